@@ -63,7 +63,8 @@ enum {
   TQ_DEV_PAGE_RANGE = 2,    /* a page-table entry outside [0, pages); the tile read zeros */
   TQ_DEV_SEQ_RANGE = 4,     /* a seq_id outside [0, sequences); the token was left empty  */
   TQ_DEV_TABLE_SHORT = 8,   /* kv_len beyond 64 * page-table width; clamped              */
-  TQ_DEV_WORK_OVERFLOW = 16 /* total page work does not fit 31 bits; nothing computed     */
+  TQ_DEV_WORK_OVERFLOW = 16,/* total page work does not fit 31 bits; nothing computed     */
+  TQ_DEV_POOL_EMPTY = 32    /* the free list ran out: the pages it lacked are -1           */
 };
 
 /* One tensor declaration (contracts.rs:109-125). rank <= 3; unused trailing axes ignored. */
@@ -349,6 +350,58 @@ int32_t tq_mla_prologue_validate(const TqPrologueSpec* spec, TqContractError* er
 int32_t tq_mla_prologue_workspace_bytes(const TqPrologueSpec* spec, uint64_t* bytes);
 int32_t tq_mla_prologue(const TqPrologueSpec* spec, void* workspace, uint64_t workspace_bytes,
                         int32_t* device_flags, void* stream, TqContractError* err);
+
+/* Step plan: the metadata of one serving step, built on the device from its request lengths. It
+ * makes the page_table / seq_id / q_pos / kv_len tensors that every call of this header takes,
+ * and the pool row of each new token. No reference counterpart: the reference plans its block
+ * tables on the host (docs/ARCHITECTURE.md:65-80).
+ *   cached_len i32 [S]     tokens of each request already in the cache
+ *   new_len    i32 [S]     new tokens of each request in this step
+ *   page_table i32 [S, L]  in/out: the first ceil(cached_len / 64) columns of a row are read as
+ *                          they are, the columns that the step grows by are written, all others
+ *                          keep their values
+ *   free_pages i32 [F]     a stack of free pages; free_count i32 [1] of them are free
+ *   q_start    i32 [S + 1] out: first token row of each request, and the number of token rows
+ *   kv_len     i32 [S]     out: cached_len + new_len
+ *   seq_id, q_pos, slot    i32 [T] out: request, position and pool row (page * 64 + position % 64)
+ *                          of each token row; rows from q_start[S] on get -1 (a batch padded to
+ *                          a captured size). `slot` may have rank 0: it is then not written.
+ *   free_left  i32 [1]     out: free_count less the pages taken; may not be free_count itself
+ * The o-th page that the batch takes, request by request and in position order, is
+ * free_pages[free_count - 1 - o]. The call changes none of its inputs but the grown columns, so
+ * the same call again gives the same result. In `device_flags` (a device int32, may be null):
+ * TQ_DEV_SEQ_RANGE (a negative length, counted as 0), TQ_DEV_TABLE_SHORT (a request needs more
+ * than L pages: kv_len is cut to 64 L), TQ_DEV_POOL_EMPTY (the missing pages are -1 and kv_len is
+ * cut to what the pages hold), TQ_DEV_WORK_OVERFLOW (more than T new tokens: q_start is cut to T),
+ * TQ_DEV_PAGE_RANGE (a page whose rows pass 31 bits). A token without a page has slot -1.
+ * One launch; the grid depends only on S and T. */
+typedef struct {
+  TqTensorSpec cached_len, new_len, page_table, free_pages, free_count;
+  TqTensorSpec q_start, kv_len, seq_id, q_pos, slot, free_left;
+} TqStepPlanSpec;
+int32_t tq_step_plan_validate(const TqStepPlanSpec* spec, TqContractError* err);
+int32_t tq_step_plan(const TqStepPlanSpec* spec, int32_t* device_flags, void* stream,
+                     TqContractError* err);
+
+/* Block norm: the step between two blocks of a layer, fused: the norm of a block's output, its
+ * gate and scaled residual sum, and the norm in front of the next block (the x of
+ * tq_mla_prologue). With rms(v) = v / sqrt(mean(v^2) + eps):
+ *   b   = post_weight given ? rms(y, post_eps) * post_weight : y
+ *   out = residual + scale * gate * b
+ *   x   = rms(out, pre_eps) * pre_weight        (from the unrounded sum)
+ *   y           bf16 [T, D]            residual, out  bf16 or f32 [T, D], one type
+ *   gate        bf16 [D], [T, D], or rank 0 (1)
+ *   post_weight bf16 [D], or rank 0    pre_weight bf16 [D] and x bf16 [T, D], or both rank 0
+ * Everything is f32 between the reads and the one rounding of each output. D is a multiple of 8
+ * up to 32768; addresses and row strides are multiples of 16, rows may be padded. `out` may be
+ * the residual itself, and x may be y itself (same address and strides); no other overlap.
+ * scale is finite. One launch of T blocks. */
+typedef struct {
+  TqTensorSpec y, residual, gate, post_weight, pre_weight, out, x;
+  float scale, post_eps, pre_eps;
+} TqBlockNormSpec;
+int32_t tq_block_norm_validate(const TqBlockNormSpec* spec, TqContractError* err);
+int32_t tq_block_norm(const TqBlockNormSpec* spec, void* stream, TqContractError* err);
 
 /* Measurement hook, no reference counterpart. Makes later tq_mla_decode / tq_mla_prefill calls
  * on the calling thread record `begin_event` right before and `end_event` right after the

@@ -385,7 +385,136 @@ int32_t prologue_validate_impl(const TqPrologueSpec* spec, TqContractError* err)
   return TQ_OK;
 }
 
+// Step plan: whole-number tensors, packed; no output overlaps an input or another output.
+int32_t step_plan_validate_impl(const TqStepPlanSpec* spec, TqContractError* err) {
+  Failure f{nullptr, TQ_OK};
+  auto fail = [&](const char* field, int32_t kind) {
+    if (err) { err->field = field; err->kind = kind; }
+    return kind;
+  };
+  if (!spec) return fail("spec", TQ_ERR_INVALID_ARGUMENT);
+  const TqStepPlanSpec& s = *spec;
+  if (s.cached_len.rank != 1) return fail("cached_len", TQ_SHAPE);
+  if (s.page_table.rank != 2) return fail("page_table", TQ_SHAPE);
+  if (s.free_pages.rank != 1) return fail("free_pages", TQ_SHAPE);
+  if (s.seq_id.rank != 1) return fail("seq_id", TQ_SHAPE);
+  const uint64_t reqs[1] = {s.cached_len.shape[0]}, starts[1] = {s.cached_len.shape[0] + 1};
+  const uint64_t table[2] = {reqs[0], s.page_table.shape[1]}, one[1] = {1};
+  const uint64_t pool[1] = {s.free_pages.shape[0]}, tok[1] = {s.seq_id.shape[0]};
+  Extent in[4], out[7];
+  int n_out = 6;
+  const int32_t i32 = TQ_DTYPE_I32;
+  const Layout packed = Layout::Packed;
+  if (!check("cached_len", s.cached_len, reqs, 1, i32, packed, true, &in[0], &f) ||
+      !check("new_len", s.new_len, reqs, 1, i32, packed, true, &in[1], &f) ||
+      !check("page_table", s.page_table, table, 2, i32, packed, true, &out[0], &f) ||
+      !check("free_pages", s.free_pages, pool, 1, i32, packed, true, &in[2], &f) ||
+      !check("free_count", s.free_count, one, 1, i32, packed, true, &in[3], &f) ||
+      !check("q_start", s.q_start, starts, 1, i32, packed, true, &out[1], &f) ||
+      !check("kv_len", s.kv_len, reqs, 1, i32, packed, true, &out[2], &f) ||
+      !check("seq_id", s.seq_id, tok, 1, i32, packed, true, &out[3], &f) ||
+      !check("q_pos", s.q_pos, tok, 1, i32, packed, true, &out[4], &f) ||
+      !check("free_left", s.free_left, one, 1, i32, packed, true, &out[5], &f))
+    return fail(f.field, f.kind);
+  if (s.slot.rank != 0) {
+    if (!check("slot", s.slot, tok, 1, i32, packed, true, &out[6], &f))
+      return fail(f.field, f.kind);
+    n_out = 7;
+  }
+  if (!check_aliases(in, 4, out, n_out, &f)) return fail(f.field, f.kind);
+  if (err) { err->field = nullptr; err->kind = TQ_OK; }
+  return TQ_OK;
+}
+
+// Two declarations of the same elements: an output written in place over its input.
+bool same_place(const TqTensorSpec& a, const TqTensorSpec& b) {
+  return a.device_address == b.device_address && a.dtype == b.dtype &&
+         a.strides_bytes[0] == b.strides_bytes[0] && a.strides_bytes[1] == b.strides_bytes[1];
+}
+
+int32_t block_norm_validate_impl(const TqBlockNormSpec* spec, TqContractError* err) {
+  Failure f{nullptr, TQ_OK};
+  auto fail = [&](const char* field, int32_t kind) {
+    if (err) { err->field = field; err->kind = kind; }
+    return kind;
+  };
+  if (!spec) return fail("spec", TQ_ERR_INVALID_ARGUMENT);
+  const TqBlockNormSpec& s = *spec;
+  if (s.y.rank != 2) return fail("y", TQ_SHAPE);
+  const uint64_t rows = s.y.shape[0], width = s.y.shape[1];
+  if (width == 0 || width % 8 || width > 32768) return fail("y", TQ_SHAPE);
+  const uint64_t shape[2] = {rows, width}, w_shape[1] = {width};
+  const bool launching = rows != 0;
+  if (s.residual.dtype != TQ_DTYPE_BF16 && s.residual.dtype != TQ_DTYPE_F32)
+    return fail("residual", TQ_DTYPE);
+  const int32_t bf = TQ_DTYPE_BF16, kind = s.residual.dtype;
+  Extent y, res, others[3], out, x;
+  int n = 0;
+  x.present = false;
+  if (!check("y", s.y, shape, 2, bf, Layout::PaddedOuter, launching, &y, &f) ||
+      !check("residual", s.residual, shape, 2, kind, Layout::PaddedOuter, launching, &res, &f))
+    return fail(f.field, f.kind);
+  if (s.gate.rank != 0) {
+    if (s.gate.rank == 1 ? !check("gate", s.gate, w_shape, 1, bf, Layout::Packed, launching,
+                                  &others[n++], &f)
+                         : !check("gate", s.gate, shape, 2, bf, Layout::PaddedOuter, launching,
+                                  &others[n++], &f))
+      return fail(f.field, f.kind);
+  }
+  if (s.post_weight.rank != 0 &&
+      !check("post_weight", s.post_weight, w_shape, 1, bf, Layout::Packed, launching,
+             &others[n++], &f))
+    return fail(f.field, f.kind);
+  if ((s.pre_weight.rank != 0) != (s.x.rank != 0)) return fail("x", TQ_SHAPE);
+  if (s.x.rank != 0 &&
+      (!check("pre_weight", s.pre_weight, w_shape, 1, bf, Layout::Packed, launching,
+              &others[n++], &f) ||
+       !check("x", s.x, shape, 2, bf, Layout::PaddedOuter, launching, &x, &f)))
+    return fail(f.field, f.kind);
+  if (!check("out", s.out, shape, 2, kind, Layout::PaddedOuter, launching, &out, &f))
+    return fail(f.field, f.kind);
+  if (launching) {
+    const TqTensorSpec* all[7] = {&s.y, &s.residual, &s.gate, &s.post_weight, &s.pre_weight,
+                                  &s.out, &s.x};
+    const char* names[7] = {"y", "residual", "gate", "post_weight", "pre_weight", "out", "x"};
+    for (int i = 0; i < 7; ++i) {
+      if (all[i]->rank == 0) continue;
+      if (all[i]->device_address % 16) return fail(names[i], TQ_ALIGNMENT);
+      if (all[i]->rank == 2 && all[i]->strides_bytes[0] % 16) return fail(names[i], TQ_STRIDE);
+    }
+  }
+  if (!std::isfinite(s.scale)) return fail("scale", TQ_SCALE);
+  if (s.post_weight.rank != 0 && !(std::isfinite(s.post_eps) && s.post_eps > 0.f))
+    return fail("post_eps", TQ_SCALE);
+  if (s.x.rank != 0 && !(std::isfinite(s.pre_eps) && s.pre_eps > 0.f))
+    return fail("pre_eps", TQ_SCALE);
+  // A row is read whole before any of it is written, so out over the residual and x over y are
+  // fine row by row; any other overlap is not.
+  Extent in[6];
+  int m = 0;
+  for (int i = 0; i < n; ++i) in[m++] = others[i];
+  const int shared = m;
+  in[m++] = y;
+  if (!same_place(s.out, s.residual)) in[m++] = res;
+  if (!check_aliases(in, m, &out, 1, &f)) return fail(f.field, f.kind);
+  m = shared;
+  in[m++] = res;
+  in[m++] = out;
+  if (s.x.rank != 0 && !same_place(s.x, s.y)) in[m++] = y;
+  if (!check_aliases(in, m, &x, 1, &f)) return fail(f.field, f.kind);
+  if (err) { err->field = nullptr; err->kind = TQ_OK; }
+  return TQ_OK;
+}
+
 }  // namespace
+
+int32_t step_plan_validate(const TqStepPlanSpec* spec, TqContractError* err) {
+  return step_plan_validate_impl(spec, err);
+}
+
+int32_t block_norm_validate(const TqBlockNormSpec* spec, TqContractError* err) {
+  return block_norm_validate_impl(spec, err);
+}
 
 int32_t prologue_validate(const TqPrologueSpec* spec, TqContractError* err) {
   return prologue_validate_impl(spec, err);
@@ -468,6 +597,14 @@ int32_t tq_kv_write_validate(const TqKvWriteSpec* spec, TqContractError* err) {
 
 int32_t tq_mla_prologue_validate(const TqPrologueSpec* spec, TqContractError* err) {
   return tq::prologue_validate(spec, err);
+}
+
+int32_t tq_step_plan_validate(const TqStepPlanSpec* spec, TqContractError* err) {
+  return tq::step_plan_validate(spec, err);
+}
+
+int32_t tq_block_norm_validate(const TqBlockNormSpec* spec, TqContractError* err) {
+  return tq::block_norm_validate(spec, err);
 }
 
 int32_t tq_mla_should_launch(const TqMlaParams* params) {

@@ -64,6 +64,12 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ long long ld_cluster_s64(uint32_t addr) {
+  long long v;
+  asm volatile("ld.shared::cluster.s64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t a) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" :: "r"(addr), "r"(a) : "memory");
 }

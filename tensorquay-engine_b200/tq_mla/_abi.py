@@ -21,6 +21,7 @@ STATUS = {
     105: "Range", 106: "Comm",
 }
 DEV_WAIT_TIMEOUT, DEV_PAGE_RANGE, DEV_SEQ_RANGE, DEV_TABLE_SHORT, DEV_WORK_OVERFLOW = 1, 2, 4, 8, 16
+DEV_POOL_EMPTY = 32
 
 
 class TqTensorSpec(ctypes.Structure):
@@ -103,6 +104,18 @@ class TqPrologueSpec(ctypes.Structure):
                 "q_eps", "kv_eps", "rope_theta")]
 
 
+class TqStepPlanSpec(ctypes.Structure):
+    _fields_ = [(name, TqTensorSpec) for name in (
+        "cached_len", "new_len", "page_table", "free_pages", "free_count", "q_start", "kv_len",
+        "seq_id", "q_pos", "slot", "free_left")]
+
+
+class TqBlockNormSpec(ctypes.Structure):
+    _fields_ = [(name, TqTensorSpec) for name in (
+        "y", "residual", "gate", "post_weight", "pre_weight", "out", "x")] + [
+            (name, ctypes.c_float) for name in ("scale", "post_eps", "pre_eps")]
+
+
 # Every exported symbol of include/tq_mla.h, with its ctypes prototype.
 _P = ctypes.POINTER
 _U64, _I32, _VP = ctypes.c_uint64, ctypes.c_int32, ctypes.c_void_p
@@ -140,6 +153,10 @@ PROTOTYPES = {
     "tq_mla_prologue_validate": (_I32, [_P(TqPrologueSpec), _P(TqContractError)]),
     "tq_mla_prologue_workspace_bytes": (_I32, [_P(TqPrologueSpec), _P(_U64)]),
     "tq_mla_prologue": (_I32, [_P(TqPrologueSpec), _VP, _U64, _VP, _VP, _P(TqContractError)]),
+    "tq_step_plan_validate": (_I32, [_P(TqStepPlanSpec), _P(TqContractError)]),
+    "tq_step_plan": (_I32, [_P(TqStepPlanSpec), _VP, _VP, _P(TqContractError)]),
+    "tq_block_norm_validate": (_I32, [_P(TqBlockNormSpec), _P(TqContractError)]),
+    "tq_block_norm": (_I32, [_P(TqBlockNormSpec), _VP, _P(TqContractError)]),
     "tq_philox_block": (None, [_P(ctypes.c_uint32), _P(ctypes.c_uint32), _P(ctypes.c_uint32)]),
     "tq_philox_words": (_I32, [_U64, _U64, _U64, _P(ctypes.c_uint32), _U64]),
     "tq_philox_uniform_f32": (ctypes.c_float, [ctypes.c_uint32]),

@@ -8,6 +8,7 @@ in dense paged form): it owns nothing but a workspace, and every launch goes thr
 and to name the current stream.
 """
 
+import collections
 import ctypes
 import math
 
@@ -299,6 +300,129 @@ def mla_prologue(x, w_qa, q_norm, w_qb, w_uk, w_kva, kv_norm, pos, seq_id, page_
         q = torch.empty((x.shape[0], heads, 512 + rope_dim), dtype=torch.bfloat16, device=x.device)
     return MlaPrologue(x, w_qa, q_norm, w_qb, w_uk, w_kva, kv_norm, pos, seq_id, page_table, kv, q,
                        heads=heads, nope_dim=nope_dim, rope_dim=rope_dim, **kw)(flags, stream)
+
+
+class _Launch:
+    """A validated call bound to its tensors (kept referenced): what a serving loop makes once and
+    calls every step. It launches on the device that holds its tensors, whichever is current, on
+    ``stream`` or that device's current stream."""
+
+    def _bind(self, *tensors):
+        self._keep = tensors
+        devices = {t.device for t in tensors if t is not None}
+        if len(devices) != 1 or next(iter(devices)).type != "cuda":
+            raise ValueError(f"the tensors must be on one CUDA device, not on {sorted(map(str, devices))}")
+        self.device = next(iter(devices))
+
+    def _run(self, launch, stream):
+        if torch.cuda.current_device() == self.device.index:
+            return launch(_stream_handle(stream))
+        with torch.cuda.device(self.device):
+            return launch(_stream_handle(stream))
+
+
+def _flags_pointer(flags):
+    return ctypes.c_void_p(flags.data_ptr()) if flags is not None else None
+
+
+#: What ``StepPlan`` fills: the step's metadata as the other operators take it.
+StepTables = collections.namedtuple(
+    "StepTables", "q_start kv_len seq_id q_pos slot page_table free_left")
+
+
+def step_plan_spec(cached_len, new_len, page_table, free_pages, free_count, q_start, kv_len, seq_id,
+                   q_pos, slot, free_left):
+    """Declaration of a step plan (``tq_step_plan``); ``slot`` may be None."""
+    s = _abi.TqStepPlanSpec()
+    for name, t in (("cached_len", cached_len), ("new_len", new_len), ("page_table", page_table),
+                    ("free_pages", free_pages), ("free_count", free_count), ("q_start", q_start),
+                    ("kv_len", kv_len), ("seq_id", seq_id), ("q_pos", q_pos), ("slot", slot),
+                    ("free_left", free_left)):
+        if t is not None:
+            setattr(s, name, spec_of(t))
+    return s
+
+
+class StepPlan(_Launch):
+    """The metadata of one serving step, built on the device from its request lengths.
+
+    ``cached_len``/``new_len`` i32 ``[S]``; ``page_table`` i32 ``[S, L]`` (in/out: the columns that
+    the step grows by are filled from the stack ``free_pages[:free_count]``, last page first);
+    ``tokens`` token rows. A call fills ``tables`` (``StepTables``): ``q_start [S + 1]``,
+    ``kv_len [S]``, ``seq_id``/``q_pos``/``slot [tokens]`` (-1 behind the last token),
+    ``page_table`` and ``free_left [1]``. Nothing else changes, so the next step starts from
+    ``kv_len`` as its ``cached_len`` and ``free_left`` as its ``free_count``.
+    """
+
+    def __init__(self, cached_len, new_len, page_table, free_pages, free_count, *, tokens):
+        n, dev = cached_len.shape[0], cached_len.device
+        new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=dev)  # noqa: E731
+        self.tables = StepTables(new(n + 1), new(n), new(tokens), new(tokens), new(tokens), page_table,
+                                 new(1))
+        t = self.tables
+        self._bind(cached_len, new_len, page_table, free_pages, free_count, t.q_start, t.seq_id)
+        self.spec = step_plan_spec(cached_len, new_len, page_table, free_pages, free_count, t.q_start,
+                                   t.kv_len, t.seq_id, t.q_pos, t.slot, t.free_left)
+        err = _abi.TqContractError()
+        raise_for(lib.tq_step_plan_validate(ctypes.byref(self.spec), ctypes.byref(err)), err)
+
+    def __call__(self, flags=None, stream=None):
+        err = _abi.TqContractError()
+        raise_for(self._run(lambda s: lib.tq_step_plan(ctypes.byref(self.spec), _flags_pointer(flags), s,
+                                                       ctypes.byref(err)), stream), err)
+        return self.tables
+
+
+def step_plan(cached_len, new_len, page_table, free_pages, free_count, *, tokens, flags=None,
+              stream=None):
+    """One step plan (see ``StepPlan``); returns its ``StepTables``."""
+    return StepPlan(cached_len, new_len, page_table, free_pages, free_count, tokens=tokens)(flags, stream)
+
+
+def block_norm_spec(y, residual, out, x=None, *, post_weight=None, gate=None, scale=1.0,
+                    pre_weight=None, eps=1e-6, post_eps=None):
+    """Declaration of a block norm (``tq_block_norm``); ``eps`` is both norms' unless ``post_eps``."""
+    s = _abi.TqBlockNormSpec()
+    for name, t in (("y", y), ("residual", residual), ("gate", gate), ("post_weight", post_weight),
+                    ("pre_weight", pre_weight), ("out", out), ("x", x)):
+        if t is not None:
+            setattr(s, name, spec_of(t))
+    s.scale = float(scale)
+    s.pre_eps = float(eps)
+    s.post_eps = float(eps if post_eps is None else post_eps)
+    return s
+
+
+class BlockNorm(_Launch):
+    """The step between two blocks: ``out = residual + scale * gate * b`` with ``b`` the block's
+    output ``y``, RMS-normalised when ``post_weight`` is given, and ``x = rms(out) * pre_weight``,
+    the next block's input, when ``pre_weight`` and ``x`` are. One pass over the rows.
+
+    ``y`` bf16 ``[T, D]``; ``residual``/``out`` bf16 or f32 ``[T, D]`` (``out`` may be ``residual``);
+    ``gate`` bf16 ``[D]`` or ``[T, D]``; weights bf16 ``[D]``; ``x`` bf16 ``[T, D]`` (may be ``y``).
+    """
+
+    def __init__(self, y, residual, out, x=None, **kw):
+        self._bind(y, residual, out, x, kw.get("post_weight"), kw.get("gate"), kw.get("pre_weight"))
+        self.spec = block_norm_spec(y, residual, out, x, **kw)
+        err = _abi.TqContractError()
+        raise_for(lib.tq_block_norm_validate(ctypes.byref(self.spec), ctypes.byref(err)), err)
+        self.out, self.x = out, x
+
+    def __call__(self, stream=None):
+        err = _abi.TqContractError()
+        raise_for(self._run(lambda s: lib.tq_block_norm(ctypes.byref(self.spec), s, ctypes.byref(err)),
+                            stream), err)
+        return self.out, self.x
+
+
+def block_norm(y, residual, *, pre_weight=None, out=None, x=None, stream=None, **kw):
+    """One block norm (see ``BlockNorm``); returns ``(out, x)``, ``x`` None without ``pre_weight``."""
+    if out is None:
+        out = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
+    if x is None and pre_weight is not None:
+        x = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    return BlockNorm(y, residual, out, x, pre_weight=pre_weight, **kw)(stream)
 
 
 def combine_parts(part_out, part_lse, out=None, lse=None, stream=None):
