@@ -403,6 +403,49 @@ typedef struct {
 int32_t tq_block_norm_validate(const TqBlockNormSpec* spec, TqContractError* err);
 int32_t tq_block_norm(const TqBlockNormSpec* spec, void* stream, TqContractError* err);
 
+/* Chunk attention: each sequence's chunk of new tokens over its paged latent rows, with per-head
+ * keys and values expanded from them. It is the same attention as tq_mla_prefill without the
+ * weights folded into the query and the output: a (query, key, head) triple costs
+ * 2 (Dn + Dr + Dv) FLOP instead of 2 (1024 + Dr), and each cached row costs 1024 (Dn + Dv) FLOP
+ * a head once per call, so it is the cheaper form from about 170 query tokens per cached row on
+ * (tq_mla_prefill is below that, tq_mla_decode for single tokens). For sequence s, rows
+ * t in [q_start[s], q_start[s + 1]) and cached rows n < kv_len[s]:
+ *   k[n, h] = bf16(latent[n] . w_uk[h]^T), followed by the row's Dr RoPE values
+ *   v[n, h] = bf16(latent[n] . w_uv[h]^T)
+ *   out[t, h] = sum_n softmax_n(softmax_scale * q[t, h] . k[n, h]) v[n, h]  over the rows
+ *               n < min(kv_len[s], q_pos[t] + 1);      lse[t, h] = log sum_n exp(score)
+ *   q          bf16 [T, H, Dn + Dr]   as the prologue makes it without absorption, RoPE applied
+ *   w_uk       bf16 [H, Dn, 512]      w_uv bf16 [H, Dv, 512] (outer strides may be padded: both
+ *                                     may be slices of one [H, Dn + Dv, 512] weight)
+ *   kv         u8   [P, 64, payload]  page_table i32 [S, L]
+ *   q_start    i32  [S + 1]           q_pos i32 [T]          kv_len i32 [S]
+ *   out        bf16 or f32 [T, H, Dv] lse f32 [T, H], or rank 0
+ * H is 1 to 128. 576-wide rows (TQ_KV_BF16_ROPE576): Dn = Dv = 128, Dr = 64; 512-wide rows
+ * (TQ_KV_BF16, TQ_KV_FP8_E4M3): Dn = Dv = 256, Dr = 0. softmax_scale is any finite f32 > 0.
+ * Addresses and strides of q, w_uk, w_uv and out are multiples of 16; T and max_keys are at most
+ * 2^24, and max_keys + 127 min(S, T) at most 2^25. `max_keys` is the host's bound on the summed kv_len of the sequences that have tokens: it
+ * sizes the workspace. A token without a visible row gets zeros and lse -inf; rows of q before
+ * q_start[0] and from q_start[S] on are not computed and their outputs are left as they were. A
+ * cached row that is not finite makes every output that sees it NaN and no other; FP8 rows are
+ * dequantized to bf16 first. Rounding points: k and v to bf16 (the model's own), the softmax
+ * weights to bf16 before the value product; statistics and sums are f32.
+ * Device error flags (tq_mla_read_device_error): TQ_DEV_PAGE_RANGE (a page-table entry outside
+ * the pool: its rows read as zeros), TQ_DEV_TABLE_SHORT (kv_len past 64 L, cut),
+ * TQ_DEV_SEQ_RANGE (q_start not ascending within [0, T]: nothing is computed),
+ * TQ_DEV_WORK_OVERFLOW (more rows than max_keys: nothing is computed), TQ_DEV_WAIT_TIMEOUT.
+ * The workspace is 256-byte aligned; calls that share one must be ordered on one stream. The
+ * launches depend only on the spec, so a captured call replays for new contents. */
+typedef struct {
+  TqTensorSpec q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse;
+  int32_t kv_format;
+  float softmax_scale;
+  uint64_t max_keys;
+} TqMlaChunkSpec;
+int32_t tq_mla_chunk_validate(const TqMlaChunkSpec* spec, TqContractError* err);
+int32_t tq_mla_chunk_workspace_bytes(const TqMlaChunkSpec* spec, int32_t device, uint64_t* bytes);
+int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace, uint64_t workspace_bytes,
+                     void* stream, TqContractError* err);
+
 /* Measurement hook, no reference counterpart. Makes later tq_mla_decode / tq_mla_prefill calls
  * on the calling thread record `begin_event` right before and `end_event` right after the
  * attention kernel, on the launch stream (both are cudaEvent_t created by the caller). Pass two

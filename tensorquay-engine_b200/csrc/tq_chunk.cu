@@ -1,0 +1,511 @@
+// Chunk attention (tq_mla_chunk): each sequence's chunk of new tokens over its paged latent rows,
+// with per-head keys and values expanded from them once per call:
+//   k[n, h] = bf16(latent[n] . w_uk[h]^T) | rope[n]      v[n, h] = bf16(latent[n] . w_uv[h]^T)
+//   out[t, h] = softmax_n(scale * q[t, h] . k[n, h]) v[n, h],  n < min(kv_len, q_pos[t] + 1)
+//
+// Launches, in order on the caller's stream:
+//   1. plan_kernel    one block: each sequence's cached rows laid end to end in a compact row space
+//                     (every sequence padded to kRowTile rows), its query blocks of kQueryTile
+//                     tokens with the number of row tiles each of them sees.
+//   2. gather_kernel  the cached rows through the page table into that space, as bf16 (FP8 rows
+//                     dequantized, rounded once): zeros past kv_len, and zeros with a mark for a
+//                     row that is not finite, so that neither stale rows nor such a row can reach
+//                     an output that does not see it through 0 * NaN.
+//   3. expand_kernel  k and v of every head from the compact rows.
+//   4. attend_kernel  attention of every (query block, head).
+// Heads are taken in passes that bound the scratch of step 3 (kScratchBytes).
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "tq_contracts.h"
+#include "tq_ptx.cuh"
+
+namespace tq {
+namespace chunk {
+
+constexpr int kPage = 64;
+constexpr int kLatent = 512;
+constexpr int kRopeDim = 64;
+constexpr int kRowTile = 128;    // keys per attention step; sequences are padded to it
+constexpr int kQueryTile = 256;  // query tokens of one attention unit
+constexpr uint64_t kScratchBytes = 8ull << 30;
+
+enum Header : int {
+  kHdrError = 0,
+  kHdrRows = 1,    // compact rows in use (padded)
+  kHdrBlocks = 2,  // query blocks
+  kHdrMarked = 3,  // rows that are not finite
+  kHdrWords = 64
+};
+
+// One query block of one sequence.
+struct Block {
+  int row0, rows;   // query tokens
+  int key0, tiles;  // first compact row, row tiles seen
+};
+
+struct Work {
+  int* header;
+  int* seq_key0;   // [S + 1] first compact row of each sequence
+  int* seq_keys;   // [S] cached rows in use
+  int* seq_block;  // [S + 1] first query block of each sequence
+  Block* blocks;
+  uint8_t* marked;  // [cap] 1 where a compact row is not finite
+  uint16_t* rows;   // bf16 [cap, 512]
+  uint16_t* rope;   // bf16 [cap, 64]
+  uint16_t* k;      // bf16 [heads of a pass, cap, Dn]
+  uint16_t* v;      // bf16 [heads of a pass, cap, Dv]
+};
+
+struct Args {
+  Work w;
+  const uint8_t* q;
+  const uint8_t* kv;
+  const uint16_t* w_uk;
+  const uint16_t* w_uv;
+  const int* page_table;
+  const int* q_start;
+  const int* q_pos;
+  const int* kv_len;
+  uint8_t* out;
+  float* lse;  // may be null
+  long long q_st, q_sh, out_st, out_sh;           // bytes
+  long long uk_sh, uk_sr, uv_sh, uv_sr;           // elements
+  long long row_stride;
+  int tokens, heads, seqs, slots, pages, cap, max_blocks;
+  int head0, pass_heads;
+  int dn, dr, dv, fp8, out_f32;
+  float scale_log2;
+};
+
+// ------------------------------------------------------------------------------ plan
+__device__ __forceinline__ int warp_inclusive(int v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// Inclusive sum over the 1024 threads of a block.
+__device__ __forceinline__ int block_inclusive(int v, int* part) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int inc = warp_inclusive(v);
+  if (lane == 31) part[warp] = inc;
+  __syncthreads();
+  if (warp == 0) part[lane] = warp_inclusive(part[lane]);
+  __syncthreads();
+  const int out = inc + (warp ? part[warp - 1] : 0);
+  __syncthreads();
+  return out;
+}
+
+__device__ __forceinline__ int last_at_or_below(const int* start, int n, int x) {
+  int b = 0, e = n;
+  while (e - b > 1) {
+    const int m = (b + e) >> 1;
+    if (start[m] <= x) b = m; else e = m;
+  }
+  return b;
+}
+
+__global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
+  __shared__ int part[32];
+  __shared__ int s_rows, s_blocks, s_over;
+  const Work& w = a.w;
+  const int tid = threadIdx.x;
+  if (tid < kHdrWords) w.header[tid] = 0;
+  if (tid == 0) { s_rows = 0; s_blocks = 0; s_over = 0; }
+  __syncthreads();
+  int bad = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += 1024) {
+    const int s = s0 + tid;
+    int keys = 0, blocks = 0;
+    if (s < a.seqs) {
+      const int b = a.q_start[s], e = a.q_start[s + 1];
+      int n = e - b;
+      if (b < 0 || e < b || e > a.tokens) {
+        // Sequences that overlap would write each other's outputs: the whole call is left out.
+        bad |= TQ_DEV_SEQ_RANGE;
+        s_over = 1;
+        n = 0;
+      }
+      if (n > 0) {
+        const long long room = (long long)kPage * a.slots;
+        keys = max(a.kv_len[s], 0);
+        if (keys > room) {
+          keys = int(room);
+          bad |= TQ_DEV_TABLE_SHORT;
+        }
+        // A sequence past the bound alone; keeps the sums below in range.
+        if (keys > a.cap) { s_over = 1; keys = 0; }
+      }
+      blocks = (n + kQueryTile - 1) / kQueryTile;
+    }
+    const int padded = (keys + kRowTile - 1) / kRowTile * kRowTile;
+    const int rows_end = block_inclusive(padded, part), blocks_end = block_inclusive(blocks, part);
+    const int rows0 = s_rows, blocks0 = s_blocks;
+    __syncthreads();
+    // 1024 sequences of at most cap <= 2^25 rows may pass 2^31: a warp's 32 are summed in 64 bits
+    // below, and 32 warps within cap stay below 2^30.
+    if (s < a.seqs) {
+      w.seq_key0[s] = rows0 + rows_end - padded;
+      w.seq_keys[s] = keys;
+      w.seq_block[s] = blocks0 + blocks_end - blocks;
+    }
+    long long sum = padded;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if ((tid & 31) == 0 && sum > a.cap) s_over = 1;
+    if (rows_end < 0 || rows_end > a.cap - rows0 || blocks0 + blocks_end > a.max_blocks)
+      s_over = 1;
+    if (tid == 1023) {
+      s_rows = rows0 + rows_end;
+      s_blocks = blocks0 + blocks_end;
+    }
+    __syncthreads();
+    if (s_over) break;
+  }
+  if (bad) atomicOr(w.header + kHdrError, bad);
+  if (s_over) {
+    const int range = __syncthreads_or(bad & TQ_DEV_SEQ_RANGE);
+    if (tid == 0) {
+      if (!range) atomicOr(w.header + kHdrError, TQ_DEV_WORK_OVERFLOW);
+      w.header[kHdrRows] = 0;
+      w.header[kHdrBlocks] = 0;
+    }
+    return;
+  }
+  if (tid == 0) {
+    w.seq_key0[a.seqs] = s_rows;
+    w.seq_block[a.seqs] = s_blocks;
+    w.header[kHdrRows] = s_rows;
+    w.header[kHdrBlocks] = s_blocks;
+  }
+  __syncthreads();
+  // Query blocks, one warp each: the tiles that its furthest-seeing token sees.
+  const int lane = tid & 31;
+  for (int b = tid >> 5; b < s_blocks; b += 32) {
+    const int s = last_at_or_below(w.seq_block, a.seqs, b);
+    const int row0 = a.q_start[s] + (b - w.seq_block[s]) * kQueryTile;
+    const int rows = min(kQueryTile, a.q_start[s + 1] - row0);
+    int far = -1;
+    for (int i = lane; i < rows; i += 32) far = max(far, a.q_pos[row0 + i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) far = max(far, __shfl_xor_sync(0xFFFFFFFFu, far, o));
+    const int keys = w.seq_keys[s];
+    const int seen = far >= keys ? keys : far + 1;
+    if (lane == 0) w.blocks[b] = {row0, rows, w.seq_key0[s], (seen + kRowTile - 1) / kRowTile};
+  }
+}
+
+// ------------------------------------------------------------------------------ gather
+__device__ __forceinline__ bool finite_bf16x2(uint32_t u) {
+  return (u & 0x7F80u) != 0x7F80u && (u & 0x7F800000u) != 0x7F800000u;
+}
+
+// One block per kRowTile compact rows, one warp per row at a time: lane i takes the 16 latent
+// values from 16 i on, and two of the 64 RoPE values.
+__global__ void __launch_bounds__(256) gather_kernel(const Args a) {
+  const Work& w = a.w;
+  const int r0 = int(blockIdx.x) * kRowTile;
+  if (r0 >= w.header[kHdrRows]) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int s = last_at_or_below(w.seq_key0, a.seqs, r0);
+  const int first = r0 - w.seq_key0[s], keys = w.seq_keys[s];
+#pragma unroll 4
+  for (int i = warp; i < kRowTile; i += 8) {
+    const int p = first + i;
+    uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
+    uint32_t rp = 0;
+    if (p < keys) {
+      const int page = a.page_table[(long long)s * a.slots + p / kPage];
+      if (page >= 0 && page < a.pages) {
+        const uint8_t* src = a.kv + ((long long)page * kPage + p % kPage) * a.row_stride;
+        if (a.fp8) {
+          const uint4 c = *reinterpret_cast<const uint4*>(src + 16 * lane);
+          const float sc = *reinterpret_cast<const float*>(src + kLatent + 4 * (lane >> 3));
+          v0 = make_uint4(ptx::e4m3x2_scaled_bf16x2(c.x & 0xFFFF, sc),
+                          ptx::e4m3x2_scaled_bf16x2(c.x >> 16, sc),
+                          ptx::e4m3x2_scaled_bf16x2(c.y & 0xFFFF, sc),
+                          ptx::e4m3x2_scaled_bf16x2(c.y >> 16, sc));
+          v1 = make_uint4(ptx::e4m3x2_scaled_bf16x2(c.z & 0xFFFF, sc),
+                          ptx::e4m3x2_scaled_bf16x2(c.z >> 16, sc),
+                          ptx::e4m3x2_scaled_bf16x2(c.w & 0xFFFF, sc),
+                          ptx::e4m3x2_scaled_bf16x2(c.w >> 16, sc));
+        } else {
+          v0 = *reinterpret_cast<const uint4*>(src + 32 * lane);
+          v1 = *reinterpret_cast<const uint4*>(src + 32 * lane + 16);
+          if (a.dr) rp = *reinterpret_cast<const uint32_t*>(src + 2 * kLatent + 4 * lane);
+        }
+      } else if (lane == 0) {
+        atomicOr(w.header + kHdrError, TQ_DEV_PAGE_RANGE);
+      }
+    }
+    const bool ok = finite_bf16x2(v0.x) && finite_bf16x2(v0.y) && finite_bf16x2(v0.z) &&
+                    finite_bf16x2(v0.w) && finite_bf16x2(v1.x) && finite_bf16x2(v1.y) &&
+                    finite_bf16x2(v1.z) && finite_bf16x2(v1.w) && finite_bf16x2(rp);
+    const bool row_ok = __all_sync(0xFFFFFFFFu, ok);
+    if (!row_ok) {
+      v0 = v1 = make_uint4(0, 0, 0, 0);
+      rp = 0;
+    }
+    const long long r = r0 + i;
+    uint16_t* dst = w.rows + r * kLatent + 16 * lane;
+    *reinterpret_cast<uint4*>(dst) = v0;
+    *reinterpret_cast<uint4*>(dst + 8) = v1;
+    if (a.dr) *reinterpret_cast<uint32_t*>(w.rope + r * kRopeDim + 2 * lane) = rp;
+    if (lane == 0) {
+      w.marked[r] = row_ok ? 0 : 1;
+      if (!row_ok) atomicAdd(w.header + kHdrMarked, 1);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------ expand
+// 64 compact rows x 64 columns of one head's [k | v] per block, 16 x 16 threads of 4 x 4.
+__global__ void __launch_bounds__(256) expand_kernel(const Args a) {
+  const Work& w = a.w;
+  const int r0 = int(blockIdx.x) * 64;
+  if (r0 >= w.header[kHdrRows]) return;
+  const int c0 = int(blockIdx.y) * 64, h = int(blockIdx.z);
+  const bool is_v = c0 >= a.dn;
+  const int c = is_v ? c0 - a.dn : c0;
+  const uint16_t* weight = is_v ? a.w_uv + (a.head0 + h) * a.uv_sh + c * a.uv_sr
+                                : a.w_uk + (a.head0 + h) * a.uk_sh + c * a.uk_sr;
+  const long long wr = is_v ? a.uv_sr : a.uk_sr;
+  __shared__ float xs[32][65], ws[32][65];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float acc[4][4] = {};
+  for (int k0 = 0; k0 < kLatent; k0 += 32) {
+    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
+      const int r = i >> 5, k = i & 31;
+      xs[k][r] = __uint_as_float(uint32_t(w.rows[(long long)(r0 + r) * kLatent + k0 + k]) << 16);
+      ws[k][r] = __uint_as_float(uint32_t(weight[r * wr + k0 + k]) << 16);
+    }
+    __syncthreads();
+    for (int k = 0; k < 32; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[k][ty * 4 + i], ws[k][tx * 4 + j], acc[i][j]);
+    __syncthreads();
+  }
+  const int width = is_v ? a.dv : a.dn;
+  uint16_t* dst = is_v ? w.v : w.k;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t* o = reinterpret_cast<uint32_t*>(
+        dst + ((long long)h * a.cap + r0 + ty * 4 + i) * width + c + tx * 4);
+    o[0] = ptx::pack_bf16x2(acc[i][0], acc[i][1]);
+    o[1] = ptx::pack_bf16x2(acc[i][2], acc[i][3]);
+  }
+}
+
+// ------------------------------------------------------------------------------ attend
+// One block per (query token, head): 128 threads, one key each per step, then one or two value
+// columns each.
+__global__ void __launch_bounds__(128) attend_kernel(const Args a) {
+  const Work& w = a.w;
+  const int t = int(blockIdx.x), h = int(blockIdx.y), tid = int(threadIdx.x);
+  if (!w.header[kHdrBlocks]) return;
+  // The token's sequence: the last block that starts at or before it, if it covers it.
+  int b = 0, e = w.header[kHdrBlocks];
+  while (e - b > 1) {
+    const int m = (b + e) >> 1;
+    if (w.blocks[m].row0 <= t) b = m; else e = m;
+  }
+  const Block blk = w.blocks[b];
+  if (t < blk.row0 || t >= blk.row0 + blk.rows) return;
+  const int s = last_at_or_below(w.seq_block, a.seqs, b);
+  const int pos = a.q_pos[t], keys = w.seq_keys[s];
+  const int n = pos >= keys ? keys : max(pos + 1, 0);
+  __shared__ float qs[256], ps[128], red[8];
+  const int dq = a.dn + a.dr;
+  const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q + t * a.q_st + (a.head0 + h) * a.q_sh);
+  for (int i = tid; i < dq; i += 128) qs[i] = __uint_as_float(uint32_t(q[i]) << 16);
+  __syncthreads();
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int k0 = 0; k0 < n; k0 += 128) {
+    const long long r = blk.key0 + k0 + tid;
+    float x = -INFINITY;
+    if (k0 + tid < n) {
+      const uint16_t* k = w.k + ((long long)h * a.cap + r) * a.dn;
+      float d = 0.f;
+      for (int i = 0; i < a.dn; ++i) d = fmaf(qs[i], __uint_as_float(uint32_t(k[i]) << 16), d);
+      for (int i = 0; i < a.dr; ++i)
+        d = fmaf(qs[a.dn + i], __uint_as_float(uint32_t(w.rope[r * kRopeDim + i]) << 16), d);
+      x = w.marked[r] ? NAN : d * a.scale_log2;
+    }
+    float mx = x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+    if ((tid & 31) == 0) red[tid >> 5] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float m1 = fmaxf(m, mx), use = m1 == -INFINITY ? 0.f : m1;
+    const float keep = exp2f(m - use);
+    const float p = exp2f(x - use);
+    ps[tid] = p;
+    float sum = p;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if ((tid & 31) == 0) red[4 + (tid >> 5)] = sum;
+    __syncthreads();
+    l = l * keep + red[4] + red[5] + red[6] + red[7];
+    o0 *= keep;
+    o1 *= keep;
+    const uint16_t* v = w.v + ((long long)h * a.cap + blk.key0 + k0) * a.dv;
+    const int lim = min(128, n - k0);
+    for (int j = 0; j < lim; ++j) {
+      o0 = fmaf(ps[j], __uint_as_float(uint32_t(v[(long long)j * a.dv + tid]) << 16), o0);
+      if (a.dv > 128)
+        o1 = fmaf(ps[j], __uint_as_float(uint32_t(v[(long long)j * a.dv + 128 + tid]) << 16), o1);
+    }
+    m = m1;
+    __syncthreads();
+  }
+  const float inv = n > 0 ? 1.f / l : 0.f;
+  uint8_t* out = a.out + t * a.out_st + (a.head0 + h) * a.out_sh;
+  for (int c = 0; c < a.dv / 128; ++c) {
+    const float o = (c ? o1 : o0) * inv;
+    if (a.out_f32)
+      reinterpret_cast<float*>(out)[c * 128 + tid] = o;
+    else
+      reinterpret_cast<__nv_bfloat16*>(out)[c * 128 + tid] = __float2bfloat16(o);
+  }
+  if (a.lse && tid == 0)
+    a.lse[(long long)t * a.heads + a.head0 + h] =
+        n > 0 ? 0.69314718055994531f * (m + log2f(l)) : -INFINITY;
+}
+
+// ------------------------------------------------------------------------------ host
+struct Layout {
+  uint64_t header, seq_key0, seq_keys, seq_block, blocks, marked, rows, rope, k, v, total;
+  uint64_t cap, max_blocks, pass_heads;
+};
+
+uint64_t round256(uint64_t v) { return (v + 255) & ~uint64_t(255); }
+
+Layout layout_of(const TqMlaChunkSpec& s) {
+  const uint64_t T = s.q.shape[0], H = s.q.shape[1], S = s.page_table.shape[0];
+  const uint64_t dn = s.w_uk.shape[1], dv = s.w_uv.shape[1];
+  const uint64_t busy = S < T ? S : T;  // sequences that can have tokens
+  Layout l;
+  // Every busy sequence may end inside a row tile; whole pairs of tiles for the expansion.
+  l.cap = (s.max_keys + busy * (kRowTile - 1) + 255) / 256 * 256;
+  if (l.cap == 0) l.cap = 256;
+  l.max_blocks = T / kQueryTile + busy;
+  const uint64_t per_head = l.cap * (dn + dv) * 2;
+  l.pass_heads = kScratchBytes / per_head;
+  if (l.pass_heads < 1) l.pass_heads = 1;
+  if (l.pass_heads > H) l.pass_heads = H;
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t here = at;
+    at += round256(bytes);
+    return here;
+  };
+  l.header = take(kHdrWords * 4);
+  l.seq_key0 = take((S + 1) * 4);
+  l.seq_keys = take((S + 1) * 4);
+  l.seq_block = take((S + 1) * 4);
+  l.blocks = take(l.max_blocks * sizeof(Block));
+  l.marked = take(l.cap);
+  l.rows = take(l.cap * kLatent * 2);
+  l.rope = take(l.cap * kRopeDim * 2);
+  l.k = take(l.pass_heads * l.cap * dn * 2);
+  l.v = take(l.pass_heads * l.cap * dv * 2);
+  l.total = at;
+  return l;
+}
+
+}  // namespace chunk
+}  // namespace tq
+
+extern "C" int32_t tq_mla_chunk_workspace_bytes(const TqMlaChunkSpec* spec, int32_t device,
+                                                uint64_t* bytes) {
+  TqContractError e{nullptr, TQ_OK};
+  const int32_t st = tq::chunk_validate(spec, &e);
+  if (st != TQ_OK) return st;
+  if (!bytes || device < 0) return TQ_ERR_INVALID_ARGUMENT;
+  *bytes = tq::chunk::layout_of(*spec).total;
+  return TQ_OK;
+}
+
+extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
+                                uint64_t workspace_bytes, void* stream, TqContractError* err) {
+  using namespace tq::chunk;
+  auto fail = [&](const char* field, int32_t kind) {
+    if (err) { err->field = field; err->kind = kind; }
+    return kind;
+  };
+  const int32_t st = tq::chunk_validate(spec, err);
+  if (st != TQ_OK) return st;
+  const TqMlaChunkSpec& s = *spec;
+  const uint64_t T = s.q.shape[0], S = s.page_table.shape[0];
+  if (T == 0 || S == 0) return fail(nullptr, TQ_OK);
+  const Layout l = layout_of(s);
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < l.total)
+    return fail("workspace", TQ_ERR_WORKSPACE);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  Args a = {};
+  a.w.header = reinterpret_cast<int*>(ws + l.header);
+  a.w.seq_key0 = reinterpret_cast<int*>(ws + l.seq_key0);
+  a.w.seq_keys = reinterpret_cast<int*>(ws + l.seq_keys);
+  a.w.seq_block = reinterpret_cast<int*>(ws + l.seq_block);
+  a.w.blocks = reinterpret_cast<Block*>(ws + l.blocks);
+  a.w.marked = ws + l.marked;
+  a.w.rows = reinterpret_cast<uint16_t*>(ws + l.rows);
+  a.w.rope = reinterpret_cast<uint16_t*>(ws + l.rope);
+  a.w.k = reinterpret_cast<uint16_t*>(ws + l.k);
+  a.w.v = reinterpret_cast<uint16_t*>(ws + l.v);
+  auto ints = [](const TqTensorSpec& t) { return reinterpret_cast<const int*>(t.device_address); };
+  a.q = reinterpret_cast<const uint8_t*>(s.q.device_address);
+  a.kv = reinterpret_cast<const uint8_t*>(s.kv.device_address);
+  a.w_uk = reinterpret_cast<const uint16_t*>(s.w_uk.device_address);
+  a.w_uv = reinterpret_cast<const uint16_t*>(s.w_uv.device_address);
+  a.page_table = ints(s.page_table);
+  a.q_start = ints(s.q_start);
+  a.q_pos = ints(s.q_pos);
+  a.kv_len = ints(s.kv_len);
+  a.out = reinterpret_cast<uint8_t*>(s.out.device_address);
+  a.lse = s.lse.rank ? reinterpret_cast<float*>(s.lse.device_address) : nullptr;
+  a.q_st = (long long)s.q.strides_bytes[0];
+  a.q_sh = (long long)s.q.strides_bytes[1];
+  a.out_st = (long long)s.out.strides_bytes[0];
+  a.out_sh = (long long)s.out.strides_bytes[1];
+  a.uk_sh = (long long)(s.w_uk.strides_bytes[0] / 2);
+  a.uk_sr = (long long)(s.w_uk.strides_bytes[1] / 2);
+  a.uv_sh = (long long)(s.w_uv.strides_bytes[0] / 2);
+  a.uv_sr = (long long)(s.w_uv.strides_bytes[1] / 2);
+  a.row_stride = (long long)s.kv.strides_bytes[1];
+  a.tokens = int(T);
+  a.heads = int(s.q.shape[1]);
+  a.seqs = int(S);
+  a.slots = int(s.page_table.shape[1]);
+  a.pages = int(s.kv.shape[0]);
+  a.cap = int(l.cap);
+  a.max_blocks = int(l.max_blocks);
+  a.dn = int(s.w_uk.shape[1]);
+  a.dv = int(s.w_uv.shape[1]);
+  a.dr = int(s.q.shape[2]) - a.dn;
+  a.fp8 = s.kv_format == TQ_KV_FP8_E4M3;
+  a.out_f32 = s.out.dtype == TQ_DTYPE_F32;
+  a.scale_log2 = s.softmax_scale * 1.4426950408889634f;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  plan_kernel<<<1, 1024, 0, cs>>>(a);
+  gather_kernel<<<a.cap / kRowTile, 256, 0, cs>>>(a);
+  for (a.head0 = 0; a.head0 < a.heads; a.head0 += int(l.pass_heads)) {
+    a.pass_heads = a.heads - a.head0 < int(l.pass_heads) ? a.heads - a.head0 : int(l.pass_heads);
+    expand_kernel<<<dim3(a.cap / 64, (a.dn + a.dv) / 64, a.pass_heads), 256, 0, cs>>>(a);
+    attend_kernel<<<dim3(a.tokens, a.pass_heads), 128, 0, cs>>>(a);
+  }
+  if (cudaGetLastError() != cudaSuccess) return fail("launch", TQ_ERR_CUDA);
+  return fail(nullptr, TQ_OK);
+}

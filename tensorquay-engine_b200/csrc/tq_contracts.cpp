@@ -506,7 +506,75 @@ int32_t block_norm_validate_impl(const TqBlockNormSpec* spec, TqContractError* e
   return TQ_OK;
 }
 
+// Chunk attention: the attention plan's declarations with per-head widths and expansion weights.
+int32_t chunk_validate_impl(const TqMlaChunkSpec* spec, TqContractError* err) {
+  Failure f{nullptr, TQ_OK};
+  auto fail = [&](const char* field, int32_t kind) {
+    if (err) { err->field = field; err->kind = kind; }
+    return kind;
+  };
+  if (!spec) return fail("spec", TQ_ERR_INVALID_ARGUMENT);
+  const TqMlaChunkSpec& s = *spec;
+  uint64_t payload = 0, dn = 256, dr = 0, dv = 256;
+  switch (s.kv_format) {
+    case TQ_KV_BF16: payload = 1024; break;
+    case TQ_KV_FP8_E4M3: payload = 528; break;
+    case TQ_KV_BF16_ROPE576: payload = 1152; dn = 128; dr = 64; dv = 128; break;
+    default: return fail("kv_format", TQ_SHAPE);
+  }
+  if (s.q.rank != 3) return fail("q", TQ_SHAPE);
+  const uint64_t T = s.q.shape[0], H = s.q.shape[1];
+  if (H < 1 || H > 128 || T > (1u << 24)) return fail("q", TQ_SHAPE);
+  if (!(std::isfinite(s.softmax_scale) && s.softmax_scale > 0.f))
+    return fail("softmax_scale", TQ_SCALE);
+  if (s.page_table.rank != 2) return fail("page_table", TQ_SHAPE);
+  const uint64_t S = s.page_table.shape[0], L = s.page_table.shape[1];
+  if (s.max_keys > (1u << 24) || s.max_keys + 127 * (S < T ? S : T) > (1u << 25))
+    return fail("max_keys", TQ_CAPACITY);
+  const bool launching = T != 0 && S != 0;
+  if (!check_kv_strides(s.kv, payload, &f)) return fail(f.field, f.kind);
+  const uint64_t q[3] = {T, H, dn + dr}, uk[3] = {H, dn, 512}, uv[3] = {H, dv, 512};
+  const uint64_t pool[3] = {s.kv.shape[0], kPageRows, payload}, table[2] = {S, L};
+  const uint64_t tok[1] = {T}, seqs[1] = {S}, starts[1] = {S + 1};
+  const uint64_t o[3] = {T, H, dv}, l[2] = {T, H};
+  if (s.kv.shape[0] >= kDimensionLimit / kPageRows) return fail("kv", TQ_DIMENSION);
+  Extent in[8], out[2];
+  const int32_t bf = TQ_DTYPE_BF16, i32 = TQ_DTYPE_I32;
+  const Layout padded = Layout::PaddedOuter, packed = Layout::Packed;
+  const int32_t out_dtype = s.out.dtype == TQ_DTYPE_F32 ? TQ_DTYPE_F32 : TQ_DTYPE_BF16;
+  if (!check("q", s.q, q, 3, bf, padded, launching, &in[0], &f) ||
+      !check("w_uk", s.w_uk, uk, 3, bf, padded, launching, &in[1], &f) ||
+      !check("w_uv", s.w_uv, uv, 3, bf, padded, launching, &in[2], &f) ||
+      !check("kv", s.kv, pool, 3, TQ_DTYPE_U8, Layout::Checked, launching, &in[3], &f) ||
+      !check("page_table", s.page_table, table, 2, i32, packed, launching, &in[4], &f) ||
+      !check("q_start", s.q_start, starts, 1, i32, packed, launching, &in[5], &f) ||
+      !check("q_pos", s.q_pos, tok, 1, i32, packed, launching, &in[6], &f) ||
+      !check("kv_len", s.kv_len, seqs, 1, i32, packed, launching, &in[7], &f) ||
+      !check("out", s.out, o, 3, out_dtype, padded, launching, &out[0], &f))
+    return fail(f.field, f.kind);
+  out[1].present = false;
+  if (s.lse.rank != 0 &&
+      !check("lse", s.lse, l, 2, TQ_DTYPE_F32, packed, launching, &out[1], &f))
+    return fail(f.field, f.kind);
+  if (launching) {
+    const TqTensorSpec* all[4] = {&s.q, &s.w_uk, &s.w_uv, &s.out};
+    const char* names[4] = {"q", "w_uk", "w_uv", "out"};
+    for (int i = 0; i < 4; ++i) {
+      if (all[i]->device_address % 16) return fail(names[i], TQ_ALIGNMENT);
+      if (all[i]->strides_bytes[0] % 16 || all[i]->strides_bytes[1] % 16)
+        return fail(names[i], TQ_STRIDE);
+    }
+  }
+  if (!check_aliases(in, 8, out, 2, &f)) return fail(f.field, f.kind);
+  if (err) { err->field = nullptr; err->kind = TQ_OK; }
+  return TQ_OK;
+}
+
 }  // namespace
+
+int32_t chunk_validate(const TqMlaChunkSpec* spec, TqContractError* err) {
+  return chunk_validate_impl(spec, err);
+}
 
 int32_t step_plan_validate(const TqStepPlanSpec* spec, TqContractError* err) {
   return step_plan_validate_impl(spec, err);
@@ -605,6 +673,10 @@ int32_t tq_step_plan_validate(const TqStepPlanSpec* spec, TqContractError* err) 
 
 int32_t tq_block_norm_validate(const TqBlockNormSpec* spec, TqContractError* err) {
   return tq::block_norm_validate(spec, err);
+}
+
+int32_t tq_mla_chunk_validate(const TqMlaChunkSpec* spec, TqContractError* err) {
+  return tq::chunk_validate(spec, err);
 }
 
 int32_t tq_mla_should_launch(const TqMlaParams* params) {

@@ -116,6 +116,13 @@ class TqBlockNormSpec(ctypes.Structure):
             (name, ctypes.c_float) for name in ("scale", "post_eps", "pre_eps")]
 
 
+class TqMlaChunkSpec(ctypes.Structure):
+    _fields_ = [(name, TqTensorSpec) for name in (
+        "q", "w_uk", "w_uv", "kv", "page_table", "q_start", "q_pos", "kv_len", "out", "lse")] + [
+            ("kv_format", ctypes.c_int32), ("softmax_scale", ctypes.c_float),
+            ("max_keys", ctypes.c_uint64)]
+
+
 # Every exported symbol of include/tq_mla.h, with its ctypes prototype.
 _P = ctypes.POINTER
 _U64, _I32, _VP = ctypes.c_uint64, ctypes.c_int32, ctypes.c_void_p
@@ -157,6 +164,9 @@ PROTOTYPES = {
     "tq_step_plan": (_I32, [_P(TqStepPlanSpec), _VP, _VP, _P(TqContractError)]),
     "tq_block_norm_validate": (_I32, [_P(TqBlockNormSpec), _P(TqContractError)]),
     "tq_block_norm": (_I32, [_P(TqBlockNormSpec), _VP, _P(TqContractError)]),
+    "tq_mla_chunk_validate": (_I32, [_P(TqMlaChunkSpec), _P(TqContractError)]),
+    "tq_mla_chunk_workspace_bytes": (_I32, [_P(TqMlaChunkSpec), _I32, _P(_U64)]),
+    "tq_mla_chunk": (_I32, [_P(TqMlaChunkSpec), _VP, _U64, _VP, _P(TqContractError)]),
     "tq_philox_block": (None, [_P(ctypes.c_uint32), _P(ctypes.c_uint32), _P(ctypes.c_uint32)]),
     "tq_philox_words": (_I32, [_U64, _U64, _U64, _P(ctypes.c_uint32), _U64]),
     "tq_philox_uniform_f32": (ctypes.c_float, [ctypes.c_uint32]),

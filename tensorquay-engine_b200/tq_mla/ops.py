@@ -425,6 +425,76 @@ def block_norm(y, residual, *, pre_weight=None, out=None, x=None, stream=None, *
     return BlockNorm(y, residual, out, x, pre_weight=pre_weight, **kw)(stream)
 
 
+def chunk_spec(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse=None, *, scale,
+               max_keys, kv_format=None):
+    """Declaration of a chunk attention call (``tq_mla_chunk``)."""
+    if kv_format is None:
+        kv_format = _abi.KV_BF16_ROPE576 if q.shape[-1] == 192 else _abi.KV_BF16
+    s = _abi.TqMlaChunkSpec()
+    for name, t in (("q", q), ("w_uk", w_uk), ("w_uv", w_uv), ("page_table", page_table),
+                    ("q_start", q_start), ("q_pos", q_pos), ("kv_len", kv_len), ("out", out),
+                    ("lse", lse)):
+        if t is not None:
+            setattr(s, name, spec_of(t))
+    s.kv = pool_spec(kv, kv_format)
+    s.kv_format, s.softmax_scale, s.max_keys = kv_format, float(scale), int(max_keys)
+    return s
+
+
+class MlaChunk(_Launch):
+    """Attention of each sequence's chunk of new tokens over its paged latent rows, with per-head
+    keys and values expanded from them: the prefill form for chunks of a few hundred tokens and
+    more (``MlaLaunch(prefill=True)`` is cheaper below, decode for single tokens).
+
+    ``q`` bf16 ``[T, H, Dn + Dr]`` with RoPE applied; ``w_uk [H, Dn, 512]``, ``w_uv [H, Dv, 512]``;
+    rows ``q_start[s]`` to ``q_start[s + 1]`` of ``q`` belong to sequence ``s`` and see its cached
+    rows below ``min(kv_len[s], q_pos + 1)``; ``out`` bf16 or f32 ``[T, H, Dv]``, ``lse`` f32
+    ``[T, H]`` or None. ``max_keys`` bounds the summed ``kv_len`` of the sequences with tokens.
+    Owns only its workspace.
+    """
+
+    def __init__(self, q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse=None, *, scale,
+                 max_keys, kv_format=None, workspace=None):
+        self._bind(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse, workspace)
+        self.spec = chunk_spec(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse,
+                               scale=scale, max_keys=max_keys, kv_format=kv_format)
+        err = _abi.TqContractError()
+        raise_for(lib.tq_mla_chunk_validate(ctypes.byref(self.spec), ctypes.byref(err)), err)
+        need = ctypes.c_uint64()
+        raise_for(lib.tq_mla_chunk_workspace_bytes(ctypes.byref(self.spec), self.device.index,
+                                                   ctypes.byref(need)))
+        if workspace is None:
+            workspace = torch.empty(need.value, dtype=torch.uint8, device=self.device)
+        if workspace.numel() * workspace.element_size() < need.value:
+            raise TqError(102, "workspace")
+        self.workspace, self.out, self.lse = workspace, out, lse
+
+    def __call__(self, stream=None):
+        err = _abi.TqContractError()
+        raise_for(self._run(lambda s: lib.tq_mla_chunk(
+            ctypes.byref(self.spec), ctypes.c_void_p(self.workspace.data_ptr()),
+            self.workspace.numel() * self.workspace.element_size(), s, ctypes.byref(err)), stream), err)
+        return self.out if self.lse is None else (self.out, self.lse)
+
+    def device_error(self, stream=None):
+        flags = ctypes.c_int32()
+        raise_for(self._run(lambda s: lib.tq_mla_read_device_error(
+            ctypes.c_void_p(self.workspace.data_ptr()), s, ctypes.byref(flags)), stream))
+        return flags.value
+
+
+def mla_chunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, *, scale, max_keys, out=None,
+              lse=None, out_dtype=torch.bfloat16, kv_format=None, stream=None):
+    """One chunk attention call (see ``MlaChunk``); returns ``(out, lse)``."""
+    t, h = q.shape[0], q.shape[1]
+    if out is None:
+        out = torch.empty((t, h, w_uv.shape[1]), dtype=out_dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty((t, h), dtype=torch.float32, device=q.device)
+    return MlaChunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse, scale=scale,
+                    max_keys=max_keys, kv_format=kv_format)(stream)
+
+
 def combine_parts(part_out, part_lse, out=None, lse=None, stream=None):
     """Merge ``G`` partial results (``part_out f32 [G,T,H,512]``, ``part_lse f32 [G,T,H]``)."""
     g, t, h, _ = part_out.shape
