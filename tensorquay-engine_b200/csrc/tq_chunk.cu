@@ -15,10 +15,12 @@
 //   4. attend_kernel  attention of every (query block, head).
 // Heads are taken in passes that bound the scratch of step 3 (kScratchBytes).
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <mutex>
 
 #include "tq_contracts.h"
 #include "tq_ptx.cuh"
@@ -267,45 +269,226 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a) {
   }
 }
 
-// ------------------------------------------------------------------------------ expand
-// 64 compact rows x 64 columns of one head's [k | v] per block, 16 x 16 threads of 4 x 4.
-__global__ void __launch_bounds__(256) expand_kernel(const Args a) {
-  const Work& w = a.w;
-  const int r0 = int(blockIdx.x) * 64;
-  if (r0 >= w.header[kHdrRows]) return;
-  const int c0 = int(blockIdx.y) * 64, h = int(blockIdx.z);
-  const bool is_v = c0 >= a.dn;
-  const int c = is_v ? c0 - a.dn : c0;
-  const uint16_t* weight = is_v ? a.w_uv + (a.head0 + h) * a.uv_sh + c * a.uv_sr
-                                : a.w_uk + (a.head0 + h) * a.uk_sh + c * a.uk_sr;
-  const long long wr = is_v ? a.uv_sr : a.uk_sr;
-  __shared__ float xs[32][65], ws[32][65];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < kLatent; k0 += 32) {
-    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-      const int r = i >> 5, k = i & 31;
-      xs[k][r] = __uint_as_float(uint32_t(w.rows[(long long)(r0 + r) * kLatent + k0 + k]) << 16);
-      ws[k][r] = __uint_as_float(uint32_t(weight[r * wr + k0 + k]) << 16);
+// ------------------------------------------------------------------------------ waits
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr uint32_t kWaitPolls = 1u << 26;
+
+// Bounded waits of one role of a CTA pair. The first that runs out sets the error flag and both
+// CTAs' abort words; every later wait of the pair then returns false at once.
+struct Waiter {
+  int* header;
+  volatile uint32_t* abort;  // this CTA's abort word
+  uint32_t peer_abort;       // the other CTA's, in the shared::cluster window
+  bool failed;
+
+  __device__ bool on(uint32_t bar, uint32_t parity) {
+    if (failed) return false;
+    if (ptx::mbar_test_cluster(bar, parity)) return true;
+    const uint64_t t0 = ptx::global_timer_ns();
+    for (uint32_t i = 1;; ++i) {
+      if (ptx::mbar_test_cluster(bar, parity)) return true;
+      if ((i & 63) == 0) {
+        if (*abort) {
+          failed = true;
+          return false;
+        }
+        if (i >= kWaitPolls || ptx::global_timer_ns() - t0 > kWaitNs) {
+          *abort = 1;
+          ptx::st_cluster_u32(peer_abort, 1u);
+          atomicOr(header + kHdrError, TQ_DEV_WAIT_TIMEOUT);
+          failed = true;
+          return false;
+        }
+      }
     }
-    __syncthreads();
-    for (int k = 0; k < 32; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[k][ty * 4 + i], ws[k][tx * 4 + j], acc[i][j]);
-    __syncthreads();
   }
-  const int width = is_v ? a.dv : a.dn;
-  uint16_t* dst = is_v ? w.v : w.k;
+  // For a converged warp: all lanes agree.
+  __device__ bool all(uint32_t bar, uint32_t parity) {
+    const bool ok = on(bar, parity);
+    if (__all_sync(0xFFFFFFFFu, ok)) return true;
+    failed = true;
+    return false;
+  }
+  // After an abort: a millisecond in which the pair's copies and MMAs in flight land.
+  __device__ void settle() {
+    if (!*abort) return;
+    const uint64_t t0 = ptx::global_timer_ns();
+    for (uint32_t i = 0; i < (1u << 20) && ptx::global_timer_ns() - t0 < 1000000ull; ++i) {
+    }
+  }
+};
+
+// ------------------------------------------------------------------------------ expand
+// [k | v] = rows . weights^T on CTA pairs: an item is 256 compact rows by 256 output columns (one
+// head's k and v where both are 128 wide, one head's k or v where they are 256 wide), K = 512.
+//
+// What bounds it: the tensor cores, 2 x 256 x 512 FLOP a row and column block against 1 KB read and
+// 512 B written a row. The weights of a column block (256 x 512, half of them in each CTA of the
+// pair) therefore stay in shared memory while the pair walks over row tiles; only the rows
+// stream (16 KB boxes through a ring), half as many bytes per FLOP as with both operands streamed.
+// Two TMEM accumulators: the epilogue of one item runs under the MMAs of the next.
+namespace expand {
+
+constexpr int kThreads = 256;  // warp 0 loads, warp 1 MMA, warps 4-7 epilogue
+constexpr int kChunks = kLatent / 64;
+constexpr uint32_t kBox = 128 * 128;  // 128 rows x 64 values
+constexpr int kStages = 5;
+constexpr uint32_t kSmW = 0;                              // [kChunks] boxes of weights
+constexpr uint32_t kSmA = kChunks * kBox;                 // [kStages] boxes of rows
+constexpr uint32_t kSmBars = kSmA + kStages * kBox;
+constexpr int kBarAFull = 0, kBarAEmpty = kStages, kBarWFull = 2 * kStages;
+constexpr int kBarWEmpty = kBarWFull + kChunks, kBarAccFull = kBarWEmpty + kChunks;
+constexpr int kBarAccEmpty = kBarAccFull + 2, kBarDrain = kBarAccEmpty + 2, kBars = kBarDrain + 1;
+constexpr uint32_t kSmMisc = kSmBars + 8 * kBars;  // TMEM address, abort word
+constexpr uint32_t kSmBytes = kSmMisc + 16 + 1024;
+static_assert(kSmBytes <= 232448, "shared memory per CTA");
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    expand_kernel(const __grid_constant__ CUtensorMap tm_rows,
+                  const __grid_constant__ CUtensorMap tm_uk,
+                  const __grid_constant__ CUtensorMap tm_uv, const Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_addr(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* sm = smem_raw + (base - raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = int(ptx::cluster_rank());
+  const int pair = int(blockIdx.x) >> 1, pairs = int(gridDim.x) >> 1;
+  auto bar = [&](int i) { return base + kSmBars + 8u * uint32_t(i); };
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sm + kSmMisc);
+  volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(sm + kSmMisc + 4);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBars; ++i) ptx::mbar_init(bar(i), 1);
+    for (int b = 0; b < 2; ++b) ptx::mbar_init(bar(kBarAccEmpty + b), 8);  // 4 warps of each CTA
+    *abort = 0;
+    ptx::fence_mbar_init_cluster();
+    ptx::tma_prefetch_desc(&tm_rows);
+    ptx::tma_prefetch_desc(&tm_uk);
+    ptx::tma_prefetch_desc(&tm_uv);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(ptx::smem_addr(tmem_holder), 512);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::tc_fence_before();
+  ptx::cluster_sync();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  Waiter wt{a.w.header, abort, ptx::map_peer(base + kSmMisc + 4, uint32_t(rank ^ 1)), false};
+
+  // Column blocks (a head, or a head's k or v) by row tiles, one contiguous range per pair.
+  const int per_head = (a.dn + a.dv) / 256;
+  const long long tiles = (a.w.header[kHdrRows] + 255) / 256;
+  const long long items = tiles * per_head * a.pass_heads;
+  const long long first = items * pair / pairs, last = items * (pair + 1) / pairs;
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0, blocks = 0;
+      for (long long i = first; i < last && !wt.failed; ++i) {
+        const int g = int(i / tiles), tile = int(i % tiles);
+        const bool fresh = i == first || tile == 0;
+        const int h = a.head0 + (per_head == 2 ? g >> 1 : g);
+        const bool from_v = per_head == 2 ? (g & 1) != 0 : rank != 0;
+        const int w_row = per_head == 2 ? rank * 128 : 0;
+        for (int c = 0; c < kChunks; ++c) {
+          if (fresh) {
+            if (blocks > 0 && !wt.on(bar(kBarWEmpty + c), (blocks - 1) & 1u)) break;
+            if (rank == 0) ptx::mbar_expect_tx(bar(kBarWFull + c), 2 * kBox);
+            ptx::tma_load_3d_pair(base + kSmW + c * kBox, from_v ? &tm_uv : &tm_uk,
+                                  ptx::map_peer(bar(kBarWFull + c), 0), c * 64, w_row, h);
+          }
+          if (!wt.on(bar(kBarAEmpty + stage), phase ^ 1u)) break;
+          if (rank == 0) ptx::mbar_expect_tx(bar(kBarAFull + stage), 2 * kBox);
+          ptx::tma_load_2d_pair(base + kSmA + stage * kBox, &tm_rows,
+                                ptx::map_peer(bar(kBarAFull + stage), 0), c * 64,
+                                tile * 256 + rank * 128);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (fresh) ++blocks;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0) {
+      constexpr uint32_t idesc = ptx::idesc_bf16(256, 256, 0);
+      uint32_t stage = 0, phase = 0, blocks = 0, n = 0;
+      for (long long i = first; i < last && !wt.failed; ++i, ++n) {
+        const int tile = int(i % tiles);
+        const bool fresh = i == first || tile == 0, done = i + 1 == last || tile == tiles - 1;
+        const uint32_t buf = n & 1u;
+        if (n >= 2 && !wt.all(bar(kBarAccEmpty + buf), ((n >> 1) - 1) & 1u)) break;
+        ptx::tc_fence_after();
+        const uint32_t d = tmem + buf * 256;
+        for (int c = 0; c < kChunks; ++c) {
+          if (fresh && !wt.all(bar(kBarWFull + c), blocks & 1u)) break;
+          if (!wt.all(bar(kBarAFull + stage), phase)) break;
+          ptx::tc_fence_after();
+          const uint64_t ad = ptx::smem_desc(base + kSmA + stage * kBox, 16, 1024, 2);
+          const uint64_t bd = ptx::smem_desc(base + kSmW + c * kBox, 16, 1024, 2);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t* o = reinterpret_cast<uint32_t*>(
-        dst + ((long long)h * a.cap + r0 + ty * 4 + i) * width + c + tx * 4);
-    o[0] = ptx::pack_bf16x2(acc[i][0], acc[i][1]);
-    o[1] = ptx::pack_bf16x2(acc[i][2], acc[i][3]);
+          for (int k = 0; k < 4; ++k)
+            ptx::mma_ss_pair(d, ad + uint64_t(2 * k), bd + uint64_t(2 * k), idesc,
+                             (c > 0 || k > 0) ? 1u : 0u);
+          ptx::mma_commit_pair(bar(kBarAEmpty + stage));
+          if (done) ptx::mma_commit_pair(bar(kBarWEmpty + c));
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        ptx::mma_commit_pair(bar(kBarAccFull + buf));
+        if (fresh) ++blocks;
+      }
+      ptx::mma_commit_pair(bar(kBarDrain));
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    const int quad = warp & 3, row = quad * 32 + lane;
+    uint32_t n = 0;
+    for (long long i = first; i < last; ++i, ++n) {
+      const int g = int(i / tiles), tile = int(i % tiles);
+      const uint32_t buf = n & 1u;
+      if (!wt.all(bar(kBarAccFull + buf), (n >> 1) & 1u)) break;
+      ptx::tc_fence_after();
+      const long long r = (long long)tile * 256 + rank * 128 + row;
+      const int h = per_head == 2 ? g >> 1 : g;  // of this pass
+      uint16_t* kd = a.w.k + ((long long)h * a.cap + r) * a.dn;
+      uint16_t* vd = a.w.v + ((long long)h * a.cap + r) * a.dv;
+      uint16_t* lo = per_head == 2 ? ((g & 1) ? vd : kd) : kd;
+      uint16_t* hi = per_head == 2 ? lo + 128 : vd;
+      const uint32_t src = tmem + buf * 256 + (uint32_t(quad * 32) << 16);
+#pragma unroll
+      for (int c = 0; c < 256; c += 32) {
+        uint32_t x[32], y[16];
+        ptx::tmem_ld32(src + c, x);
+        ptx::tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          y[j] = ptx::pack_bf16x2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+        uint16_t* dst = c < 128 ? lo + c : hi + (c - 128);
+        ptx::st_global_v8(dst, y);
+        ptx::st_global_v8(dst + 16, y + 8);
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_peer(bar(kBarAccEmpty + buf), 0));
+    }
+  }
+  // Every commit of the leader has arrived in both CTAs before either leaves.
+  wt.on(bar(kBarDrain), 0);
+  wt.settle();
+  ptx::tc_fence_before();
+  ptx::cluster_sync();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc_pair(tmem, 512);
   }
 }
+
+}  // namespace expand
 
 // ------------------------------------------------------------------------------ attend
 // One block per (query token, head): 128 threads, one key each per step, then one or two value
@@ -425,6 +608,55 @@ Layout layout_of(const TqMlaChunkSpec& s) {
   return l;
 }
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// bf16 boxes of 64 values by `box` rows (and one of the third axis) with 128-byte swizzle.
+bool encode(CUtensorMap* map, const void* addr, uint64_t width, uint64_t rows, uint64_t planes,
+            uint64_t row_bytes, uint64_t plane_bytes, uint32_t box, uint32_t box_planes = 1) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {width, rows, planes};
+  const cuuint64_t strides[2] = {row_bytes, plane_bytes};
+  const cuuint32_t boxes[3] = {64, box, box_planes};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, planes ? 3 : 2, const_cast<void*>(addr), dims,
+            strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Per device: CTA pairs (two SMs each), and the kernels' shared memory granted. 0 on failure.
+int pairs_on(int device) {
+  static std::mutex mu;
+  static int cached[128] = {0};
+  if (device < 0 || device >= 128) return 0;
+  std::lock_guard<std::mutex> lock(mu);
+  if (cached[device]) return cached[device];
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
+      cudaFuncSetAttribute(expand::expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           int(expand::kSmBytes)) != cudaSuccess)
+    return 0;
+  cached[device] = sms / 2;
+  return cached[device];
+}
+
 }  // namespace chunk
 }  // namespace tq
 
@@ -498,12 +730,24 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
   a.fp8 = s.kv_format == TQ_KV_FP8_E4M3;
   a.out_f32 = s.out.dtype == TQ_DTYPE_F32;
   a.scale_log2 = s.softmax_scale * 1.4426950408889634f;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return fail("device", TQ_ERR_CUDA);
+  const int pairs = pairs_on(device);
+  if (pairs <= 0) return fail("device", TQ_ERR_CUDA);
+  CUtensorMap tm_rows, tm_uk, tm_uv;
+  if (!encode(&tm_rows, a.w.rows, kLatent, l.cap, 0, kLatent * 2, 0, 128) ||
+      !encode(&tm_uk, a.w_uk, kLatent, uint64_t(a.dn), s.w_uk.shape[0], s.w_uk.strides_bytes[1],
+              s.w_uk.strides_bytes[0], 128) ||
+      !encode(&tm_uv, a.w_uv, kLatent, uint64_t(a.dv), s.w_uv.shape[0], s.w_uv.strides_bytes[1],
+              s.w_uv.strides_bytes[0], 128))
+    return fail("tensor_map", TQ_ERR_CUDA);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   plan_kernel<<<1, 1024, 0, cs>>>(a);
   gather_kernel<<<a.cap / kRowTile, 256, 0, cs>>>(a);
   for (a.head0 = 0; a.head0 < a.heads; a.head0 += int(l.pass_heads)) {
     a.pass_heads = a.heads - a.head0 < int(l.pass_heads) ? a.heads - a.head0 : int(l.pass_heads);
-    expand_kernel<<<dim3(a.cap / 64, (a.dn + a.dv) / 64, a.pass_heads), 256, 0, cs>>>(a);
+    expand::expand_kernel<<<2 * pairs, expand::kThreads, expand::kSmBytes, cs>>>(tm_rows, tm_uk,
+                                                                                 tm_uv, a);
     attend_kernel<<<dim3(a.tokens, a.pass_heads), 128, 0, cs>>>(a);
   }
   if (cudaGetLastError() != cudaSuccess) return fail("launch", TQ_ERR_CUDA);

@@ -1,8 +1,11 @@
 """GPU: chunk attention against its float64 oracle.
 
-Tolerances. With h = 2^-8, bf16's largest relative rounding error, an expanded key is off by at most
-h of itself (2h + h^2 for FP8 rows, whose latent values are rounded to bf16 first; that rounding
-enters a key through sum_r |latent_r w_r|), so a score is off by at most
+Tolerances. With h = 2^-8, bf16's largest relative rounding error, an expanded key or value is off by
+at most h of itself, after a sum of 512 products in f32: each of the 512 additions rounds by at most
+2^-24 of a partial sum, and no partial sum exceeds sum_r |latent_r w_r|, so that sum is off by at most
+512 * 2^-24 = 2^-15 of sum_r |latent_r w_r| (it matters where the sum cancels, in a row that sees one
+key). FP8 rows' latent values are rounded to bf16 first, which adds h of the same sum. A score is off
+by at most
 d = scale * sum |q| |key error|, a softmax weight by a factor within exp(+-2d), and it is rounded
 once more, as is the value. The output is then off by at most
   sum_n p_n |value error|  +  (exp(2d) - 1 + h)(1 + h) sum_n p_n |v_n|  +  half a step of its type,
@@ -122,8 +125,9 @@ class Case:
             hidden = pos[None] >= np.minimum(n, self.q_pos[b:e, None] + 1)
             for h in range(self.heads):
                 k, v = lat @ uk[h].T, lat @ uv[h].T
-                k_off = H * np.abs(k) + (1 + H) * latent_off * (np.abs(lat) @ np.abs(uk[h]).T)
-                v_off = H * np.abs(v) + (1 + H) * latent_off * (np.abs(lat) @ np.abs(uv[h]).T)
+                before = (1 + H) * (latent_off + 2.0 ** -15)
+                k_off = H * np.abs(k) + before * (np.abs(lat) @ np.abs(uk[h]).T)
+                v_off = H * np.abs(v) + before * (np.abs(lat) @ np.abs(uv[h]).T)
                 full = np.concatenate([k, kv[:, 512:]], axis=1)
                 score = self.scale * (signed[b:e, h] @ full.T)
                 f32 = 2.0 ** -16 * self.scale * (q[b:e, h] @ np.abs(full).T)
