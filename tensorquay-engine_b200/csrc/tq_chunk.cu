@@ -491,81 +491,374 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }  // namespace expand
 
 // ------------------------------------------------------------------------------ attend
-// One block per (query token, head): 128 threads, one key each per step, then one or two value
-// columns each.
-__global__ void __launch_bounds__(128) attend_kernel(const Args a) {
+// Attention of one unit (a block of kQueryTile query tokens, one head) on a CTA pair, row tiles of
+// kRowTile keys one after the other with the running maximum and sum of a softmax:
+//   S_j = Q K_j^T (M = 256 over the pair, N = 128)  ->  P_j = exp2(c S_j - c m)  ->  O += P_j V_j
+// Each CTA holds its 128 query rows of S, P and O in TMEM and Q in shared memory; of B operands
+// it loads half: 64 of a tile's keys for QK^T, half the value columns for PV. So a pair moves
+// K_j and V_j once for 256 queries, and the shared memory left holds several tiles ahead.
+//   warp 0      TMA loads of this CTA's halves; their bytes complete on the leader's barriers
+//   warp 1      (leader) all MMAs. S_j has kS buffers in TMEM: S_{j+kS} is issued right after
+//               PV_j, whose P_j lies in the same columns; MMAs run in issue order
+//               (a softmax warp may be up to kS tiles ahead of PV, so the completion of PV_j has a
+//               barrier per buffer: S_j, which a waiter has seen, lies behind PV_{j-kS})
+//   warps 4-11  softmax: a row's 128 scores are split between two threads (warps 4-7 the first 64
+//               keys, 8-11 the rest), which exchange their maxima through shared memory. P goes to
+//               TMEM as bf16 over the scores. The maximum that p is taken against moves only when
+//               it would grow by more than 2^8 (kSlack): then O and the sum are rescaled, after
+//               the last PV; otherwise p stays below 2^8 and the final division makes it exact.
+//
+// What bounds it: per 128 x 128 tile and CTA the tensor cores need (2 (Dqk + Dv) 128 128) / 8192
+// cycles (1280 at 192 + 128, 2048 at 256 + 256), the exponentials 128 128 / 16 = 1024.
+namespace attend {
+
+constexpr int kThreads = 384;
+constexpr float kSlack = 8.f;  // log2 units
+
+template <int kDq, int kDv>
+struct Shape {
+  static constexpr int kQChunks = kDq / 64;
+  static constexpr int kVChunks = kDv / 128;              // of this CTA's half
+  static constexpr int kS = (512 - kDv) / 128 < 3 ? (512 - kDv) / 128 : 3;  // score buffers
+  static constexpr int kKv = kDv == 128 ? 4 : 2;          // K and V stages each
+  static constexpr uint32_t kQBytes = kQChunks * 128 * 128;
+  static constexpr uint32_t kKBytes = kQChunks * 64 * 128;
+  static constexpr uint32_t kVBytes = kVChunks * 128 * 128;
+  static constexpr uint32_t kSmK = kQBytes;
+  static constexpr uint32_t kSmV = kSmK + kKv * kKBytes;
+  static constexpr uint32_t kSmExch = kSmV + kKv * kVBytes;  // f32 [2][2][128]
+  static constexpr uint32_t kSmBars = kSmExch + 2048;
+  static constexpr int kQFull = 0, kQEmpty = 1, kKFull = 2, kKEmpty = kKFull + kKv;
+  static constexpr int kVFull = kKEmpty + kKv, kVEmpty = kVFull + kKv;
+  static constexpr int kSFull = kVEmpty + kKv, kPFull = kSFull + kS;
+  static constexpr int kPvDone = kPFull + kS, kOFree = kPvDone + kS, kDrain = kOFree + 1;
+  static constexpr int kBars = kDrain + 1;
+  static constexpr uint32_t kSmMisc = kSmBars + 8 * kBars;
+  static constexpr uint32_t kSmBytes = kSmMisc + 16 + 1024;
+  static constexpr uint32_t kTmemO = kS * 128;
+  static_assert(kSmBytes <= 232448, "shared memory per CTA");
+  static_assert(kTmemO + kDv <= 512, "TMEM columns");
+};
+
+struct Unit {
+  Block blk;
+  int head;  // of this pass
+  int seq;
+};
+
+// Units in order: sequence, head, query block from the last (which sees the most) to the first, so
+// that the pairs at work at one time share the keys and values of few heads in L2.
+__device__ __forceinline__ Unit unit_at(const Args& a, int u) {
   const Work& w = a.w;
-  const int t = int(blockIdx.x), h = int(blockIdx.y), tid = int(threadIdx.x);
-  if (!w.header[kHdrBlocks]) return;
-  // The token's sequence: the last block that starts at or before it, if it covers it.
-  int b = 0, e = w.header[kHdrBlocks];
-  while (e - b > 1) {
-    const int m = (b + e) >> 1;
-    if (w.blocks[m].row0 <= t) b = m; else e = m;
-  }
-  const Block blk = w.blocks[b];
-  if (t < blk.row0 || t >= blk.row0 + blk.rows) return;
+  const int b = u / a.pass_heads;
   const int s = last_at_or_below(w.seq_block, a.seqs, b);
-  const int pos = a.q_pos[t], keys = w.seq_keys[s];
-  const int n = pos >= keys ? keys : max(pos + 1, 0);
-  __shared__ float qs[256], ps[128], red[8];
-  const int dq = a.dn + a.dr;
-  const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q + t * a.q_st + (a.head0 + h) * a.q_sh);
-  for (int i = tid; i < dq; i += 128) qs[i] = __uint_as_float(uint32_t(q[i]) << 16);
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int k0 = 0; k0 < n; k0 += 128) {
-    const long long r = blk.key0 + k0 + tid;
-    float x = -INFINITY;
-    if (k0 + tid < n) {
-      const uint16_t* k = w.k + ((long long)h * a.cap + r) * a.dn;
-      float d = 0.f;
-      for (int i = 0; i < a.dn; ++i) d = fmaf(qs[i], __uint_as_float(uint32_t(k[i]) << 16), d);
-      for (int i = 0; i < a.dr; ++i)
-        d = fmaf(qs[a.dn + i], __uint_as_float(uint32_t(w.rope[r * kRopeDim + i]) << 16), d);
-      x = w.marked[r] ? NAN : d * a.scale_log2;
-    }
-    float mx = x;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-    if ((tid & 31) == 0) red[tid >> 5] = mx;
-    __syncthreads();
-    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float m1 = fmaxf(m, mx), use = m1 == -INFINITY ? 0.f : m1;
-    const float keep = exp2f(m - use);
-    const float p = exp2f(x - use);
-    ps[tid] = p;
-    float sum = p;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    if ((tid & 31) == 0) red[4 + (tid >> 5)] = sum;
-    __syncthreads();
-    l = l * keep + red[4] + red[5] + red[6] + red[7];
-    o0 *= keep;
-    o1 *= keep;
-    const uint16_t* v = w.v + ((long long)h * a.cap + blk.key0 + k0) * a.dv;
-    const int lim = min(128, n - k0);
-    for (int j = 0; j < lim; ++j) {
-      o0 = fmaf(ps[j], __uint_as_float(uint32_t(v[(long long)j * a.dv + tid]) << 16), o0);
-      if (a.dv > 128)
-        o1 = fmaf(ps[j], __uint_as_float(uint32_t(v[(long long)j * a.dv + 128 + tid]) << 16), o1);
-    }
-    m = m1;
-    __syncthreads();
-  }
-  const float inv = n > 0 ? 1.f / l : 0.f;
-  uint8_t* out = a.out + t * a.out_st + (a.head0 + h) * a.out_sh;
-  for (int c = 0; c < a.dv / 128; ++c) {
-    const float o = (c ? o1 : o0) * inv;
-    if (a.out_f32)
-      reinterpret_cast<float*>(out)[c * 128 + tid] = o;
-    else
-      reinterpret_cast<__nv_bfloat16*>(out)[c * 128 + tid] = __float2bfloat16(o);
-  }
-  if (a.lse && tid == 0)
-    a.lse[(long long)t * a.heads + a.head0 + h] =
-        n > 0 ? 0.69314718055994531f * (m + log2f(l)) : -INFINITY;
+  const int b0 = w.seq_block[s], n = w.seq_block[s + 1] - b0;
+  const int r = u - b0 * a.pass_heads;
+  Unit x;
+  x.head = r / n;
+  x.blk = w.blocks[b0 + n - 1 - r % n];
+  x.seq = s;
+  return x;
 }
+
+template <int kDq, int kDv>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    attend_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_rope,
+                  const __grid_constant__ CUtensorMap tm_v, const Args a) {
+  using C = Shape<kDq, kDv>;
+  constexpr bool kRope = kDq == 192;
+  constexpr int kNopeChunks = kRope ? 2 : C::kQChunks;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_addr(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* sm = smem_raw + (base - raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = int(ptx::cluster_rank());
+  const int pair = int(blockIdx.x) >> 1, pairs = int(gridDim.x) >> 1;
+  auto bar = [&](int i) { return base + C::kSmBars + 8u * uint32_t(i); };
+  auto lead = [&](int i) { return ptx::map_peer(bar(i), 0); };
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sm + C::kSmMisc);
+  volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(sm + C::kSmMisc + 4);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kBars; ++i) {
+      // P of a tile and the release of O: one arrival per softmax warp of either CTA.
+      const bool joint = (i >= C::kPFull && i < C::kPFull + C::kS) || i == C::kOFree;
+      ptx::mbar_init(bar(i), joint ? 16 : 1);
+    }
+    *abort = 0;
+    ptx::fence_mbar_init_cluster();
+    ptx::tma_prefetch_desc(&tm_q);
+    ptx::tma_prefetch_desc(&tm_k);
+    ptx::tma_prefetch_desc(&tm_v);
+    if (kRope) ptx::tma_prefetch_desc(&tm_rope);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(ptx::smem_addr(tmem_holder), 512);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::tc_fence_before();
+  ptx::cluster_sync();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  Waiter wt{a.w.header, abort, ptx::map_peer(base + C::kSmMisc + 4, uint32_t(rank ^ 1)), false};
+  const int units = a.w.header[kHdrBlocks] * a.pass_heads;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0, useq = 0;
+      for (int u = pair; u < units && !wt.failed; u += pairs) {
+        const Unit x = unit_at(a, u);
+        if (!x.blk.tiles) continue;
+        if (!wt.on(bar(C::kQEmpty), (useq & 1u) ^ 1u)) break;
+        if (rank == 0) ptx::mbar_expect_tx(bar(C::kQFull), 2 * C::kQBytes);
+#pragma unroll
+        for (int c = 0; c < C::kQChunks; ++c)
+          ptx::tma_load_3d_pair(base + c * 16384, &tm_q, lead(C::kQFull), c * 64, a.head0 + x.head,
+                                x.blk.row0 + rank * 128);
+        ++useq;
+        for (int j = 0; j < x.blk.tiles; ++j, ++it) {
+          const uint32_t st = it % C::kKv, ph = ((it / C::kKv) & 1u) ^ 1u;
+          const int key = x.blk.key0 + j * kRowTile;
+          if (!wt.on(bar(C::kKEmpty + st), ph)) break;
+          if (rank == 0) ptx::mbar_expect_tx(bar(C::kKFull + st), 2 * C::kKBytes);
+          const uint32_t kd = base + C::kSmK + st * C::kKBytes;
+#pragma unroll
+          for (int c = 0; c < kNopeChunks; ++c)
+            ptx::tma_load_3d_pair(kd + c * 8192, &tm_k, lead(C::kKFull + st), c * 64,
+                                  key + rank * 64, x.head);
+          if (kRope)
+            ptx::tma_load_2d_pair(kd + 2 * 8192, &tm_rope, lead(C::kKFull + st), 0,
+                                  key + rank * 64);
+          if (!wt.on(bar(C::kVEmpty + st), ph)) break;
+          if (rank == 0) ptx::mbar_expect_tx(bar(C::kVFull + st), 2 * C::kVBytes);
+          const uint32_t vd = base + C::kSmV + st * C::kVBytes;
+#pragma unroll
+          for (int c = 0; c < C::kVChunks; ++c)
+            ptx::tma_load_3d_pair(vd + c * 16384, &tm_v, lead(C::kVFull + st),
+                                  rank * (kDv / 2) + c * 64, key, x.head);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0) {
+      constexpr uint32_t idesc_qk = ptx::idesc_bf16(256, 128, 0);
+      constexpr uint32_t idesc_pv = ptx::idesc_bf16(256, kDv, 1);
+      uint32_t it0 = 0, useq = 0;  // tiles of earlier units, units with tiles
+      auto issue_qk = [&](uint32_t it) -> bool {
+        const uint32_t st = it % C::kKv;
+        if (!wt.all(bar(C::kKFull + st), (it / C::kKv) & 1u)) return false;
+        ptx::tc_fence_after();
+        const uint64_t qd = ptx::smem_desc(base, 16, 1024, 2);
+        const uint64_t kd = ptx::smem_desc(base + C::kSmK + st * C::kKBytes, 16, 1024, 2);
+        const uint32_t d = tmem + (it % C::kS) * 128;
+#pragma unroll
+        for (int k = 0; k < kDq / 16; ++k)
+          ptx::mma_ss_pair(d, qd + uint64_t(((k >> 2) * 16384 + (k & 3) * 32) >> 4),
+                           kd + uint64_t(((k >> 2) * 8192 + (k & 3) * 32) >> 4), idesc_qk,
+                           k > 0 ? 1u : 0u);
+        ptx::mma_commit_pair(bar(C::kSFull + it % C::kS));
+        ptx::mma_commit_pair(bar(C::kKEmpty + st));
+        return true;
+      };
+      for (int u = pair; u < units && !wt.failed; u += pairs) {
+        const Unit x = unit_at(a, u);
+        const int tiles = x.blk.tiles;
+        if (!tiles) continue;
+        if (!wt.all(bar(C::kQFull), useq & 1u)) break;
+        ptx::tc_fence_after();
+        for (int j = 0; j < C::kS && j < tiles; ++j)
+          if (!issue_qk(it0 + j)) break;
+        if (tiles <= C::kS) ptx::mma_commit_pair(bar(C::kQEmpty));
+        for (int j = 0; j < tiles && !wt.failed; ++j) {
+          const uint32_t it = it0 + j, sb = it % C::kS, st = it % C::kKv;
+          // The unit before must have read its output before this one's first PV replaces it.
+          if (j == 0 && useq > 0 && !wt.all(bar(C::kOFree), (useq - 1) & 1u)) break;
+          if (!wt.all(bar(C::kVFull + st), (it / C::kKv) & 1u)) break;
+          if (!wt.all(bar(C::kPFull + sb), (it / C::kS) & 1u)) break;
+          ptx::tc_fence_after();
+          // V as B, MN-major: 64 value columns are a chunk of [128 keys][128 B], 8-key groups 1 KB
+          // apart; a step of 16 keys is 2 KB.
+          const uint64_t vd = ptx::smem_desc(base + C::kSmV + st * C::kVBytes, 16384, 1024, 2);
+#pragma unroll
+          for (int k = 0; k < kRowTile / 16; ++k)
+            ptx::mma_ts_pair(tmem + C::kTmemO, tmem + sb * 128 + k * 8, vd + uint64_t(k * 128),
+                             idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
+          ptx::mma_commit_pair(bar(C::kVEmpty + st));
+          ptx::mma_commit_pair(bar(C::kPvDone + sb));
+          if (j + C::kS < tiles) {
+            if (!issue_qk(it + C::kS)) break;
+            if (j + C::kS + 1 == tiles) ptx::mma_commit_pair(bar(C::kQEmpty));
+          }
+        }
+        it0 += uint32_t(tiles);
+        ++useq;
+      }
+      ptx::mma_commit_pair(bar(C::kDrain));
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    const int half = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t lanes = uint32_t(quad * 32) << 16;
+    float* exch = reinterpret_cast<float*>(sm + C::kSmExch);
+    const bool marked = a.w.header[kHdrMarked] != 0;
+    const float c = a.scale_log2, slack = kSlack / c;
+    uint32_t it = 0;
+    // A wait that ran out is not left for: the two warps of a row go through the same barriers to
+    // the end, over whatever TMEM holds; the error flag is set.
+    for (int u = pair; u < units; u += pairs) {
+      const Unit x = unit_at(a, u);
+      const int t = x.blk.row0 + rank * 128 + row;
+      const bool mine = rank * 128 + row < x.blk.rows;
+      int n = 0;  // keys that this row sees
+      if (mine) {
+        const int keys = a.w.seq_keys[x.seq], pos = a.q_pos[t];
+        n = pos >= keys ? keys : max(pos + 1, 0);
+      }
+      float m = -INFINITY, sum = 0.f;
+      for (int j = 0; j < x.blk.tiles; ++j, ++it) {
+        const uint32_t sb = it % C::kS;
+        wt.all(bar(C::kSFull + sb), (it / C::kS) & 1u);
+        ptx::tc_fence_after();
+        uint32_t r[2][32];
+        const uint32_t src = tmem + sb * 128 + half * 64 + lanes;
+        ptx::tmem_ld32(src, r[0]);
+        ptx::tmem_ld32(src + 32, r[1]);
+        ptx::tmem_wait_ld();
+        float(&s0)[32] = reinterpret_cast<float(&)[32]>(r[0]);
+        float(&s1)[32] = reinterpret_cast<float(&)[32]>(r[1]);
+        const int key = j * kRowTile + half * 64;
+        if (!__all_sync(0xFFFFFFFFu, n >= key + 64)) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (key + i >= n) s0[i] = -INFINITY;
+            if (key + 32 + i >= n) s1[i] = -INFINITY;
+          }
+        }
+        if (marked) {
+          const uint8_t* mk = a.w.marked + x.blk.key0 + key;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (mk[i] && key + i < n) s0[i] = NAN;
+            if (mk[32 + i] && key + 32 + i < n) s1[i] = NAN;
+          }
+        }
+        float top = s0[0];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) top = fmaxf(top, s0[i]);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = fmaxf(top, s1[i]);
+        float* ex = exch + (it & 1u) * 256;
+        ex[half * 128 + row] = top;
+        ptx::named_barrier(1 + quad, 64);
+        top = fmaxf(top, ex[(half ^ 1) * 128 + row]);
+        if (j == 0) {
+          m = top;
+        } else {
+          const bool grow = top > m + slack;
+          if (__any_sync(0xFFFFFFFFu, grow)) {
+            const float keep = !grow ? 1.f : m == -INFINITY ? 0.f : ptx::ex2((m - top) * c);
+            if (grow) m = top;
+            sum *= keep;
+            wt.all(bar(C::kPvDone + (it - 1) % C::kS), ((it - 1) / C::kS) & 1u);
+            ptx::tc_fence_after();
+            const uint32_t o = tmem + C::kTmemO + half * (kDv / 2) + lanes;
+            for (int i = 0; i < kDv / 2; i += 32) {
+              uint32_t v[32];
+              ptx::tmem_ld32(o + i, v);
+              ptx::tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * keep);
+              ptx::tmem_st32(o + i, v);
+            }
+          }
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c;
+        uint32_t p[32];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float p0 = ptx::ex2(fmaf(s0[i], c, -mc)), p1 = ptx::ex2(fmaf(s0[i + 1], c, -mc));
+          sum += p0 + p1;
+          p[i / 2] = ptx::pack_bf16x2(p0, p1);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float p0 = ptx::ex2(fmaf(s1[i], c, -mc)), p1 = ptx::ex2(fmaf(s1[i + 1], c, -mc));
+          sum += p0 + p1;
+          p[16 + i / 2] = ptx::pack_bf16x2(p0, p1);
+        }
+        ptx::tmem_st32(tmem + sb * 128 + half * 32 + lanes, p);
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(lead(C::kPFull + sb));
+      }
+      // The row's whole sum, then O / sum to the output: this thread's half of the columns.
+      float* ex = exch + (it & 1u) * 256;
+      ex[half * 128 + row] = sum;
+      ptx::named_barrier(1 + quad, 64);
+      sum += ex[(half ^ 1) * 128 + row];
+      // Both have read before either writes its next maximum there (two tiles on at the earliest,
+      // or at once when the next unit has no tiles).
+      ptx::named_barrier(1 + quad, 64);
+      const float inv = n > 0 ? 1.f / sum : 0.f;
+      if (x.blk.tiles) {
+        wt.all(bar(C::kPvDone + (it - 1) % C::kS), ((it - 1) / C::kS) & 1u);
+        ptx::tc_fence_after();
+      }
+      const int head = a.head0 + x.head;
+      uint8_t* out = a.out + (long long)t * a.out_st + (long long)head * a.out_sh;
+      const uint32_t o = tmem + C::kTmemO + half * (kDv / 2) + lanes;
+#pragma unroll
+      for (int i = 0; i < kDv / 2; i += 32) {
+        uint32_t v[32];
+        if (x.blk.tiles) {
+          ptx::tmem_ld32(o + i, v);
+          ptx::tmem_wait_ld();
+        }
+        if (mine) {
+          const int col = half * (kDv / 2) + i;
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            v[k] = n > 0 ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
+          if (a.out_f32) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<uint4*>(out + 4 * (col + k)) =
+                  make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8)
+              *reinterpret_cast<uint4*>(out + 2 * (col + k)) = make_uint4(
+                  ptx::pack_bf16x2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])),
+                  ptx::pack_bf16x2(__uint_as_float(v[k + 2]), __uint_as_float(v[k + 3])),
+                  ptx::pack_bf16x2(__uint_as_float(v[k + 4]), __uint_as_float(v[k + 5])),
+                  ptx::pack_bf16x2(__uint_as_float(v[k + 6]), __uint_as_float(v[k + 7])));
+          }
+        }
+      }
+      if (x.blk.tiles) {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(lead(C::kOFree));
+      }
+      if (a.lse && mine && half == 0)
+        a.lse[(long long)t * a.heads + head] =
+            n > 0 ? 0.69314718055994531f * (m * c + log2f(sum)) : -INFINITY;
+    }
+  }
+  wt.on(bar(C::kDrain), 0);
+  wt.settle();
+  ptx::tc_fence_before();
+  ptx::cluster_sync();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+}  // namespace attend
 
 // ------------------------------------------------------------------------------ host
 struct Layout {
@@ -651,7 +944,13 @@ int pairs_on(int device) {
   int sms = 0;
   if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
       cudaFuncSetAttribute(expand::expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           int(expand::kSmBytes)) != cudaSuccess)
+                           int(expand::kSmBytes)) != cudaSuccess ||
+      cudaFuncSetAttribute(attend::attend_kernel<192, 128>,
+                           cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           int(attend::Shape<192, 128>::kSmBytes)) != cudaSuccess ||
+      cudaFuncSetAttribute(attend::attend_kernel<256, 256>,
+                           cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           int(attend::Shape<256, 256>::kSmBytes)) != cudaSuccess)
     return 0;
   cached[device] = sms / 2;
   return cached[device];
@@ -734,8 +1033,16 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
   if (cudaGetDevice(&device) != cudaSuccess) return fail("device", TQ_ERR_CUDA);
   const int pairs = pairs_on(device);
   if (pairs <= 0) return fail("device", TQ_ERR_CUDA);
-  CUtensorMap tm_rows, tm_uk, tm_uv;
-  if (!encode(&tm_rows, a.w.rows, kLatent, l.cap, 0, kLatent * 2, 0, 128) ||
+  CUtensorMap tm_rows, tm_uk, tm_uv, tm_q, tm_k, tm_rope, tm_v;
+  // q: 64 values by one head by 128 tokens, tokens past T as zeros.
+  if (!encode(&tm_q, a.q, uint64_t(a.dn + a.dr), s.q.shape[1], T, s.q.strides_bytes[1],
+              s.q.strides_bytes[0], 1, 128) ||
+      !encode(&tm_k, a.w.k, uint64_t(a.dn), l.cap, l.pass_heads, uint64_t(a.dn) * 2,
+              l.cap * uint64_t(a.dn) * 2, 64) ||
+      !encode(&tm_v, a.w.v, uint64_t(a.dv), l.cap, l.pass_heads, uint64_t(a.dv) * 2,
+              l.cap * uint64_t(a.dv) * 2, 128) ||
+      !encode(&tm_rope, a.w.rope, kRopeDim, l.cap, 0, kRopeDim * 2, 0, 64) ||
+      !encode(&tm_rows, a.w.rows, kLatent, l.cap, 0, kLatent * 2, 0, 128) ||
       !encode(&tm_uk, a.w_uk, kLatent, uint64_t(a.dn), s.w_uk.shape[0], s.w_uk.strides_bytes[1],
               s.w_uk.strides_bytes[0], 128) ||
       !encode(&tm_uv, a.w_uv, kLatent, uint64_t(a.dv), s.w_uv.shape[0], s.w_uv.strides_bytes[1],
@@ -748,7 +1055,14 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
     a.pass_heads = a.heads - a.head0 < int(l.pass_heads) ? a.heads - a.head0 : int(l.pass_heads);
     expand::expand_kernel<<<2 * pairs, expand::kThreads, expand::kSmBytes, cs>>>(tm_rows, tm_uk,
                                                                                  tm_uv, a);
-    attend_kernel<<<dim3(a.tokens, a.pass_heads), 128, 0, cs>>>(a);
+    if (a.dr)
+      attend::attend_kernel<192, 128>
+          <<<2 * pairs, attend::kThreads, attend::Shape<192, 128>::kSmBytes, cs>>>(tm_q, tm_k,
+                                                                                   tm_rope, tm_v, a);
+    else
+      attend::attend_kernel<256, 256>
+          <<<2 * pairs, attend::kThreads, attend::Shape<256, 256>::kSmBytes, cs>>>(tm_q, tm_k,
+                                                                                   tm_rope, tm_v, a);
   }
   if (cudaGetLastError() != cudaSuccess) return fail("launch", TQ_ERR_CUDA);
   return fail(nullptr, TQ_OK);
