@@ -12,13 +12,16 @@
 //                     row that is not finite, so that neither stale rows nor such a row can reach
 //                     an output that does not see it through 0 * NaN.
 //   3. expand_kernel  k and v of every head from the compact rows.
-//   4. attend_kernel  attention of every (query block, head).
+//   4. attend_kernel  attention of every (query block, head); where those are few, each is split
+//                     into pieces of its row tiles, and
+//   5. join_kernel    merges the pieces by their log sums.
 // Heads are taken in passes that bound the scratch of step 3 (kScratchBytes).
 
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <climits>
 #include <cstdint>
 #include <mutex>
 
@@ -34,19 +37,35 @@ constexpr int kRopeDim = 64;
 constexpr int kRowTile = 128;    // keys per attention step; sequences are padded to it
 constexpr int kQueryTile = 256;  // query tokens of one attention unit
 constexpr uint64_t kScratchBytes = 8ull << 30;
+// Splitting: at most this many units once split, about four per CTA pair (their partial outputs are
+// kept in the workspace), and what a piece costs beside its tiles (query load, pipeline fill,
+// output), in tiles.
+constexpr int kSplitUnits = 320;
+constexpr int kPieceCost = 4;
 
 enum Header : int {
   kHdrError = 0,
   kHdrRows = 1,    // compact rows in use (padded)
   kHdrBlocks = 2,  // query blocks
   kHdrMarked = 3,  // rows that are not finite
+  kHdrPieces = 4,  // pieces of all blocks: units of one head
+  kHdrSplit = 5,   // 1 if some block has more than one piece
   kHdrWords = 64
 };
 
 // One query block of one sequence.
 struct Block {
-  int row0, rows;   // query tokens
-  int key0, tiles;  // first compact row, row tiles seen
+  int row0, rows;       // query tokens
+  int key0, tiles;      // first compact row, row tiles seen
+  int seq;
+  int piece0, pieces;   // its pieces
+  int unused;
+};
+
+// Row tiles tile0 .. tile0 + tiles - 1 of a block.
+struct __align__(16) Piece {
+  int row0, rows, key0, tile0;
+  int tiles, seq, whole, block;  // whole: the block's only piece
 };
 
 struct Work {
@@ -55,6 +74,9 @@ struct Work {
   int* seq_keys;   // [S] cached rows in use
   int* seq_block;  // [S + 1] first query block of each sequence
   Block* blocks;
+  Piece* pieces;
+  float* part_out;  // f32 [units, kQueryTile, Dv] of split blocks, each normalised
+  float* part_lse;  // f32 [units, kQueryTile] base-2 log sums
   uint8_t* marked;  // [cap] 1 where a compact row is not finite
   uint16_t* rows;   // bf16 [cap, 512]
   uint16_t* rope;   // bf16 [cap, 64]
@@ -79,6 +101,8 @@ struct Args {
   long long row_stride;
   int tokens, heads, seqs, slots, pages, cap, max_blocks;
   int head0, pass_heads;
+  int split_units;  // most units of a pass after splitting; 0: blocks are not split
+  int pairs;
   int dn, dr, dv, fp8, out_f32;
   float scale_log2;
 };
@@ -191,8 +215,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
   }
   __syncthreads();
   // Query blocks, one warp each: the tiles that its furthest-seeing token sees.
-  const int lane = tid & 31;
-  for (int b = tid >> 5; b < s_blocks; b += 32) {
+  const int lane = tid & 31, warp = tid >> 5;
+  for (int b = warp; b < s_blocks; b += 32) {
     const int s = last_at_or_below(w.seq_block, a.seqs, b);
     const int row0 = a.q_start[s] + (b - w.seq_block[s]) * kQueryTile;
     const int rows = min(kQueryTile, a.q_start[s + 1] - row0);
@@ -202,8 +226,65 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
     for (int o = 16; o > 0; o >>= 1) far = max(far, __shfl_xor_sync(0xFFFFFFFFu, far, o));
     const int keys = w.seq_keys[s];
     const int seen = far >= keys ? keys : far + 1;
-    if (lane == 0) w.blocks[b] = {row0, rows, w.seq_key0[s], (seen + kRowTile - 1) / kRowTile};
+    if (lane == 0)
+      w.blocks[b] = {row0, rows, w.seq_key0[s], (seen + kRowTile - 1) / kRowTile, s, b, 1, 0};
   }
+  __syncthreads();
+  // The most tiles that a piece gets. Warp k weighs cutting the longest block into k + 1: the
+  // rounds that the CTA pairs need for all units, each as long as such a piece.
+  __shared__ int s_cost[32], s_len[32];
+  int longest = 1;
+  for (int b = lane; b < s_blocks; b += 32) longest = max(longest, w.blocks[b].tiles);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xFFFFFFFFu, longest, o));
+  {
+    const int len = (longest + warp) / (warp + 1);
+    int count = 0;
+    if (a.split_units)
+      for (int b = lane; b < s_blocks; b += 32)
+        count += max(1, (w.blocks[b].tiles + len - 1) / len);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) count += __shfl_xor_sync(0xFFFFFFFFu, count, o);
+    const long long units = (long long)count * a.pass_heads;
+    if (lane == 0) {
+      s_len[warp] = len;
+      s_cost[warp] = INT_MAX;
+      if (a.split_units && units <= a.split_units)
+        s_cost[warp] = int((units + a.pairs - 1) / a.pairs) * (len + kPieceCost) +
+                       (warp ? 2 * kPieceCost : 0);
+    }
+  }
+  __syncthreads();
+  int best = 0;
+  for (int k = 1; k < 32; ++k)
+    if (s_cost[k] < s_cost[best]) best = k;
+  const int len = best ? s_len[best] : longest;
+  // Number the pieces, 1024 blocks at a time.
+  __syncthreads();
+  if (tid == 0) s_rows = 0;
+  __syncthreads();
+  for (int b0 = 0; b0 < s_blocks; b0 += 1024) {
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < s_blocks) n = max(1, (w.blocks[b].tiles + len - 1) / len);
+    const int end = block_inclusive(n, part), at = s_rows;
+    if (b < s_blocks) {
+      Block blk = w.blocks[b];
+      blk.piece0 = at + end - n;
+      blk.pieces = n;
+      w.blocks[b] = blk;
+      // Pieces of one length, the last one shorter by less than one tile a piece.
+      const int each = max(1, (blk.tiles + n - 1) / n);
+      for (int i = 0; i < n; ++i)
+        w.pieces[blk.piece0 + i] = {blk.row0, blk.rows, blk.key0, i * each,
+                                    max(0, min(each, blk.tiles - i * each)), blk.seq, n == 1, b};
+      if (n > 1) w.header[kHdrSplit] = 1;
+    }
+    __syncthreads();
+    if (tid == 1023) s_rows = at + end;
+    __syncthreads();
+  }
+  if (tid == 0) w.header[kHdrPieces] = s_rows;
 }
 
 // ------------------------------------------------------------------------------ gather
@@ -273,7 +354,10 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a) {
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr uint32_t kWaitPolls = 1u << 26;
 
-// Bounded waits of one role of a CTA pair. The first that runs out sets the error flag and both
+// Bounded waits of one role of a CTA pair. What they wait for lies in TMEM or is written and read by
+// the asynchronous proxies (TMA, MMA), ordered by the barriers and tcgen05 fences themselves: no wait
+// or arrival here needs the cluster-scope release or acquire of generic memory, which cost a
+// memory barrier per tile (2.0 of 9.8 warps stalled in it). The first that runs out sets the error flag and both
 // CTAs' abort words; every later wait of the pair then returns false at once.
 struct Waiter {
   int* header;
@@ -283,10 +367,10 @@ struct Waiter {
 
   __device__ bool on(uint32_t bar, uint32_t parity) {
     if (failed) return false;
-    if (ptx::mbar_test_cluster(bar, parity)) return true;
+    if (ptx::mbar_test(bar, parity)) return true;
     const uint64_t t0 = ptx::global_timer_ns();
     for (uint32_t i = 1;; ++i) {
-      if (ptx::mbar_test_cluster(bar, parity)) return true;
+      if (ptx::mbar_test(bar, parity)) return true;
       if ((i & 63) == 0) {
         if (*abort) {
           failed = true;
@@ -474,7 +558,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_peer(bar(kBarAccEmpty + buf), 0));
+      if (lane == 0) ptx::mbar_arrive_cluster_relaxed(ptx::map_peer(bar(kBarAccEmpty + buf), 0));
     }
   }
   // Every commit of the leader has arrived in both CTAs before either leaves.
@@ -541,23 +625,18 @@ struct Shape {
 };
 
 struct Unit {
-  Block blk;
+  Piece p;
   int head;  // of this pass
-  int seq;
 };
 
-// Units in order: sequence, head, query block from the last (which sees the most) to the first, so
-// that the pairs at work at one time share the keys and values of few heads in L2.
-__device__ __forceinline__ Unit unit_at(const Args& a, int u) {
-  const Work& w = a.w;
-  const int b = u / a.pass_heads;
-  const int s = last_at_or_below(w.seq_block, a.seqs, b);
-  const int b0 = w.seq_block[s], n = w.seq_block[s + 1] - b0;
-  const int r = u - b0 * a.pass_heads;
+// Units in order: head, so that the pairs at work at one time share the keys and values of few heads
+// in L2, then query block from the last, which sees the most of its sequence, to the first.
+__device__ __forceinline__ Unit unit_at(const Args& a, int u, int pieces) {
   Unit x;
-  x.head = r / n;
-  x.blk = w.blocks[b0 + n - 1 - r % n];
-  x.seq = s;
+  x.head = u / pieces;
+  const int4* src = reinterpret_cast<const int4*>(a.w.pieces + (pieces - 1 - (u - x.head * pieces)));
+  const int4 lo = src[0], hi = src[1];
+  x.p = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
   return x;
 }
 
@@ -602,24 +681,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   Waiter wt{a.w.header, abort, ptx::map_peer(base + C::kSmMisc + 4, uint32_t(rank ^ 1)), false};
-  const int units = a.w.header[kHdrBlocks] * a.pass_heads;
+  const int pieces = a.w.header[kHdrPieces], units = pieces * a.pass_heads;
 
+  // 384 threads start with 168 registers each; the softmax warpgroups take what the first gives up:
+  // 128 * 96 + 256 * 200 = 63488 of 64512.
   if (warp == 0) {
+    ptx::registers_down<96>();
     if (lane == 0) {
       uint32_t it = 0, useq = 0;
       for (int u = pair; u < units && !wt.failed; u += pairs) {
-        const Unit x = unit_at(a, u);
-        if (!x.blk.tiles) continue;
+        const Unit x = unit_at(a, u, pieces);
+        if (!x.p.tiles) continue;
         if (!wt.on(bar(C::kQEmpty), (useq & 1u) ^ 1u)) break;
         if (rank == 0) ptx::mbar_expect_tx(bar(C::kQFull), 2 * C::kQBytes);
 #pragma unroll
         for (int c = 0; c < C::kQChunks; ++c)
           ptx::tma_load_3d_pair(base + c * 16384, &tm_q, lead(C::kQFull), c * 64, a.head0 + x.head,
-                                x.blk.row0 + rank * 128);
+                                x.p.row0 + rank * 128);
         ++useq;
-        for (int j = 0; j < x.blk.tiles; ++j, ++it) {
+        for (int j = 0; j < x.p.tiles; ++j, ++it) {
           const uint32_t st = it % C::kKv, ph = ((it / C::kKv) & 1u) ^ 1u;
-          const int key = x.blk.key0 + j * kRowTile;
+          const int key = x.p.key0 + (x.p.tile0 + j) * kRowTile;
           if (!wt.on(bar(C::kKEmpty + st), ph)) break;
           if (rank == 0) ptx::mbar_expect_tx(bar(C::kKFull + st), 2 * C::kKBytes);
           const uint32_t kd = base + C::kSmK + st * C::kKBytes;
@@ -642,6 +724,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
+    ptx::registers_down<96>();
     if (rank == 0) {
       constexpr uint32_t idesc_qk = ptx::idesc_bf16(256, 128, 0);
       constexpr uint32_t idesc_pv = ptx::idesc_bf16(256, kDv, 1);
@@ -663,8 +746,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         return true;
       };
       for (int u = pair; u < units && !wt.failed; u += pairs) {
-        const Unit x = unit_at(a, u);
-        const int tiles = x.blk.tiles;
+        const Unit x = unit_at(a, u, pieces);
+        const int tiles = x.p.tiles;
         if (!tiles) continue;
         if (!wt.all(bar(C::kQFull), useq & 1u)) break;
         ptx::tc_fence_after();
@@ -698,57 +781,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       ptx::mma_commit_pair(bar(C::kDrain));
     }
     __syncwarp();
-  } else if (warp >= 4) {
+  } else if (warp < 4) {
+    ptx::registers_down<96>();
+  } else {
+    ptx::registers_up<200>();
     const int half = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = uint32_t(quad * 32) << 16;
     float* exch = reinterpret_cast<float*>(sm + C::kSmExch);
     const bool marked = a.w.header[kHdrMarked] != 0;
     const float c = a.scale_log2, slack = kSlack / c;
+    const uint64_t c2 = ptx::pack_f32x2(c, c);
     uint32_t it = 0;
     // A wait that ran out is not left for: the two warps of a row go through the same barriers to
     // the end, over whatever TMEM holds; the error flag is set.
     for (int u = pair; u < units; u += pairs) {
-      const Unit x = unit_at(a, u);
-      const int t = x.blk.row0 + rank * 128 + row;
-      const bool mine = rank * 128 + row < x.blk.rows;
+      const Unit x = unit_at(a, u, pieces);
+      const int t = x.p.row0 + rank * 128 + row;
+      const bool mine = rank * 128 + row < x.p.rows;
       int n = 0;  // keys that this row sees
       if (mine) {
-        const int keys = a.w.seq_keys[x.seq], pos = a.q_pos[t];
+        const int keys = a.w.seq_keys[x.p.seq], pos = a.q_pos[t];
         n = pos >= keys ? keys : max(pos + 1, 0);
       }
-      float m = -INFINITY, sum = 0.f;
-      for (int j = 0; j < x.blk.tiles; ++j, ++it) {
+      float m = -INFINITY;
+      uint64_t sum0 = 0, sum1 = 0;  // pairs of f32 partial sums
+      for (int j = 0; j < x.p.tiles; ++j, ++it) {
         const uint32_t sb = it % C::kS;
         wt.all(bar(C::kSFull + sb), (it / C::kS) & 1u);
         ptx::tc_fence_after();
-        uint32_t r[2][32];
+        float s[64];
         const uint32_t src = tmem + sb * 128 + half * 64 + lanes;
-        ptx::tmem_ld32(src, r[0]);
-        ptx::tmem_ld32(src + 32, r[1]);
-        ptx::tmem_wait_ld();
-        float(&s0)[32] = reinterpret_cast<float(&)[32]>(r[0]);
-        float(&s1)[32] = reinterpret_cast<float(&)[32]>(r[1]);
-        const int key = j * kRowTile + half * 64;
+        {
+          uint32_t lo[32], hi[32];
+          ptx::tmem_ld32(src, lo);
+          ptx::tmem_ld32(src + 32, hi);
+          ptx::tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            s[i] = __uint_as_float(lo[i]);
+            s[32 + i] = __uint_as_float(hi[i]);
+          }
+        }
+        const int key = (x.p.tile0 + j) * kRowTile + half * 64;
         if (!__all_sync(0xFFFFFFFFu, n >= key + 64)) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (key + i >= n) s0[i] = -INFINITY;
-            if (key + 32 + i >= n) s1[i] = -INFINITY;
-          }
+          for (int i = 0; i < 64; ++i)
+            if (key + i >= n) s[i] = -INFINITY;
         }
         if (marked) {
-          const uint8_t* mk = a.w.marked + x.blk.key0 + key;
+          const uint8_t* mk = a.w.marked + x.p.key0 + key;
+          const uint32_t bits[2] = {__ballot_sync(0xFFFFFFFFu, mk[lane] != 0),
+                                    __ballot_sync(0xFFFFFFFFu, mk[32 + lane] != 0)};
+          if (bits[0] | bits[1]) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (mk[i] && key + i < n) s0[i] = NAN;
-            if (mk[32 + i] && key + 32 + i < n) s1[i] = NAN;
+            for (int i = 0; i < 64; ++i)
+              if (((bits[i >> 5] >> (i & 31)) & 1u) && key + i < n) s[i] = NAN;
           }
         }
-        float top = s0[0];
+        float top = s[0], top1 = s[32];
 #pragma unroll
-        for (int i = 1; i < 32; ++i) top = fmaxf(top, s0[i]);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) top = fmaxf(top, s1[i]);
+        for (int i = 1; i < 32; ++i) {
+          top = fmaxf(top, s[i]);
+          top1 = fmaxf(top1, s[32 + i]);
+        }
+        top = fmaxf(top, top1);
         float* ex = exch + (it & 1u) * 256;
         ex[half * 128 + row] = top;
         ptx::named_barrier(1 + quad, 64);
@@ -760,7 +856,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (__any_sync(0xFFFFFFFFu, grow)) {
             const float keep = !grow ? 1.f : m == -INFINITY ? 0.f : ptx::ex2((m - top) * c);
             if (grow) m = top;
-            sum *= keep;
+            const uint64_t keep2 = ptx::pack_f32x2(keep, keep), zero = 0;
+            sum0 = ptx::fma_f32x2(sum0, keep2, zero);
+            sum1 = ptx::fma_f32x2(sum1, keep2, zero);
             wt.all(bar(C::kPvDone + (it - 1) % C::kS), ((it - 1) / C::kS) & 1u);
             ptx::tc_fence_after();
             const uint32_t o = tmem + C::kTmemO + half * (kDv / 2) + lanes;
@@ -774,27 +872,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float mc = m == -INFINITY ? 0.f : m * c;
+        const float mc = m == -INFINITY ? 0.f : -m * c;
+        const uint64_t mc2 = ptx::pack_f32x2(mc, mc);
         uint32_t p[32];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float p0 = ptx::ex2(fmaf(s0[i], c, -mc)), p1 = ptx::ex2(fmaf(s0[i + 1], c, -mc));
-          sum += p0 + p1;
+        for (int i = 0; i < 64; i += 2) {
+          float p0, p1;
+          ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(s[i], s[i + 1]), c2, mc2), p0, p1);
+          p0 = ptx::ex2(p0);
+          p1 = ptx::ex2(p1);
+          if (i & 2)
+            sum1 = ptx::add_f32x2(sum1, ptx::pack_f32x2(p0, p1));
+          else
+            sum0 = ptx::add_f32x2(sum0, ptx::pack_f32x2(p0, p1));
           p[i / 2] = ptx::pack_bf16x2(p0, p1);
-        }
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float p0 = ptx::ex2(fmaf(s1[i], c, -mc)), p1 = ptx::ex2(fmaf(s1[i + 1], c, -mc));
-          sum += p0 + p1;
-          p[16 + i / 2] = ptx::pack_bf16x2(p0, p1);
         }
         ptx::tmem_st32(tmem + sb * 128 + half * 32 + lanes, p);
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive_cluster(lead(C::kPFull + sb));
+        if (lane == 0) ptx::mbar_arrive_cluster_relaxed(lead(C::kPFull + sb));
       }
       // The row's whole sum, then O / sum to the output: this thread's half of the columns.
+      float sum, odd;
+      ptx::unpack_f32x2(ptx::add_f32x2(sum0, sum1), sum, odd);
+      sum += odd;
       float* ex = exch + (it & 1u) * 256;
       ex[half * 128 + row] = sum;
       ptx::named_barrier(1 + quad, 64);
@@ -802,18 +904,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // Both have read before either writes its next maximum there (two tiles on at the earliest,
       // or at once when the next unit has no tiles).
       ptx::named_barrier(1 + quad, 64);
-      const float inv = n > 0 ? 1.f / sum : 0.f;
-      if (x.blk.tiles) {
+      const bool sees = n > x.p.tile0 * kRowTile;  // in this piece
+      const float inv = sees ? 1.f / sum : 0.f;
+      if (x.p.tiles) {
         wt.all(bar(C::kPvDone + (it - 1) % C::kS), ((it - 1) / C::kS) & 1u);
         ptx::tc_fence_after();
       }
       const int head = a.head0 + x.head;
-      uint8_t* out = a.out + (long long)t * a.out_st + (long long)head * a.out_sh;
+      const long long part = (long long)u * kQueryTile + rank * 128 + row;
+      uint8_t* out = x.p.whole ? a.out + (long long)t * a.out_st + (long long)head * a.out_sh
+                               : reinterpret_cast<uint8_t*>(a.w.part_out + part * kDv);
       const uint32_t o = tmem + C::kTmemO + half * (kDv / 2) + lanes;
 #pragma unroll
       for (int i = 0; i < kDv / 2; i += 32) {
         uint32_t v[32];
-        if (x.blk.tiles) {
+        if (x.p.tiles) {
           ptx::tmem_ld32(o + i, v);
           ptx::tmem_wait_ld();
         }
@@ -821,8 +926,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const int col = half * (kDv / 2) + i;
 #pragma unroll
           for (int k = 0; k < 32; ++k)
-            v[k] = n > 0 ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
-          if (a.out_f32) {
+            v[k] = sees ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
+          if (a.out_f32 || !x.p.whole) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4)
               *reinterpret_cast<uint4*>(out + 4 * (col + k)) =
@@ -838,14 +943,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (x.blk.tiles) {
+      if (x.p.tiles) {
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive_cluster(lead(C::kOFree));
+        if (lane == 0) ptx::mbar_arrive_cluster_relaxed(lead(C::kOFree));
       }
-      if (a.lse && mine && half == 0)
-        a.lse[(long long)t * a.heads + head] =
-            n > 0 ? 0.69314718055994531f * (m * c + log2f(sum)) : -INFINITY;
+      if (mine && half == 0) {
+        const float l2 = sees ? m * c + log2f(sum) : -INFINITY;
+        if (!x.p.whole)
+          a.w.part_lse[part] = l2;
+        else if (a.lse)
+          a.lse[(long long)t * a.heads + head] = l2 * 0.69314718055994531f;
+      }
     }
   }
   wt.on(bar(C::kDrain), 0);
@@ -860,10 +969,64 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 }  // namespace attend
 
+// ------------------------------------------------------------------------------ join
+// Merges the pieces of split blocks: out = sum_i 2^(l_i - l) out_i, l = log2 sum_i 2^l_i, in piece
+// order. One thread takes 8 columns of one row and head, all pieces' loads ahead of their use.
+// Reads the partial outputs once from L2, where the attention left them.
+__global__ void __launch_bounds__(256) join_kernel(const Args a) {
+  const Work& w = a.w;
+  if (!w.header[kHdrSplit]) return;
+  const int pieces = w.header[kHdrPieces], groups = a.dv / 8;
+  const long long all = (long long)w.header[kHdrBlocks] * a.pass_heads * kQueryTile * groups;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all;
+       i += (long long)gridDim.x * 256) {
+    const int g = int(i % groups);
+    long long r = i / groups;
+    const int row = int(r % kQueryTile);
+    r /= kQueryTile;
+    const int head = int(r % a.pass_heads);
+    const Block blk = w.blocks[r / a.pass_heads];
+    if (blk.pieces == 1 || row >= blk.rows) continue;
+    const long long p0 = ((long long)head * pieces + blk.piece0) * kQueryTile + row;
+    float top = -INFINITY;
+    for (int k = 0; k < blk.pieces; ++k) top = fmaxf(top, w.part_lse[p0 + (long long)k * kQueryTile]);
+    const float use = top == -INFINITY ? 0.f : top;
+    float o[8] = {}, sum = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < blk.pieces; ++k) {
+      const long long p = p0 + (long long)k * kQueryTile;
+      const float f = ptx::ex2(w.part_lse[p] - use);
+      const float4* src = reinterpret_cast<const float4*>(w.part_out + p * a.dv + 8 * g);
+      const float4 x = src[0], y = src[1];
+      sum += f;
+      o[0] = fmaf(f, x.x, o[0]); o[1] = fmaf(f, x.y, o[1]);
+      o[2] = fmaf(f, x.z, o[2]); o[3] = fmaf(f, x.w, o[3]);
+      o[4] = fmaf(f, y.x, o[4]); o[5] = fmaf(f, y.y, o[5]);
+      o[6] = fmaf(f, y.z, o[6]); o[7] = fmaf(f, y.w, o[7]);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] *= inv;
+    const long long t = blk.row0 + row;
+    uint8_t* out = a.out + t * a.out_st + (long long)(a.head0 + head) * a.out_sh;
+    if (a.out_f32) {
+      reinterpret_cast<float4*>(out + 32 * g)[0] = make_float4(o[0], o[1], o[2], o[3]);
+      reinterpret_cast<float4*>(out + 32 * g)[1] = make_float4(o[4], o[5], o[6], o[7]);
+    } else {
+      *reinterpret_cast<uint4*>(out + 16 * g) =
+          make_uint4(ptx::pack_bf16x2(o[0], o[1]), ptx::pack_bf16x2(o[2], o[3]),
+                     ptx::pack_bf16x2(o[4], o[5]), ptx::pack_bf16x2(o[6], o[7]));
+    }
+    if (a.lse && g == 0)
+      a.lse[t * a.heads + a.head0 + head] =
+          sum == 0.f ? -INFINITY : 0.69314718055994531f * (use + log2f(sum));
+  }
+}
+
 // ------------------------------------------------------------------------------ host
 struct Layout {
-  uint64_t header, seq_key0, seq_keys, seq_block, blocks, marked, rows, rope, k, v, total;
-  uint64_t cap, max_blocks, pass_heads;
+  uint64_t header, seq_key0, seq_keys, seq_block, blocks, pieces, part_out, part_lse, marked, rows, rope, k, v, total;
+  uint64_t cap, max_blocks, pass_heads, split_units;
 };
 
 uint64_t round256(uint64_t v) { return (v + 255) & ~uint64_t(255); }
@@ -881,6 +1044,9 @@ Layout layout_of(const TqMlaChunkSpec& s) {
   l.pass_heads = kScratchBytes / per_head;
   if (l.pass_heads < 1) l.pass_heads = 1;
   if (l.pass_heads > H) l.pass_heads = H;
+  // Blocks are split only where even full query blocks would be fewer than the units allowed.
+  const uint64_t full = (T + kQueryTile - 1) / kQueryTile * l.pass_heads;
+  l.split_units = full <= kSplitUnits ? kSplitUnits : 0;
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
     const uint64_t here = at;
@@ -892,6 +1058,9 @@ Layout layout_of(const TqMlaChunkSpec& s) {
   l.seq_keys = take((S + 1) * 4);
   l.seq_block = take((S + 1) * 4);
   l.blocks = take(l.max_blocks * sizeof(Block));
+  l.pieces = take((l.max_blocks + l.split_units) * sizeof(Piece));
+  l.part_out = take(l.split_units * kQueryTile * dv * 4);
+  l.part_lse = take(l.split_units * kQueryTile * 4);
   l.marked = take(l.cap);
   l.rows = take(l.cap * kLatent * 2);
   l.rope = take(l.cap * kRopeDim * 2);
@@ -934,7 +1103,8 @@ bool encode(CUtensorMap* map, const void* addr, uint64_t width, uint64_t rows, u
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Per device: CTA pairs (two SMs each), and the kernels' shared memory granted. 0 on failure.
+// CTA pairs (two SMs each) of the current device, once the kernels have their shared memory granted
+// on it; 0 on failure.
 int pairs_on(int device) {
   static std::mutex mu;
   static int cached[128] = {0};
@@ -981,6 +1151,10 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
   const TqMlaChunkSpec& s = *spec;
   const uint64_t T = s.q.shape[0], S = s.page_table.shape[0];
   if (T == 0 || S == 0) return fail(nullptr, TQ_OK);
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return fail("device", TQ_ERR_CUDA);
+  const int pairs = pairs_on(device);
+  if (pairs <= 0) return fail("device", TQ_ERR_CUDA);
   const Layout l = layout_of(s);
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < l.total)
     return fail("workspace", TQ_ERR_WORKSPACE);
@@ -991,6 +1165,9 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
   a.w.seq_keys = reinterpret_cast<int*>(ws + l.seq_keys);
   a.w.seq_block = reinterpret_cast<int*>(ws + l.seq_block);
   a.w.blocks = reinterpret_cast<Block*>(ws + l.blocks);
+  a.w.pieces = reinterpret_cast<Piece*>(ws + l.pieces);
+  a.w.part_out = reinterpret_cast<float*>(ws + l.part_out);
+  a.w.part_lse = reinterpret_cast<float*>(ws + l.part_lse);
   a.w.marked = ws + l.marked;
   a.w.rows = reinterpret_cast<uint16_t*>(ws + l.rows);
   a.w.rope = reinterpret_cast<uint16_t*>(ws + l.rope);
@@ -1023,16 +1200,15 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
   a.pages = int(s.kv.shape[0]);
   a.cap = int(l.cap);
   a.max_blocks = int(l.max_blocks);
+  a.split_units = int(l.split_units);
+  a.pairs = pairs;
+  a.pass_heads = int(l.pass_heads);
   a.dn = int(s.w_uk.shape[1]);
   a.dv = int(s.w_uv.shape[1]);
   a.dr = int(s.q.shape[2]) - a.dn;
   a.fp8 = s.kv_format == TQ_KV_FP8_E4M3;
   a.out_f32 = s.out.dtype == TQ_DTYPE_F32;
   a.scale_log2 = s.softmax_scale * 1.4426950408889634f;
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return fail("device", TQ_ERR_CUDA);
-  const int pairs = pairs_on(device);
-  if (pairs <= 0) return fail("device", TQ_ERR_CUDA);
   CUtensorMap tm_rows, tm_uk, tm_uv, tm_q, tm_k, tm_rope, tm_v;
   // q: 64 values by one head by 128 tokens, tokens past T as zeros.
   if (!encode(&tm_q, a.q, uint64_t(a.dn + a.dr), s.q.shape[1], T, s.q.strides_bytes[1],
@@ -1063,6 +1239,7 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
       attend::attend_kernel<256, 256>
           <<<2 * pairs, attend::kThreads, attend::Shape<256, 256>::kSmBytes, cs>>>(tm_q, tm_k,
                                                                                    tm_rope, tm_v, a);
+    if (a.split_units) join_kernel<<<4 * pairs, 256, 0, cs>>>(a);
   }
   if (cudaGetLastError() != cudaSuccess) return fail("launch", TQ_ERR_CUDA);
   return fail(nullptr, TQ_OK);
