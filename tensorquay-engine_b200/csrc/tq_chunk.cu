@@ -8,9 +8,10 @@
 //                     (every sequence padded to kRowTile rows), its query blocks of kQueryTile
 //                     tokens with the number of row tiles each of them sees.
 //   2. gather_kernel  the cached rows through the page table into that space, as bf16 (FP8 rows
-//                     dequantized, rounded once): zeros past kv_len, and zeros with a mark for a
-//                     row that is not finite, so that neither stale rows nor such a row can reach
-//                     an output that does not see it through 0 * NaN.
+//                     dequantized, rounded once): zeros past kv_len and for a row that is not
+//                     finite, so that neither stale rows nor such a row can reach an output that
+//                     does not see it through 0 * NaN. The first such row of a sequence is kept:
+//                     the outputs of the tokens that see it become NaN at the end.
 //   3. expand_kernel  k and v of every head from the compact rows.
 //   4. attend_kernel  attention of every (query block, head); where those are few, each is split
 //                     into pieces of its row tiles, and
@@ -47,9 +48,8 @@ enum Header : int {
   kHdrError = 0,
   kHdrRows = 1,    // compact rows in use (padded)
   kHdrBlocks = 2,  // query blocks
-  kHdrMarked = 3,  // rows that are not finite
-  kHdrPieces = 4,  // pieces of all blocks: units of one head
-  kHdrSplit = 5,   // 1 if some block has more than one piece
+  kHdrPieces = 3,  // pieces of all blocks: units of one head
+  kHdrSplit = 4,   // 1 if some block has more than one piece
   kHdrWords = 64
 };
 
@@ -73,11 +73,11 @@ struct Work {
   int* seq_key0;   // [S + 1] first compact row of each sequence
   int* seq_keys;   // [S] cached rows in use
   int* seq_block;  // [S + 1] first query block of each sequence
+  int* seq_spoilt; // [S] first cached row that is not finite (INT_MAX: none)
   Block* blocks;
   Piece* pieces;
   float* part_out;  // f32 [units, kQueryTile, Dv] of split blocks, each normalised
   float* part_lse;  // f32 [units, kQueryTile] base-2 log sums
-  uint8_t* marked;  // [cap] 1 where a compact row is not finite
   uint16_t* rows;   // bf16 [cap, 512]
   uint16_t* rope;   // bf16 [cap, 64]
   uint16_t* k;      // bf16 [heads of a pass, cap, Dn]
@@ -182,6 +182,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
     if (s < a.seqs) {
       w.seq_key0[s] = rows0 + rows_end - padded;
       w.seq_keys[s] = keys;
+      w.seq_spoilt[s] = INT_MAX;
       w.seq_block[s] = blocks0 + blocks_end - blocks;
     }
     long long sum = padded;
@@ -343,10 +344,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a) {
     *reinterpret_cast<uint4*>(dst) = v0;
     *reinterpret_cast<uint4*>(dst + 8) = v1;
     if (a.dr) *reinterpret_cast<uint32_t*>(w.rope + r * kRopeDim + 2 * lane) = rp;
-    if (lane == 0) {
-      w.marked[r] = row_ok ? 0 : 1;
-      if (!row_ok) atomicAdd(w.header + kHdrMarked, 1);
-    }
+    if (lane == 0 && !row_ok) atomicMin(w.seq_spoilt + s, p);
   }
 }
 
@@ -361,24 +359,25 @@ constexpr uint32_t kWaitPolls = 1u << 26;
 // CTAs' abort words; every later wait of the pair then returns false at once.
 struct Waiter {
   int* header;
-  volatile uint32_t* abort;  // this CTA's abort word
-  uint32_t peer_abort;       // the other CTA's, in the shared::cluster window
+  uint32_t abort;  // shared address of this CTA's abort word
+  int rank;
   bool failed;
 
   __device__ bool on(uint32_t bar, uint32_t parity) {
     if (failed) return false;
-    if (ptx::mbar_test(bar, parity)) return true;
-    const uint64_t t0 = ptx::global_timer_ns();
+    uint64_t t0 = 0;  // reading the timer is slow: only a wait of many polls does
     for (uint32_t i = 1;; ++i) {
-      if (ptx::mbar_test(bar, parity)) return true;
-      if ((i & 63) == 0) {
-        if (*abort) {
+      if (ptx::mbar_try(bar, parity)) return true;
+      if ((i & 15) == 0) {
+        if (ptx::ld_shared_u32(abort)) {
           failed = true;
           return false;
         }
-        if (i >= kWaitPolls || ptx::global_timer_ns() - t0 > kWaitNs) {
-          *abort = 1;
-          ptx::st_cluster_u32(peer_abort, 1u);
+        const uint64_t now = ptx::global_timer_ns();
+        if (t0 == 0) t0 = now;
+        if (i >= kWaitPolls || now - t0 > kWaitNs) {
+          ptx::st_cluster_u32(ptx::map_peer(abort, uint32_t(rank)), 1u);
+          ptx::st_cluster_u32(ptx::map_peer(abort, uint32_t(rank ^ 1)), 1u);
           atomicOr(header + kHdrError, TQ_DEV_WAIT_TIMEOUT);
           failed = true;
           return false;
@@ -395,7 +394,7 @@ struct Waiter {
   }
   // After an abort: a millisecond in which the pair's copies and MMAs in flight land.
   __device__ void settle() {
-    if (!*abort) return;
+    if (!ptx::ld_shared_u32(abort)) return;
     const uint64_t t0 = ptx::global_timer_ns();
     for (uint32_t i = 0; i < (1u << 20) && ptx::global_timer_ns() - t0 < 1000000ull; ++i) {
     }
@@ -440,11 +439,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int pair = int(blockIdx.x) >> 1, pairs = int(gridDim.x) >> 1;
   auto bar = [&](int i) { return base + kSmBars + 8u * uint32_t(i); };
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sm + kSmMisc);
-  volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(sm + kSmMisc + 4);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBars; ++i) ptx::mbar_init(bar(i), 1);
     for (int b = 0; b < 2; ++b) ptx::mbar_init(bar(kBarAccEmpty + b), 8);  // 4 warps of each CTA
-    *abort = 0;
+    tmem_holder[1] = 0;  // the abort word
     ptx::fence_mbar_init_cluster();
     ptx::tma_prefetch_desc(&tm_rows);
     ptx::tma_prefetch_desc(&tm_uk);
@@ -458,7 +456,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::cluster_sync();
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  Waiter wt{a.w.header, abort, ptx::map_peer(base + kSmMisc + 4, uint32_t(rank ^ 1)), false};
+  Waiter wt{a.w.header, base + kSmMisc + 4, rank, false};
 
   // Column blocks (a head, or a head's k or v) by row tiles, one contiguous range per pair.
   const int per_head = (a.dn + a.dv) / 256;
@@ -498,6 +496,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     if (rank == 0) {
       constexpr uint32_t idesc = ptx::idesc_bf16(256, 256, 0);
+      const uint32_t elected = ptx::elect_one();
       uint32_t stage = 0, phase = 0, blocks = 0, n = 0;
       for (long long i = first; i < last && !wt.failed; ++i, ++n) {
         const int tile = int(i % tiles);
@@ -512,10 +511,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ptx::tc_fence_after();
           const uint64_t ad = ptx::smem_desc(base + kSmA + stage * kBox, 16, 1024, 2);
           const uint64_t bd = ptx::smem_desc(base + kSmW + c * kBox, 16, 1024, 2);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            ptx::mma_ss_pair(d, ad + uint64_t(2 * k), bd + uint64_t(2 * k), idesc,
-                             (c > 0 || k > 0) ? 1u : 0u);
+          ptx::mma_ss_pair_x4(elected, d, ad, bd, idesc, c > 0 ? 1u : 0u);
           ptx::mma_commit_pair(bar(kBarAEmpty + stage));
           if (done) ptx::mma_commit_pair(bar(kBarWEmpty + c));
           if (++stage == kStages) {
@@ -561,8 +557,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (lane == 0) ptx::mbar_arrive_cluster_relaxed(ptx::map_peer(bar(kBarAccEmpty + buf), 0));
     }
   }
-  // Every commit of the leader has arrived in both CTAs before either leaves.
-  wt.on(bar(kBarDrain), 0);
+  // Every commit of the leader has arrived in both CTAs before either leaves. One warp polls for it;
+  // the others go on to the cluster barrier, which costs no issue slots.
+  if (warp == 0) wt.on(bar(kBarDrain), 0);
   wt.settle();
   ptx::tc_fence_before();
   ptx::cluster_sync();
@@ -582,15 +579,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // it loads half: 64 of a tile's keys for QK^T, half the value columns for PV. So a pair moves
 // K_j and V_j once for 256 queries, and the shared memory left holds several tiles ahead.
 //   warp 0      TMA loads of this CTA's halves; their bytes complete on the leader's barriers
-//   warp 1      (leader) all MMAs. S_j has kS buffers in TMEM: S_{j+kS} is issued right after
-//               PV_j, whose P_j lies in the same columns; MMAs run in issue order
-//               (a softmax warp may be up to kS tiles ahead of PV, so the completion of PV_j has a
-//               barrier per buffer: S_j, which a waiter has seen, lies behind PV_{j-kS})
-//   warps 4-11  softmax: a row's 128 scores are split between two threads (warps 4-7 the first 64
-//               keys, 8-11 the rest), which exchange their maxima through shared memory. P goes to
-//               TMEM as bf16 over the scores. The maximum that p is taken against moves only when
-//               it would grow by more than 2^8 (kSlack): then O and the sum are rescaled, after
-//               the last PV; otherwise p stays below 2^8 and the final division makes it exact.
+//   warps 1, 2  (leader) the MMAs of QK^T and of PV, a warp each, so that the waits of one run
+//               under the MMAs of the other (one warp for both left the tensor cores idle half of
+//               the time). S_j has kS buffers in TMEM; P_j lies in S_j's columns, so S_{j+kS}
+//               waits for PV_j. A softmax warp may be several tiles ahead of PV, so the
+//               completion of PV_j has a barrier per buffer: a waiter has seen S_j, which lies
+//               behind PV_{j-kS}, and its phase is the next.
+//   warps 4-11  softmax: two groups of four warps take the tiles in turn, a thread a row, so that
+//               one group's exponentials run under the other's loads, maxima and waits (both
+//               groups on each tile's halves in step took 2990 cycles a tile, of them 1350 in the
+//               exponentials). P goes to TMEM as bf16 over the scores. The reference maximum of a
+//               row passes from group to group through shared memory. It moves only when it would
+//               grow by more than 2^8 (kSlack): then O is rescaled, after the last PV; otherwise p
+//               stays below 2^8 and the final division makes it exact. Each thread's sum is over
+//               its own tiles.
 //
 // What bounds it: per 128 x 128 tile and CTA the tensor cores need (2 (Dqk + Dv) 128 128) / 8192
 // cycles (1280 at 192 + 128, 2048 at 256 + 256), the exponentials 128 128 / 16 = 1024.
@@ -598,19 +600,20 @@ namespace attend {
 
 constexpr int kThreads = 384;
 constexpr float kSlack = 8.f;  // log2 units
+constexpr int kTurn = 1;       // quarter of a tile's exponentials after which the turn passes
 
 template <int kDq, int kDv>
 struct Shape {
   static constexpr int kQChunks = kDq / 64;
   static constexpr int kVChunks = kDv / 128;              // of this CTA's half
   static constexpr int kS = (512 - kDv) / 128 < 3 ? (512 - kDv) / 128 : 3;  // score buffers
-  static constexpr int kKv = kDv == 128 ? 4 : 2;          // K and V stages each
+  static constexpr int kKv = kS;                         // K and V stages each
   static constexpr uint32_t kQBytes = kQChunks * 128 * 128;
   static constexpr uint32_t kKBytes = kQChunks * 64 * 128;
   static constexpr uint32_t kVBytes = kVChunks * 128 * 128;
   static constexpr uint32_t kSmK = kQBytes;
   static constexpr uint32_t kSmV = kSmK + kKv * kKBytes;
-  static constexpr uint32_t kSmExch = kSmV + kKv * kVBytes;  // f32 [2][2][128]
+  static constexpr uint32_t kSmExch = kSmV + kKv * kVBytes;  // f32 [3][128]
   static constexpr uint32_t kSmBars = kSmExch + 2048;
   static constexpr int kQFull = 0, kQEmpty = 1, kKFull = 2, kKEmpty = kKFull + kKv;
   static constexpr int kVFull = kKEmpty + kKv, kVEmpty = kVFull + kKv;
@@ -622,6 +625,26 @@ struct Shape {
   static constexpr uint32_t kTmemO = kS * 128;
   static_assert(kSmBytes <= 232448, "shared memory per CTA");
   static_assert(kTmemO + kDv <= 512, "TMEM columns");
+};
+
+// Parities of the N barriers of a ring that every unit enters at its first stage (so that a tile's
+// stage is its number within the unit mod N): bit i is the parity of stage i's next use.
+template <int N>
+struct Phases {
+  uint32_t bits = 0;
+  // The parity of stage i's next use, which is now taken.
+  __device__ uint32_t take(uint32_t i) {
+    const uint32_t b = (bits >> i) & 1u;
+    bits ^= 1u << i;
+    return b;
+  }
+  // The parity of stage i's use number k from here on.
+  __device__ uint32_t at(uint32_t i, int k) const { return ((bits >> i) ^ uint32_t(k)) & 1u; }
+  // A unit of `tiles` tiles is over.
+  __device__ void pass(int tiles) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) bits ^= uint32_t(((tiles - i + N - 1) / N) & 1) << i;
+  }
 };
 
 struct Unit {
@@ -658,14 +681,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   auto bar = [&](int i) { return base + C::kSmBars + 8u * uint32_t(i); };
   auto lead = [&](int i) { return ptx::map_peer(bar(i), 0); };
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sm + C::kSmMisc);
-  volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(sm + C::kSmMisc + 4);
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kBars; ++i) {
-      // P of a tile and the release of O: one arrival per softmax warp of either CTA.
-      const bool joint = (i >= C::kPFull && i < C::kPFull + C::kS) || i == C::kOFree;
-      ptx::mbar_init(bar(i), joint ? 16 : 1);
+      // P of a tile: its group's four warps in either CTA; the release of O: all softmax warps; the
+      // end: both MMA warps.
+      const bool joint = i >= C::kPFull && i < C::kPFull + C::kS;
+      ptx::mbar_init(bar(i), joint ? 8 : i == C::kOFree ? 16 : i == C::kDrain ? 2 : 1);
     }
-    *abort = 0;
+    tmem_holder[1] = 0;  // the abort word
     ptx::fence_mbar_init_cluster();
     ptx::tma_prefetch_desc(&tm_q);
     ptx::tma_prefetch_desc(&tm_k);
@@ -680,7 +703,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::cluster_sync();
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  Waiter wt{a.w.header, abort, ptx::map_peer(base + C::kSmMisc + 4, uint32_t(rank ^ 1)), false};
+  Waiter wt{a.w.header, base + C::kSmMisc + 4, rank, false};
+  // All 512 columns are this CTA's, so they start at 0.
   const int pieces = a.w.header[kHdrPieces], units = pieces * a.pass_heads;
 
   // 384 threads start with 168 registers each; the softmax warpgroups take what the first gives up:
@@ -688,7 +712,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     ptx::registers_down<96>();
     if (lane == 0) {
-      uint32_t it = 0, useq = 0;
+      uint32_t useq = 0;
+      Phases<C::kKv> free;  // of the K and V stages, which are taken together
       for (int u = pair; u < units && !wt.failed; u += pairs) {
         const Unit x = unit_at(a, u, pieces);
         if (!x.p.tiles) continue;
@@ -699,8 +724,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ptx::tma_load_3d_pair(base + c * 16384, &tm_q, lead(C::kQFull), c * 64, a.head0 + x.head,
                                 x.p.row0 + rank * 128);
         ++useq;
-        for (int j = 0; j < x.p.tiles; ++j, ++it) {
-          const uint32_t st = it % C::kKv, ph = ((it / C::kKv) & 1u) ^ 1u;
+        for (int j = 0; j < x.p.tiles; ++j) {
+          const uint32_t st = uint32_t(j % C::kKv), ph = free.take(st) ^ 1u;
           const int key = x.p.key0 + (x.p.tile0 + j) * kRowTile;
           if (!wt.on(bar(C::kKEmpty + st), ph)) break;
           if (rank == 0) ptx::mbar_expect_tx(bar(C::kKFull + st), 2 * C::kKBytes);
@@ -726,56 +751,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     ptx::registers_down<96>();
     if (rank == 0) {
-      constexpr uint32_t idesc_qk = ptx::idesc_bf16(256, 128, 0);
-      constexpr uint32_t idesc_pv = ptx::idesc_bf16(256, kDv, 1);
-      uint32_t it0 = 0, useq = 0;  // tiles of earlier units, units with tiles
-      auto issue_qk = [&](uint32_t it) -> bool {
-        const uint32_t st = it % C::kKv;
-        if (!wt.all(bar(C::kKFull + st), (it / C::kKv) & 1u)) return false;
-        ptx::tc_fence_after();
-        const uint64_t qd = ptx::smem_desc(base, 16, 1024, 2);
-        const uint64_t kd = ptx::smem_desc(base + C::kSmK + st * C::kKBytes, 16, 1024, 2);
-        const uint32_t d = tmem + (it % C::kS) * 128;
-#pragma unroll
-        for (int k = 0; k < kDq / 16; ++k)
-          ptx::mma_ss_pair(d, qd + uint64_t(((k >> 2) * 16384 + (k & 3) * 32) >> 4),
-                           kd + uint64_t(((k >> 2) * 8192 + (k & 3) * 32) >> 4), idesc_qk,
-                           k > 0 ? 1u : 0u);
-        ptx::mma_commit_pair(bar(C::kSFull + it % C::kS));
-        ptx::mma_commit_pair(bar(C::kKEmpty + st));
-        return true;
-      };
+      constexpr uint32_t idesc = ptx::idesc_bf16(256, 128, 0);
+      const uint32_t elected = ptx::elect_one();
+      uint32_t useq = 0;  // units with tiles so far
+      Phases<C::kS> k_full, s_free;
       for (int u = pair; u < units && !wt.failed; u += pairs) {
-        const Unit x = unit_at(a, u, pieces);
-        const int tiles = x.p.tiles;
+        const int tiles = unit_at(a, u, pieces).p.tiles;
         if (!tiles) continue;
         if (!wt.all(bar(C::kQFull), useq & 1u)) break;
-        ptx::tc_fence_after();
-        for (int j = 0; j < C::kS && j < tiles; ++j)
-          if (!issue_qk(it0 + j)) break;
-        if (tiles <= C::kS) ptx::mma_commit_pair(bar(C::kQEmpty));
-        for (int j = 0; j < tiles && !wt.failed; ++j) {
-          const uint32_t it = it0 + j, sb = it % C::kS, st = it % C::kKv;
-          // The unit before must have read its output before this one's first PV replaces it.
-          if (j == 0 && useq > 0 && !wt.all(bar(C::kOFree), (useq - 1) & 1u)) break;
-          if (!wt.all(bar(C::kVFull + st), (it / C::kKv) & 1u)) break;
-          if (!wt.all(bar(C::kPFull + sb), (it / C::kS) & 1u)) break;
-          ptx::tc_fence_after();
-          // V as B, MN-major: 64 value columns are a chunk of [128 keys][128 B], 8-key groups 1 KB
-          // apart; a step of 16 keys is 2 KB.
-          const uint64_t vd = ptx::smem_desc(base + C::kSmV + st * C::kVBytes, 16384, 1024, 2);
+        for (int j0 = 0; j0 < tiles && !wt.failed; j0 += C::kS) {
+          // Stage and score buffer `st` are constants in each copy of the body, and so are the MMA
+          // operands.
 #pragma unroll
-          for (int k = 0; k < kRowTile / 16; ++k)
-            ptx::mma_ts_pair(tmem + C::kTmemO, tmem + sb * 128 + k * 8, vd + uint64_t(k * 128),
-                             idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
-          ptx::mma_commit_pair(bar(C::kVEmpty + st));
-          ptx::mma_commit_pair(bar(C::kPvDone + sb));
-          if (j + C::kS < tiles) {
-            if (!issue_qk(it + C::kS)) break;
-            if (j + C::kS + 1 == tiles) ptx::mma_commit_pair(bar(C::kQEmpty));
+          for (int st = 0; st < C::kS; ++st) {
+            const int j = j0 + st;
+            if (j >= tiles || wt.failed) break;
+            if (!wt.all(bar(C::kKFull + st), k_full.take(st))) break;
+            if (!wt.all(bar(C::kPvDone + st), s_free.take(st) ^ 1u)) break;
+            ptx::tc_fence_after();
+            const uint64_t qd = ptx::smem_desc(base, 16, 1024, 2);
+            const uint64_t kd = ptx::smem_desc(base + C::kSmK + st * C::kKBytes, 16, 1024, 2);
+            if constexpr (kDq == 192)
+              ptx::mma_ss_pair_x12(elected, st * 128, qd, kd, idesc, 0u);
+            else
+              ptx::mma_ss_pair_x16(elected, st * 128, qd, kd, idesc, 0u);
+            ptx::mma_commit_pair(bar(C::kSFull + st));
+            ptx::mma_commit_pair(bar(C::kKEmpty + st));
           }
         }
-        it0 += uint32_t(tiles);
+        ptx::mma_commit_pair(bar(C::kQEmpty));
+        ++useq;
+      }
+      ptx::mma_commit_pair(bar(C::kDrain));
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    ptx::registers_down<96>();
+    if (rank == 0) {
+      constexpr uint32_t idesc = ptx::idesc_bf16(256, kDv, 1);
+      const uint32_t elected = ptx::elect_one();
+      uint32_t useq = 0;
+      Phases<C::kS> v_full, p_full;
+      for (int u = pair; u < units && !wt.failed; u += pairs) {
+        const int tiles = unit_at(a, u, pieces).p.tiles;
+        if (!tiles) continue;
+        // The unit before must have read its output before this one's first PV replaces it.
+        if (useq > 0 && !wt.all(bar(C::kOFree), (useq - 1) & 1u)) break;
+        for (int j0 = 0; j0 < tiles && !wt.failed; j0 += C::kS) {
+#pragma unroll
+          for (int st = 0; st < C::kS; ++st) {
+            const int j = j0 + st;
+            if (j >= tiles || wt.failed) break;
+            if (!wt.all(bar(C::kVFull + st), v_full.take(st))) break;
+            if (!wt.all(bar(C::kPFull + st), p_full.take(st))) break;
+            ptx::tc_fence_after();
+            // V as B, MN-major: 64 value columns are a chunk of [128 keys][128 B], 8-key groups
+            // 1 KB apart; a step of 16 keys is 2 KB.
+            const uint64_t vd = ptx::smem_desc(base + C::kSmV + st * C::kVBytes, 16384, 1024, 2);
+            ptx::mma_ts_pair_x8(elected, C::kTmemO, st * 128, vd, idesc, j > 0 ? 1u : 0u);
+            ptx::mma_commit_pair(bar(C::kVEmpty + st));
+            ptx::mma_commit_pair(bar(C::kPvDone + st));
+          }
+        }
         ++useq;
       }
       ptx::mma_commit_pair(bar(C::kDrain));
@@ -785,13 +822,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::registers_down<96>();
   } else {
     ptx::registers_up<200>();
-    const int half = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
+    const int group = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = uint32_t(quad * 32) << 16;
-    float* exch = reinterpret_cast<float*>(sm + C::kSmExch);
-    const bool marked = a.w.header[kHdrMarked] != 0;
+    float* shared_m = reinterpret_cast<float*>(sm + C::kSmExch);  // [128]
+    float* shared_sum = shared_m + 128;                           // [2][128]
     const float c = a.scale_log2, slack = kSlack / c;
-    const uint64_t c2 = ptx::pack_f32x2(c, c);
-    uint32_t it = 0;
+    uint32_t it0 = 0;  // tiles of earlier units
+    Phases<C::kS> s_full, pv_done;
     // A wait that ran out is not left for: the two warps of a row go through the same barriers to
     // the end, over whatever TMEM holds; the error flag is set.
     for (int u = pair; u < units; u += pairs) {
@@ -803,118 +840,115 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int keys = a.w.seq_keys[x.p.seq], pos = a.q_pos[t];
         n = pos >= keys ? keys : max(pos + 1, 0);
       }
-      float m = -INFINITY;
-      uint64_t sum0 = 0, sum1 = 0;  // pairs of f32 partial sums
-      for (int j = 0; j < x.p.tiles; ++j, ++it) {
-        const uint32_t sb = it % C::kS;
-        wt.all(bar(C::kSFull + sb), (it / C::kS) & 1u);
+      float m = -INFINITY;           // what this thread's sum is taken against
+      float sum[2][2] = {};          // partial sums over this thread's tiles
+      const int odd = int((it0 ^ uint32_t(group)) & 1u);  // the unit's first tile of this group
+      for (int j = odd; j < x.p.tiles; j += 2) {
+        const uint32_t it = it0 + uint32_t(j), sb = uint32_t(j % C::kS);
+        wt.all(bar(C::kSFull + sb), s_full.at(sb, j / C::kS));
         ptx::tc_fence_after();
-        float s[64];
-        const uint32_t src = tmem + sb * 128 + half * 64 + lanes;
-        {
-          uint32_t lo[32], hi[32];
-          ptx::tmem_ld32(src, lo);
-          ptx::tmem_ld32(src + 32, hi);
-          ptx::tmem_wait_ld();
+        const uint32_t src = tmem + sb * 128 + lanes;
+        const int key = (x.p.tile0 + j) * kRowTile;
+        uint32_t r[4][32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            s[i] = __uint_as_float(lo[i]);
-            s[32 + i] = __uint_as_float(hi[i]);
-          }
-        }
-        const int key = (x.p.tile0 + j) * kRowTile + half * 64;
-        if (!__all_sync(0xFFFFFFFFu, n >= key + 64)) {
+        for (int g = 0; g < 4; ++g) ptx::tmem_ld32(src + 32 * g, r[g]);
+        ptx::tmem_wait_ld();
+        if (!__all_sync(0xFFFFFFFFu, n >= key + kRowTile)) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (key + i >= n) s[i] = -INFINITY;
-        }
-        if (marked) {
-          const uint8_t* mk = a.w.marked + x.p.key0 + key;
-          const uint32_t bits[2] = {__ballot_sync(0xFFFFFFFFu, mk[lane] != 0),
-                                    __ballot_sync(0xFFFFFFFFu, mk[32 + lane] != 0)};
-          if (bits[0] | bits[1]) {
+          for (int g = 0; g < 4; ++g)
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (((bits[i >> 5] >> (i & 31)) & 1u) && key + i < n) s[i] = NAN;
-          }
+            for (int i = 0; i < 32; ++i)
+              if (key + 32 * g + i >= n) r[g][i] = 0xFF800000u;  // -inf
         }
-        float top = s[0], top1 = s[32];
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 1; i < 32; ++i) {
-          top = fmaxf(top, s[i]);
-          top1 = fmaxf(top1, s[32 + i]);
-        }
-        top = fmaxf(top, top1);
-        float* ex = exch + (it & 1u) * 256;
-        ex[half * 128 + row] = top;
-        ptx::named_barrier(1 + quad, 64);
-        top = fmaxf(top, ex[(half ^ 1) * 128 + row]);
-        if (j == 0) {
-          m = top;
-        } else {
-          const bool grow = top > m + slack;
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              top[k] = fmaxf(fmaxf(top[k], __uint_as_float(r[g][i + k])),
+                             __uint_as_float(r[g][i + 4 + k]));
+        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        // The turn passes from tile to tile, and so from group to group, with the row's reference
+        // maximum: one group at a time is in its exponentials.
+        if (it > 0) ptx::named_barrier(1 + quad + 4 * int(it & 1u), 64);
+        float ref = j == 0 ? high : shared_m[row];
+        if (j > 0) {
+          const bool grow = high > ref + slack;
           if (__any_sync(0xFFFFFFFFu, grow)) {
-            const float keep = !grow ? 1.f : m == -INFINITY ? 0.f : ptx::ex2((m - top) * c);
-            if (grow) m = top;
-            const uint64_t keep2 = ptx::pack_f32x2(keep, keep), zero = 0;
-            sum0 = ptx::fma_f32x2(sum0, keep2, zero);
-            sum1 = ptx::fma_f32x2(sum1, keep2, zero);
-            wt.all(bar(C::kPvDone + (it - 1) % C::kS), ((it - 1) / C::kS) & 1u);
+            const float keep =
+                !grow ? 1.f : ref == -INFINITY ? 0.f : ptx::ex2((ref - high) * c);
+            if (grow) ref = high;
+            const int b = j - 1;
+            wt.all(bar(C::kPvDone + b % C::kS), pv_done.at(b % C::kS, b / C::kS));
             ptx::tc_fence_after();
-            const uint32_t o = tmem + C::kTmemO + half * (kDv / 2) + lanes;
-            for (int i = 0; i < kDv / 2; i += 32) {
-              uint32_t v[32];
-              ptx::tmem_ld32(o + i, v);
+            const uint32_t o = tmem + C::kTmemO + lanes;
+            for (int i = 0; i < kDv; i += 16) {
+              uint32_t v[16];
+              ptx::tmem_ld16(o + i, v);
               ptx::tmem_wait_ld();
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * keep);
-              ptx::tmem_st32(o + i, v);
+              for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * keep);
+              ptx::tmem_st16(o + i, v);
             }
           }
         }
-        const float mc = m == -INFINITY ? 0.f : -m * c;
-        const uint64_t mc2 = ptx::pack_f32x2(mc, mc);
-        uint32_t p[32];
-#pragma unroll
-        for (int i = 0; i < 64; i += 2) {
-          float p0, p1;
-          ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(s[i], s[i + 1]), c2, mc2), p0, p1);
-          p0 = ptx::ex2(p0);
-          p1 = ptx::ex2(p1);
-          if (i & 2)
-            sum1 = ptx::add_f32x2(sum1, ptx::pack_f32x2(p0, p1));
-          else
-            sum0 = ptx::add_f32x2(sum0, ptx::pack_f32x2(p0, p1));
-          p[i / 2] = ptx::pack_bf16x2(p0, p1);
+        shared_m[row] = ref;
+        if (__any_sync(0xFFFFFFFFu, ref != m)) {
+          const float keep = m == ref ? 1.f : m == -INFINITY ? 0.f : ptx::ex2((m - ref) * c);
+          sum[0][0] *= keep;
+          sum[0][1] *= keep;
+          sum[1][0] *= keep;
+          sum[1][1] *= keep;
+          m = ref;
         }
-        ptx::tmem_st32(tmem + sb * 128 + half * 32 + lanes, p);
+        const float mc = ref == -INFINITY ? 0.f : -ref * c;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float p0 = ptx::ex2(fmaf(__uint_as_float(r[g][i]), c, mc));
+            const float p1 = ptx::ex2(fmaf(__uint_as_float(r[g][i + 1]), c, mc));
+            sum[(i >> 1) & 1][0] += p0;
+            sum[(i >> 1) & 1][1] += p1;
+            p[i / 2] = ptx::pack_bf16x2(p0, p1);
+          }
+          ptx::tmem_st16(src + 16 * g, p);  // over the scores
+          if (g == kTurn) ptx::named_barrier_arrive(1 + quad + 4 * int((it + 1) & 1u), 64);
+        }
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive_cluster_relaxed(lead(C::kPFull + sb));
       }
-      // The row's whole sum, then O / sum to the output: this thread's half of the columns.
-      float sum, odd;
-      ptx::unpack_f32x2(ptx::add_f32x2(sum0, sum1), sum, odd);
-      sum += odd;
-      float* ex = exch + (it & 1u) * 256;
-      ex[half * 128 + row] = sum;
-      ptx::named_barrier(1 + quad, 64);
-      sum += ex[(half ^ 1) * 128 + row];
-      // Both have read before either writes its next maximum there (two tiles on at the earliest,
-      // or at once when the next unit has no tiles).
-      ptx::named_barrier(1 + quad, 64);
+      it0 += uint32_t(x.p.tiles);
+      const int last = x.p.tiles - 1;
+      const uint32_t last_phase = last >= 0 ? pv_done.at(last % C::kS, last / C::kS) : 0u;
+      s_full.pass(x.p.tiles);
+      pv_done.pass(x.p.tiles);
+      // The row's last reference maximum and its whole sum, then O / sum to the output: this
+      // thread's half of the columns.
+      ptx::named_barrier(9 + quad, 64);
+      const float ref = x.p.tiles ? shared_m[row] : -INFINITY;
+      float total = (sum[0][0] + sum[0][1]) + (sum[1][0] + sum[1][1]);
+      if (m != ref) total = m == -INFINITY ? 0.f : total * ptx::ex2((m - ref) * c);
+      shared_sum[group * 128 + row] = total;
+      ptx::named_barrier(9 + quad, 64);
+      total = shared_sum[row] + shared_sum[128 + row];
+      if (n > a.w.seq_spoilt[x.p.seq]) total = NAN;
       const bool sees = n > x.p.tile0 * kRowTile;  // in this piece
-      const float inv = sees ? 1.f / sum : 0.f;
+      const float inv = sees ? 1.f / total : 0.f;
       if (x.p.tiles) {
-        wt.all(bar(C::kPvDone + (it - 1) % C::kS), ((it - 1) / C::kS) & 1u);
+        wt.all(bar(C::kPvDone + last % C::kS), last_phase);
         ptx::tc_fence_after();
       }
       const int head = a.head0 + x.head;
       const long long part = (long long)u * kQueryTile + rank * 128 + row;
       uint8_t* out = x.p.whole ? a.out + (long long)t * a.out_st + (long long)head * a.out_sh
                                : reinterpret_cast<uint8_t*>(a.w.part_out + part * kDv);
-      const uint32_t o = tmem + C::kTmemO + half * (kDv / 2) + lanes;
+      const uint32_t o = tmem + C::kTmemO + group * (kDv / 2) + lanes;
 #pragma unroll
       for (int i = 0; i < kDv / 2; i += 32) {
         uint32_t v[32];
@@ -923,7 +957,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ptx::tmem_wait_ld();
         }
         if (mine) {
-          const int col = half * (kDv / 2) + i;
+          const int col = group * (kDv / 2) + i;
 #pragma unroll
           for (int k = 0; k < 32; ++k)
             v[k] = sees ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
@@ -948,8 +982,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive_cluster_relaxed(lead(C::kOFree));
       }
-      if (mine && half == 0) {
-        const float l2 = sees ? m * c + log2f(sum) : -INFINITY;
+      if (mine && group == 0) {
+        const float l2 = sees ? ref * c + log2f(total) : -INFINITY;
         if (!x.p.whole)
           a.w.part_lse[part] = l2;
         else if (a.lse)
@@ -957,7 +991,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
   }
-  wt.on(bar(C::kDrain), 0);
+  if (warp == 0) wt.on(bar(C::kDrain), 0);
   wt.settle();
   ptx::tc_fence_before();
   ptx::cluster_sync();
@@ -1025,7 +1059,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
 
 // ------------------------------------------------------------------------------ host
 struct Layout {
-  uint64_t header, seq_key0, seq_keys, seq_block, blocks, pieces, part_out, part_lse, marked, rows, rope, k, v, total;
+  uint64_t header, seq_key0, seq_keys, seq_block, seq_spoilt, blocks, pieces, part_out, part_lse, rows, rope, k, v, total;
   uint64_t cap, max_blocks, pass_heads, split_units;
 };
 
@@ -1057,11 +1091,11 @@ Layout layout_of(const TqMlaChunkSpec& s) {
   l.seq_key0 = take((S + 1) * 4);
   l.seq_keys = take((S + 1) * 4);
   l.seq_block = take((S + 1) * 4);
+  l.seq_spoilt = take((S + 1) * 4);
   l.blocks = take(l.max_blocks * sizeof(Block));
   l.pieces = take((l.max_blocks + l.split_units) * sizeof(Piece));
   l.part_out = take(l.split_units * kQueryTile * dv * 4);
   l.part_lse = take(l.split_units * kQueryTile * 4);
-  l.marked = take(l.cap);
   l.rows = take(l.cap * kLatent * 2);
   l.rope = take(l.cap * kRopeDim * 2);
   l.k = take(l.pass_heads * l.cap * dn * 2);
@@ -1164,11 +1198,11 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
   a.w.seq_key0 = reinterpret_cast<int*>(ws + l.seq_key0);
   a.w.seq_keys = reinterpret_cast<int*>(ws + l.seq_keys);
   a.w.seq_block = reinterpret_cast<int*>(ws + l.seq_block);
+  a.w.seq_spoilt = reinterpret_cast<int*>(ws + l.seq_spoilt);
   a.w.blocks = reinterpret_cast<Block*>(ws + l.blocks);
   a.w.pieces = reinterpret_cast<Piece*>(ws + l.pieces);
   a.w.part_out = reinterpret_cast<float*>(ws + l.part_out);
   a.w.part_lse = reinterpret_cast<float*>(ws + l.part_lse);
-  a.w.marked = ws + l.marked;
   a.w.rows = reinterpret_cast<uint16_t*>(ws + l.rows);
   a.w.rope = reinterpret_cast<uint16_t*>(ws + l.rope);
   a.w.k = reinterpret_cast<uint16_t*>(ws + l.k);

@@ -64,6 +64,12 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 __device__ __forceinline__ long long ld_cluster_s64(uint32_t addr) {
   long long v;
   asm volatile("ld.shared::cluster.s64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
@@ -132,6 +138,19 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+
+// A test that may suspend the thread until the phase completes or a time that the hardware sets runs
+// out. A suspended waiter issues nothing; a spinning one keeps the queue busy that shared-memory
+// and special-function instructions of the other warps go through.
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
@@ -348,24 +367,80 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols
                : "memory");
 }
 
-__device__ __forceinline__ void mma_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                            uint32_t idesc, uint32_t accumulate) {
+// One lane of a converged warp, the same one every time: 1 there, 0 elsewhere. The MMA wrappers below
+// take it, so that a run of MMAs elects once.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e;
 }
 
-__device__ __forceinline__ void mma_ts_pair(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                            uint32_t idesc, uint32_t accumulate) {
+// Runs of MMAs of a pair as one instruction sequence, K = 16 a step: one predicate for the elected
+// lane, descriptors advanced in place (the high half of a shared-memory descriptor does not change
+// while its 14-bit address field does not carry). Issued one by one, with their own predicate and
+// 64-bit descriptors, they took 80 to 95 cycles each; an M = 256, N = 128 step executes in 64.
+#define TQ_MMA_SS_STEP(A, B, ACC)                                    \
+  "add.u32 al, %1, " #A ";\n\tmov.b64 ad, {al, %2};\n\t"            \
+  "add.u32 bl, %3, " #B ";\n\tmov.b64 bd, {bl, %4};\n\t"            \
+  "@e tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %5, " #ACC ";\n\t"
+// Four steps of one 64-value chunk (32 bytes apart inside the 128-byte swizzle).
+#define TQ_MMA_SS_CHUNK(A0, A1, A2, A3, B0, B1, B2, B3, FIRST)       \
+  TQ_MMA_SS_STEP(A0, B0, FIRST) TQ_MMA_SS_STEP(A1, B1, t)            \
+  TQ_MMA_SS_STEP(A2, B2, t) TQ_MMA_SS_STEP(A3, B3, t)
+#define TQ_MMA_SS_BEGIN                                              \
+  "{\n\t.reg .pred e, f, t;\n\t.reg .b32 al, bl;\n\t.reg .b64 ad, bd;\n\t" \
+  "setp.ne.b32 e, %6, 0;\n\tsetp.ne.b32 f, %7, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+#define TQ_MMA_SS_ARGS                                               \
+  :: "r"(d_tmem), "r"(uint32_t(a_desc)), "r"(uint32_t(a_desc >> 32)),  \
+     "r"(uint32_t(b_desc)), "r"(uint32_t(b_desc >> 32)), "r"(idesc), "r"(elected), "r"(accumulate)
+
+// One chunk of 64: both operands advance 2 descriptor units (32 bytes) a step.
+__device__ __forceinline__ void mma_ss_pair_x4(uint32_t elected, uint32_t d_tmem, uint64_t a_desc,
+                                               uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(TQ_MMA_SS_BEGIN TQ_MMA_SS_CHUNK(0, 2, 4, 6, 0, 2, 4, 6, f) "}"
+               TQ_MMA_SS_ARGS : "memory");
+}
+// Three or four chunks: A's chunks are 16 KB apart (128 rows), B's 8 KB (64 rows).
+__device__ __forceinline__ void mma_ss_pair_x12(uint32_t elected, uint32_t d_tmem, uint64_t a_desc,
+                                                uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(TQ_MMA_SS_BEGIN
+               TQ_MMA_SS_CHUNK(0, 2, 4, 6, 0, 2, 4, 6, f)
+               TQ_MMA_SS_CHUNK(0x400, 0x402, 0x404, 0x406, 0x200, 0x202, 0x204, 0x206, t)
+               TQ_MMA_SS_CHUNK(0x800, 0x802, 0x804, 0x806, 0x400, 0x402, 0x404, 0x406, t) "}"
+               TQ_MMA_SS_ARGS : "memory");
+}
+__device__ __forceinline__ void mma_ss_pair_x16(uint32_t elected, uint32_t d_tmem, uint64_t a_desc,
+                                                uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(TQ_MMA_SS_BEGIN
+               TQ_MMA_SS_CHUNK(0, 2, 4, 6, 0, 2, 4, 6, f)
+               TQ_MMA_SS_CHUNK(0x400, 0x402, 0x404, 0x406, 0x200, 0x202, 0x204, 0x206, t)
+               TQ_MMA_SS_CHUNK(0x800, 0x802, 0x804, 0x806, 0x400, 0x402, 0x404, 0x406, t)
+               TQ_MMA_SS_CHUNK(0xC00, 0xC02, 0xC04, 0xC06, 0x600, 0x602, 0x604, 0x606, t) "}"
+               TQ_MMA_SS_ARGS : "memory");
+}
+// Eight steps with A in TMEM (8 columns a step) and B advancing 128 descriptor units (2 KB).
+#define TQ_MMA_TS_STEP(A, B, ACC)                                    \
+  "add.u32 al, %1, " #A ";\n\tadd.u32 bl, %2, " #B ";\n\tmov.b64 bd, {bl, %3};\n\t" \
+  "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [al], bd, %4, " #ACC ";\n\t"
+__device__ __forceinline__ void mma_ts_pair_x8(uint32_t elected, uint32_t d_tmem, uint32_t a_tmem,
+                                               uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      :: "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+      "{\n\t.reg .pred e, f, t;\n\t.reg .b32 al, bl;\n\t.reg .b64 bd;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\tsetp.ne.b32 f, %6, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      TQ_MMA_TS_STEP(0, 0, f) TQ_MMA_TS_STEP(8, 128, t) TQ_MMA_TS_STEP(16, 256, t)
+      TQ_MMA_TS_STEP(24, 384, t) TQ_MMA_TS_STEP(32, 512, t) TQ_MMA_TS_STEP(40, 640, t)
+      TQ_MMA_TS_STEP(48, 768, t) TQ_MMA_TS_STEP(56, 896, t) "}"
+      :: "r"(d_tmem), "r"(a_tmem), "r"(uint32_t(b_desc)), "r"(uint32_t(b_desc >> 32)), "r"(idesc),
+         "r"(elected), "r"(accumulate)
+      : "memory");
 }
 
 // Arrive once on the mbarrier at the same offset in both CTAs when all prior MMAs are complete.
@@ -403,6 +478,10 @@ __device__ __forceinline__ void st_global_v8(void* p, const uint32_t* r) {
                :: "l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
                   "r"(r[6]), "r"(r[7])
                : "memory");
+}
+
+__device__ __forceinline__ void named_barrier_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" :: "r"(id), "r"(threads) : "memory");
 }
 
 __device__ __forceinline__ void named_barrier(int id, int threads) {
