@@ -579,12 +579,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // it loads half: 64 of a tile's keys for QK^T, half the value columns for PV. So a pair moves
 // K_j and V_j once for 256 queries, and the shared memory left holds several tiles ahead.
 //   warp 0      TMA loads of this CTA's halves; their bytes complete on the leader's barriers
-//   warps 1, 2  (leader) the MMAs of QK^T and of PV, a warp each, so that the waits of one run
-//               under the MMAs of the other (one warp for both left the tensor cores idle half of
-//               the time). S_j has kS buffers in TMEM; P_j lies in S_j's columns, so S_{j+kS}
-//               waits for PV_j. A softmax warp may be several tiles ahead of PV, so the
-//               completion of PV_j has a barrier per buffer: a waiter has seen S_j, which lies
-//               behind PV_{j-kS}, and its phase is the next.
+//   warp 1      (leader) all MMAs. S_j has kS buffers in TMEM: S_{j+kS} is issued right after
+//               PV_j, whose P_j lies in the same columns; MMAs run in issue order. PV_j starts
+//               on the first 64 keys while the other half's exponentials run. A softmax warp may
+//               be several tiles ahead of PV, so the completion of PV_j has a barrier per buffer:
+//               a waiter has seen S_j, which lies behind PV_{j-kS}, and its phase is the next.
 //   warps 4-11  softmax: two groups of four warps take the tiles in turn, a thread a row, so that
 //               one group's exponentials run under the other's loads, maxima and waits (both
 //               groups on each tile's halves in step took 2990 cycles a tile, of them 1350 in the
@@ -600,7 +599,7 @@ namespace attend {
 
 constexpr int kThreads = 384;
 constexpr float kSlack = 8.f;  // log2 units
-constexpr int kTurn = 1;       // quarter of a tile's exponentials after which the turn passes
+constexpr int kTurn = 0;       // quarter of a tile's exponentials after which the turn passes
 
 template <int kDq, int kDv>
 struct Shape {
@@ -618,7 +617,7 @@ struct Shape {
   static constexpr int kQFull = 0, kQEmpty = 1, kKFull = 2, kKEmpty = kKFull + kKv;
   static constexpr int kVFull = kKEmpty + kKv, kVEmpty = kVFull + kKv;
   static constexpr int kSFull = kVEmpty + kKv, kPFull = kSFull + kS;
-  static constexpr int kPvDone = kPFull + kS, kOFree = kPvDone + kS, kDrain = kOFree + 1;
+  static constexpr int kPvDone = kPFull + 2 * kS, kOFree = kPvDone + kS, kDrain = kOFree + 1;
   static constexpr int kBars = kDrain + 1;
   static constexpr uint32_t kSmMisc = kSmBars + 8 * kBars;
   static constexpr uint32_t kSmBytes = kSmMisc + 16 + 1024;
@@ -683,10 +682,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sm + C::kSmMisc);
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kBars; ++i) {
-      // P of a tile: its group's four warps in either CTA; the release of O: all softmax warps; the
-      // end: both MMA warps.
-      const bool joint = i >= C::kPFull && i < C::kPFull + C::kS;
-      ptx::mbar_init(bar(i), joint ? 8 : i == C::kOFree ? 16 : i == C::kDrain ? 2 : 1);
+      // P of half a tile: its group's four warps in either CTA; the release of O: all softmax warps.
+      const bool joint = i >= C::kPFull && i < C::kPFull + 2 * C::kS;
+      ptx::mbar_init(bar(i), joint ? 8 : i == C::kOFree ? 16 : 1);
     }
     tmem_holder[1] = 0;  // the abort word
     ptx::fence_mbar_init_cluster();
@@ -751,50 +749,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     ptx::registers_down<96>();
     if (rank == 0) {
-      constexpr uint32_t idesc = ptx::idesc_bf16(256, 128, 0);
+      constexpr uint32_t idesc_qk = ptx::idesc_bf16(256, 128, 0);
+      constexpr uint32_t idesc_pv = ptx::idesc_bf16(256, kDv, 1);
       const uint32_t elected = ptx::elect_one();
       uint32_t useq = 0;  // units with tiles so far
-      Phases<C::kS> k_full, s_free;
+      Phases<C::kS> k_full, v_full, p_full;
+      // The tile in stage and score buffer `st`, a constant in every call: the MMA operands are
+      // then constants too.
+      auto issue_qk = [&](uint32_t st) -> bool {
+        if (!wt.all(bar(C::kKFull + st), k_full.take(st))) return false;
+        ptx::tc_fence_after();
+        const uint64_t qd = ptx::smem_desc(base, 16, 1024, 2);
+        const uint64_t kd = ptx::smem_desc(base + C::kSmK + st * C::kKBytes, 16, 1024, 2);
+        if constexpr (kDq == 192)
+          ptx::mma_ss_pair_x12(elected, st * 128, qd, kd, idesc_qk, 0u);
+        else
+          ptx::mma_ss_pair_x16(elected, st * 128, qd, kd, idesc_qk, 0u);
+        ptx::mma_commit_pair(bar(C::kSFull + st));
+        ptx::mma_commit_pair(bar(C::kKEmpty + st));
+        return true;
+      };
       for (int u = pair; u < units && !wt.failed; u += pairs) {
         const int tiles = unit_at(a, u, pieces).p.tiles;
         if (!tiles) continue;
         if (!wt.all(bar(C::kQFull), useq & 1u)) break;
-        for (int j0 = 0; j0 < tiles && !wt.failed; j0 += C::kS) {
-          // Stage and score buffer `st` are constants in each copy of the body, and so are the MMA
-          // operands.
 #pragma unroll
-          for (int st = 0; st < C::kS; ++st) {
-            const int j = j0 + st;
-            if (j >= tiles || wt.failed) break;
-            if (!wt.all(bar(C::kKFull + st), k_full.take(st))) break;
-            if (!wt.all(bar(C::kPvDone + st), s_free.take(st) ^ 1u)) break;
-            ptx::tc_fence_after();
-            const uint64_t qd = ptx::smem_desc(base, 16, 1024, 2);
-            const uint64_t kd = ptx::smem_desc(base + C::kSmK + st * C::kKBytes, 16, 1024, 2);
-            if constexpr (kDq == 192)
-              ptx::mma_ss_pair_x12(elected, st * 128, qd, kd, idesc, 0u);
-            else
-              ptx::mma_ss_pair_x16(elected, st * 128, qd, kd, idesc, 0u);
-            ptx::mma_commit_pair(bar(C::kSFull + st));
-            ptx::mma_commit_pair(bar(C::kKEmpty + st));
-          }
-        }
-        ptx::mma_commit_pair(bar(C::kQEmpty));
-        ++useq;
-      }
-      ptx::mma_commit_pair(bar(C::kDrain));
-    }
-    __syncwarp();
-  } else if (warp == 2) {
-    ptx::registers_down<96>();
-    if (rank == 0) {
-      constexpr uint32_t idesc = ptx::idesc_bf16(256, kDv, 1);
-      const uint32_t elected = ptx::elect_one();
-      uint32_t useq = 0;
-      Phases<C::kS> v_full, p_full;
-      for (int u = pair; u < units && !wt.failed; u += pairs) {
-        const int tiles = unit_at(a, u, pieces).p.tiles;
-        if (!tiles) continue;
+        for (int j = 0; j < C::kS; ++j)
+          if (j < tiles && !wt.failed) issue_qk(j);
+        if (tiles <= C::kS) ptx::mma_commit_pair(bar(C::kQEmpty));
         // The unit before must have read its output before this one's first PV replaces it.
         if (useq > 0 && !wt.all(bar(C::kOFree), (useq - 1) & 1u)) break;
         for (int j0 = 0; j0 < tiles && !wt.failed; j0 += C::kS) {
@@ -803,14 +785,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int j = j0 + st;
             if (j >= tiles || wt.failed) break;
             if (!wt.all(bar(C::kVFull + st), v_full.take(st))) break;
-            if (!wt.all(bar(C::kPFull + st), p_full.take(st))) break;
-            ptx::tc_fence_after();
             // V as B, MN-major: 64 value columns are a chunk of [128 keys][128 B], 8-key groups
-            // 1 KB apart; a step of 16 keys is 2 KB.
+            // 1 KB apart; a step of 16 keys is 2 KB. The first 64 keys go ahead of the rest.
             const uint64_t vd = ptx::smem_desc(base + C::kSmV + st * C::kVBytes, 16384, 1024, 2);
-            ptx::mma_ts_pair_x8(elected, C::kTmemO, st * 128, vd, idesc, j > 0 ? 1u : 0u);
+            const uint32_t phase = p_full.take(st);
+            if (!wt.all(bar(C::kPFull + 2 * st), phase)) break;
+            ptx::tc_fence_after();
+            ptx::mma_ts_pair_x4(elected, C::kTmemO, st * 128, vd, idesc_pv, j > 0 ? 1u : 0u);
+            if (!wt.all(bar(C::kPFull + 2 * st + 1), phase)) break;
+            ptx::tc_fence_after();
+            ptx::mma_ts_pair_x4(elected, C::kTmemO, st * 128 + 32, vd + 512, idesc_pv, 1u);
             ptx::mma_commit_pair(bar(C::kVEmpty + st));
             ptx::mma_commit_pair(bar(C::kPvDone + st));
+            if (j + C::kS < tiles) {
+              if (!issue_qk(st)) break;
+              if (j + C::kS + 1 == tiles) ptx::mma_commit_pair(bar(C::kQEmpty));
+            }
           }
         }
         ++useq;
@@ -917,11 +907,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
           ptx::tmem_st16(src + 16 * g, p);  // over the scores
           if (g == kTurn) ptx::named_barrier_arrive(1 + quad + 4 * int((it + 1) & 1u), 64);
+          if (g & 1) {
+            ptx::tmem_wait_st();
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+              ptx::mbar_arrive_cluster_relaxed(lead(C::kPFull + 2 * int(sb) + (g >> 1)));
+          }
         }
-        ptx::tmem_wait_st();
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive_cluster_relaxed(lead(C::kPFull + sb));
       }
       it0 += uint32_t(x.p.tiles);
       const int last = x.p.tiles - 1;

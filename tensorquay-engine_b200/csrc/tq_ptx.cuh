@@ -425,19 +425,18 @@ __device__ __forceinline__ void mma_ss_pair_x16(uint32_t elected, uint32_t d_tme
                TQ_MMA_SS_CHUNK(0xC00, 0xC02, 0xC04, 0xC06, 0x600, 0x602, 0x604, 0x606, t) "}"
                TQ_MMA_SS_ARGS : "memory");
 }
-// Eight steps with A in TMEM (8 columns a step) and B advancing 128 descriptor units (2 KB).
+// Four steps with A in TMEM (8 columns a step) and B advancing 128 descriptor units (2 KB).
 #define TQ_MMA_TS_STEP(A, B, ACC)                                    \
   "add.u32 al, %1, " #A ";\n\tadd.u32 bl, %2, " #B ";\n\tmov.b64 bd, {bl, %3};\n\t" \
   "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [al], bd, %4, " #ACC ";\n\t"
-__device__ __forceinline__ void mma_ts_pair_x8(uint32_t elected, uint32_t d_tmem, uint32_t a_tmem,
+__device__ __forceinline__ void mma_ts_pair_x4(uint32_t elected, uint32_t d_tmem, uint32_t a_tmem,
                                                uint64_t b_desc, uint32_t idesc,
                                                uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred e, f, t;\n\t.reg .b32 al, bl;\n\t.reg .b64 bd;\n\t"
       "setp.ne.b32 e, %5, 0;\n\tsetp.ne.b32 f, %6, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
       TQ_MMA_TS_STEP(0, 0, f) TQ_MMA_TS_STEP(8, 128, t) TQ_MMA_TS_STEP(16, 256, t)
-      TQ_MMA_TS_STEP(24, 384, t) TQ_MMA_TS_STEP(32, 512, t) TQ_MMA_TS_STEP(40, 640, t)
-      TQ_MMA_TS_STEP(48, 768, t) TQ_MMA_TS_STEP(56, 896, t) "}"
+      TQ_MMA_TS_STEP(24, 384, t) "}"
       :: "r"(d_tmem), "r"(a_tmem), "r"(uint32_t(b_desc)), "r"(uint32_t(b_desc >> 32)), "r"(idesc),
          "r"(elected), "r"(accumulate)
       : "memory");
