@@ -578,7 +578,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // Each CTA holds its 128 query rows of S, P and O in TMEM and Q in shared memory; of B operands
 // it loads half: 64 of a tile's keys for QK^T, half the value columns for PV. So a pair moves
 // K_j and V_j once for 256 queries, and the shared memory left holds several tiles ahead.
-//   warp 0      TMA loads of this CTA's halves; their bytes complete on the leader's barriers
+//   warps 0, 2  TMA loads of this CTA's halves of Q and K, and of V; their bytes complete on the
+//               leader's barriers (one warp for all waited for V's stages before K's next one)
+//   warp 3      fetches the next unit's rows for the softmax warps
 //   warp 1      (leader) all MMAs. S_j has kS buffers in TMEM: S_{j+kS} is issued right after
 //               PV_j, whose P_j lies in the same columns; MMAs run in issue order. PV_j starts
 //               on the first 64 keys while the other half's exponentials run. A softmax warp may
@@ -599,7 +601,15 @@ namespace attend {
 
 constexpr int kThreads = 384;
 constexpr float kSlack = 8.f;  // log2 units
-constexpr int kTurn = 0;       // quarter of a tile's exponentials after which the turn passes
+
+// What the softmax warps need of a unit, fetched ahead by warp 3.
+struct Info {
+  int seen[128];  // keys that each of this CTA's query rows sees; kSpoilt: one is not finite
+  int row0, rows, tile0, tiles, head, whole, unused0, unused1;
+};
+constexpr int kSpoilt = 1 << 30;
+// A warp's 32 output rows of 64 bytes, 80 bytes apart (16-byte accesses without bank conflicts).
+constexpr uint32_t kTurnBytes = 32 * 80;
 
 template <int kDq, int kDv>
 struct Shape {
@@ -612,16 +622,24 @@ struct Shape {
   static constexpr uint32_t kVBytes = kVChunks * 128 * 128;
   static constexpr uint32_t kSmK = kQBytes;
   static constexpr uint32_t kSmV = kSmK + kKv * kKBytes;
-  static constexpr uint32_t kSmExch = kSmV + kKv * kVBytes;  // f32 [3][128]
-  static constexpr uint32_t kSmBars = kSmExch + 2048;
+  static constexpr uint32_t kSmExch = kSmV + kKv * kVBytes;  // f32 [3][128], int [4]
+  static constexpr uint32_t kSmInfo = kSmExch + 1552;         // 2 x Info
+  static constexpr uint32_t kSmTurn = kSmInfo + 2 * sizeof(Info);  // output rows, kTurnBytes a warp
+  static constexpr uint32_t kSmBars = kSmTurn + 8 * kTurnBytes;
   static constexpr int kQFull = 0, kQEmpty = 1, kKFull = 2, kKEmpty = kKFull + kKv;
   static constexpr int kVFull = kKEmpty + kKv, kVEmpty = kVFull + kKv;
   static constexpr int kSFull = kVEmpty + kKv, kPFull = kSFull + kS;
   static constexpr int kPvDone = kPFull + 2 * kS, kOFree = kPvDone + kS, kDrain = kOFree + 1;
-  static constexpr int kBars = kDrain + 1;
+  static constexpr int kInfoFull = kDrain + 1, kInfoEmpty = kInfoFull + 2;
+  static constexpr int kBars = kInfoEmpty + 2;
   static constexpr uint32_t kSmMisc = kSmBars + 8 * kBars;
   static constexpr uint32_t kSmBytes = kSmMisc + 16 + 1024;
   static constexpr uint32_t kTmemO = kS * 128;
+  // Quarter of a tile's exponentials after which the turn passes. The earlier, the more the two
+  // groups' exponentials overlap and slow each other; the later, the longer a tile takes. With three
+  // score buffers the first is best (2 x 2048 tokens, 128 heads: 2.05 ms after the first quarter, 2.25
+  // after the third), with two the third (4096 tokens, 64 heads: 703 us, 716 after the first).
+  static constexpr int kTurn = kS == 3 ? 0 : 2;
   static_assert(kSmBytes <= 232448, "shared memory per CTA");
   static_assert(kTmemO + kDv <= 512, "TMEM columns");
 };
@@ -684,9 +702,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int i = 0; i < C::kBars; ++i) {
       // P of half a tile: its group's four warps in either CTA; the release of O: all softmax warps.
       const bool joint = i >= C::kPFull && i < C::kPFull + 2 * C::kS;
-      ptx::mbar_init(bar(i), joint ? 8 : i == C::kOFree ? 16 : 1);
+      const bool read = i >= C::kInfoEmpty;  // eight warps have taken a unit's info
+      ptx::mbar_init(bar(i), joint || read ? 8 : i == C::kOFree ? 16 : 1);
     }
     tmem_holder[1] = 0;  // the abort word
+    for (int i = 0; i < 4; ++i) reinterpret_cast<int*>(sm + C::kSmExch + 1536)[i] = 0;
     ptx::fence_mbar_init_cluster();
     ptx::tma_prefetch_desc(&tm_q);
     ptx::tma_prefetch_desc(&tm_k);
@@ -711,7 +731,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::registers_down<96>();
     if (lane == 0) {
       uint32_t useq = 0;
-      Phases<C::kKv> free;  // of the K and V stages, which are taken together
+      Phases<C::kKv> free;
       for (int u = pair; u < units && !wt.failed; u += pairs) {
         const Unit x = unit_at(a, u, pieces);
         if (!x.p.tiles) continue;
@@ -735,13 +755,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (kRope)
             ptx::tma_load_2d_pair(kd + 2 * 8192, &tm_rope, lead(C::kKFull + st), 0,
                                   key + rank * 64);
-          if (!wt.on(bar(C::kVEmpty + st), ph)) break;
-          if (rank == 0) ptx::mbar_expect_tx(bar(C::kVFull + st), 2 * C::kVBytes);
-          const uint32_t vd = base + C::kSmV + st * C::kVBytes;
-#pragma unroll
-          for (int c = 0; c < C::kVChunks; ++c)
-            ptx::tma_load_3d_pair(vd + c * 16384, &tm_v, lead(C::kVFull + st),
-                                  rank * (kDv / 2) + c * 64, key, x.head);
         }
       }
     }
@@ -808,37 +821,87 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       ptx::mma_commit_pair(bar(C::kDrain));
     }
     __syncwarp();
-  } else if (warp < 4) {
+  } else if (warp == 2) {
     ptx::registers_down<96>();
+    if (lane == 0) {
+      Phases<C::kKv> free;
+      for (int u = pair; u < units && !wt.failed; u += pairs) {
+        const Unit x = unit_at(a, u, pieces);
+        for (int j = 0; j < x.p.tiles; ++j) {
+          const uint32_t st = uint32_t(j % C::kKv), ph = free.take(st) ^ 1u;
+          const int key = x.p.key0 + (x.p.tile0 + j) * kRowTile;
+          if (!wt.on(bar(C::kVEmpty + st), ph)) break;
+          if (rank == 0) ptx::mbar_expect_tx(bar(C::kVFull + st), 2 * C::kVBytes);
+          const uint32_t vd = base + C::kSmV + st * C::kVBytes;
+#pragma unroll
+          for (int c = 0; c < C::kVChunks; ++c)
+            ptx::tma_load_3d_pair(vd + c * 16384, &tm_v, lead(C::kVFull + st),
+                                  rank * (kDv / 2) + c * 64, key, x.head);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    ptx::registers_down<96>();
+    uint32_t n = 0;
+    for (int u = pair; u < units && !wt.failed; u += pairs, ++n) {
+      const Unit x = unit_at(a, u, pieces);
+      const int keys = a.w.seq_keys[x.p.seq], spoilt = a.w.seq_spoilt[x.p.seq];
+      if (!wt.all(bar(C::kInfoEmpty + int(n & 1u)), ((n >> 1) & 1u) ^ 1u)) break;
+      Info* info = reinterpret_cast<Info*>(sm + C::kSmInfo) + (n & 1u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 32 + lane, at = rank * 128 + r;
+        int seen = 0;
+        if (at < x.p.rows) {
+          const int pos = a.q_pos[x.p.row0 + at];
+          seen = pos >= keys ? keys : max(pos + 1, 0);
+          if (seen > spoilt) seen |= kSpoilt;
+        }
+        info->seen[r] = seen;
+      }
+      if (lane == 0) {
+        info->row0 = x.p.row0;
+        info->rows = x.p.rows;
+        info->tile0 = x.p.tile0;
+        info->tiles = x.p.tiles;
+        info->head = x.head;
+        info->whole = x.p.whole;
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(C::kInfoFull + int(n & 1u)));
+    }
+    __syncwarp();
   } else {
     ptx::registers_up<200>();
     const int group = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = uint32_t(quad * 32) << 16;
     float* shared_m = reinterpret_cast<float*>(sm + C::kSmExch);  // [128]
     float* shared_sum = shared_m + 128;                           // [2][128]
+    volatile int* gone = reinterpret_cast<volatile int*>(shared_m + 384);  // [4]
     const float c = a.scale_log2, slack = kSlack / c;
     uint32_t it0 = 0;  // tiles of earlier units
     Phases<C::kS> s_full, pv_done;
-    // A wait that ran out is not left for: the two warps of a row go through the same barriers to
-    // the end, over whatever TMEM holds; the error flag is set.
-    for (int u = pair; u < units; u += pairs) {
-      const Unit x = unit_at(a, u, pieces);
-      const int t = x.p.row0 + rank * 128 + row;
-      const bool mine = rank * 128 + row < x.p.rows;
-      int n = 0;  // keys that this row sees
-      if (mine) {
-        const int keys = a.w.seq_keys[x.p.seq], pos = a.q_pos[t];
-        n = pos >= keys ? keys : max(pos + 1, 0);
-      }
+    uint32_t nth = 0;  // units so far
+    for (int u = pair; u < units; u += pairs, ++nth) {
+      const Info* info = reinterpret_cast<const Info*>(sm + C::kSmInfo) + (nth & 1u);
+      wt.all(bar(C::kInfoFull + int(nth & 1u)), (nth >> 1) & 1u);
+      // A wait that ran out ends the loop here for both warps of a row, and only here: inside a unit
+      // they go through the same barriers to its end, over whatever TMEM holds.
+      if (wt.failed && lane == 0) gone[quad] = 1;
+      ptx::named_barrier(9 + quad, 64);
+      if (gone[quad]) break;
+      const int n = info->seen[row] & (kSpoilt - 1);  // keys that this row sees
+      const int tiles = info->tiles, tile0 = info->tile0;
       float m = -INFINITY;           // what this thread's sum is taken against
       float sum[2][2] = {};          // partial sums over this thread's tiles
       const int odd = int((it0 ^ uint32_t(group)) & 1u);  // the unit's first tile of this group
-      for (int j = odd; j < x.p.tiles; j += 2) {
+      for (int j = odd; j < tiles; j += 2) {
         const uint32_t it = it0 + uint32_t(j), sb = uint32_t(j % C::kS);
         wt.all(bar(C::kSFull + sb), s_full.at(sb, j / C::kS));
         ptx::tc_fence_after();
         const uint32_t src = tmem + sb * 128 + lanes;
-        const int key = (x.p.tile0 + j) * kRowTile;
+        const int key = (tile0 + j) * kRowTile;
         uint32_t r[4][32];
 #pragma unroll
         for (int g = 0; g < 4; ++g) ptx::tmem_ld32(src + 32 * g, r[g]);
@@ -906,7 +969,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             p[i / 2] = ptx::pack_bf16x2(p0, p1);
           }
           ptx::tmem_st16(src + 16 * g, p);  // over the scores
-          if (g == kTurn) ptx::named_barrier_arrive(1 + quad + 4 * int((it + 1) & 1u), 64);
+          if (g == C::kTurn) ptx::named_barrier_arrive(1 + quad + 4 * int((it + 1) & 1u), 64);
           if (g & 1) {
             ptx::tmem_wait_st();
             ptx::tc_fence_before();
@@ -916,71 +979,94 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       }
-      it0 += uint32_t(x.p.tiles);
-      const int last = x.p.tiles - 1;
+      it0 += uint32_t(tiles);
+      const int last = tiles - 1;
       const uint32_t last_phase = last >= 0 ? pv_done.at(last % C::kS, last / C::kS) : 0u;
-      s_full.pass(x.p.tiles);
-      pv_done.pass(x.p.tiles);
+      s_full.pass(tiles);
+      pv_done.pass(tiles);
       // The row's last reference maximum and its whole sum, then O / sum to the output: this
       // thread's half of the columns.
       ptx::named_barrier(9 + quad, 64);
-      const float ref = x.p.tiles ? shared_m[row] : -INFINITY;
+      const float ref = tiles ? shared_m[row] : -INFINITY;
       float total = (sum[0][0] + sum[0][1]) + (sum[1][0] + sum[1][1]);
       if (m != ref) total = m == -INFINITY ? 0.f : total * ptx::ex2((m - ref) * c);
       shared_sum[group * 128 + row] = total;
       ptx::named_barrier(9 + quad, 64);
       total = shared_sum[row] + shared_sum[128 + row];
-      if (n > a.w.seq_spoilt[x.p.seq]) total = NAN;
-      const bool sees = n > x.p.tile0 * kRowTile;  // in this piece
+      if (info->seen[row] & kSpoilt) total = NAN;
+      const bool sees = n > tile0 * kRowTile;  // in this piece
       const float inv = sees ? 1.f / total : 0.f;
-      if (x.p.tiles) {
+      if (tiles) {
         wt.all(bar(C::kPvDone + last % C::kS), last_phase);
         ptx::tc_fence_after();
       }
-      const int head = a.head0 + x.head;
-      const long long part = (long long)u * kQueryTile + rank * 128 + row;
-      uint8_t* out = x.p.whole ? a.out + (long long)t * a.out_st + (long long)head * a.out_sh
-                               : reinterpret_cast<uint8_t*>(a.w.part_out + part * kDv);
-      const uint32_t o = tmem + C::kTmemO + group * (kDv / 2) + lanes;
+      // The rest of the unit's info, and the info buffer is free.
+      const int head = a.head0 + info->head, rows = info->rows - rank * 128;
+      const int t0 = info->row0 + rank * 128;
+      const bool whole = info->whole != 0;
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(C::kInfoEmpty + int(nth & 1u)));
+      // Rows of this warp: through shared memory 64 bytes a row at a time, so that four lanes store
+      // 64 consecutive bytes (a lane a row stored 16 bytes each to 32 lines at once: 7500 cycles a
+      // unit at 256 columns).
+      const bool f32 = a.out_f32 || !whole;
+      const long long part = (long long)u * kQueryTile + rank * 128;
+      uint8_t* out0 = whole ? a.out + (long long)t0 * a.out_st + (long long)head * a.out_sh
+                            : reinterpret_cast<uint8_t*>(a.w.part_out + part * kDv);
+      const long long out_row = whole ? a.out_st : (long long)kDv * 4;
+      uint8_t* turn = sm + C::kSmTurn + (warp - 4) * kTurnBytes;
+      auto emit = [&](const uint32_t (&v)[16], int byte) {
 #pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<uint4*>(turn + lane * 80 + k * 16) =
+              make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = k * 8 + (lane >> 2), at = quad * 32 + r;
+          const uint4 w = *reinterpret_cast<const uint4*>(turn + r * 80 + (lane & 3) * 16);
+          if (at < rows)
+            *reinterpret_cast<uint4*>(out0 + at * out_row + byte + (lane & 3) * 16) = w;
+        }
+        __syncwarp();
+      };
+      const uint32_t o = tmem + C::kTmemO + group * (kDv / 2) + lanes;
+#pragma unroll 1
       for (int i = 0; i < kDv / 2; i += 32) {
-        uint32_t v[32];
-        if (x.p.tiles) {
+        const int col = group * (kDv / 2) + i;
+        uint32_t v[32], y[16];
+        if (tiles) {
           ptx::tmem_ld32(o + i, v);
           ptx::tmem_wait_ld();
         }
-        if (mine) {
-          const int col = group * (kDv / 2) + i;
 #pragma unroll
-          for (int k = 0; k < 32; ++k)
-            v[k] = sees ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
-          if (a.out_f32 || !x.p.whole) {
+        for (int k = 0; k < 32; ++k)
+          v[k] = sees ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
+        if (f32) {
+#pragma unroll 1
+          for (int g = 0; g < 2; ++g) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<uint4*>(out + 4 * (col + k)) =
-                  make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; k += 8)
-              *reinterpret_cast<uint4*>(out + 2 * (col + k)) = make_uint4(
-                  ptx::pack_bf16x2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])),
-                  ptx::pack_bf16x2(__uint_as_float(v[k + 2]), __uint_as_float(v[k + 3])),
-                  ptx::pack_bf16x2(__uint_as_float(v[k + 4]), __uint_as_float(v[k + 5])),
-                  ptx::pack_bf16x2(__uint_as_float(v[k + 6]), __uint_as_float(v[k + 7])));
+            for (int k = 0; k < 16; ++k) y[k] = g ? v[16 + k] : v[k];
+            emit(y, 4 * col + 64 * g);
           }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            y[k] = ptx::pack_bf16x2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
+          emit(y, 2 * col);
         }
       }
-      if (x.p.tiles) {
+      if (tiles) {
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive_cluster_relaxed(lead(C::kOFree));
       }
-      if (mine && group == 0) {
+      if (row < rows && group == 0) {
         const float l2 = sees ? ref * c + log2f(total) : -INFINITY;
-        if (!x.p.whole)
-          a.w.part_lse[part] = l2;
+        if (!whole)
+          a.w.part_lse[part + row] = l2;
         else if (a.lse)
-          a.lse[(long long)t * a.heads + head] = l2 * 0.69314718055994531f;
+          a.lse[(long long)(t0 + row) * a.heads + head] = l2 * 0.69314718055994531f;
       }
     }
   }
