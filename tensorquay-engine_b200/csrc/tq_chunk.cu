@@ -142,18 +142,20 @@ __device__ __forceinline__ int last_at_or_below(const int* start, int n, int x) 
 
 __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
   __shared__ int part[32];
-  __shared__ int s_rows, s_blocks, s_over;
+  __shared__ int s_rows, s_blocks, s_over, s_split;
+  // The first 1024 sequences and blocks again, near: the steps below read each other's results.
+  __shared__ int n_q0[1025], n_block[1025], n_key0[1024], n_keys[1024], n_tiles[1024];
   const Work& w = a.w;
   const int tid = threadIdx.x;
   if (tid < kHdrWords) w.header[tid] = 0;
-  if (tid == 0) { s_rows = 0; s_blocks = 0; s_over = 0; }
+  if (tid == 0) { s_rows = 0; s_blocks = 0; s_over = 0; s_split = 0; }
   __syncthreads();
   int bad = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += 1024) {
     const int s = s0 + tid;
     int keys = 0, blocks = 0;
     if (s < a.seqs) {
-      const int b = a.q_start[s], e = a.q_start[s + 1];
+      const int b = a.q_start[s], e = a.q_start[s + 1], len = a.kv_len[s];
       int n = e - b;
       if (b < 0 || e < b || e > a.tokens) {
         // Sequences that overlap would write each other's outputs: the whole call is left out.
@@ -163,7 +165,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
       }
       if (n > 0) {
         const long long room = (long long)kPage * a.slots;
-        keys = max(a.kv_len[s], 0);
+        keys = max(len, 0);
         if (keys > room) {
           keys = int(room);
           bad |= TQ_DEV_TABLE_SHORT;
@@ -172,6 +174,11 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
         if (keys > a.cap) { s_over = 1; keys = 0; }
       }
       blocks = (n + kQueryTile - 1) / kQueryTile;
+      if (s < 1024) {
+        n_q0[s] = b;
+        n_q0[s + 1] = e;  // the same value from both sides
+        n_keys[s] = keys;
+      }
     }
     const int padded = (keys + kRowTile - 1) / kRowTile * kRowTile;
     const int rows_end = block_inclusive(padded, part), blocks_end = block_inclusive(blocks, part);
@@ -184,6 +191,10 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
       w.seq_keys[s] = keys;
       w.seq_spoilt[s] = INT_MAX;
       w.seq_block[s] = blocks0 + blocks_end - blocks;
+      if (s < 1024) {
+        n_key0[s] = rows0 + rows_end - padded;
+        n_block[s] = blocks0 + blocks_end - blocks;
+      }
     }
     long long sum = padded;
 #pragma unroll
@@ -196,7 +207,9 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
       s_blocks = blocks0 + blocks_end;
     }
     __syncthreads();
-    if (s_over) break;
+    const int over = s_over;
+    __syncthreads();  // before the next round may set it
+    if (over) break;
   }
   if (bad) atomicOr(w.header + kHdrError, bad);
   if (s_over) {
@@ -213,79 +226,102 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
     w.seq_block[a.seqs] = s_blocks;
     w.header[kHdrRows] = s_rows;
     w.header[kHdrBlocks] = s_blocks;
+    if (a.seqs <= 1024) n_block[a.seqs] = s_blocks;
   }
   __syncthreads();
+  const bool near = a.seqs <= 1024;
+  const int* seq_block = near ? n_block : w.seq_block;
+  const int* q_start = near ? n_q0 : a.q_start;
+  const int* seq_keys = near ? n_keys : w.seq_keys;
+  const int* seq_key0 = near ? n_key0 : w.seq_key0;
+  const int blocks = s_blocks;
   // Query blocks, one warp each: the tiles that its furthest-seeing token sees.
   const int lane = tid & 31, warp = tid >> 5;
-  for (int b = warp; b < s_blocks; b += 32) {
-    const int s = last_at_or_below(w.seq_block, a.seqs, b);
-    const int row0 = a.q_start[s] + (b - w.seq_block[s]) * kQueryTile;
-    const int rows = min(kQueryTile, a.q_start[s + 1] - row0);
+  for (int b = warp; b < blocks; b += 32) {
+    const int s = last_at_or_below(seq_block, a.seqs, b);
+    const int row0 = q_start[s] + (b - seq_block[s]) * kQueryTile;
+    const int rows = min(kQueryTile, q_start[s + 1] - row0);
     int far = -1;
-    for (int i = lane; i < rows; i += 32) far = max(far, a.q_pos[row0 + i]);
+#pragma unroll
+    for (int i = 0; i < kQueryTile; i += 32)
+      if (i + lane < rows) far = max(far, a.q_pos[row0 + i + lane]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) far = max(far, __shfl_xor_sync(0xFFFFFFFFu, far, o));
-    const int keys = w.seq_keys[s];
-    const int seen = far >= keys ? keys : far + 1;
-    if (lane == 0)
-      w.blocks[b] = {row0, rows, w.seq_key0[s], (seen + kRowTile - 1) / kRowTile, s, b, 1, 0};
+    const int keys = seq_keys[s];
+    const int tiles = ((far >= keys ? keys : far + 1) + kRowTile - 1) / kRowTile;
+    if (lane == 0) {
+      if (b < 1024) n_tiles[b] = tiles;
+      else w.blocks[b].tiles = tiles;
+    }
   }
   __syncthreads();
+  auto tiles_of = [&](int b) { return b < 1024 ? n_tiles[b] : w.blocks[b].tiles; };
   // The most tiles that a piece gets. Warp k weighs cutting the longest block into k + 1: the
   // rounds that the CTA pairs need for all units, each as long as such a piece.
-  __shared__ int s_cost[32], s_len[32];
-  int longest = 1;
-  for (int b = lane; b < s_blocks; b += 32) longest = max(longest, w.blocks[b].tiles);
+  int len = 1 << 30;  // whole blocks
+  if (a.split_units) {
+    __shared__ int s_cost[32], s_len[32];
+    int longest = 1, count = 0;
+    for (int b = lane; b < blocks; b += 32) longest = max(longest, tiles_of(b));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xFFFFFFFFu, longest, o));
-  {
-    const int len = (longest + warp) / (warp + 1);
-    int count = 0;
-    if (a.split_units)
-      for (int b = lane; b < s_blocks; b += 32)
-        count += max(1, (w.blocks[b].tiles + len - 1) / len);
+    for (int o = 16; o > 0; o >>= 1)
+      longest = max(longest, __shfl_xor_sync(0xFFFFFFFFu, longest, o));
+    const int cut = (longest + warp) / (warp + 1);
+    for (int b = lane; b < blocks; b += 32) count += max(1, (tiles_of(b) + cut - 1) / cut);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) count += __shfl_xor_sync(0xFFFFFFFFu, count, o);
     const long long units = (long long)count * a.pass_heads;
     if (lane == 0) {
-      s_len[warp] = len;
-      s_cost[warp] = INT_MAX;
-      if (a.split_units && units <= a.split_units)
-        s_cost[warp] = int((units + a.pairs - 1) / a.pairs) * (len + kPieceCost) +
-                       (warp ? 2 * kPieceCost : 0);
+      s_len[warp] = cut;
+      s_cost[warp] = units <= a.split_units
+                         ? int((units + a.pairs - 1) / a.pairs) * (cut + kPieceCost) +
+                               (warp ? 2 * kPieceCost : 0)
+                         : INT_MAX;
     }
+    __syncthreads();
+    int cost = s_cost[lane], best = lane;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const int c = __shfl_xor_sync(0xFFFFFFFFu, cost, o), k = __shfl_xor_sync(0xFFFFFFFFu, best, o);
+      if (c < cost || (c == cost && k < best)) {
+        cost = c;
+        best = k;
+      }
+    }
+    if (best) len = s_len[best];
   }
-  __syncthreads();
-  int best = 0;
-  for (int k = 1; k < 32; ++k)
-    if (s_cost[k] < s_cost[best]) best = k;
-  const int len = best ? s_len[best] : longest;
   // Number the pieces, 1024 blocks at a time.
   __syncthreads();
   if (tid == 0) s_rows = 0;
   __syncthreads();
-  for (int b0 = 0; b0 < s_blocks; b0 += 1024) {
+  for (int b0 = 0; b0 < blocks; b0 += 1024) {
     const int b = b0 + tid;
-    int n = 0;
-    if (b < s_blocks) n = max(1, (w.blocks[b].tiles + len - 1) / len);
-    const int end = block_inclusive(n, part), at = s_rows;
-    if (b < s_blocks) {
-      Block blk = w.blocks[b];
-      blk.piece0 = at + end - n;
-      blk.pieces = n;
-      w.blocks[b] = blk;
-      // Pieces of one length, the last one shorter by less than one tile a piece.
-      const int each = max(1, (blk.tiles + n - 1) / n);
+    int n = 0, tiles = 0;
+    if (b < blocks) {
+      tiles = tiles_of(b);
+      n = max(1, (tiles + len - 1) / len);
+    }
+    const int end = block_inclusive(n, part), at = s_rows + end - n;
+    if (b < blocks) {
+      const int s = last_at_or_below(seq_block, a.seqs, b);
+      const int row0 = q_start[s] + (b - seq_block[s]) * kQueryTile;
+      const int rows = min(kQueryTile, q_start[s + 1] - row0), key0 = seq_key0[s];
+      w.blocks[b] = {row0, rows, key0, tiles, s, at, n, 0};
+      // Pieces of one length, the last ones shorter.
+      const int each = max(1, (tiles + n - 1) / n);
       for (int i = 0; i < n; ++i)
-        w.pieces[blk.piece0 + i] = {blk.row0, blk.rows, blk.key0, i * each,
-                                    max(0, min(each, blk.tiles - i * each)), blk.seq, n == 1, b};
-      if (n > 1) w.header[kHdrSplit] = 1;
+        w.pieces[at + i] = {row0, rows, key0, i * each, max(0, min(each, tiles - i * each)), s,
+                            n == 1, b};
+      if (n > 1) s_split = 1;
     }
     __syncthreads();
-    if (tid == 1023) s_rows = at + end;
+    if (tid == 1023) s_rows = at + n;
     __syncthreads();
   }
-  if (tid == 0) w.header[kHdrPieces] = s_rows;
+  if (tid == 0) {
+    w.header[kHdrPieces] = s_rows;
+    w.header[kHdrSplit] = s_split;
+  }
 }
 
 // ------------------------------------------------------------------------------ gather
@@ -293,58 +329,72 @@ __device__ __forceinline__ bool finite_bf16x2(uint32_t u) {
   return (u & 0x7F80u) != 0x7F80u && (u & 0x7F800000u) != 0x7F800000u;
 }
 
-// One block per kRowTile compact rows, one warp per row at a time: lane i takes the 16 latent
-// values from 16 i on, and two of the 64 RoPE values.
+// One block per kGatherRows compact rows, four rows a warp with all their loads in flight: lane i
+// takes the 16 latent values from 16 i on, and two of the 64 RoPE values. What bounds it: the chain
+// of dependent loads (sequence, page, row) for small calls, so rows are spread over many blocks;
+// HBM for large ones (a row read and written once).
+constexpr int kGatherRows = 32;
+static_assert(kRowTile % kGatherRows == 0, "a block's rows lie in one sequence");
+
 __global__ void __launch_bounds__(256) gather_kernel(const Args a) {
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   const Work& w = a.w;
-  const int r0 = int(blockIdx.x) * kRowTile;
+  const int r0 = int(blockIdx.x) * kGatherRows;
   if (r0 >= w.header[kHdrRows]) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int s = last_at_or_below(w.seq_key0, a.seqs, r0);
-  const int first = r0 - w.seq_key0[s], keys = w.seq_keys[s];
-#pragma unroll 4
-  for (int i = warp; i < kRowTile; i += 8) {
-    const int p = first + i;
-    uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
-    uint32_t rp = 0;
-    if (p < keys) {
-      const int page = a.page_table[(long long)s * a.slots + p / kPage];
-      if (page >= 0 && page < a.pages) {
-        const uint8_t* src = a.kv + ((long long)page * kPage + p % kPage) * a.row_stride;
-        if (a.fp8) {
-          const uint4 c = *reinterpret_cast<const uint4*>(src + 16 * lane);
-          const float sc = *reinterpret_cast<const float*>(src + kLatent + 4 * (lane >> 3));
-          v0 = make_uint4(ptx::e4m3x2_scaled_bf16x2(c.x & 0xFFFF, sc),
-                          ptx::e4m3x2_scaled_bf16x2(c.x >> 16, sc),
-                          ptx::e4m3x2_scaled_bf16x2(c.y & 0xFFFF, sc),
-                          ptx::e4m3x2_scaled_bf16x2(c.y >> 16, sc));
-          v1 = make_uint4(ptx::e4m3x2_scaled_bf16x2(c.z & 0xFFFF, sc),
-                          ptx::e4m3x2_scaled_bf16x2(c.z >> 16, sc),
-                          ptx::e4m3x2_scaled_bf16x2(c.w & 0xFFFF, sc),
-                          ptx::e4m3x2_scaled_bf16x2(c.w >> 16, sc));
-        } else {
-          v0 = *reinterpret_cast<const uint4*>(src + 32 * lane);
-          v1 = *reinterpret_cast<const uint4*>(src + 32 * lane + 16);
-          if (a.dr) rp = *reinterpret_cast<const uint32_t*>(src + 2 * kLatent + 4 * lane);
-        }
-      } else if (lane == 0) {
-        atomicOr(w.header + kHdrError, TQ_DEV_PAGE_RANGE);
+  const int p0 = r0 - w.seq_key0[s] + warp * 4, keys = w.seq_keys[s];
+  int page[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    page[i] = p0 + i < keys ? a.page_table[(long long)s * a.slots + (p0 + i) / kPage] : 0;
+  uint4 v0[4], v1[4];
+  uint32_t rp[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v0[i] = v1[i] = make_uint4(0, 0, 0, 0);
+    rp[i] = 0;
+    const bool live = p0 + i < keys, known = page[i] >= 0 && page[i] < a.pages;
+    if (live && known) {
+      const uint8_t* src = a.kv + ((long long)page[i] * kPage + (p0 + i) % kPage) * a.row_stride;
+      if (a.fp8) {
+        v0[i] = *reinterpret_cast<const uint4*>(src + 16 * lane);
+        rp[i] = *reinterpret_cast<const uint32_t*>(src + kLatent + 4 * (lane >> 3));  // scale
+      } else {
+        v0[i] = *reinterpret_cast<const uint4*>(src + 32 * lane);
+        v1[i] = *reinterpret_cast<const uint4*>(src + 32 * lane + 16);
+        if (a.dr) rp[i] = *reinterpret_cast<const uint32_t*>(src + 2 * kLatent + 4 * lane);
       }
     }
-    const bool ok = finite_bf16x2(v0.x) && finite_bf16x2(v0.y) && finite_bf16x2(v0.z) &&
-                    finite_bf16x2(v0.w) && finite_bf16x2(v1.x) && finite_bf16x2(v1.y) &&
-                    finite_bf16x2(v1.z) && finite_bf16x2(v1.w) && finite_bf16x2(rp);
-    const bool row_ok = __all_sync(0xFFFFFFFFu, ok);
-    if (!row_ok) {
-      v0 = v1 = make_uint4(0, 0, 0, 0);
-      rp = 0;
+    if (live && !known && lane == 0) atomicOr(w.header + kHdrError, TQ_DEV_PAGE_RANGE);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (a.fp8) {
+      const uint4 c = v0[i];
+      const float sc = __uint_as_float(rp[i]);
+      rp[i] = 0;
+      v0[i] = make_uint4(
+          ptx::e4m3x2_scaled_bf16x2(c.x & 0xFFFF, sc), ptx::e4m3x2_scaled_bf16x2(c.x >> 16, sc),
+          ptx::e4m3x2_scaled_bf16x2(c.y & 0xFFFF, sc), ptx::e4m3x2_scaled_bf16x2(c.y >> 16, sc));
+      v1[i] = make_uint4(
+          ptx::e4m3x2_scaled_bf16x2(c.z & 0xFFFF, sc), ptx::e4m3x2_scaled_bf16x2(c.z >> 16, sc),
+          ptx::e4m3x2_scaled_bf16x2(c.w & 0xFFFF, sc), ptx::e4m3x2_scaled_bf16x2(c.w >> 16, sc));
     }
-    const long long r = r0 + i;
+    const bool ok = finite_bf16x2(v0[i].x) && finite_bf16x2(v0[i].y) && finite_bf16x2(v0[i].z) &&
+                    finite_bf16x2(v0[i].w) && finite_bf16x2(v1[i].x) && finite_bf16x2(v1[i].y) &&
+                    finite_bf16x2(v1[i].z) && finite_bf16x2(v1[i].w) && finite_bf16x2(rp[i]);
+    if (!__all_sync(0xFFFFFFFFu, ok)) {
+      v0[i] = v1[i] = make_uint4(0, 0, 0, 0);
+      rp[i] = 0;
+      if (lane == 0) atomicMin(w.seq_spoilt + s, p0 + i);
+    }
+    const long long r = r0 + warp * 4 + i;
     uint16_t* dst = w.rows + r * kLatent + 16 * lane;
-    *reinterpret_cast<uint4*>(dst) = v0;
-    *reinterpret_cast<uint4*>(dst + 8) = v1;
-    if (a.dr) *reinterpret_cast<uint32_t*>(w.rope + r * kRopeDim + 2 * lane) = rp;
-    if (lane == 0 && !row_ok) atomicMin(w.seq_spoilt + s, p);
+    *reinterpret_cast<uint4*>(dst) = v0[i];
+    *reinterpret_cast<uint4*>(dst + 8) = v1[i];
+    if (a.dr) *reinterpret_cast<uint32_t*>(w.rope + r * kRopeDim + 2 * lane) = rp[i];
   }
 }
 
@@ -458,10 +508,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_holder;
   Waiter wt{a.w.header, base + kSmMisc + 4, rank, false};
 
-  // Column blocks (a head, or a head's k or v) by row tiles, one contiguous range per pair.
-  const int per_head = (a.dn + a.dv) / 256;
+  // Column blocks (a head, or a head's k or v) by row tiles, one contiguous range per pair. The
+  // first one's column block, floor(floor(tiles * blocks * pair / pairs) / tiles), does not depend
+  // on the number of row tiles, so its weights load while the rows are still being gathered.
+  const int per_head = (a.dn + a.dv) / 256, columns = per_head * a.pass_heads;
+  auto load_weights = [&](int g, int c) {
+    const bool from_v = per_head == 2 ? (g & 1) != 0 : rank != 0;
+    if (rank == 0) ptx::mbar_expect_tx(bar(kBarWFull + c), 2 * kBox);
+    ptx::tma_load_3d_pair(base + kSmW + c * kBox, from_v ? &tm_uv : &tm_uk,
+                          ptx::map_peer(bar(kBarWFull + c), 0), c * 64,
+                          per_head == 2 ? rank * 128 : 0,
+                          a.head0 + (per_head == 2 ? g >> 1 : g));
+  };
+  if (threadIdx.x == 0)
+    for (int c = 0; c < kChunks; ++c) load_weights(int((long long)columns * pair / pairs), c);
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   const long long tiles = (a.w.header[kHdrRows] + 255) / 256;
-  const long long items = tiles * per_head * a.pass_heads;
+  const long long items = tiles * columns;
   const long long first = items * pair / pairs, last = items * (pair + 1) / pairs;
   if (warp == 0) {
     if (lane == 0) {
@@ -469,15 +533,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (long long i = first; i < last && !wt.failed; ++i) {
         const int g = int(i / tiles), tile = int(i % tiles);
         const bool fresh = i == first || tile == 0;
-        const int h = a.head0 + (per_head == 2 ? g >> 1 : g);
-        const bool from_v = per_head == 2 ? (g & 1) != 0 : rank != 0;
-        const int w_row = per_head == 2 ? rank * 128 : 0;
         for (int c = 0; c < kChunks; ++c) {
-          if (fresh) {
-            if (blocks > 0 && !wt.on(bar(kBarWEmpty + c), (blocks - 1) & 1u)) break;
-            if (rank == 0) ptx::mbar_expect_tx(bar(kBarWFull + c), 2 * kBox);
-            ptx::tma_load_3d_pair(base + kSmW + c * kBox, from_v ? &tm_uv : &tm_uk,
-                                  ptx::map_peer(bar(kBarWFull + c), 0), c * 64, w_row, h);
+          if (fresh && blocks > 0) {
+            if (!wt.on(bar(kBarWEmpty + c), (blocks - 1) & 1u)) break;
+            load_weights(g, c);
           }
           if (!wt.on(bar(kBarAEmpty + stage), phase ^ 1u)) break;
           if (rank == 0) ptx::mbar_expect_tx(bar(kBarAFull + stage), 2 * kBox);
@@ -522,6 +581,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ptx::mma_commit_pair(bar(kBarAccFull + buf));
         if (fresh) ++blocks;
       }
+      // A pair without items has its weights in flight all the same.
+      if (first >= last)
+        for (int c = 0; c < kChunks; ++c) wt.all(bar(kBarWFull + c), 0);
       ptx::mma_commit_pair(bar(kBarDrain));
     }
     __syncwarp();
@@ -722,6 +784,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   Waiter wt{a.w.header, base + C::kSmMisc + 4, rank, false};
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   // All 512 columns are this CTA's, so they start at 0.
   const int pieces = a.w.header[kHdrPieces], units = pieces * a.pass_heads;
 
@@ -1087,6 +1151,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // order. One thread takes 8 columns of one row and head, all pieces' loads ahead of their use.
 // Reads the partial outputs once from L2, where the attention left them.
 __global__ void __launch_bounds__(256) join_kernel(const Args a) {
+  ptx::grid_dependency_wait();
   const Work& w = a.w;
   if (!w.header[kHdrSplit]) return;
   const int pieces = w.header[kHdrPieces], groups = a.dv / 8;
@@ -1338,22 +1403,37 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
               s.w_uv.strides_bytes[0], 128))
     return fail("tensor_map", TQ_ERR_CUDA);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  // Each kernel after the first starts while the one before it ends, and waits inside for its
+  // results (griddepcontrol.wait): the setup and the loads that need none run meanwhile.
+  auto launch = [&](auto kernel, int grid, int threads, uint32_t smem, auto... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(grid), 1, 1);
+    cfg.blockDim = dim3(unsigned(threads), 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = cs;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess;
+  };
   plan_kernel<<<1, 1024, 0, cs>>>(a);
-  gather_kernel<<<a.cap / kRowTile, 256, 0, cs>>>(a);
+  if (cudaGetLastError() != cudaSuccess ||
+      !launch(gather_kernel, a.cap / kGatherRows, 256, 0, a))
+    return fail("launch", TQ_ERR_CUDA);
   for (a.head0 = 0; a.head0 < a.heads; a.head0 += int(l.pass_heads)) {
     a.pass_heads = a.heads - a.head0 < int(l.pass_heads) ? a.heads - a.head0 : int(l.pass_heads);
-    expand::expand_kernel<<<2 * pairs, expand::kThreads, expand::kSmBytes, cs>>>(tm_rows, tm_uk,
-                                                                                 tm_uv, a);
-    if (a.dr)
-      attend::attend_kernel<192, 128>
-          <<<2 * pairs, attend::kThreads, attend::Shape<192, 128>::kSmBytes, cs>>>(tm_q, tm_k,
-                                                                                   tm_rope, tm_v, a);
-    else
-      attend::attend_kernel<256, 256>
-          <<<2 * pairs, attend::kThreads, attend::Shape<256, 256>::kSmBytes, cs>>>(tm_q, tm_k,
-                                                                                   tm_rope, tm_v, a);
-    if (a.split_units) join_kernel<<<4 * pairs, 256, 0, cs>>>(a);
+    using Rope = attend::Shape<192, 128>;
+    using Wide = attend::Shape<256, 256>;
+    if (!launch(expand::expand_kernel, 2 * pairs, expand::kThreads, expand::kSmBytes, tm_rows,
+                tm_uk, tm_uv, a) ||
+        !(a.dr ? launch(attend::attend_kernel<192, 128>, 2 * pairs, attend::kThreads,
+                        Rope::kSmBytes, tm_q, tm_k, tm_rope, tm_v, a)
+               : launch(attend::attend_kernel<256, 256>, 2 * pairs, attend::kThreads,
+                        Wide::kSmBytes, tm_q, tm_k, tm_rope, tm_v, a)) ||
+        (a.split_units && !launch(join_kernel, 4 * pairs, 256, 0, a)))
+      return fail("launch", TQ_ERR_CUDA);
   }
-  if (cudaGetLastError() != cudaSuccess) return fail("launch", TQ_ERR_CUDA);
   return fail(nullptr, TQ_OK);
 }
