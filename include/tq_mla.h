@@ -329,6 +329,8 @@ int32_t tq_kv_write(const TqKvWriteSpec* spec, int32_t* device_flags, void* stre
  *   w_qb     bf16 [H * (Dn + Dr), Rq]  w_uk  bf16 [H, Dn, 512]      w_kva   bf16 [W, Dm]
  *   kv_norm  bf16 [512]                pos, seq_id i32 [T]          page_table i32 [S, L]
  *   kv       u8 [P, 64, row bytes] pool of `kv_format` rows        q  bf16 [T, H, W] (out)
+ * With w_uk of rank 0 the query is left unabsorbed, as tq_mla_chunk takes it: q is [T, H, Dn + Dr],
+ * q[t, h] = [ qf[h][:Dn] | bf16(rope(qf[h][Dn:], pos[t])) ].
  * All matrices are packed row-major with 16-byte aligned bases; Dm, Rq and Dn are multiples of
  * 8. A row whose seq_id, pos or page entry is out of range is not written and sets
  * TQ_DEV_SEQ_RANGE, TQ_DEV_TABLE_SHORT or TQ_DEV_PAGE_RANGE in `device_flags` (a device int32,

@@ -35,7 +35,7 @@ def step_plan(cached, new, table, free, count, tokens):
         for p in range(c, c + n):
             col = p // PAGE
             page = table[s, col] if col < columns else -1
-            rows.append((s, p, page * PAGE + p % PAGE if page >= 0 else -1))
+            rows.append((s, min(p, 2 ** 31 - 1), page * PAGE + p % PAGE if page >= 0 else -1))
         q_start.append(q_start[-1] + n)
     if q_start[-1] > tokens:
         flags |= WORK_OVERFLOW

@@ -354,13 +354,18 @@ int32_t prologue_validate_impl(const TqPrologueSpec* spec, TqContractError* err)
   const uint64_t wqb[2] = {H * (dn + dr), rq}, wuk[3] = {H, dn, 512}, wkva[2] = {512 + dr, dm};
   const uint64_t kvn[1] = {512}, tok[1] = {T};
   const uint64_t table[2] = {s.page_table.shape[0], s.page_table.shape[1]};
-  const uint64_t pool[3] = {s.kv.shape[0], kPageRows, payload}, q_shape[3] = {T, H, 512 + dr};
+  // Without w_uk the query is not absorbed: [Dn | Dr] per head.
+  const bool absorb = s.w_uk.rank != 0;
+  const uint64_t pool[3] = {s.kv.shape[0], kPageRows, payload};
+  const uint64_t q_shape[3] = {T, H, (absorb ? 512 : dn) + dr};
   Extent in[10], out[2];
+  in[4].present = false;
   if (!check("x", s.x, x_shape, 2, TQ_DTYPE_BF16, Layout::Packed, launching, &in[0], &f) ||
       !check("w_qa", s.w_qa, wqa, 2, TQ_DTYPE_BF16, Layout::Packed, launching, &in[1], &f) ||
       !check("q_norm", s.q_norm, qn, 1, TQ_DTYPE_BF16, Layout::Packed, launching, &in[2], &f) ||
       !check("w_qb", s.w_qb, wqb, 2, TQ_DTYPE_BF16, Layout::Packed, launching, &in[3], &f) ||
-      !check("w_uk", s.w_uk, wuk, 3, TQ_DTYPE_BF16, Layout::Packed, launching, &in[4], &f) ||
+      (absorb &&
+       !check("w_uk", s.w_uk, wuk, 3, TQ_DTYPE_BF16, Layout::Packed, launching, &in[4], &f)) ||
       !check("w_kva", s.w_kva, wkva, 2, TQ_DTYPE_BF16, Layout::Packed, launching, &in[5], &f) ||
       !check("kv_norm", s.kv_norm, kvn, 1, TQ_DTYPE_BF16, Layout::Packed, launching, &in[6], &f) ||
       !check("pos", s.pos, tok, 1, TQ_DTYPE_I32, Layout::Packed, launching, &in[7], &f) ||
@@ -375,7 +380,8 @@ int32_t prologue_validate_impl(const TqPrologueSpec* spec, TqContractError* err)
                                    &s.kv_norm, &s.q};
     const char* names[8] = {"x", "w_qa", "q_norm", "w_qb", "w_uk", "w_kva", "kv_norm", "q"};
     for (int i = 0; i < 8; ++i)
-      if (mats[i]->device_address % 16) return fail(names[i], TQ_ALIGNMENT);
+      if (mats[i]->rank != 0 && mats[i]->device_address % 16)
+        return fail(names[i], TQ_ALIGNMENT);
   }
   if (!(std::isfinite(s.q_eps) && s.q_eps > 0.f)) return fail("q_eps", TQ_SCALE);
   if (!(std::isfinite(s.kv_eps) && s.kv_eps > 0.f)) return fail("kv_eps", TQ_SCALE);

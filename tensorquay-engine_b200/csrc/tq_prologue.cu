@@ -9,6 +9,7 @@
 //   3. qf  = cq . w_qb^T                plain GEMM                       [T, H, Dn + Dr]
 //   4. q[:, :, :512] = qf[:, :, :Dn] . w_uk[h]   one strided-batched GEMM over the heads, written
 //                                       straight into q's row layout (ldc = H * W)
+//                                       (without w_uk: qf is q itself, for the chunk attention)
 //   5. q[:, :, 512:] = rope(qf[:, :, Dn:]) and kvf[:, 512:] rotated in place (rope_rows_kernel)
 //   6. kvf = x . w_kva^T                plain GEMM                       [T, W]
 //   7. tq_kv_write: bf16(rms(kvf[:512])) * kv_norm and the row written (FP8 rows quantized) to the
@@ -220,7 +221,8 @@ Layout layout_of(const TqPrologueSpec& s) {
   Layout l;
   l.cq = 0;
   l.qf = l.cq + round256(T * rq * 2);
-  l.kvf = l.qf + round256(T * H * (dn + dr) * 2);
+  // The unabsorbed query is written straight into q.
+  l.kvf = l.qf + (s.w_uk.rank ? round256(T * H * (dn + dr) * 2) : 0);
   l.scratch = l.kvf + round256(T * (kLatent + dr) * 2);
   l.total = l.scratch + kCublasScratch;
   return l;
@@ -328,10 +330,11 @@ extern "C" int32_t tq_mla_prologue(const TqPrologueSpec* spec, void* workspace,
   const int dn = s.nope_dim, dr = s.rope_dim, width = kLatent + dr;
   char* ws = static_cast<char*>(workspace);
   uint16_t* cq = reinterpret_cast<uint16_t*>(ws + l.cq);
-  uint16_t* qf = reinterpret_cast<uint16_t*>(ws + l.qf);
   uint16_t* kvf = reinterpret_cast<uint16_t*>(ws + l.kvf);
   const void* x = reinterpret_cast<const void*>(s.x.device_address);
   uint16_t* q = reinterpret_cast<uint16_t*>(s.q.device_address);
+  const bool absorb = s.w_uk.rank != 0;
+  uint16_t* qf = absorb ? reinterpret_cast<uint16_t*>(ws + l.qf) : q;
   const int* pos = reinterpret_cast<const int*>(s.pos.device_address);
   const double log2_theta = std::log2(double(s.rope_theta));
   const long long cap = 8ll * sms;
@@ -427,8 +430,8 @@ extern "C" int32_t tq_mla_prologue(const TqPrologueSpec* spec, void* workspace,
         bad = "fork";
       } else {
         rope_rows_kernel<<<dim3(unsigned(T < cap ? T : cap), unsigned((H + 63) / 64)), 256, 0,
-                           sd->stream>>>(qf + dn, dn + dr, q + kLatent, width, T, H, pos,
-                                         log2_theta);
+                           sd->stream>>>(qf + dn, dn + dr, absorb ? q + kLatent : q + dn,
+                                         absorb ? width : dn + dr, T, H, pos, log2_theta);
         if (cudaGetLastError() != cudaSuccess) bad = "launch";
       }
     }
@@ -436,7 +439,7 @@ extern "C" int32_t tq_mla_prologue(const TqPrologueSpec* spec, void* workspace,
     // q^T = w_uk[h]^T . qf^T with w_uk[h] seen as a 512 x Dn matrix (ld 512), qf[:, h] as
     // Dn x T (ld H (Dn + Dr)) and q[:, h] as 512 x T (ld H W).
     const float one = 1.f, zero = 0.f;
-    if (!bad && b->gemm_batched(h, CUBLAS_OP_N, CUBLAS_OP_N, kLatent, T, dn, &one,
+    if (!bad && absorb && b->gemm_batched(h, CUBLAS_OP_N, CUBLAS_OP_N, kLatent, T, dn, &one,
                                 reinterpret_cast<const void*>(s.w_uk.device_address), CUDA_R_16BF,
                                 kLatent, (long long)dn * kLatent, qf, CUDA_R_16BF, H * (dn + dr),
                                 dn + dr, &zero, q, CUDA_R_16BF, H * width, width, H,

@@ -254,7 +254,8 @@ def prologue_spec(x, w_qa, q_norm, w_qb, w_uk, w_kva, kv_norm, pos, seq_id, page
     for name, t in (("x", x), ("w_qa", w_qa), ("q_norm", q_norm), ("w_qb", w_qb), ("w_uk", w_uk),
                     ("w_kva", w_kva), ("kv_norm", kv_norm), ("pos", pos), ("seq_id", seq_id),
                     ("page_table", page_table), ("q", q)):
-        setattr(s, name, spec_of(t))
+        if t is not None:
+            setattr(s, name, spec_of(t))
     s.kv = pool_spec(kv, kv_format)
     s.heads, s.nope_dim, s.rope_dim, s.kv_format = int(heads), int(nope_dim), int(rope_dim), kv_format
     s.q_eps, s.kv_eps, s.rope_theta = float(q_eps), float(kv_eps), float(rope_theta)
@@ -267,7 +268,8 @@ class MlaPrologue:
     ``x`` bf16 ``[T, Dm]``; weights ``w_qa [Rq, Dm]``, ``q_norm [Rq]``, ``w_qb [H (Dn + Dr), Rq]``,
     ``w_uk [H, Dn, 512]``, ``w_kva [512 + Dr, Dm]``, ``kv_norm [512]``; ``pos``/``seq_id`` i32
     ``[T]``. Writes ``q`` bf16 ``[T, H, 512 + Dr]`` and each token's row into the paged pool
-    ``kv`` at ``pos`` of sequence ``seq_id`` (``kv_format`` rows). Owns only its workspace.
+    ``kv`` at ``pos`` of sequence ``seq_id`` (``kv_format`` rows). Without ``w_uk`` (None) ``q`` is
+    ``[T, H, Dn + Dr]``, not absorbed: what ``MlaChunk`` takes. Owns only its workspace.
     """
 
     def __init__(self, x, w_qa, q_norm, w_qb, w_uk, w_kva, kv_norm, pos, seq_id, page_table, kv,
@@ -297,7 +299,8 @@ def mla_prologue(x, w_qa, q_norm, w_qb, w_uk, w_kva, kv_norm, pos, seq_id, page_
                  heads, nope_dim, rope_dim, q=None, flags=None, stream=None, **kw):
     """One prologue call (see ``MlaPrologue``); returns ``q``."""
     if q is None:
-        q = torch.empty((x.shape[0], heads, 512 + rope_dim), dtype=torch.bfloat16, device=x.device)
+        width = (512 if w_uk is not None else nope_dim) + rope_dim
+        q = torch.empty((x.shape[0], heads, width), dtype=torch.bfloat16, device=x.device)
     return MlaPrologue(x, w_qa, q_norm, w_qb, w_uk, w_kva, kv_norm, pos, seq_id, page_table, kv, q,
                        heads=heads, nope_dim=nope_dim, rope_dim=rope_dim, **kw)(flags, stream)
 
@@ -313,16 +316,29 @@ class _Launch:
         if len(devices) != 1 or next(iter(devices)).type != "cuda":
             raise ValueError(f"the tensors must be on one CUDA device, not on {sorted(map(str, devices))}")
         self.device = next(iter(devices))
+        self._err = _abi.TqContractError()
+        self._err_ref = ctypes.byref(self._err)
 
-    def _run(self, launch, stream):
-        if torch.cuda.current_device() == self.device.index:
-            return launch(_stream_handle(stream))
-        with torch.cuda.device(self.device):
-            return launch(_stream_handle(stream))
+    def _check(self, validate):
+        """Raises for a rejected declaration; ``self.spec`` is what every launch passes on."""
+        self._spec_ref = ctypes.byref(self.spec)
+        raise_for(validate(self._spec_ref, self._err_ref), self._err)
+
+    def _run(self, fn, args, stream):
+        """``fn(spec, *args, stream, err)`` with the tensors' device current."""
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self._run(fn, args, stream)
+        # The raw handle without a Stream object around it: 2 us of a call that takes 6.
+        handle = (torch._C._cuda_getCurrentRawStream(self.device.index) if stream is None
+                  else stream.cuda_stream)
+        status = fn(self._spec_ref, *args, handle, self._err_ref)
+        if status:
+            raise_for(status, self._err)
 
 
 def _flags_pointer(flags):
-    return ctypes.c_void_p(flags.data_ptr()) if flags is not None else None
+    return flags.data_ptr() if flags is not None else None
 
 
 #: What ``StepPlan`` fills: the step's metadata as the other operators take it.
@@ -363,13 +379,10 @@ class StepPlan(_Launch):
         self._bind(cached_len, new_len, page_table, free_pages, free_count, t.q_start, t.seq_id)
         self.spec = step_plan_spec(cached_len, new_len, page_table, free_pages, free_count, t.q_start,
                                    t.kv_len, t.seq_id, t.q_pos, t.slot, t.free_left)
-        err = _abi.TqContractError()
-        raise_for(lib.tq_step_plan_validate(ctypes.byref(self.spec), ctypes.byref(err)), err)
+        self._check(lib.tq_step_plan_validate)
 
     def __call__(self, flags=None, stream=None):
-        err = _abi.TqContractError()
-        raise_for(self._run(lambda s: lib.tq_step_plan(ctypes.byref(self.spec), _flags_pointer(flags), s,
-                                                       ctypes.byref(err)), stream), err)
+        self._run(lib.tq_step_plan, (_flags_pointer(flags),), stream)
         return self.tables
 
 
@@ -405,14 +418,11 @@ class BlockNorm(_Launch):
     def __init__(self, y, residual, out, x=None, **kw):
         self._bind(y, residual, out, x, kw.get("post_weight"), kw.get("gate"), kw.get("pre_weight"))
         self.spec = block_norm_spec(y, residual, out, x, **kw)
-        err = _abi.TqContractError()
-        raise_for(lib.tq_block_norm_validate(ctypes.byref(self.spec), ctypes.byref(err)), err)
+        self._check(lib.tq_block_norm_validate)
         self.out, self.x = out, x
 
     def __call__(self, stream=None):
-        err = _abi.TqContractError()
-        raise_for(self._run(lambda s: lib.tq_block_norm(ctypes.byref(self.spec), s, ctypes.byref(err)),
-                            stream), err)
+        self._run(lib.tq_block_norm, (), stream)
         return self.out, self.x
 
 
@@ -458,28 +468,26 @@ class MlaChunk(_Launch):
         self._bind(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse, workspace)
         self.spec = chunk_spec(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse,
                                scale=scale, max_keys=max_keys, kv_format=kv_format)
-        err = _abi.TqContractError()
-        raise_for(lib.tq_mla_chunk_validate(ctypes.byref(self.spec), ctypes.byref(err)), err)
+        self._check(lib.tq_mla_chunk_validate)
         need = ctypes.c_uint64()
-        raise_for(lib.tq_mla_chunk_workspace_bytes(ctypes.byref(self.spec), self.device.index,
-                                                   ctypes.byref(need)))
+        raise_for(lib.tq_mla_chunk_workspace_bytes(self._spec_ref, self.device.index, ctypes.byref(need)))
         if workspace is None:
             workspace = torch.empty(need.value, dtype=torch.uint8, device=self.device)
-        if workspace.numel() * workspace.element_size() < need.value:
-            raise TqError(102, "workspace")
         self.workspace, self.out, self.lse = workspace, out, lse
+        self._args = (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        if self._args[1] < need.value or not workspace.is_contiguous():
+            raise TqError(102, "workspace")
 
     def __call__(self, stream=None):
-        err = _abi.TqContractError()
-        raise_for(self._run(lambda s: lib.tq_mla_chunk(
-            ctypes.byref(self.spec), ctypes.c_void_p(self.workspace.data_ptr()),
-            self.workspace.numel() * self.workspace.element_size(), s, ctypes.byref(err)), stream), err)
+        self._run(lib.tq_mla_chunk, self._args, stream)
         return self.out if self.lse is None else (self.out, self.lse)
 
     def device_error(self, stream=None):
+        """Device error flags of the last call (waits for ``stream``)."""
         flags = ctypes.c_int32()
-        raise_for(self._run(lambda s: lib.tq_mla_read_device_error(
-            ctypes.c_void_p(self.workspace.data_ptr()), s, ctypes.byref(flags)), stream))
+        with torch.cuda.device(self.device):
+            raise_for(lib.tq_mla_read_device_error(self.workspace.data_ptr(), _stream_handle(stream),
+                                                   ctypes.byref(flags)))
         return flags.value
 
 

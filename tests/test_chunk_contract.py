@@ -156,3 +156,20 @@ def test_oracle_equals_the_absorbed_core(fmt):
         ref, _, ref_lse = omla.mla_attention_core(q[b:e], lat, wide_uk, wide_uv, mask, scale=0.09)
         np.testing.assert_allclose(out[b:e], ref, rtol=1e-9, atol=1e-10)
         np.testing.assert_allclose(lse[b:e], ref_lse, rtol=1e-9)
+
+
+def test_prologue_without_w_uk_declares_the_query_of_the_chunk():
+    """A prologue whose w_uk has rank 0 takes q [T, H, Dn + Dr] and no space for a second one."""
+    import test_prologue_contract as tp
+    for dr, fmt in ((64, _abi.KV_BF16_ROPE576), (0, _abi.KV_FP8_E4M3)):
+        s = tp.spec(dr=dr, fmt=fmt)
+        n, m = ctypes.c_uint64(), ctypes.c_uint64()
+        assert _abi.lib.tq_mla_prologue_workspace_bytes(ctypes.byref(s), ctypes.byref(n)) == 0
+        s.w_uk = _abi.TqTensorSpec()
+        assert tp.verdict(s) == ("q", SHAPE)
+        s.q = tp.tensor([6, 4, 128 + dr], _abi.DTYPE_BF16, 12 * GiB, 2)
+        assert tp.verdict(s) is None
+        assert _abi.lib.tq_mla_prologue_workspace_bytes(ctypes.byref(s), ctypes.byref(m)) == 0
+        assert m.value < n.value
+        s.q.device_address = s.w_qb.device_address
+        assert tp.verdict(s) == ("q", ALIAS)

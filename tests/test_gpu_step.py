@@ -94,6 +94,26 @@ def test_plan_at_its_edges(cuda_device, case):
     _check_plan(cuda_device, cached, new, table, free, count, tokens)
 
 
+@pytest.mark.parametrize("requests,tokens", [(300, 1 << 19), (5000, 70000)])
+def test_plan_past_the_near_kernel(cuda_device, requests, tokens):
+    """Many requests, or many token rows: the scan that is split over clusters."""
+    rng = np.random.default_rng(requests)
+    cached, new = rng.integers(0, 300, requests), rng.integers(0, 20, requests)
+    table, free = _step(rng, requests, cached, new, 6)
+    _check_plan(cuda_device, cached, new, table, free, len(free) - 40, tokens)
+
+
+def test_plan_of_lengths_near_the_type_border(cuda_device):
+    top = 2 ** 31 - 1
+    cached, new = np.array([top, 5, top - 1]), np.array([3, top, 2])
+    table = np.arange(9).reshape(3, 3)
+    _check_plan(cuda_device, cached, np.array([3, 4, 2]), table, np.arange(20, 30), 10, 12)
+    got = ops.step_plan(_i32(cached, cuda_device), _i32(new, cuda_device), _i32(table, cuda_device),
+                        _i32([40], cuda_device), _i32([1], cuda_device), tokens=10)
+    assert got.q_start.tolist() == [0, 3, 10, 10] and got.kv_len.tolist() == [192, 128, 192]
+    assert got.q_pos.tolist() == [top] * 3 + list(range(5, 12))   # positions past 31 bits stay at the top
+
+
 def test_plan_of_no_requests(cuda_device):
     e = torch.empty(0, dtype=torch.int32, device=cuda_device)
     got = ops.step_plan(e, e, e.view(0, 3), _i32([4, 5], cuda_device), _i32([2], cuda_device), tokens=3)
