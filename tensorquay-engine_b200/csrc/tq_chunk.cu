@@ -50,6 +50,8 @@ enum Header : int {
   kHdrBlocks = 2,  // query blocks
   kHdrPieces = 3,  // pieces of all blocks: units of one head
   kHdrSplit = 4,   // 1 if some block has more than one piece
+  kHdrWhere = 8,   // first wait that ran out: shared address of its barrier
+  kHdrWho = 9,     // its block, and the kernel's block size << 16
   kHdrWords = 64
 };
 
@@ -403,22 +405,24 @@ constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr uint32_t kWaitPolls = 1u << 26;
 
 // Bounded waits of one role of a CTA pair. What they wait for lies in TMEM or is written and read by
-// the asynchronous proxies (TMA, MMA), ordered by the barriers and tcgen05 fences themselves: no wait
-// or arrival here needs the cluster-scope release or acquire of generic memory, which cost a
-// memory barrier per tile (2.0 of 9.8 warps stalled in it). The first that runs out sets the error flag and both
-// CTAs' abort words; every later wait of the pair then returns false at once.
+// the asynchronous proxies (TMA, MMA), ordered by the barriers and tcgen05 fences themselves: no
+// wait or arrival here needs the cluster-scope release or acquire of generic memory, which cost a
+// memory barrier per tile (2.0 of 9.8 warps stalled in it). The first wait that runs out writes its
+// barrier into both CTAs' abort words, and every later wait of the pair returns false soon; the
+// error flag is set at the end, in one place: a wait is inlined at two dozen places, and every
+// instruction of it competes for the instruction caches with the loops that it stands in.
 struct Waiter {
-  int* header;
   uint32_t abort;  // shared address of this CTA's abort word
-  int rank;
   bool failed;
 
+  // Polls: a suspended wait (mbarrier.try_wait) can resume long after its phase completed, or not
+  // within its bound.
   __device__ bool on(uint32_t bar, uint32_t parity) {
     if (failed) return false;
     uint64_t t0 = 0;  // reading the timer is slow: only a wait of many polls does
     for (uint32_t i = 1;; ++i) {
-      if (ptx::mbar_try(bar, parity)) return true;
-      if ((i & 15) == 0) {
+      if (ptx::mbar_test(bar, parity)) return true;
+      if ((i & 1023) == 0) {
         if (ptx::ld_shared_u32(abort)) {
           failed = true;
           return false;
@@ -426,9 +430,8 @@ struct Waiter {
         const uint64_t now = ptx::global_timer_ns();
         if (t0 == 0) t0 = now;
         if (i >= kWaitPolls || now - t0 > kWaitNs) {
-          ptx::st_cluster_u32(ptx::map_peer(abort, uint32_t(rank)), 1u);
-          ptx::st_cluster_u32(ptx::map_peer(abort, uint32_t(rank ^ 1)), 1u);
-          atomicOr(header + kHdrError, TQ_DEV_WAIT_TIMEOUT);
+          ptx::st_cluster_u32(ptx::map_peer(abort, 0), bar);
+          ptx::st_cluster_u32(ptx::map_peer(abort, 1), bar);
           failed = true;
           return false;
         }
@@ -442,9 +445,16 @@ struct Waiter {
     failed = true;
     return false;
   }
-  // After an abort: a millisecond in which the pair's copies and MMAs in flight land.
-  __device__ void settle() {
-    if (!ptx::ld_shared_u32(abort)) return;
+  // The end of an aborted CTA: the error flag, and a millisecond in which the pair's copies and MMAs
+  // in flight land.
+  __device__ void settle(int* header) {
+    const uint32_t bar = ptx::ld_shared_u32(abort);
+    if (!bar) return;
+    if (threadIdx.x == 0) {
+      atomicOr(header + kHdrError, TQ_DEV_WAIT_TIMEOUT);
+      if (atomicCAS(header + kHdrWhere, 0, int(bar)) == 0)
+        header[kHdrWho] = int(blockIdx.x | (blockDim.x << 16));
+    }
     const uint64_t t0 = ptx::global_timer_ns();
     for (uint32_t i = 0; i < (1u << 20) && ptx::global_timer_ns() - t0 < 1000000ull; ++i) {
     }
@@ -506,7 +516,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::cluster_sync();
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  Waiter wt{a.w.header, base + kSmMisc + 4, rank, false};
+  Waiter wt{base + kSmMisc + 4, false};
 
   // Column blocks (a head, or a head's k or v) by row tiles, one contiguous range per pair. The
   // first one's column block, floor(floor(tiles * blocks * pair / pairs) / tiles), does not depend
@@ -521,34 +531,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                           a.head0 + (per_head == 2 ? g >> 1 : g));
   };
   if (threadIdx.x == 0)
-    for (int c = 0; c < kChunks; ++c) load_weights(int((long long)columns * pair / pairs), c);
+    for (int c = 0; c < kChunks; ++c) load_weights(columns * pair / pairs, c);
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const long long tiles = (a.w.header[kHdrRows] + 255) / 256;
-  const long long items = tiles * columns;
-  const long long first = items * pair / pairs, last = items * (pair + 1) / pairs;
+  // At most kScratchBytes of 128 KB items, or the 2^17 row tiles of one head: 32 bits hold the
+  // products with the pairs.
+  const uint32_t tiles = uint32_t(a.w.header[kHdrRows] + 255) / 256;
+  const uint32_t items = tiles * uint32_t(columns);
+  const uint32_t first = items * uint32_t(pair) / uint32_t(pairs);
+  const uint32_t last = items * uint32_t(pair + 1) / uint32_t(pairs);
+  const uint32_t g0 = tiles ? first / tiles : 0u, tile0 = first - g0 * tiles;
   if (warp == 0) {
     if (lane == 0) {
       uint32_t stage = 0, phase = 0, blocks = 0;
-      for (long long i = first; i < last && !wt.failed; ++i) {
-        const int g = int(i / tiles), tile = int(i % tiles);
+      uint32_t g = g0, tile = tile0;
+      for (uint32_t i = first; i < last && !wt.failed; ++i) {
         const bool fresh = i == first || tile == 0;
         for (int c = 0; c < kChunks; ++c) {
           if (fresh && blocks > 0) {
             if (!wt.on(bar(kBarWEmpty + c), (blocks - 1) & 1u)) break;
-            load_weights(g, c);
+            load_weights(int(g), c);
           }
           if (!wt.on(bar(kBarAEmpty + stage), phase ^ 1u)) break;
           if (rank == 0) ptx::mbar_expect_tx(bar(kBarAFull + stage), 2 * kBox);
           ptx::tma_load_2d_pair(base + kSmA + stage * kBox, &tm_rows,
                                 ptx::map_peer(bar(kBarAFull + stage), 0), c * 64,
-                                tile * 256 + rank * 128);
+                                int(tile) * 256 + rank * 128);
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
         if (fresh) ++blocks;
+        if (++tile == tiles) {
+          tile = 0;
+          ++g;
+        }
       }
     }
     __syncwarp();
@@ -556,9 +574,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (rank == 0) {
       constexpr uint32_t idesc = ptx::idesc_bf16(256, 256, 0);
       const uint32_t elected = ptx::elect_one();
-      uint32_t stage = 0, phase = 0, blocks = 0, n = 0;
-      for (long long i = first; i < last && !wt.failed; ++i, ++n) {
-        const int tile = int(i % tiles);
+      uint32_t stage = 0, phase = 0, blocks = 0, n = 0, tile = tile0;
+      for (uint32_t i = first; i < last && !wt.failed; ++i, ++n) {
         const bool fresh = i == first || tile == 0, done = i + 1 == last || tile == tiles - 1;
         const uint32_t buf = n & 1u;
         if (n >= 2 && !wt.all(bar(kBarAccEmpty + buf), ((n >> 1) - 1) & 1u)) break;
@@ -580,6 +597,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         ptx::mma_commit_pair(bar(kBarAccFull + buf));
         if (fresh) ++blocks;
+        if (++tile == tiles) tile = 0;
       }
       // A pair without items has its weights in flight all the same.
       if (first >= last)
@@ -589,20 +607,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp >= 4) {
     const int quad = warp & 3, row = quad * 32 + lane;
-    uint32_t n = 0;
-    for (long long i = first; i < last; ++i, ++n) {
-      const int g = int(i / tiles), tile = int(i % tiles);
+    uint32_t n = 0, g = g0, tile = tile0;
+    for (uint32_t i = first; i < last; ++i, ++n) {
       const uint32_t buf = n & 1u;
       if (!wt.all(bar(kBarAccFull + buf), (n >> 1) & 1u)) break;
       ptx::tc_fence_after();
       const long long r = (long long)tile * 256 + rank * 128 + row;
-      const int h = per_head == 2 ? g >> 1 : g;  // of this pass
+      const uint32_t h = per_head == 2 ? g >> 1 : g;  // of this pass
       uint16_t* kd = a.w.k + ((long long)h * a.cap + r) * a.dn;
       uint16_t* vd = a.w.v + ((long long)h * a.cap + r) * a.dv;
       uint16_t* lo = per_head == 2 ? ((g & 1) ? vd : kd) : kd;
       uint16_t* hi = per_head == 2 ? lo + 128 : vd;
       const uint32_t src = tmem + buf * 256 + (uint32_t(quad * 32) << 16);
-#pragma unroll
+#pragma unroll 2
       for (int c = 0; c < 256; c += 32) {
         uint32_t x[32], y[16];
         ptx::tmem_ld32(src + c, x);
@@ -617,12 +634,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive_cluster_relaxed(ptx::map_peer(bar(kBarAccEmpty + buf), 0));
+      if (++tile == tiles) {
+        tile = 0;
+        ++g;
+      }
     }
   }
   // Every commit of the leader has arrived in both CTAs before either leaves. One warp polls for it;
   // the others go on to the cluster barrier, which costs no issue slots.
   if (warp == 0) wt.on(bar(kBarDrain), 0);
-  wt.settle();
+  wt.settle(a.w.header);
   ptx::tc_fence_before();
   ptx::cluster_sync();
   if (warp == 1) {
@@ -698,10 +719,9 @@ struct Shape {
   static constexpr uint32_t kSmBytes = kSmMisc + 16 + 1024;
   static constexpr uint32_t kTmemO = kS * 128;
   // Quarter of a tile's exponentials after which the turn passes. The earlier, the more the two
-  // groups' exponentials overlap and slow each other; the later, the longer a tile takes. With three
-  // score buffers the first is best (2 x 2048 tokens, 128 heads: 2.05 ms after the first quarter, 2.25
-  // after the third), with two the third (4096 tokens, 64 heads: 703 us, 716 after the first).
-  static constexpr int kTurn = kS == 3 ? 0 : 2;
+  // groups' exponentials overlap and slow each other; the later, the longer a tile takes (after the
+  // first quarter 1553 us of attention for 2 x 2048 tokens of 128 heads, after the second 1545).
+  static constexpr int kTurn = 1;
   static_assert(kSmBytes <= 232448, "shared memory per CTA");
   static_assert(kTmemO + kDv <= 512, "TMEM columns");
 };
@@ -783,16 +803,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::cluster_sync();
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  Waiter wt{a.w.header, base + C::kSmMisc + 4, rank, false};
+  Waiter wt{base + C::kSmMisc + 4, false};
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   // All 512 columns are this CTA's, so they start at 0.
   const int pieces = a.w.header[kHdrPieces], units = pieces * a.pass_heads;
 
-  // 384 threads start with 168 registers each; the softmax warpgroups take what the first gives up:
-  // 128 * 96 + 256 * 200 = 63488 of 64512.
   if (warp == 0) {
-    ptx::registers_down<96>();
     if (lane == 0) {
       uint32_t useq = 0;
       Phases<C::kKv> free;
@@ -824,15 +841,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    ptx::registers_down<96>();
     if (rank == 0) {
       constexpr uint32_t idesc_qk = ptx::idesc_bf16(256, 128, 0);
       constexpr uint32_t idesc_pv = ptx::idesc_bf16(256, kDv, 1);
       const uint32_t elected = ptx::elect_one();
       uint32_t useq = 0;  // units with tiles so far
       Phases<C::kS> k_full, v_full, p_full;
-      // The tile in stage and score buffer `st`, a constant in every call: the MMA operands are
-      // then constants too.
       auto issue_qk = [&](uint32_t st) -> bool {
         if (!wt.all(bar(C::kKFull + st), k_full.take(st))) return false;
         ptx::tc_fence_after();
@@ -850,43 +864,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int tiles = unit_at(a, u, pieces).p.tiles;
         if (!tiles) continue;
         if (!wt.all(bar(C::kQFull), useq & 1u)) break;
-#pragma unroll
-        for (int j = 0; j < C::kS; ++j)
-          if (j < tiles && !wt.failed) issue_qk(j);
-        if (tiles <= C::kS) ptx::mma_commit_pair(bar(C::kQEmpty));
-        // The unit before must have read its output before this one's first PV replaces it.
-        if (useq > 0 && !wt.all(bar(C::kOFree), (useq - 1) & 1u)) break;
-        for (int j0 = 0; j0 < tiles && !wt.failed; j0 += C::kS) {
-#pragma unroll
+        // Tile j's PV and, in its place, tile j + kS's QK^T; the first kS tiles' QK^T lead.
+        for (int j0 = -C::kS; j0 < tiles && !wt.failed; j0 += C::kS) {
+#pragma unroll 1
           for (int st = 0; st < C::kS; ++st) {
             const int j = j0 + st;
             if (j >= tiles || wt.failed) break;
-            if (!wt.all(bar(C::kVFull + st), v_full.take(st))) break;
-            // V as B, MN-major: 64 value columns are a chunk of [128 keys][128 B], 8-key groups
-            // 1 KB apart; a step of 16 keys is 2 KB. The first 64 keys go ahead of the rest.
-            const uint64_t vd = ptx::smem_desc(base + C::kSmV + st * C::kVBytes, 16384, 1024, 2);
-            const uint32_t phase = p_full.take(st);
-            if (!wt.all(bar(C::kPFull + 2 * st), phase)) break;
-            ptx::tc_fence_after();
-            ptx::mma_ts_pair_x4(elected, C::kTmemO, st * 128, vd, idesc_pv, j > 0 ? 1u : 0u);
-            if (!wt.all(bar(C::kPFull + 2 * st + 1), phase)) break;
-            ptx::tc_fence_after();
-            ptx::mma_ts_pair_x4(elected, C::kTmemO, st * 128 + 32, vd + 512, idesc_pv, 1u);
-            ptx::mma_commit_pair(bar(C::kVEmpty + st));
-            ptx::mma_commit_pair(bar(C::kPvDone + st));
+            if (j >= 0) {
+              // The unit before must have read its output before this one's first PV replaces it.
+              if (j == 0 && useq > 0 && !wt.all(bar(C::kOFree), (useq - 1) & 1u)) break;
+              if (!wt.all(bar(C::kVFull + st), v_full.take(st))) break;
+              // V as B, MN-major: 64 value columns are a chunk of [128 keys][128 B], 8-key groups
+              // 1 KB apart; a step of 16 keys is 2 KB. The first 64 keys go ahead of the rest.
+              const uint64_t vd =
+                  ptx::smem_desc(base + C::kSmV + st * C::kVBytes, 16384, 1024, 2);
+              const uint32_t phase = p_full.take(st);
+              if (!wt.all(bar(C::kPFull + 2 * st), phase)) break;
+              ptx::tc_fence_after();
+              ptx::mma_ts_pair_x4(elected, C::kTmemO, st * 128, vd, idesc_pv, j > 0 ? 1u : 0u);
+              if (!wt.all(bar(C::kPFull + 2 * st + 1), phase)) break;
+              ptx::tc_fence_after();
+              ptx::mma_ts_pair_x4(elected, C::kTmemO, st * 128 + 32, vd + 512, idesc_pv, 1u);
+              ptx::mma_commit_pair(bar(C::kVEmpty + st));
+              ptx::mma_commit_pair(bar(C::kPvDone + st));
+            }
             if (j + C::kS < tiles) {
               if (!issue_qk(st)) break;
               if (j + C::kS + 1 == tiles) ptx::mma_commit_pair(bar(C::kQEmpty));
             }
           }
         }
-        ++useq;
+      ++useq;
       }
       ptx::mma_commit_pair(bar(C::kDrain));
     }
     __syncwarp();
   } else if (warp == 2) {
-    ptx::registers_down<96>();
     if (lane == 0) {
       Phases<C::kKv> free;
       for (int u = pair; u < units && !wt.failed; u += pairs) {
@@ -906,7 +919,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 3) {
-    ptx::registers_down<96>();
     uint32_t n = 0;
     for (int u = pair; u < units && !wt.failed; u += pairs, ++n) {
       const Unit x = unit_at(a, u, pieces);
@@ -937,7 +949,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else {
-    ptx::registers_up<200>();
     const int group = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = uint32_t(quad * 32) << 16;
     float* shared_m = reinterpret_cast<float*>(sm + C::kSmExch);  // [128]
@@ -966,26 +977,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ptx::tc_fence_after();
         const uint32_t src = tmem + sb * 128 + lanes;
         const int key = (tile0 + j) * kRowTile;
-        uint32_t r[4][32];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) ptx::tmem_ld32(src + 32 * g, r[g]);
-        ptx::tmem_wait_ld();
-        if (!__all_sync(0xFFFFFFFFu, n >= key + kRowTile)) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
+        const bool whole = __all_sync(0xFFFFFFFFu, n >= key + kRowTile);
+        auto scores = [&](uint32_t (&r)[32], int g) {
+          ptx::tmem_ld32(src + 32 * g, r);
+          ptx::tmem_wait_ld();
+          if (!whole) {
+            const int see = n - key - 32 * g;
+            const uint32_t bits = see >= 32 ? 0xFFFFFFFFu : see <= 0 ? 0u : (1u << see) - 1u;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (key + 32 * g + i >= n) r[g][i] = 0xFF800000u;  // -inf
-        }
+              if (!(bits & (1u << i))) r[i] = 0xFF800000u;  // -inf
+          }
+        };
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
+#pragma unroll 1
+        for (int g = 0; g < 4; ++g) {
+          uint32_t r[32];
+          scores(r, g);
 #pragma unroll
           for (int i = 0; i < 32; i += 8)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              top[k] = fmaxf(fmaxf(top[k], __uint_as_float(r[g][i + k])),
-                             __uint_as_float(r[g][i + 4 + k]));
+              top[k] = fmaxf(fmaxf(top[k], __uint_as_float(r[i + k])), __uint_as_float(r[i + 4 + k]));
+        }
         const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         // The turn passes from tile to tile, and so from group to group, with the row's reference
         // maximum: one group at a time is in its exponentials.
@@ -1001,6 +1015,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             wt.all(bar(C::kPvDone + b % C::kS), pv_done.at(b % C::kS, b / C::kS));
             ptx::tc_fence_after();
             const uint32_t o = tmem + C::kTmemO + lanes;
+#pragma unroll 1
             for (int i = 0; i < kDv; i += 16) {
               uint32_t v[16];
               ptx::tmem_ld16(o + i, v);
@@ -1021,13 +1036,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           m = ref;
         }
         const float mc = ref == -INFINITY ? 0.f : -ref * c;
-#pragma unroll
+#pragma unroll 1
         for (int g = 0; g < 4; ++g) {
-          uint32_t p[16];
+          uint32_t r[32], p[16];
+          scores(r, g);
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const float p0 = ptx::ex2(fmaf(__uint_as_float(r[g][i]), c, mc));
-            const float p1 = ptx::ex2(fmaf(__uint_as_float(r[g][i + 1]), c, mc));
+            const float p0 = ptx::ex2(fmaf(__uint_as_float(r[i]), c, mc));
+            const float p1 = ptx::ex2(fmaf(__uint_as_float(r[i + 1]), c, mc));
             sum[(i >> 1) & 1][0] += p0;
             sum[(i >> 1) & 1][1] += p1;
             p[i / 2] = ptx::pack_bf16x2(p0, p1);
@@ -1106,18 +1122,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < 32; ++k)
           v[k] = sees ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
-        if (f32) {
 #pragma unroll 1
-          for (int g = 0; g < 2; ++g) {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) y[k] = g ? v[16 + k] : v[k];
-            emit(y, 4 * col + 64 * g);
-          }
-        } else {
+        for (int g = 0; g <= int(f32); ++g) {
 #pragma unroll
           for (int k = 0; k < 16; ++k)
-            y[k] = ptx::pack_bf16x2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
-          emit(y, 2 * col);
+            y[k] = !f32 ? ptx::pack_bf16x2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]))
+                   : g  ? v[16 + k]
+                        : v[k];
+          emit(y, f32 ? 4 * col + 64 * g : 2 * col);
         }
       }
       if (tiles) {
@@ -1135,7 +1147,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
   }
   if (warp == 0) wt.on(bar(C::kDrain), 0);
-  wt.settle();
+  wt.settle(a.w.header);
   ptx::tc_fence_before();
   ptx::cluster_sync();
   if (warp == 1) {
