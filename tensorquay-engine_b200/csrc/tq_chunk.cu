@@ -688,7 +688,7 @@ constexpr float kSlack = 8.f;  // log2 units
 // What the softmax warps need of a unit, fetched ahead by warp 3.
 struct Info {
   int seen[128];  // keys that each of this CTA's query rows sees; kSpoilt: one is not finite
-  int row0, rows, tile0, tiles, head, whole, unused0, unused1;
+  int row0, rows, tile0, tiles, head, whole, slot, unused;
 };
 constexpr int kSpoilt = 1 << 30;
 // A warp's 32 output rows of 64 bytes, 80 bytes apart (16-byte accesses without bank conflicts).
@@ -749,6 +749,7 @@ struct Phases {
 struct Unit {
   Piece p;
   int head;  // of this pass
+  int slot;  // of its partial output: pieces of one head in piece order
 };
 
 // Units in order: head, so that the pairs at work at one time share the keys and values of few heads
@@ -756,7 +757,9 @@ struct Unit {
 __device__ __forceinline__ Unit unit_at(const Args& a, int u, int pieces) {
   Unit x;
   x.head = u / pieces;
-  const int4* src = reinterpret_cast<const int4*>(a.w.pieces + (pieces - 1 - (u - x.head * pieces)));
+  const int piece = pieces - 1 - (u - x.head * pieces);
+  x.slot = x.head * pieces + piece;
+  const int4* src = reinterpret_cast<const int4*>(a.w.pieces + piece);
   const int4 lo = src[0], hi = src[1];
   x.p = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
   return x;
@@ -943,6 +946,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         info->tiles = x.p.tiles;
         info->head = x.head;
         info->whole = x.p.whole;
+      info->slot = x.slot;
       }
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar(C::kInfoFull + int(n & 1u)));
@@ -1084,13 +1088,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int head = a.head0 + info->head, rows = info->rows - rank * 128;
       const int t0 = info->row0 + rank * 128;
       const bool whole = info->whole != 0;
+      const long long part = (long long)info->slot * kQueryTile + rank * 128;
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar(C::kInfoEmpty + int(nth & 1u)));
       // Rows of this warp: through shared memory 64 bytes a row at a time, so that four lanes store
       // 64 consecutive bytes (a lane a row stored 16 bytes each to 32 lines at once: 7500 cycles a
       // unit at 256 columns).
       const bool f32 = a.out_f32 || !whole;
-      const long long part = (long long)u * kQueryTile + rank * 128;
       uint8_t* out0 = whole ? a.out + (long long)t0 * a.out_st + (long long)head * a.out_sh
                             : reinterpret_cast<uint8_t*>(a.w.part_out + part * kDv);
       const long long out_row = whole ? a.out_st : (long long)kDv * 4;

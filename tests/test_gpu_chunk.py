@@ -210,6 +210,18 @@ def test_one_long_row_of_work(cuda_device):
     c.check()
 
 
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("new,cached,heads", [([18, 353, 1], [3651, 0, 0], 3), ([2, 312], [4219, 403], 5),
+                                              ([345, 6, 2, 75], [2130, 38, 101, 14], 2),
+                                              ([1, 3, 280, 17, 4], [2231, 477, 3024, 0, 3], 2)])
+def test_split_and_whole_blocks_together(cuda_device, fmt, new, cached, heads):
+    """Blocks of very different lengths in one call: some are split over their keys, in different
+    numbers of pieces, some are not."""
+    c = Case(cuda_device, fmt, new, cached, heads=heads, seed=len(new))
+    c.launch()()
+    c.check()
+
+
 def test_many_sequences(cuda_device):
     rng = np.random.default_rng(8)
     new, cached = rng.integers(0, 30, 1100), rng.integers(0, 3, 1100)
