@@ -50,9 +50,10 @@ enum Header : int {
   kHdrBlocks = 2,  // query blocks
   kHdrPieces = 3,  // pieces of all blocks: units of one head
   kHdrSplit = 4,   // 1 if some block has more than one piece
-  kHdrWhere = 8,   // first wait that ran out: shared address of its barrier
-  kHdrWho = 9,     // its block, and the kernel's block size << 16
-  kHdrWords = 64
+  kHdrWhere = 5,   // first wait that ran out: shared address of its barrier
+  kHdrWho = 6,     // its block, and the kernel's block size << 16
+  kHdrNext = 8,    // [128] next unit of each pass over the heads
+  kHdrWords = 136
 };
 
 // One query block of one sequence.
@@ -67,7 +68,7 @@ struct Block {
 // Row tiles tile0 .. tile0 + tiles - 1 of a block.
 struct __align__(16) Piece {
   int row0, rows, key0, tile0;
-  int tiles, seq, whole, block;  // whole: the block's only piece
+  int tiles, seq, whole, index;  // whole: the block's only piece; index: in block order
 };
 
 struct Work {
@@ -77,7 +78,8 @@ struct Work {
   int* seq_block;  // [S + 1] first query block of each sequence
   int* seq_spoilt; // [S] first cached row that is not finite (INT_MAX: none)
   Block* blocks;
-  Piece* pieces;
+  Piece* pieces;    // in block order
+  Piece* order;     // in the order in which they run
   float* part_out;  // f32 [units, kQueryTile, Dv] of split blocks, each normalised
   float* part_lse;  // f32 [units, kQueryTile] base-2 log sums
   uint16_t* rows;   // bf16 [cap, 512]
@@ -102,7 +104,7 @@ struct Args {
   long long uk_sh, uk_sr, uv_sh, uv_sr;           // elements
   long long row_stride;
   int tokens, heads, seqs, slots, pages, cap, max_blocks;
-  int head0, pass_heads;
+  int head0, pass_heads, pass;
   int split_units;  // most units of a pass after splitting; 0: blocks are not split
   int pairs;
   int dn, dr, dv, fp8, out_f32;
@@ -147,6 +149,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
   __shared__ int s_rows, s_blocks, s_over, s_split;
   // The first 1024 sequences and blocks again, near: the steps below read each other's results.
   __shared__ int n_q0[1025], n_block[1025], n_key0[1024], n_keys[1024], n_tiles[1024];
+  __shared__ int n_length[1024];  // tiles of the pieces
   const Work& w = a.w;
   const int tid = threadIdx.x;
   if (tid < kHdrWords) w.header[tid] = 0;
@@ -311,17 +314,33 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
       w.blocks[b] = {row0, rows, key0, tiles, s, at, n, 0};
       // Pieces of one length, the last ones shorter.
       const int each = max(1, (tiles + n - 1) / n);
-      for (int i = 0; i < n; ++i)
-        w.pieces[at + i] = {row0, rows, key0, i * each, max(0, min(each, tiles - i * each)), s,
-                            n == 1, b};
+      for (int i = 0; i < n; ++i) {
+        const int length = max(0, min(each, tiles - i * each));
+        w.pieces[at + i] = {row0, rows, key0, i * each, length, s, n == 1, at + i};
+        if (at + i < 1024) n_length[at + i] = length;
+      }
       if (n > 1) s_split = 1;
     }
     __syncthreads();
     if (tid == 1023) s_rows = at + n;
     __syncthreads();
   }
+  // The order in which a head's pieces run: the longest first, so that the last ones to run are
+  // short (up to 1024 pieces; more are left in their order).
+  const int pieces = s_rows;
+  if (tid < pieces && pieces <= 1024) {
+    const int mine = n_length[tid];
+    int rank = 0;
+    for (int i = 0; i < pieces; ++i) {
+      const int other = n_length[i];
+      rank += other > mine || (other == mine && i < tid);
+    }
+    w.order[rank] = w.pieces[tid];
+  } else if (pieces > 1024) {
+    for (int i = tid; i < pieces; i += 1024) w.order[i] = w.pieces[i];
+  }
   if (tid == 0) {
-    w.header[kHdrPieces] = s_rows;
+    w.header[kHdrPieces] = pieces;
     w.header[kHdrSplit] = s_split;
   }
 }
@@ -685,10 +704,11 @@ namespace attend {
 constexpr int kThreads = 384;
 constexpr float kSlack = 8.f;  // log2 units
 
-// What the softmax warps need of a unit, fetched ahead by warp 3.
+// A unit as the warps of a CTA take it, fetched ahead by warp 3. tiles < 0: there are no more.
 struct Info {
   int seen[128];  // keys that each of this CTA's query rows sees; kSpoilt: one is not finite
-  int row0, rows, tile0, tiles, head, whole, slot, unused;
+  int row0, rows, key0, tile0;
+  int tiles, whole, head, slot;  // head of this pass; slot of a piece's partial output
 };
 constexpr int kSpoilt = 1 << 30;
 // A warp's 32 output rows of 64 bytes, 80 bytes apart (16-byte accesses without bank conflicts).
@@ -705,8 +725,8 @@ struct Shape {
   static constexpr uint32_t kVBytes = kVChunks * 128 * 128;
   static constexpr uint32_t kSmK = kQBytes;
   static constexpr uint32_t kSmV = kSmK + kKv * kKBytes;
-  static constexpr uint32_t kSmExch = kSmV + kKv * kVBytes;  // f32 [3][128], int [4]
-  static constexpr uint32_t kSmInfo = kSmExch + 1552;         // 2 x Info
+  static constexpr uint32_t kSmExch = kSmV + kKv * kVBytes;  // f32 [3][128], int [4], mail
+  static constexpr uint32_t kSmInfo = kSmExch + 1568;         // 2 x Info
   static constexpr uint32_t kSmTurn = kSmInfo + 2 * sizeof(Info);  // output rows, kTurnBytes a warp
   static constexpr uint32_t kSmBars = kSmTurn + 8 * kTurnBytes;
   static constexpr int kQFull = 0, kQEmpty = 1, kKFull = 2, kKEmpty = kKFull + kKv;
@@ -714,7 +734,8 @@ struct Shape {
   static constexpr int kSFull = kVEmpty + kKv, kPFull = kSFull + kS;
   static constexpr int kPvDone = kPFull + 2 * kS, kOFree = kPvDone + kS, kDrain = kOFree + 1;
   static constexpr int kInfoFull = kDrain + 1, kInfoEmpty = kInfoFull + 2;
-  static constexpr int kBars = kInfoEmpty + 2;
+  static constexpr int kMailFull = kInfoEmpty + 2, kMailEmpty = kMailFull + 1;
+  static constexpr int kBars = kMailEmpty + 1;
   static constexpr uint32_t kSmMisc = kSmBars + 8 * kBars;
   static constexpr uint32_t kSmBytes = kSmMisc + 16 + 1024;
   static constexpr uint32_t kTmemO = kS * 128;
@@ -749,17 +770,26 @@ struct Phases {
 struct Unit {
   Piece p;
   int head;  // of this pass
-  int slot;  // of its partial output: pieces of one head in piece order
 };
 
-// Units in order: head, so that the pairs at work at one time share the keys and values of few heads
-// in L2, then query block from the last, which sees the most of its sequence, to the first.
-__device__ __forceinline__ Unit unit_at(const Args& a, int u, int pieces) {
+// Units in the order in which they are taken: head by head, so that the pairs at work at one time
+// share the keys and values of few heads in L2, and within a head the longest piece first. The last
+// two rounds' worth of heads go piece by piece instead, so that the call ends on short units (with a
+// fixed round-robin of units the longest pair had 11% more than the mean at 4096 tokens, 12% in a
+// ragged batch; now about 2%).
+__device__ __forceinline__ Unit unit_at(const Args& a, int u, int pieces, int pairs) {
+  const int last = min(a.pass_heads, (2 * pairs + pieces - 1) / pieces);
+  const int first = (a.pass_heads - last) * pieces;  // units of the heads before those
   Unit x;
-  x.head = u / pieces;
-  const int piece = pieces - 1 - (u - x.head * pieces);
-  x.slot = x.head * pieces + piece;
-  const int4* src = reinterpret_cast<const int4*>(a.w.pieces + piece);
+  int piece;
+  if (u < first) {
+    x.head = u / pieces;
+    piece = u - x.head * pieces;
+  } else {
+    piece = (u - first) / last;
+    x.head = a.pass_heads - last + (u - first) - piece * last;
+  }
+  const int4* src = reinterpret_cast<const int4*>(a.w.order + piece);
   const int4 lo = src[0], hi = src[1];
   x.p = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
   return x;
@@ -779,7 +809,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint8_t* sm = smem_raw + (base - raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = int(ptx::cluster_rank());
-  const int pair = int(blockIdx.x) >> 1, pairs = int(gridDim.x) >> 1;
+  const int pairs = int(gridDim.x) >> 1;
   auto bar = [&](int i) { return base + C::kSmBars + 8u * uint32_t(i); };
   auto lead = [&](int i) { return ptx::map_peer(bar(i), 0); };
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sm + C::kSmMisc);
@@ -787,8 +817,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int i = 0; i < C::kBars; ++i) {
       // P of half a tile: its group's four warps in either CTA; the release of O: all softmax warps.
       const bool joint = i >= C::kPFull && i < C::kPFull + 2 * C::kS;
-      const bool read = i >= C::kInfoEmpty;  // eight warps have taken a unit's info
-      ptx::mbar_init(bar(i), joint || read ? 8 : i == C::kOFree ? 16 : 1);
+      // A unit's info: every warp but the one that fetches it and a follower's idle warp 1.
+      const bool read = i >= C::kInfoEmpty && i < C::kInfoEmpty + 2;
+      ptx::mbar_init(bar(i), joint ? 8 : read ? 11 - rank : i == C::kOFree ? 16 : 1);
     }
     tmem_holder[1] = 0;  // the abort word
     for (int i = 0; i < 4; ++i) reinterpret_cast<int*>(sm + C::kSmExch + 1536)[i] = 0;
@@ -811,24 +842,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::grid_launch_dependents();
   // All 512 columns are this CTA's, so they start at 0.
   const int pieces = a.w.header[kHdrPieces], units = pieces * a.pass_heads;
+  // The n-th unit, for one lane of a load warp; the MMA warp takes it as a whole.
+  struct UnitRef {
+    int row0, key0, tiles, head;
+  };
+  auto next_unit = [&](uint32_t n) -> UnitRef {
+    const int slot = int(n & 1u);
+    if (!wt.on(bar(C::kInfoFull + slot), (n >> 1) & 1u)) return {0, 0, -1, 0};
+    const Info* info = reinterpret_cast<const Info*>(sm + C::kSmInfo) + slot;
+    const UnitRef x = {info->row0, info->key0, info->tiles, info->head};
+    ptx::mbar_arrive(bar(C::kInfoEmpty + slot));
+    return x;
+  };
 
   if (warp == 0) {
     if (lane == 0) {
       uint32_t useq = 0;
       Phases<C::kKv> free;
-      for (int u = pair; u < units && !wt.failed; u += pairs) {
-        const Unit x = unit_at(a, u, pieces);
-        if (!x.p.tiles) continue;
+      for (uint32_t n = 0;; ++n) {
+        const UnitRef x = next_unit(n);
+        if (x.tiles < 0) break;
+        if (!x.tiles) continue;
         if (!wt.on(bar(C::kQEmpty), (useq & 1u) ^ 1u)) break;
         if (rank == 0) ptx::mbar_expect_tx(bar(C::kQFull), 2 * C::kQBytes);
 #pragma unroll
         for (int c = 0; c < C::kQChunks; ++c)
           ptx::tma_load_3d_pair(base + c * 16384, &tm_q, lead(C::kQFull), c * 64, a.head0 + x.head,
-                                x.p.row0 + rank * 128);
+                                x.row0 + rank * 128);
         ++useq;
-        for (int j = 0; j < x.p.tiles; ++j) {
+        for (int j = 0; j < x.tiles; ++j) {
           const uint32_t st = uint32_t(j % C::kKv), ph = free.take(st) ^ 1u;
-          const int key = x.p.key0 + (x.p.tile0 + j) * kRowTile;
+          const int key = x.key0 + j * kRowTile;
           if (!wt.on(bar(C::kKEmpty + st), ph)) break;
           if (rank == 0) ptx::mbar_expect_tx(bar(C::kKFull + st), 2 * C::kKBytes);
           const uint32_t kd = base + C::kSmK + st * C::kKBytes;
@@ -863,8 +907,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ptx::mma_commit_pair(bar(C::kKEmpty + st));
         return true;
       };
-      for (int u = pair; u < units && !wt.failed; u += pairs) {
-        const int tiles = unit_at(a, u, pieces).p.tiles;
+      for (uint32_t n = 0;; ++n) {
+        const int slot = int(n & 1u);
+        if (!wt.all(bar(C::kInfoFull + slot), (n >> 1) & 1u)) break;
+        const int tiles = __shfl_sync(
+            0xFFFFFFFFu, (reinterpret_cast<const Info*>(sm + C::kSmInfo) + slot)->tiles, 0);
+        if (lane == 0) ptx::mbar_arrive(bar(C::kInfoEmpty + slot));
+        if (tiles < 0) break;
         if (!tiles) continue;
         if (!wt.all(bar(C::kQFull), useq & 1u)) break;
         // Tile j's PV and, in its place, tile j + kS's QK^T; the first kS tiles' QK^T lead.
@@ -905,11 +954,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 2) {
     if (lane == 0) {
       Phases<C::kKv> free;
-      for (int u = pair; u < units && !wt.failed; u += pairs) {
-        const Unit x = unit_at(a, u, pieces);
-        for (int j = 0; j < x.p.tiles; ++j) {
+      for (uint32_t n = 0;; ++n) {
+        const UnitRef x = next_unit(n);
+        if (x.tiles < 0) break;
+        for (int j = 0; j < x.tiles; ++j) {
           const uint32_t st = uint32_t(j % C::kKv), ph = free.take(st) ^ 1u;
-          const int key = x.p.key0 + (x.p.tile0 + j) * kRowTile;
+          const int key = x.key0 + j * kRowTile;
           if (!wt.on(bar(C::kVEmpty + st), ph)) break;
           if (rank == 0) ptx::mbar_expect_tx(bar(C::kVFull + st), 2 * C::kVBytes);
           const uint32_t vd = base + C::kSmV + st * C::kVBytes;
@@ -922,10 +972,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 3) {
-    uint32_t n = 0;
-    for (int u = pair; u < units && !wt.failed; u += pairs, ++n) {
-      const Unit x = unit_at(a, u, pieces);
-      const int keys = a.w.seq_keys[x.p.seq], spoilt = a.w.seq_spoilt[x.p.seq];
+    // The first unit is the pair's own; then the leader takes the next one from the pass's counter and
+    // tells the other CTA.
+    const uint32_t mail = base + C::kSmExch + 1552;
+    for (uint32_t n = 0;; ++n) {
+      int u = int(blockIdx.x) >> 1;
+      if (n == 0) {
+      } else if (rank == 0) {
+        if (!wt.all(bar(C::kMailEmpty), n & 1u)) break;
+        if (lane == 0) {
+          u = pairs + atomicAdd(a.w.header + kHdrNext + a.pass, 1);
+          ptx::st_cluster_u32(ptx::map_peer(mail, 1), uint32_t(u));
+          ptx::mbar_arrive_cluster(ptx::map_peer(bar(C::kMailFull), 1));
+        }
+        u = __shfl_sync(0xFFFFFFFFu, u, 0);
+      } else {
+        if (!wt.all(bar(C::kMailFull), (n & 1u) ^ 1u)) break;
+        ptx::mbar_test_cluster(bar(C::kMailFull), (n & 1u) ^ 1u);  // acquires the leader's store
+        u = __shfl_sync(0xFFFFFFFFu, int(ptx::ld_shared_u32(mail)), 0);
+        if (lane == 0) ptx::mbar_arrive_cluster_relaxed(ptx::map_peer(bar(C::kMailEmpty), 0));
+      }
+      const bool end = u >= units;
+      Unit x = {};
+      int keys = 0, spoilt = INT_MAX;
+      if (!end) {
+        x = unit_at(a, u, pieces, pairs);
+        keys = a.w.seq_keys[x.p.seq];
+        spoilt = a.w.seq_spoilt[x.p.seq];
+      }
       if (!wt.all(bar(C::kInfoEmpty + int(n & 1u)), ((n >> 1) & 1u) ^ 1u)) break;
       Info* info = reinterpret_cast<Info*>(sm + C::kSmInfo) + (n & 1u);
 #pragma unroll
@@ -942,14 +1016,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         info->row0 = x.p.row0;
         info->rows = x.p.rows;
+        info->key0 = x.p.key0 + x.p.tile0 * kRowTile;
         info->tile0 = x.p.tile0;
-        info->tiles = x.p.tiles;
-        info->head = x.head;
+        info->tiles = end ? -1 : x.p.tiles;
         info->whole = x.p.whole;
-      info->slot = x.slot;
+        info->head = x.head;
+        info->slot = x.head * pieces + x.p.index;
       }
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar(C::kInfoFull + int(n & 1u)));
+      if (end) break;
     }
     __syncwarp();
   } else {
@@ -961,8 +1037,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const float c = a.scale_log2, slack = kSlack / c;
     uint32_t it0 = 0;  // tiles of earlier units
     Phases<C::kS> s_full, pv_done;
-    uint32_t nth = 0;  // units so far
-    for (int u = pair; u < units; u += pairs, ++nth) {
+    for (uint32_t nth = 0;; ++nth) {
       const Info* info = reinterpret_cast<const Info*>(sm + C::kSmInfo) + (nth & 1u);
       wt.all(bar(C::kInfoFull + int(nth & 1u)), (nth >> 1) & 1u);
       // A wait that ran out ends the loop here for both warps of a row, and only here: inside a unit
@@ -972,6 +1047,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (gone[quad]) break;
       const int n = info->seen[row] & (kSpoilt - 1);  // keys that this row sees
       const int tiles = info->tiles, tile0 = info->tile0;
+      if (tiles < 0) break;
       float m = -INFINITY;           // what this thread's sum is taken against
       float sum[2][2] = {};          // partial sums over this thread's tiles
       const int odd = int((it0 ^ uint32_t(group)) & 1u);  // the unit's first tile of this group
@@ -1219,7 +1295,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
 
 // ------------------------------------------------------------------------------ host
 struct Layout {
-  uint64_t header, seq_key0, seq_keys, seq_block, seq_spoilt, blocks, pieces, part_out, part_lse, rows, rope, k, v, total;
+  uint64_t header, seq_key0, seq_keys, seq_block, seq_spoilt, blocks, pieces, order, part_out, part_lse, rows, rope, k, v, total;
   uint64_t cap, max_blocks, pass_heads, split_units;
 };
 
@@ -1254,6 +1330,7 @@ Layout layout_of(const TqMlaChunkSpec& s) {
   l.seq_spoilt = take((S + 1) * 4);
   l.blocks = take(l.max_blocks * sizeof(Block));
   l.pieces = take((l.max_blocks + l.split_units) * sizeof(Piece));
+  l.order = take((l.max_blocks + l.split_units) * sizeof(Piece));
   l.part_out = take(l.split_units * kQueryTile * dv * 4);
   l.part_lse = take(l.split_units * kQueryTile * 4);
   l.rows = take(l.cap * kLatent * 2);
@@ -1361,6 +1438,7 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
   a.w.seq_spoilt = reinterpret_cast<int*>(ws + l.seq_spoilt);
   a.w.blocks = reinterpret_cast<Block*>(ws + l.blocks);
   a.w.pieces = reinterpret_cast<Piece*>(ws + l.pieces);
+  a.w.order = reinterpret_cast<Piece*>(ws + l.order);
   a.w.part_out = reinterpret_cast<float*>(ws + l.part_out);
   a.w.part_lse = reinterpret_cast<float*>(ws + l.part_lse);
   a.w.rows = reinterpret_cast<uint16_t*>(ws + l.rows);
@@ -1438,7 +1516,7 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
   if (cudaGetLastError() != cudaSuccess ||
       !launch(gather_kernel, a.cap / kGatherRows, 256, 0, a))
     return fail("launch", TQ_ERR_CUDA);
-  for (a.head0 = 0; a.head0 < a.heads; a.head0 += int(l.pass_heads)) {
+  for (a.head0 = 0; a.head0 < a.heads; a.head0 += int(l.pass_heads), ++a.pass) {
     a.pass_heads = a.heads - a.head0 < int(l.pass_heads) ? a.heads - a.head0 : int(l.pass_heads);
     using Rope = attend::Shape<192, 128>;
     using Wide = attend::Shape<256, 256>;
