@@ -725,8 +725,8 @@ struct Shape {
   static constexpr uint32_t kVBytes = kVChunks * 128 * 128;
   static constexpr uint32_t kSmK = kQBytes;
   static constexpr uint32_t kSmV = kSmK + kKv * kKBytes;
-  static constexpr uint32_t kSmExch = kSmV + kKv * kVBytes;  // f32 [3][128], int [4], mail
-  static constexpr uint32_t kSmInfo = kSmExch + 1568;         // 2 x Info
+  static constexpr uint32_t kSmExch = kSmV + kKv * kVBytes;  // f32 [6][128], int [4], mail
+  static constexpr uint32_t kSmInfo = kSmExch + 3104;         // 2 x Info
   static constexpr uint32_t kSmTurn = kSmInfo + 2 * sizeof(Info);  // output rows, kTurnBytes a warp
   static constexpr uint32_t kSmBars = kSmTurn + 8 * kTurnBytes;
   static constexpr int kQFull = 0, kQEmpty = 1, kKFull = 2, kKEmpty = kKFull + kKv;
@@ -739,9 +739,14 @@ struct Shape {
   static constexpr uint32_t kSmMisc = kSmBars + 8 * kBars;
   static constexpr uint32_t kSmBytes = kSmMisc + 16 + 1024;
   static constexpr uint32_t kTmemO = kS * 128;
-  // Quarter of a tile's exponentials after which the turn passes. The earlier, the more the two
-  // groups' exponentials overlap and slow each other; the later, the longer a tile takes (after the
-  // first quarter 1553 us of attention for 2 x 2048 tokens of 128 heads, after the second 1545).
+  // With two score buffers a tile's own chain (scores, softmax, PV, the next scores in the buffer)
+  // is the limit, and both softmax groups work on every tile, half of its keys each; with three the
+  // groups take the tiles in turn, and one's exponentials run under the other's loads and maxima.
+  static constexpr bool kHalves = kS == 2;
+  // In turn: the quarter of a tile's exponentials after which the turn passes. The earlier, the more
+  // the two groups' exponentials overlap and slow each other; the later, the longer a tile takes
+  // (after the first quarter 1553 us of attention for 2 x 2048 tokens of 128 heads, after the second
+  // 1545).
   static constexpr int kTurn = 1;
   static_assert(kSmBytes <= 232448, "shared memory per CTA");
   static_assert(kTmemO + kDv <= 512, "TMEM columns");
@@ -822,7 +827,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       ptx::mbar_init(bar(i), joint ? 8 : read ? 11 - rank : i == C::kOFree ? 16 : 1);
     }
     tmem_holder[1] = 0;  // the abort word
-    for (int i = 0; i < 4; ++i) reinterpret_cast<int*>(sm + C::kSmExch + 1536)[i] = 0;
+    for (int i = 0; i < 4; ++i) reinterpret_cast<int*>(sm + C::kSmExch + 3072)[i] = 0;
     ptx::fence_mbar_init_cluster();
     ptx::tma_prefetch_desc(&tm_q);
     ptx::tma_prefetch_desc(&tm_k);
@@ -974,7 +979,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 3) {
     // The first unit is the pair's own; then the leader takes the next one from the pass's counter and
     // tells the other CTA.
-    const uint32_t mail = base + C::kSmExch + 1552;
+    const uint32_t mail = base + C::kSmExch + 3088;
     for (uint32_t n = 0;; ++n) {
       int u = int(blockIdx.x) >> 1;
       if (n == 0) {
@@ -1031,9 +1036,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else {
     const int group = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = uint32_t(quad * 32) << 16;
-    float* shared_m = reinterpret_cast<float*>(sm + C::kSmExch);  // [128]
-    float* shared_sum = shared_m + 128;                           // [2][128]
-    volatile int* gone = reinterpret_cast<volatile int*>(shared_m + 384);  // [4]
+    float* shared_m = reinterpret_cast<float*>(sm + C::kSmExch);  // [128], or [2][2][128] in halves
+    float* shared_sum = shared_m + 512;                           // [2][128]
+    volatile int* gone = reinterpret_cast<volatile int*>(shared_m + 768);  // [4]
     const float c = a.scale_log2, slack = kSlack / c;
     uint32_t it0 = 0;  // tiles of earlier units
     Phases<C::kS> s_full, pv_done;
@@ -1048,94 +1053,154 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int n = info->seen[row] & (kSpoilt - 1);  // keys that this row sees
       const int tiles = info->tiles, tile0 = info->tile0;
       if (tiles < 0) break;
-      float m = -INFINITY;           // what this thread's sum is taken against
-      float sum[2][2] = {};          // partial sums over this thread's tiles
-      const int odd = int((it0 ^ uint32_t(group)) & 1u);  // the unit's first tile of this group
-      for (int j = odd; j < tiles; j += 2) {
+      float m = -INFINITY;   // what this thread's sum is taken against
+      float sum[2][2] = {};  // partial sums over this thread's keys
+      // Where a row's maximum grew by more than the slack: columns `first` on of its part of O are
+      // rescaled, after the PV of the tile before tile j.
+      auto rescale = [&](int j, float keep, int first, int columns) {
+        const int b = j - 1;
+        wt.all(bar(C::kPvDone + b % C::kS), pv_done.at(b % C::kS, b / C::kS));
+        ptx::tc_fence_after();
+        const uint32_t o = tmem + C::kTmemO + first + lanes;
+#pragma unroll 1
+        for (int i = 0; i < columns; i += 16) {
+          uint32_t v[16];
+          ptx::tmem_ld16(o + i, v);
+          ptx::tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * keep);
+          ptx::tmem_st16(o + i, v);
+        }
+      };
+      // Of 32 scores, those behind the first `see` become -inf.
+      auto hide = [&](uint32_t (&r)[32], int see) {
+        const uint32_t bits = see >= 32 ? 0xFFFFFFFFu : see <= 0 ? 0u : (1u << see) - 1u;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (!(bits & (1u << i))) r[i] = 0xFF800000u;
+      };
+      float top[4];
+      auto raise = [&](const uint32_t (&r)[32]) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            top[k] = fmaxf(fmaxf(top[k], __uint_as_float(r[i + k])), __uint_as_float(r[i + 4 + k]));
+      };
+      // 32 softmax weights, against mc = -c * reference, to TMEM as 16 columns of bf16 pairs.
+      auto weigh = [&](const uint32_t (&r)[32], float mc, uint32_t dst) {
+        uint32_t p[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float p0 = ptx::ex2(fmaf(__uint_as_float(r[i]), c, mc));
+          const float p1 = ptx::ex2(fmaf(__uint_as_float(r[i + 1]), c, mc));
+          sum[(i >> 1) & 1][0] += p0;
+          sum[(i >> 1) & 1][1] += p1;
+          p[i / 2] = ptx::pack_bf16x2(p0, p1);
+        }
+        ptx::tmem_st16(dst, p);
+      };
+      auto weighed = [&](int half, uint32_t sb) {
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster_relaxed(lead(C::kPFull + 2 * int(sb) + half));
+      };
+      const int odd = C::kHalves ? 0 : int((it0 ^ uint32_t(group)) & 1u);
+      for (int j = odd; j < tiles; j += C::kHalves ? 1 : 2) {
         const uint32_t it = it0 + uint32_t(j), sb = uint32_t(j % C::kS);
         wt.all(bar(C::kSFull + sb), s_full.at(sb, j / C::kS));
         ptx::tc_fence_after();
         const uint32_t src = tmem + sb * 128 + lanes;
         const int key = (tile0 + j) * kRowTile;
-        const bool whole = __all_sync(0xFFFFFFFFu, n >= key + kRowTile);
-        auto scores = [&](uint32_t (&r)[32], int g) {
-          ptx::tmem_ld32(src + 32 * g, r);
+        top[0] = top[1] = top[2] = top[3] = -INFINITY;
+        if constexpr (C::kHalves) {
+          // This group's 64 keys of every tile.
+          uint32_t r0[32], r1[32];
+          ptx::tmem_ld32(src + group * 64, r0);
+          ptx::tmem_ld32(src + group * 64 + 32, r1);
           ptx::tmem_wait_ld();
-          if (!whole) {
-            const int see = n - key - 32 * g;
-            const uint32_t bits = see >= 32 ? 0xFFFFFFFFu : see <= 0 ? 0u : (1u << see) - 1u;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(bits & (1u << i))) r[i] = 0xFF800000u;  // -inf
+          const int see = n - key - group * 64;
+          if (!__all_sync(0xFFFFFFFFu, see >= 64)) {
+            hide(r0, see);
+            hide(r1, see - 32);
           }
-        };
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-        for (int g = 0; g < 4; ++g) {
-          uint32_t r[32];
-          scores(r, g);
-#pragma unroll
-          for (int i = 0; i < 32; i += 8)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              top[k] = fmaxf(fmaxf(top[k], __uint_as_float(r[i + k])), __uint_as_float(r[i + 4 + k]));
-        }
-        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        // The turn passes from tile to tile, and so from group to group, with the row's reference
-        // maximum: one group at a time is in its exponentials.
-        if (it > 0) ptx::named_barrier(1 + quad + 4 * int(it & 1u), 64);
-        float ref = j == 0 ? high : shared_m[row];
-        if (j > 0) {
-          const bool grow = high > ref + slack;
-          if (__any_sync(0xFFFFFFFFu, grow)) {
-            const float keep =
-                !grow ? 1.f : ref == -INFINITY ? 0.f : ptx::ex2((ref - high) * c);
-            if (grow) ref = high;
-            const int b = j - 1;
-            wt.all(bar(C::kPvDone + b % C::kS), pv_done.at(b % C::kS, b / C::kS));
-            ptx::tc_fence_after();
-            const uint32_t o = tmem + C::kTmemO + lanes;
-#pragma unroll 1
-            for (int i = 0; i < kDv; i += 16) {
-              uint32_t v[16];
-              ptx::tmem_ld16(o + i, v);
-              ptx::tmem_wait_ld();
-#pragma unroll
-              for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * keep);
-              ptx::tmem_st16(o + i, v);
+          raise(r0);
+          raise(r1);
+          float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          // The two threads of a row exchange their maxima, and keep the same reference. Past the
+          // barrier both have read their scores, which P may now replace.
+          float* ex = shared_m + (it & 1u) * 256;
+          ex[group * 128 + row] = high;
+          ptx::named_barrier(1 + quad, 64);
+          high = fmaxf(high, ex[(group ^ 1) * 128 + row]);
+          if (j == 0) {
+            m = high;
+          } else {
+            const bool grow = high > m + slack;
+            if (__any_sync(0xFFFFFFFFu, grow)) {
+              const float keep =
+                  !grow ? 1.f : m == -INFINITY ? 0.f : ptx::ex2((m - high) * c);
+              if (grow) m = high;
+              rescale(j, keep, group * (kDv / 2), kDv / 2);
+              sum[0][0] *= keep;
+              sum[0][1] *= keep;
+              sum[1][0] *= keep;
+              sum[1][1] *= keep;
             }
           }
-        }
-        shared_m[row] = ref;
-        if (__any_sync(0xFFFFFFFFu, ref != m)) {
-          const float keep = m == ref ? 1.f : m == -INFINITY ? 0.f : ptx::ex2((m - ref) * c);
-          sum[0][0] *= keep;
-          sum[0][1] *= keep;
-          sum[1][0] *= keep;
-          sum[1][1] *= keep;
-          m = ref;
-        }
-        const float mc = ref == -INFINITY ? 0.f : -ref * c;
+          const float mc = m == -INFINITY ? 0.f : -m * c;
+          weigh(r0, mc, src + group * 32);
+          weigh(r1, mc, src + group * 32 + 16);
+          weighed(group, sb);
+        } else {
+          // Every other tile, all of its keys; its scores are read twice, a quarter at a time.
+          // (Holding them from the maximum to the exponentials, or unrolling the quarters, makes
+          // code that crowds the instruction caches which all roles share: 1690 to 1780 us of
+          // attention for 2 x 2048 tokens of 128 heads instead of 1545.)
+          const bool whole = __all_sync(0xFFFFFFFFu, n >= key + kRowTile);
 #pragma unroll 1
-        for (int g = 0; g < 4; ++g) {
-          uint32_t r[32], p[16];
-          scores(r, g);
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float p0 = ptx::ex2(fmaf(__uint_as_float(r[i]), c, mc));
-            const float p1 = ptx::ex2(fmaf(__uint_as_float(r[i + 1]), c, mc));
-            sum[(i >> 1) & 1][0] += p0;
-            sum[(i >> 1) & 1][1] += p1;
-            p[i / 2] = ptx::pack_bf16x2(p0, p1);
+          for (int g = 0; g < 4; ++g) {
+            uint32_t r[32];
+            ptx::tmem_ld32(src + 32 * g, r);
+            ptx::tmem_wait_ld();
+            if (!whole) hide(r, n - key - 32 * g);
+            raise(r);
           }
-          ptx::tmem_st16(src + 16 * g, p);  // over the scores
-          if (g == C::kTurn) ptx::named_barrier_arrive(1 + quad + 4 * int((it + 1) & 1u), 64);
-          if (g & 1) {
-            ptx::tmem_wait_st();
-            ptx::tc_fence_before();
-            __syncwarp();
-            if (lane == 0)
-              ptx::mbar_arrive_cluster_relaxed(lead(C::kPFull + 2 * int(sb) + (g >> 1)));
+          const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          // The turn passes from tile to tile, and so from group to group, with the row's reference
+          // maximum.
+          if (it > 0) ptx::named_barrier(1 + quad + 4 * int(it & 1u), 64);
+          float ref = j == 0 ? high : shared_m[row];
+          if (j > 0) {
+            const bool grow = high > ref + slack;
+            if (__any_sync(0xFFFFFFFFu, grow)) {
+              const float keep =
+                  !grow ? 1.f : ref == -INFINITY ? 0.f : ptx::ex2((ref - high) * c);
+              if (grow) ref = high;
+              rescale(j, keep, 0, kDv);
+            }
+          }
+          shared_m[row] = ref;
+          if (__any_sync(0xFFFFFFFFu, ref != m)) {
+            const float keep = m == ref ? 1.f : m == -INFINITY ? 0.f : ptx::ex2((m - ref) * c);
+            sum[0][0] *= keep;
+            sum[0][1] *= keep;
+            sum[1][0] *= keep;
+            sum[1][1] *= keep;
+            m = ref;
+          }
+          const float mc = ref == -INFINITY ? 0.f : -ref * c;
+#pragma unroll 1
+          for (int g = 0; g < 4; ++g) {
+            uint32_t r[32];
+            ptx::tmem_ld32(src + 32 * g, r);
+            ptx::tmem_wait_ld();
+            if (!whole) hide(r, n - key - 32 * g);
+            weigh(r, mc, src + 16 * g);  // over scores that are read
+            if (g == C::kTurn)
+              ptx::named_barrier_arrive(1 + quad + 4 * int((it + 1) & 1u), 64);
+            if (g & 1) weighed(g >> 1, sb);
           }
         }
       }
@@ -1147,7 +1212,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // The row's last reference maximum and its whole sum, then O / sum to the output: this
       // thread's half of the columns.
       ptx::named_barrier(9 + quad, 64);
-      const float ref = tiles ? shared_m[row] : -INFINITY;
+      const float ref = C::kHalves ? m : tiles ? shared_m[row] : -INFINITY;
       float total = (sum[0][0] + sum[0][1]) + (sum[1][0] + sum[1][1]);
       if (m != ref) total = m == -INFINITY ? 0.f : total * ptx::ex2((m - ref) * c);
       shared_sum[group * 128 + row] = total;
