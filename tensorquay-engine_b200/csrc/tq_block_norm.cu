@@ -64,6 +64,9 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
 template <int kThreads, int kSteps, bool kF32>
 __global__ void __launch_bounds__(kThreads) block_norm_kernel(const Args a) {
   __shared__ float part[2][kThreads / 32];
+  // Launched while the kernel before it ends; its results are waited for here.
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   const long long row = blockIdx.x;
   const uint8_t* y = a.y + row * a.y_stride;
   const uint8_t* res = a.res + row * a.res_stride;
@@ -147,11 +150,17 @@ __global__ void __launch_bounds__(kThreads) block_norm_kernel(const Args a) {
 
 template <int kThreads, int kSteps>
 cudaError_t launch(const Args& a, bool f32, cudaStream_t stream) {
-  if (f32)
-    block_norm_kernel<kThreads, kSteps, true><<<a.rows, kThreads, 0, stream>>>(a);
-  else
-    block_norm_kernel<kThreads, kSteps, false><<<a.rows, kThreads, 0, stream>>>(a);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(a.rows), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return f32 ? cudaLaunchKernelEx(&cfg, block_norm_kernel<kThreads, kSteps, true>, a)
+             : cudaLaunchKernelEx(&cfg, block_norm_kernel<kThreads, kSteps, false>, a);
 }
 
 }  // namespace norm

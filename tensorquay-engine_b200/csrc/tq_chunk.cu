@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
   __shared__ int n_length[1024];  // tiles of the pieces
   const Work& w = a.w;
   const int tid = threadIdx.x;
+  ptx::grid_dependency_wait();
   if (tid < kHdrWords) w.header[tid] = 0;
   if (tid == 0) { s_rows = 0; s_blocks = 0; s_over = 0; s_split = 0; }
   __syncthreads();
@@ -1562,8 +1563,8 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
               s.w_uv.strides_bytes[0], 128))
     return fail("tensor_map", TQ_ERR_CUDA);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  // Each kernel after the first starts while the one before it ends, and waits inside for its
-  // results (griddepcontrol.wait): the setup and the loads that need none run meanwhile.
+  // Each kernel starts while the one before it ends, and waits inside for its results
+  // (griddepcontrol.wait): the setup and the loads that need none run meanwhile.
   auto launch = [&](auto kernel, int grid, int threads, uint32_t smem, auto... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(grid), 1, 1);
@@ -1577,8 +1578,7 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess;
   };
-  plan_kernel<<<1, 1024, 0, cs>>>(a);
-  if (cudaGetLastError() != cudaSuccess ||
+  if (!launch(plan_kernel, 1, 1024, 0, a) ||
       !launch(gather_kernel, a.cap / kGatherRows, 256, 0, a))
     return fail("launch", TQ_ERR_CUDA);
   for (a.head0 = 0; a.head0 < a.heads; a.head0 += int(l.pass_heads), ++a.pass) {

@@ -148,6 +148,9 @@ __global__ void __launch_bounds__(kT) near_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t raw[];
   NearShared<kN>& sh = *reinterpret_cast<NearShared<kN>*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // Launched while the kernel before it ends; its results are waited for here.
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   const int pool = min(max(*a.free_count, 0), a.pool);
   int bad = 0;
   Request r[4];
@@ -279,8 +282,17 @@ template <int kT>
 cudaError_t launch_near(const Args& a, cudaStream_t stream) {
   long long ctas = (a.tokens + 4ll * kT - 1) / (4 * kT);
   ctas = ctas < 1 ? 1 : ctas > 296 ? 296 : ctas;
-  near_kernel<kT><<<int(ctas), kT, sizeof(NearShared<4 * kT>), stream>>>(a);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(ctas), 1, 1);
+  cfg.blockDim = dim3(kT, 1, 1);
+  cfg.dynamicSmemBytes = sizeof(NearShared<4 * kT>);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, near_kernel<kT>, a);
 }
 
 __global__ void __launch_bounds__(kThreads) plan_kernel(const Args a) {
