@@ -429,14 +429,17 @@ int32_t tq_block_norm(const TqBlockNormSpec* spec, void* stream, TqContractError
  * sizes the workspace. A token without a visible row gets zeros and lse -inf; rows of q before
  * q_start[0] and from q_start[S] on are not computed and their outputs are left as they were. A
  * cached row that is not finite makes every output that sees it NaN and no other; FP8 rows are
- * dequantized to bf16 first. Rounding points: k and v to bf16 (the model's own), the softmax
- * weights to bf16 before the value product; statistics and sums are f32.
+ * dequantized to bf16 first. Rounding points: k and v to bf16 (the model's own; a value past bf16's
+ * range becomes its largest), the softmax weights to bf16 before the value product; statistics and
+ * sums are f32.
  * Device error flags (tq_mla_read_device_error): TQ_DEV_PAGE_RANGE (a page-table entry outside
  * the pool: its rows read as zeros), TQ_DEV_TABLE_SHORT (kv_len past 64 L, cut),
  * TQ_DEV_SEQ_RANGE (q_start not ascending within [0, T]: nothing is computed),
  * TQ_DEV_WORK_OVERFLOW (more rows than max_keys: nothing is computed), TQ_DEV_WAIT_TIMEOUT.
- * The workspace is 256-byte aligned; calls that share one must be ordered on one stream. The
- * launches depend only on the spec, so a captured call replays for new contents. */
+ * The workspace is 256-byte aligned; calls that share one must be ordered on one stream. It holds
+ * the cached rows as bf16 (1.2 KB for each of max_keys) and their expanded keys and values, of as
+ * many heads at a time as fit 8 GiB (for one head 512 or 1024 bytes a row). The launches depend
+ * only on the spec, so a captured call replays for new contents. */
 typedef struct {
   TqTensorSpec q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse;
   int32_t kv_format;

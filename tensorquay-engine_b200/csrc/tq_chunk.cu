@@ -489,7 +489,9 @@ struct Waiter {
 // 512 B written a row. The weights of a column block (256 x 512, half of them in each CTA of the
 // pair) therefore stay in shared memory while the pair walks over row tiles; only the rows
 // stream (16 KB boxes through a ring), half as many bytes per FLOP as with both operands streamed.
-// Two TMEM accumulators: the epilogue of one item runs under the MMAs of the next.
+// Two TMEM accumulators: the epilogue of one item runs under the MMAs of the next. Products past
+// bf16's range become its largest value: an infinite value would reach the tile's other query rows
+// as 0 * infinity.
 namespace expand {
 
 constexpr int kThreads = 256;  // warp 0 loads, warp 1 MMA, warps 4-7 epilogue
@@ -646,7 +648,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ptx::tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          y[j] = ptx::pack_bf16x2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+          y[j] = ptx::pack_bf16x2_finite(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
         uint16_t* dst = c < 128 ? lo + c : hi + (c - 128);
         ptx::st_global_v8(dst, y);
         ptx::st_global_v8(dst + 16, y + 8);

@@ -537,6 +537,13 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return r;
 }
 
+// As pack_bf16x2, and a value past bf16's largest becomes the largest instead of infinity.
+__device__ __forceinline__ uint32_t pack_bf16x2_finite(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 // Two E4M3 codes (bits 0-7: first, bits 8-15: second) times `scale`, as packed bf16 (first in
 // the low half). The codes widen exactly to f16, then to f32; only the final bf16 rounds.
 __device__ __forceinline__ uint32_t e4m3x2_scaled_bf16x2(uint32_t codes, float scale) {

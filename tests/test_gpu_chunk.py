@@ -283,6 +283,38 @@ def test_a_row_that_is_not_finite_reaches_only_those_who_see_it(cuda_device, fmt
 
 
 @pytest.mark.parametrize("fmt", [0, 2])
+def test_a_row_whose_expansion_overflows_reaches_only_those_who_see_it(cuda_device, fmt):
+    """Finite latent values of 3e38: keys and values past bf16's range."""
+    c = Case(cuda_device, fmt, [200], [50], seed=3)
+    c.launch()()
+    clean, clean_lse = c.out, c.lse
+    row = int(c.table[0, 220 // 64]) * 64 + 220 % 64
+    c.kv.view(-1, c.kv.shape[-1])[row, :1024] = torch.full((512,), 3e38, dtype=torch.bfloat16).view(torch.uint8).to(cuda_device)
+    c.w_uv[0, 3] = c.w_uv[0, 3].abs()
+    c.w_uk[1, 5] = c.w_uk[1, 5].abs()
+    first = Case(cuda_device, fmt, [200], [50], seed=3)
+    first.w_uv, first.w_uk = c.w_uv, c.w_uk
+    first.launch()()
+    c.launch()()
+    seen = 170                       # tokens 0 to 169 are at positions below 220
+    assert torch.equal(c.out[:seen], first.out[:seen]) and torch.equal(c.lse[:seen], first.lse[:seen])
+    assert not torch.equal(clean[:seen], first.out[:seen])
+
+
+@pytest.mark.parametrize("fmt", [0, 2])
+def test_heads_in_several_passes(cuda_device, fmt):
+    """A bound so large that the expanded keys and values of all heads do not fit the scratch."""
+    c = Case(cuda_device, fmt, [140, 30], [200, 1500], heads=5, seed=8)
+    launch = c.launch(max_keys=1 << 22)
+    assert launch.workspace.numel() < 20 << 30
+    launch()
+    assert launch.device_error() == 0
+    c.check()
+    del launch
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("fmt", [0, 2])
 def test_a_query_that_is_not_finite_stays_in_its_row(cuda_device, fmt):
     c = Case(cuda_device, fmt, [140], [20], seed=5)
     c.q[13, 1, 4] = float("nan")

@@ -3,9 +3,12 @@ tq_block_norm_validate) and their oracles, CPU only: fake numeric addresses, the
 violation kinds of the other contracts."""
 
 import ctypes
+import subprocess
 
 import numpy as np
 import pytest
+
+from conftest import ROOT
 
 from oracle import step as ostep
 from tq_mla import _abi
@@ -188,3 +191,19 @@ def test_norm_oracle_without_its_parts_is_a_sum():
     out, x = ostep.block_norm(y, h, pre_weight=np.ones(16), post_weight=np.ones(16), eps=1e-12)
     np.testing.assert_allclose((x * x).mean(axis=1), 1.0, rtol=1e-9)
     np.testing.assert_allclose(((out - h) ** 2).mean(axis=1), 1.0, rtol=1e-9)
+
+
+def test_struct_layout_matches_a_c_compiler(tmp_path):
+    structs = {name: getattr(_abi, name) for name in ("TqStepPlanSpec", "TqBlockNormSpec", "TqMlaChunkSpec")}
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{ROOT / "include" / "tq_mla.h"}"', "int main(){"]
+    for name, cls in structs.items():
+        lines.append(f'printf("{name} %zu\\n", sizeof({name}));')
+        lines += [f'printf("{name}.{f} %zu\\n", offsetof({name}, {f}));' for f, _ in cls._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["return 0;}"]))
+    subprocess.run(["gcc", "-std=c11", "-o", str(exe), str(src)], check=True)
+    got = dict(line.split() for line in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines())
+    for name, cls in structs.items():
+        assert int(got[name]) == ctypes.sizeof(cls), name
+        for f, _ in cls._fields_:
+            assert int(got[f"{name}.{f}"]) == getattr(cls, f).offset, (name, f)
