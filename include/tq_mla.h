@@ -409,8 +409,11 @@ int32_t tq_block_norm(const TqBlockNormSpec* spec, void* stream, TqContractError
  * keys and values expanded from them. It is the same attention as tq_mla_prefill without the
  * weights folded into the query and the output: a (query, key, head) triple costs
  * 2 (Dn + Dr + Dv) FLOP instead of 2 (1024 + Dr), and each cached row costs 1024 (Dn + Dv) FLOP
- * a head once per call, so it is the cheaper form from about 170 query tokens per cached row on
- * (tq_mla_prefill is below that, tq_mla_decode for single tokens). For sequence s, rows
+ * a head once per call. So it is the cheaper form for sequences of many new tokens: at 128 heads
+ * of 576-wide rows, one sequence over 8000 cached rows takes 377 us for 128 tokens and 382 for 256
+ * where tq_mla_prefill takes 312 and 597, eight over 1000 rows 435 and 475 where it takes 474 and
+ * 915 (and its caller still folds the weights). A sequence of fewer tokens over a long cache
+ * belongs in a tq_mla_prefill or tq_mla_decode call beside this one. For sequence s, rows
  * t in [q_start[s], q_start[s + 1]) and cached rows n < kv_len[s]:
  *   k[n, h] = bf16(latent[n] . w_uk[h]^T), followed by the row's Dr RoPE values
  *   v[n, h] = bf16(latent[n] . w_uv[h]^T)
@@ -425,13 +428,13 @@ int32_t tq_block_norm(const TqBlockNormSpec* spec, void* stream, TqContractError
  * H is 1 to 128. 576-wide rows (TQ_KV_BF16_ROPE576): Dn = Dv = 128, Dr = 64; 512-wide rows
  * (TQ_KV_BF16, TQ_KV_FP8_E4M3): Dn = Dv = 256, Dr = 0. softmax_scale is any finite f32 > 0.
  * Addresses and strides of q, w_uk, w_uv and out are multiples of 16; T and max_keys are at most
- * 2^24, and max_keys + 127 min(S, T) at most 2^25. `max_keys` is the host's bound on the summed kv_len of the sequences that have tokens: it
- * sizes the workspace. A token without a visible row gets zeros and lse -inf; rows of q before
- * q_start[0] and from q_start[S] on are not computed and their outputs are left as they were. A
- * cached row that is not finite makes every output that sees it NaN and no other; FP8 rows are
- * dequantized to bf16 first. Rounding points: k and v to bf16 (the model's own; a value past bf16's
- * range becomes its largest), the softmax weights to bf16 before the value product; statistics and
- * sums are f32.
+ * 2^24, and max_keys + 127 min(S, T) at most 2^25. `max_keys` is the host's bound on the summed
+ * kv_len of the sequences that have tokens: it sizes the workspace. A token without a visible row
+ * gets zeros and lse -inf; rows of q before q_start[0] and from q_start[S] on are not computed and
+ * their outputs are left as they were. A cached row that is not finite makes every output that sees
+ * it NaN and no other; FP8 rows are dequantized to bf16 first. Rounding points: k and v to bf16
+ * (the model's own; a value past bf16's range becomes its largest), the softmax weights to bf16
+ * before the value product; statistics and sums are f32 (a score past f32's range gives NaN).
  * Device error flags (tq_mla_read_device_error): TQ_DEV_PAGE_RANGE (a page-table entry outside
  * the pool: its rows read as zeros), TQ_DEV_TABLE_SHORT (kv_len past 64 L, cut),
  * TQ_DEV_SEQ_RANGE (q_start not ascending within [0, T]: nothing is computed),

@@ -5,13 +5,14 @@
 //
 // Launches, in order on the caller's stream:
 //   1. plan_kernel    one block: each sequence's cached rows laid end to end in a compact row space
-//                     (every sequence padded to kRowTile rows), its query blocks of kQueryTile
-//                     tokens with the number of row tiles each of them sees.
+//                     (every sequence padded to kRowTile rows) and its query blocks of kQueryTile
+//                     tokens.
 //   2. gather_kernel  the cached rows through the page table into that space, as bf16 (FP8 rows
 //                     dequantized, rounded once): zeros past kv_len and for a row that is not
 //                     finite, so that neither stale rows nor such a row can reach an output that
 //                     does not see it through 0 * NaN. The first such row of a sequence is kept:
-//                     the outputs of the tokens that see it become NaN at the end.
+//                     the outputs of the tokens that see it become NaN at the end. One block of
+//                     its grid cuts the query blocks into pieces of the row tiles that they see.
 //   3. expand_kernel  k and v of every head from the compact rows.
 //   4. attend_kernel  attention of every (query block, head); where those are few, each is split
 //                     into pieces of its row tiles, and
@@ -122,13 +123,14 @@ __device__ __forceinline__ int warp_inclusive(int v) {
   return v;
 }
 
-// Inclusive sum over the 1024 threads of a block.
+// Inclusive sum over the kWarps warps of a block.
+template <int kWarps>
 __device__ __forceinline__ int block_inclusive(int v, int* part) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int inc = warp_inclusive(v);
   if (lane == 31) part[warp] = inc;
   __syncthreads();
-  if (warp == 0) part[lane] = warp_inclusive(part[lane]);
+  if (warp == 0) part[lane] = warp_inclusive(lane < kWarps ? part[lane] : 0);
   __syncthreads();
   const int out = inc + (warp ? part[warp - 1] : 0);
   __syncthreads();
@@ -146,15 +148,12 @@ __device__ __forceinline__ int last_at_or_below(const int* start, int n, int x) 
 
 __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
   __shared__ int part[32];
-  __shared__ int s_rows, s_blocks, s_over, s_split;
-  // The first 1024 sequences and blocks again, near: the steps below read each other's results.
-  __shared__ int n_q0[1025], n_block[1025], n_key0[1024], n_keys[1024], n_tiles[1024];
-  __shared__ int n_length[1024];  // tiles of the pieces
+  __shared__ int s_rows, s_blocks, s_over;
   const Work& w = a.w;
   const int tid = threadIdx.x;
   ptx::grid_dependency_wait();
   if (tid < kHdrWords) w.header[tid] = 0;
-  if (tid == 0) { s_rows = 0; s_blocks = 0; s_over = 0; s_split = 0; }
+  if (tid == 0) { s_rows = 0; s_blocks = 0; s_over = 0; }
   __syncthreads();
   int bad = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += 1024) {
@@ -180,14 +179,10 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
         if (keys > a.cap) { s_over = 1; keys = 0; }
       }
       blocks = (n + kQueryTile - 1) / kQueryTile;
-      if (s < 1024) {
-        n_q0[s] = b;
-        n_q0[s + 1] = e;  // the same value from both sides
-        n_keys[s] = keys;
-      }
     }
     const int padded = (keys + kRowTile - 1) / kRowTile * kRowTile;
-    const int rows_end = block_inclusive(padded, part), blocks_end = block_inclusive(blocks, part);
+    const int rows_end = block_inclusive<32>(padded, part);
+    const int blocks_end = block_inclusive<32>(blocks, part);
     const int rows0 = s_rows, blocks0 = s_blocks;
     __syncthreads();
     // 1024 sequences of at most cap <= 2^25 rows may pass 2^31: a warp's 32 are summed in 64 bits
@@ -197,10 +192,6 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
       w.seq_keys[s] = keys;
       w.seq_spoilt[s] = INT_MAX;
       w.seq_block[s] = blocks0 + blocks_end - blocks;
-      if (s < 1024) {
-        n_key0[s] = rows0 + rows_end - padded;
-        n_block[s] = blocks0 + blocks_end - blocks;
-      }
     }
     long long sum = padded;
 #pragma unroll
@@ -232,18 +223,48 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
     w.seq_block[a.seqs] = s_blocks;
     w.header[kHdrRows] = s_rows;
     w.header[kHdrBlocks] = s_blocks;
-    if (a.seqs <= 1024) n_block[a.seqs] = s_blocks;
   }
+}
+
+// The query blocks and their pieces, by one block of the gather's grid: only the attention reads
+// them, so they run beside the gathering of rows (24 tokens over 124 rows, replayed from a graph:
+// 27 us with this in plan_kernel, 22 here and with the attention's first fetch ahead of its wait).
+constexpr int kGatherThreads = 256, kGatherWarps = kGatherThreads / 32;
+
+struct PlanShared {
+  // The first sequences, blocks and pieces again, near: the steps read each other's results.
+  static constexpr int kSeqs = 256, kBlocks = 1024;
+  int part[32], at, split;
+  int q0[kSeqs + 1], block[kSeqs + 1], key0[kSeqs], keys[kSeqs];
+  int tiles[kBlocks], length[kBlocks];  // of blocks; of pieces
+  int cost[32], len[32];
+};
+
+__device__ void plan_pieces(const Args& a, PlanShared& sh) {
+  const Work& w = a.w;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int blocks = w.header[kHdrBlocks];
+  const bool near = a.seqs <= PlanShared::kSeqs;
+  if (near) {
+#pragma unroll 1
+    for (int s = tid; s <= a.seqs; s += kGatherThreads) {
+      sh.q0[s] = a.q_start[s];
+      sh.block[s] = w.seq_block[s];
+      if (s < a.seqs) {
+        sh.key0[s] = w.seq_key0[s];
+        sh.keys[s] = w.seq_keys[s];
+      }
+    }
+  }
+  if (tid == 0) { sh.at = 0; sh.split = 0; }
   __syncthreads();
-  const bool near = a.seqs <= 1024;
-  const int* seq_block = near ? n_block : w.seq_block;
-  const int* q_start = near ? n_q0 : a.q_start;
-  const int* seq_keys = near ? n_keys : w.seq_keys;
-  const int* seq_key0 = near ? n_key0 : w.seq_key0;
-  const int blocks = s_blocks;
+  const int* seq_block = near ? sh.block : w.seq_block;
+  const int* q_start = near ? sh.q0 : a.q_start;
+  const int* seq_keys = near ? sh.keys : w.seq_keys;
+  const int* seq_key0 = near ? sh.key0 : w.seq_key0;
   // Query blocks, one warp each: the tiles that its furthest-seeing token sees.
-  const int lane = tid & 31, warp = tid >> 5;
-  for (int b = warp; b < blocks; b += 32) {
+#pragma unroll 1
+  for (int b = warp; b < blocks; b += kGatherWarps) {
     const int s = last_at_or_below(seq_block, a.seqs, b);
     const int row0 = q_start[s] + (b - seq_block[s]) * kQueryTile;
     const int rows = min(kQueryTile, q_start[s + 1] - row0);
@@ -256,58 +277,61 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
     const int keys = seq_keys[s];
     const int tiles = ((far >= keys ? keys : far + 1) + kRowTile - 1) / kRowTile;
     if (lane == 0) {
-      if (b < 1024) n_tiles[b] = tiles;
+      if (b < PlanShared::kBlocks) sh.tiles[b] = tiles;
       else w.blocks[b].tiles = tiles;
     }
   }
   __syncthreads();
-  auto tiles_of = [&](int b) { return b < 1024 ? n_tiles[b] : w.blocks[b].tiles; };
-  // The most tiles that a piece gets. Warp k weighs cutting the longest block into k + 1: the
-  // rounds that the CTA pairs need for all units, each as long as such a piece.
+  auto tiles_of = [&](int b) { return b < PlanShared::kBlocks ? sh.tiles[b] : w.blocks[b].tiles; };
+  // The most tiles that a piece gets. Each k below 32 weighs cutting the longest block into k + 1:
+  // the rounds that the CTA pairs need for all units, each as long as such a piece.
   int len = 1 << 30;  // whole blocks
   if (a.split_units) {
-    __shared__ int s_cost[32], s_len[32];
-    int longest = 1, count = 0;
+    int longest = 1;
+#pragma unroll 1
     for (int b = lane; b < blocks; b += 32) longest = max(longest, tiles_of(b));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
       longest = max(longest, __shfl_xor_sync(0xFFFFFFFFu, longest, o));
-    const int cut = (longest + warp) / (warp + 1);
-    for (int b = lane; b < blocks; b += 32) count += max(1, (tiles_of(b) + cut - 1) / cut);
+#pragma unroll 1
+    for (int k = warp; k < 32; k += kGatherWarps) {
+      const int cut = (longest + k) / (k + 1);
+      int count = 0;
+#pragma unroll 1
+      for (int b = lane; b < blocks; b += 32) count += max(1, (tiles_of(b) + cut - 1) / cut);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) count += __shfl_xor_sync(0xFFFFFFFFu, count, o);
-    const long long units = (long long)count * a.pass_heads;
-    if (lane == 0) {
-      s_len[warp] = cut;
-      s_cost[warp] = units <= a.split_units
-                         ? int((units + a.pairs - 1) / a.pairs) * (cut + kPieceCost) +
-                               (warp ? 2 * kPieceCost : 0)
-                         : INT_MAX;
+      for (int o = 16; o > 0; o >>= 1) count += __shfl_xor_sync(0xFFFFFFFFu, count, o);
+      if (lane == 0) {
+        const int units = count <= a.split_units ? count * a.pass_heads : INT_MAX;
+        sh.len[k] = cut;
+        sh.cost[k] = units <= a.split_units ? (units + a.pairs - 1) / a.pairs * (cut + kPieceCost) +
+                                                  (k ? 2 * kPieceCost : 0)
+                                            : INT_MAX;
+      }
     }
     __syncthreads();
-    int cost = s_cost[lane], best = lane;
+    int cost = sh.cost[lane], best = lane;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      const int c = __shfl_xor_sync(0xFFFFFFFFu, cost, o), k = __shfl_xor_sync(0xFFFFFFFFu, best, o);
+      const int c = __shfl_xor_sync(0xFFFFFFFFu, cost, o);
+      const int k = __shfl_xor_sync(0xFFFFFFFFu, best, o);
       if (c < cost || (c == cost && k < best)) {
         cost = c;
         best = k;
       }
     }
-    if (best) len = s_len[best];
+    if (best) len = sh.len[best];
   }
-  // Number the pieces, 1024 blocks at a time.
-  __syncthreads();
-  if (tid == 0) s_rows = 0;
-  __syncthreads();
-  for (int b0 = 0; b0 < blocks; b0 += 1024) {
+  // Number the pieces.
+#pragma unroll 1
+  for (int b0 = 0; b0 < blocks; b0 += kGatherThreads) {
     const int b = b0 + tid;
     int n = 0, tiles = 0;
     if (b < blocks) {
       tiles = tiles_of(b);
       n = max(1, (tiles + len - 1) / len);
     }
-    const int end = block_inclusive(n, part), at = s_rows + end - n;
+    const int end = block_inclusive<kGatherWarps>(n, sh.part), at = sh.at + end - n;
     if (b < blocks) {
       const int s = last_at_or_below(seq_block, a.seqs, b);
       const int row0 = q_start[s] + (b - seq_block[s]) * kQueryTile;
@@ -315,34 +339,38 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
       w.blocks[b] = {row0, rows, key0, tiles, s, at, n, 0};
       // Pieces of one length, the last ones shorter.
       const int each = max(1, (tiles + n - 1) / n);
+#pragma unroll 1
       for (int i = 0; i < n; ++i) {
         const int length = max(0, min(each, tiles - i * each));
         w.pieces[at + i] = {row0, rows, key0, i * each, length, s, n == 1, at + i};
-        if (at + i < 1024) n_length[at + i] = length;
+        if (at + i < PlanShared::kBlocks) sh.length[at + i] = length;
       }
-      if (n > 1) s_split = 1;
+      if (n > 1) sh.split = 1;
     }
     __syncthreads();
-    if (tid == 1023) s_rows = at + n;
+    if (tid == kGatherThreads - 1) sh.at = at + n;
     __syncthreads();
   }
   // The order in which a head's pieces run: the longest first, so that the last ones to run are
-  // short (up to 1024 pieces; more are left in their order).
-  const int pieces = s_rows;
-  if (tid < pieces && pieces <= 1024) {
-    const int mine = n_length[tid];
-    int rank = 0;
-    for (int i = 0; i < pieces; ++i) {
-      const int other = n_length[i];
-      rank += other > mine || (other == mine && i < tid);
+  // short (up to kBlocks pieces; more are left in their order).
+  const int pieces = sh.at;
+#pragma unroll 1
+  for (int i = tid; i < pieces; i += kGatherThreads) {
+    int rank = i;
+    if (pieces <= PlanShared::kBlocks) {
+      const int mine = sh.length[i];
+      rank = 0;
+#pragma unroll 4
+      for (int k = 0; k < pieces; ++k) {
+        const int other = sh.length[k];
+        rank += other > mine || (other == mine && k < i);
+      }
     }
-    w.order[rank] = w.pieces[tid];
-  } else if (pieces > 1024) {
-    for (int i = tid; i < pieces; i += 1024) w.order[i] = w.pieces[i];
+    w.order[rank] = w.pieces[i];
   }
   if (tid == 0) {
     w.header[kHdrPieces] = pieces;
-    w.header[kHdrSplit] = s_split;
+    w.header[kHdrSplit] = sh.split;
   }
 }
 
@@ -351,18 +379,23 @@ __device__ __forceinline__ bool finite_bf16x2(uint32_t u) {
   return (u & 0x7F80u) != 0x7F80u && (u & 0x7F800000u) != 0x7F800000u;
 }
 
-// One block per kGatherRows compact rows, four rows a warp with all their loads in flight: lane i
-// takes the 16 latent values from 16 i on, and two of the 64 RoPE values. What bounds it: the chain
-// of dependent loads (sequence, page, row) for small calls, so rows are spread over many blocks;
-// HBM for large ones (a row read and written once).
-constexpr int kGatherRows = 32;
+// Block 0 plans the pieces. The others take kGatherRows compact rows each, four rows a warp with
+// all their loads in flight: lane i takes the 16 latent values from 16 i on, and two of the 64 RoPE
+// values. What bounds it: the chain of dependent loads (sequence, page, row) for small calls, so
+// rows are spread over many blocks; HBM for large ones (a row read and written once).
+constexpr int kGatherRows = 4 * kGatherWarps;
 static_assert(kRowTile % kGatherRows == 0, "a block's rows lie in one sequence");
 
-__global__ void __launch_bounds__(256) gather_kernel(const Args a) {
+__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Args a) {
+  __shared__ PlanShared sh;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const Work& w = a.w;
-  const int r0 = int(blockIdx.x) * kGatherRows;
+  if (blockIdx.x == 0) {
+    plan_pieces(a, sh);
+    return;
+  }
+  const int r0 = int(blockIdx.x - 1) * kGatherRows;
   if (r0 >= w.header[kHdrRows]) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int s = last_at_or_below(w.seq_key0, a.seqs, r0);
@@ -424,8 +457,8 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a) {
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr uint32_t kWaitPolls = 1u << 26;
 
-// Bounded waits of one role of a CTA pair. What they wait for lies in TMEM or is written and read by
-// the asynchronous proxies (TMA, MMA), ordered by the barriers and tcgen05 fences themselves: no
+// Bounded waits of one role of a CTA pair. What they wait for lies in TMEM or is written and read
+// by the asynchronous proxies (TMA, MMA), ordered by the barriers and tcgen05 fences themselves: no
 // wait or arrival here needs the cluster-scope release or acquire of generic memory, which cost a
 // memory barrier per tile (2.0 of 9.8 warps stalled in it). The first wait that runs out writes its
 // barrier into both CTAs' abort words, and every later wait of the pair returns false soon; the
@@ -465,8 +498,8 @@ struct Waiter {
     failed = true;
     return false;
   }
-  // The end of an aborted CTA: the error flag, and a millisecond in which the pair's copies and MMAs
-  // in flight land.
+  // The end of an aborted CTA: the error flag, and a millisecond in which the pair's copies and
+  // MMAs in flight land.
   __device__ void settle(int* header) {
     const uint32_t bar = ptx::ld_shared_u32(abort);
     if (!bar) return;
@@ -554,11 +587,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   };
   if (threadIdx.x == 0)
     for (int c = 0; c < kChunks; ++c) load_weights(columns * pair / pairs, c);
-  ptx::grid_dependency_wait();
-  ptx::grid_launch_dependents();
+  // The rows must have been gathered, and the pass before must have read the keys and values that
+  // this one replaces. Its stores follow its loads, so the load warp alone waits. The plan is in
+  // place before: the gather's blocks let this grid start after their own wait for it.
+  if (warp == 0) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+  }
   // At most kScratchBytes of 128 KB items, or the 2^17 row tiles of one head: 32 bits hold the
   // products with the pairs.
-  const uint32_t tiles = uint32_t(a.w.header[kHdrRows] + 255) / 256;
+  const uint32_t tiles = uint32_t(__ldcg(a.w.header + kHdrRows) + 255) / 256;
   const uint32_t items = tiles * uint32_t(columns);
   const uint32_t first = items * uint32_t(pair) / uint32_t(pairs);
   const uint32_t last = items * uint32_t(pair + 1) / uint32_t(pairs);
@@ -662,8 +700,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
   }
-  // Every commit of the leader has arrived in both CTAs before either leaves. One warp polls for it;
-  // the others go on to the cluster barrier, which costs no issue slots.
+  // Every commit of the leader has arrived in both CTAs before either leaves. One warp polls for
+  // it; the others go on to the cluster barrier, which costs no issue slots.
   if (warp == 0) wt.on(bar(kBarDrain), 0);
   wt.settle(a.w.header);
   ptx::tc_fence_before();
@@ -691,17 +729,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 //               on the first 64 keys while the other half's exponentials run. A softmax warp may
 //               be several tiles ahead of PV, so the completion of PV_j has a barrier per buffer:
 //               a waiter has seen S_j, which lies behind PV_{j-kS}, and its phase is the next.
-//   warps 4-11  softmax: two groups of four warps take the tiles in turn, a thread a row, so that
-//               one group's exponentials run under the other's loads, maxima and waits (both
-//               groups on each tile's halves in step took 2990 cycles a tile, of them 1350 in the
-//               exponentials). P goes to TMEM as bf16 over the scores. The reference maximum of a
-//               row passes from group to group through shared memory. It moves only when it would
-//               grow by more than 2^8 (kSlack): then O is rescaled, after the last PV; otherwise p
-//               stays below 2^8 and the final division makes it exact. Each thread's sum is over
-//               its own tiles.
+//   warps 4-11  softmax, a thread a row, in two groups of four warps. With three score buffers (192
+//               columns) the groups take the tiles in turn, so that one group's exponentials run
+//               under the other's loads, maxima and waits, and the row's reference maximum passes
+//               from group to group through shared memory; with two (256 columns) both work on
+//               every tile, half of its keys each, and exchange their maxima (Shape::kHalves). P
+//               goes to TMEM as bf16 over the scores. The reference moves only when it would grow
+//               by more than 2^8 (kSlack): then O is rescaled, after the last PV; otherwise p
+//               stays below 2^8 and the final division makes it exact. Each thread sums its own
+//               keys' weights; the two sums of a row meet at the unit's end.
 //
 // What bounds it: per 128 x 128 tile and CTA the tensor cores need (2 (Dqk + Dv) 128 128) / 8192
-// cycles (1280 at 192 + 128, 2048 at 256 + 256), the exponentials 128 128 / 16 = 1024.
+// cycles (1280 at 192 + 128, 2048 at 256 + 256), the exponentials 128 128 / 16 = 1024. Measured:
+// 64 heads of 192 + 128, 2048 tokens over 4096 cached rows 369 us, the tensor pipe active in 65% of
+// the cycles and the exponentials' unit in 52%; 64 heads of 256 + 256, 4096 tokens 419 us, 80% and
+// 40%. What is lost lies in the handoffs between a tile's scores, weights and product, and in
+// instruction fetch: the roles are seven different loops that share the caches, so that code added
+// to any of them (unrolled loops, weights by a polynomial, a second MMA warp) cost more than it
+// gained. In long calls the power limit holds the clock at 1.4 GHz of 1.97.
 namespace attend {
 
 constexpr int kThreads = 384;
@@ -743,13 +788,14 @@ struct Shape {
   static constexpr uint32_t kSmBytes = kSmMisc + 16 + 1024;
   static constexpr uint32_t kTmemO = kS * 128;
   // With two score buffers a tile's own chain (scores, softmax, PV, the next scores in the buffer)
-  // is the limit, and both softmax groups work on every tile, half of its keys each; with three the
-  // groups take the tiles in turn, and one's exponentials run under the other's loads and maxima.
+  // is the limit, and both softmax groups work on every tile, half of its keys each (4096 tokens,
+  // 64 heads of 256: 622 us a call, in turn 645); with three the groups take the tiles in turn
+  // (2 x 2048 tokens, 128 heads of 192: 2030 us, by halves 2117).
   static constexpr bool kHalves = kS == 2;
-  // In turn: the quarter of a tile's exponentials after which the turn passes. The earlier, the more
-  // the two groups' exponentials overlap and slow each other; the later, the longer a tile takes
-  // (after the first quarter 1553 us of attention for 2 x 2048 tokens of 128 heads, after the second
-  // 1545).
+  // In turn: the quarter of a tile's exponentials after which the turn passes. The earlier, the
+  // more the two groups' exponentials overlap and slow each other; the later, the longer a tile
+  // takes (after the first quarter 1553 us of attention for 2 x 2048 tokens of 128 heads, after the
+  // second 1545).
   static constexpr int kTurn = 1;
   static_assert(kSmBytes <= 232448, "shared memory per CTA");
   static_assert(kTmemO + kDv <= 512, "TMEM columns");
@@ -782,9 +828,9 @@ struct Unit {
 
 // Units in the order in which they are taken: head by head, so that the pairs at work at one time
 // share the keys and values of few heads in L2, and within a head the longest piece first. The last
-// two rounds' worth of heads go piece by piece instead, so that the call ends on short units (with a
-// fixed round-robin of units the longest pair had 11% more than the mean at 4096 tokens, 12% in a
-// ragged batch; now about 2%).
+// two rounds' worth of heads go piece by piece instead, so that the call ends on short units (with
+// a fixed round-robin of units the longest pair had 11% more than the mean at 4096 tokens, 12% in
+// a ragged batch; now about 2%).
 __device__ __forceinline__ Unit unit_at(const Args& a, int u, int pieces, int pairs) {
   const int last = min(a.pass_heads, (2 * pairs + pieces - 1) / pieces);
   const int first = (a.pass_heads - last) * pieces;  // units of the heads before those
@@ -798,7 +844,7 @@ __device__ __forceinline__ Unit unit_at(const Args& a, int u, int pieces, int pa
     x.head = a.pass_heads - last + (u - first) - piece * last;
   }
   const int4* src = reinterpret_cast<const int4*>(a.w.order + piece);
-  const int4 lo = src[0], hi = src[1];
+  const int4 lo = __ldcg(src), hi = __ldcg(src + 1);
   x.p = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
   return x;
 }
@@ -823,7 +869,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sm + C::kSmMisc);
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kBars; ++i) {
-      // P of half a tile: its group's four warps in either CTA; the release of O: all softmax warps.
+      // P of half a tile: its group's four warps in either CTA; the release of O: all softmax
+      // warps.
       const bool joint = i >= C::kPFull && i < C::kPFull + 2 * C::kS;
       // A unit's info: every warp but the one that fetches it and a follower's idle warp 1.
       const bool read = i >= C::kInfoEmpty && i < C::kInfoEmpty + 2;
@@ -846,10 +893,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   Waiter wt{base + C::kSmMisc + 4, false};
-  ptx::grid_dependency_wait();
-  ptx::grid_launch_dependents();
-  // All 512 columns are this CTA's, so they start at 0.
-  const int pieces = a.w.header[kHdrPieces], units = pieces * a.pass_heads;
+  // Only the keys and values must be waited for, by the warps that load them. The expansion lets
+  // this grid start after its own wait for the gather, so the plan and the pieces are in place, and
+  // the first unit's rows and queries are fetched under the expansion's end (from L2: lines of an
+  // earlier call may lie in L1). All 512 columns are this CTA's, so they start at 0.
+  const int pieces = __ldcg(a.w.header + kHdrPieces), units = pieces * a.pass_heads;
   // The n-th unit, for one lane of a load warp; the MMA warp takes it as a whole.
   struct UnitRef {
     int row0, key0, tiles, head;
@@ -877,7 +925,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int c = 0; c < C::kQChunks; ++c)
           ptx::tma_load_3d_pair(base + c * 16384, &tm_q, lead(C::kQFull), c * 64, a.head0 + x.head,
                                 x.row0 + rank * 128);
-        ++useq;
+        if (useq++ == 0) ptx::grid_dependency_wait();
         for (int j = 0; j < x.tiles; ++j) {
           const uint32_t st = uint32_t(j % C::kKv), ph = free.take(st) ^ 1u;
           const int key = x.key0 + j * kRowTile;
@@ -960,6 +1008,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 2) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     if (lane == 0) {
       Phases<C::kKv> free;
       for (uint32_t n = 0;; ++n) {
@@ -980,8 +1030,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 3) {
-    // The first unit is the pair's own; then the leader takes the next one from the pass's counter and
-    // tells the other CTA.
+    // The first unit is the pair's own; then the leader takes the next one from the pass's counter
+    // and tells the other CTA.
     const uint32_t mail = base + C::kSmExch + 3088;
     for (uint32_t n = 0;; ++n) {
       int u = int(blockIdx.x) >> 1;
@@ -1005,8 +1055,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int keys = 0, spoilt = INT_MAX;
       if (!end) {
         x = unit_at(a, u, pieces, pairs);
-        keys = a.w.seq_keys[x.p.seq];
-        spoilt = a.w.seq_spoilt[x.p.seq];
+        keys = __ldcg(a.w.seq_keys + x.p.seq);
+        spoilt = __ldcg(a.w.seq_spoilt + x.p.seq);
       }
       if (!wt.all(bar(C::kInfoEmpty + int(n & 1u)), ((n >> 1) & 1u) ^ 1u)) break;
       Info* info = reinterpret_cast<Info*>(sm + C::kSmInfo) + (n & 1u);
@@ -1015,7 +1065,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int r = i * 32 + lane, at = rank * 128 + r;
         int seen = 0;
         if (at < x.p.rows) {
-          const int pos = a.q_pos[x.p.row0 + at];
+          const int pos = __ldcg(a.q_pos + x.p.row0 + at);
           seen = pos >= keys ? keys : max(pos + 1, 0);
           if (seen > spoilt) seen |= kSpoilt;
         }
@@ -1048,8 +1098,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (uint32_t nth = 0;; ++nth) {
       const Info* info = reinterpret_cast<const Info*>(sm + C::kSmInfo) + (nth & 1u);
       wt.all(bar(C::kInfoFull + int(nth & 1u)), (nth >> 1) & 1u);
-      // A wait that ran out ends the loop here for both warps of a row, and only here: inside a unit
-      // they go through the same barriers to its end, over whatever TMEM holds.
+      // A wait that ran out ends the loop here for both warps of a row, and only here: inside a
+      // unit they go through the same barriers to its end, over whatever TMEM holds.
       if (wt.failed && lane == 0) gone[quad] = 1;
       ptx::named_barrier(9 + quad, 64);
       if (gone[quad]) break;
@@ -1327,7 +1377,8 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
     if (blk.pieces == 1 || row >= blk.rows) continue;
     const long long p0 = ((long long)head * pieces + blk.piece0) * kQueryTile + row;
     float top = -INFINITY;
-    for (int k = 0; k < blk.pieces; ++k) top = fmaxf(top, w.part_lse[p0 + (long long)k * kQueryTile]);
+    for (int k = 0; k < blk.pieces; ++k)
+      top = fmaxf(top, w.part_lse[p0 + (long long)k * kQueryTile]);
     const float use = top == -INFINITY ? 0.f : top;
     float o[8] = {}, sum = 0.f;
 #pragma unroll 4
@@ -1363,7 +1414,8 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
 
 // ------------------------------------------------------------------------------ host
 struct Layout {
-  uint64_t header, seq_key0, seq_keys, seq_block, seq_spoilt, blocks, pieces, order, part_out, part_lse, rows, rope, k, v, total;
+  uint64_t header, seq_key0, seq_keys, seq_block, seq_spoilt, blocks, pieces, order;
+  uint64_t part_out, part_lse, rows, rope, k, v, total;
   uint64_t cap, max_blocks, pass_heads, split_units;
 };
 
@@ -1581,7 +1633,7 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
     return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess;
   };
   if (!launch(plan_kernel, 1, 1024, 0, a) ||
-      !launch(gather_kernel, a.cap / kGatherRows, 256, 0, a))
+      !launch(gather_kernel, 1 + a.cap / kGatherRows, kGatherThreads, 0, a))
     return fail("launch", TQ_ERR_CUDA);
   for (a.head0 = 0; a.head0 < a.heads; a.head0 += int(l.pass_heads), ++a.pass) {
     a.pass_heads = a.heads - a.head0 < int(l.pass_heads) ? a.heads - a.head0 : int(l.pass_heads);

@@ -13,7 +13,7 @@
 // requests and fills its share of the tokens, finding a token's request by bisection in shared
 // memory and a new page in the free stack rather than in the table that another CTA may be writing
 // (512 requests with 14841 tokens: 4.4 us on the device, 10.5 with a scan split over a cluster and
-// bisection in global memory).
+// bisection in global memory; 5.6 us a call, 64 decode requests 4.9, 4096 requests 8.3).
 // Beyond kNear, clusters of C CTAs split the requests: each CTA sums its share, the CTAs exchange
 // their totals through distributed shared memory, scan their share with that base, and after a
 // cluster barrier fill the tokens. With more than one cluster, every cluster does the whole scan
