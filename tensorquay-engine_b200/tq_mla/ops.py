@@ -9,6 +9,7 @@ and to name the current stream.
 """
 
 import collections
+import contextlib
 import ctypes
 import math
 
@@ -298,11 +299,12 @@ class MlaPrologue:
 def mla_prologue(x, w_qa, q_norm, w_qb, w_uk, w_kva, kv_norm, pos, seq_id, page_table, kv, *,
                  heads, nope_dim, rope_dim, q=None, flags=None, stream=None, **kw):
     """One prologue call (see ``MlaPrologue``); returns ``q``."""
-    if q is None:
-        width = (512 if w_uk is not None else nope_dim) + rope_dim
-        q = torch.empty((x.shape[0], heads, width), dtype=torch.bfloat16, device=x.device)
-    return MlaPrologue(x, w_qa, q_norm, w_qb, w_uk, w_kva, kv_norm, pos, seq_id, page_table, kv, q,
-                       heads=heads, nope_dim=nope_dim, rope_dim=rope_dim, **kw)(flags, stream)
+    with _allocating_on(stream):
+        if q is None:
+            width = (512 if w_uk is not None else nope_dim) + rope_dim
+            q = torch.empty((x.shape[0], heads, width), dtype=torch.bfloat16, device=x.device)
+        return MlaPrologue(x, w_qa, q_norm, w_qb, w_uk, w_kva, kv_norm, pos, seq_id, page_table, kv,
+                           q, heads=heads, nope_dim=nope_dim, rope_dim=rope_dim, **kw)(flags, stream)
 
 
 class _Launch:
@@ -335,6 +337,12 @@ class _Launch:
         status = fn(self._spec_ref, *args, handle, self._err_ref)
         if status:
             raise_for(status, self._err)
+
+
+def _allocating_on(stream):
+    """What is allocated within belongs to ``stream``: memory freed after a launch there is not
+    handed to work of another stream while the launch still uses it."""
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
 
 
 def _flags_pointer(flags):
@@ -389,7 +397,9 @@ class StepPlan(_Launch):
 def step_plan(cached_len, new_len, page_table, free_pages, free_count, *, tokens, flags=None,
               stream=None):
     """One step plan (see ``StepPlan``); returns its ``StepTables``."""
-    return StepPlan(cached_len, new_len, page_table, free_pages, free_count, tokens=tokens)(flags, stream)
+    with _allocating_on(stream):
+        return StepPlan(cached_len, new_len, page_table, free_pages, free_count,
+                        tokens=tokens)(flags, stream)
 
 
 def block_norm_spec(y, residual, out, x=None, *, post_weight=None, gate=None, scale=1.0,
@@ -428,11 +438,12 @@ class BlockNorm(_Launch):
 
 def block_norm(y, residual, *, pre_weight=None, out=None, x=None, stream=None, **kw):
     """One block norm (see ``BlockNorm``); returns ``(out, x)``, ``x`` None without ``pre_weight``."""
-    if out is None:
-        out = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
-    if x is None and pre_weight is not None:
-        x = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    return BlockNorm(y, residual, out, x, pre_weight=pre_weight, **kw)(stream)
+    with _allocating_on(stream):
+        if out is None:
+            out = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
+        if x is None and pre_weight is not None:
+            x = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+        return BlockNorm(y, residual, out, x, pre_weight=pre_weight, **kw)(stream)
 
 
 def chunk_spec(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse=None, *, scale,
@@ -460,7 +471,8 @@ class MlaChunk(_Launch):
     rows ``q_start[s]`` to ``q_start[s + 1]`` of ``q`` belong to sequence ``s`` and see its cached
     rows below ``min(kv_len[s], q_pos + 1)``; ``out`` bf16 or f32 ``[T, H, Dv]``, ``lse`` f32
     ``[T, H]`` or None. ``max_keys`` bounds the summed ``kv_len`` of the sequences with tokens.
-    Owns only its workspace.
+    Owns only its workspace: launches of one object are ordered on one stream, and the object
+    outlives them when that is not the stream on which it was made.
     """
 
     def __init__(self, q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse=None, *, scale,
@@ -495,12 +507,13 @@ def mla_chunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, *, scale, m
               lse=None, out_dtype=torch.bfloat16, kv_format=None, stream=None):
     """One chunk attention call (see ``MlaChunk``); returns ``(out, lse)``."""
     t, h = q.shape[0], q.shape[1]
-    if out is None:
-        out = torch.empty((t, h, w_uv.shape[1]), dtype=out_dtype, device=q.device)
-    if lse is None:
-        lse = torch.empty((t, h), dtype=torch.float32, device=q.device)
-    return MlaChunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse, scale=scale,
-                    max_keys=max_keys, kv_format=kv_format)(stream)
+    with _allocating_on(stream):
+        if out is None:
+            out = torch.empty((t, h, w_uv.shape[1]), dtype=out_dtype, device=q.device)
+        if lse is None:
+            lse = torch.empty((t, h), dtype=torch.float32, device=q.device)
+        return MlaChunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse, scale=scale,
+                        max_keys=max_keys, kv_format=kv_format)(stream)
 
 
 def combine_parts(part_out, part_lse, out=None, lse=None, stream=None):

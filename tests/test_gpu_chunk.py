@@ -451,6 +451,33 @@ def test_two_launches_on_two_streams(cuda_device):
     b.check()
 
 
+def test_a_call_on_another_stream_keeps_its_memory(cuda_device):
+    """What a call allocates and drops on return is not handed to the current stream while the call
+    still runs on its own."""
+    c = Case(cuda_device, 2, [512], [1500], heads=16, seed=21)
+    launch = c.launch()
+    launch()
+    torch.cuda.synchronize()
+    need = launch.workspace.numel()
+    want, want_lse = c.out.clone(), c.lse.clone()
+    del launch
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        torch.zeros(need, dtype=torch.uint8, device=cuda_device)     # a free block of the current stream
+        outs = []
+        meta = [i32(x, cuda_device) for x in (c.table, c.q_start, c.q_pos, c.kv_len)]
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(3):
+            outs.append(ops.mla_chunk(c.q, c.w_uk, c.w_uv, c.kv, *meta, scale=c.scale,
+                                      max_keys=int(c.kv_len.sum()), stream=side))
+            torch.full((need,), 255, dtype=torch.uint8, device=cuda_device)
+        torch.cuda.synchronize()
+        for out, lse in outs:
+            assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
 def test_pages_past_four_gigabytes(cuda_device):
     c = Case(cuda_device, 2, [50], [200], seed=12)
     pages = 60000                                # 4.4 GB of 576-wide rows
