@@ -367,7 +367,8 @@ int32_t tq_mla_prologue(const TqPrologueSpec* spec, void* workspace, uint64_t wo
  *   kv_len     i32 [S]     out: cached_len + new_len
  *   seq_id, q_pos, slot    i32 [T] out: request, position and pool row (page * 64 + position % 64)
  *                          of each token row; rows from q_start[S] on get -1 (a batch padded to
- *                          a captured size). `slot` may have rank 0: it is then not written.
+ *                          a captured size; the calls that take seq_id leave such a row empty and
+ *                          set TQ_DEV_SEQ_RANGE). `slot` may have rank 0: it is then not written.
  *   free_left  i32 [1]     out: free_count less the pages taken; may not be free_count itself
  * The o-th page that the batch takes, request by request and in position order, is
  * free_pages[free_count - 1 - o]. The call changes none of its inputs but the grown columns, so

@@ -587,16 +587,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   };
   if (threadIdx.x == 0)
     for (int c = 0; c < kChunks; ++c) load_weights(columns * pair / pairs, c);
-  // The rows must have been gathered, and the pass before must have read the keys and values that
-  // this one replaces. Its stores follow its loads, so the load warp alone waits. The plan is in
-  // place before: the gather's blocks let this grid start after their own wait for it.
-  if (warp == 0) {
-    ptx::grid_dependency_wait();
-    ptx::grid_launch_dependents();
-  }
+  // The number of rows is in place ahead of the wait for the gather: its blocks let this grid start
+  // after their own wait for the plan.
+  const int rows_used = __ldcg(a.w.header + kHdrRows);
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   // At most kScratchBytes of 128 KB items, or the 2^17 row tiles of one head: 32 bits hold the
   // products with the pairs.
-  const uint32_t tiles = uint32_t(__ldcg(a.w.header + kHdrRows) + 255) / 256;
+  const uint32_t tiles = uint32_t(rows_used + 255) / 256;
   const uint32_t items = tiles * uint32_t(columns);
   const uint32_t first = items * uint32_t(pair) / uint32_t(pairs);
   const uint32_t last = items * uint32_t(pair + 1) / uint32_t(pairs);
@@ -877,7 +875,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       ptx::mbar_init(bar(i), joint ? 8 : read ? 11 - rank : i == C::kOFree ? 16 : 1);
     }
     tmem_holder[1] = 0;  // the abort word
-    for (int i = 0; i < 4; ++i) reinterpret_cast<int*>(sm + C::kSmExch + 3072)[i] = 0;
+    for (int i = 0; i < 4; ++i) reinterpret_cast<int*>(sm + C::kSmExch + 6 * 128 * 4)[i] = 0;
     ptx::fence_mbar_init_cluster();
     ptx::tma_prefetch_desc(&tm_q);
     ptx::tma_prefetch_desc(&tm_k);
@@ -893,10 +891,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   Waiter wt{base + C::kSmMisc + 4, false};
-  // Only the keys and values must be waited for, by the warps that load them. The expansion lets
-  // this grid start after its own wait for the gather, so the plan and the pieces are in place, and
-  // the first unit's rows and queries are fetched under the expansion's end (from L2: lines of an
-  // earlier call may lie in L1). All 512 columns are this CTA's, so they start at 0.
+  // The expansion lets this grid start after its own wait for the gather, so the plan and the pieces
+  // are in place ahead of the wait for the keys and values: warps 0 and 3 fetch the first unit's
+  // rows and queries before it (from L2: lines of an earlier call may lie in L1), then they wait
+  // like the others. All 512 columns are this CTA's, so they start at 0.
+  if (warp != 0 && warp != 3) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+  }
   const int pieces = __ldcg(a.w.header + kHdrPieces), units = pieces * a.pass_heads;
   // The n-th unit, for one lane of a load warp; the MMA warp takes it as a whole.
   struct UnitRef {
@@ -918,14 +920,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (uint32_t n = 0;; ++n) {
         const UnitRef x = next_unit(n);
         if (x.tiles < 0) break;
-        if (!x.tiles) continue;
-        if (!wt.on(bar(C::kQEmpty), (useq & 1u) ^ 1u)) break;
-        if (rank == 0) ptx::mbar_expect_tx(bar(C::kQFull), 2 * C::kQBytes);
+        if (x.tiles) {
+          if (!wt.on(bar(C::kQEmpty), (useq & 1u) ^ 1u)) break;
+          if (rank == 0) ptx::mbar_expect_tx(bar(C::kQFull), 2 * C::kQBytes);
 #pragma unroll
-        for (int c = 0; c < C::kQChunks; ++c)
-          ptx::tma_load_3d_pair(base + c * 16384, &tm_q, lead(C::kQFull), c * 64, a.head0 + x.head,
-                                x.row0 + rank * 128);
-        if (useq++ == 0) ptx::grid_dependency_wait();
+          for (int c = 0; c < C::kQChunks; ++c)
+            ptx::tma_load_3d_pair(base + c * 16384, &tm_q, lead(C::kQFull), c * 64,
+                                  a.head0 + x.head, x.row0 + rank * 128);
+          ++useq;
+        }
+        if (n == 0) ptx::grid_dependency_wait();
         for (int j = 0; j < x.tiles; ++j) {
           const uint32_t st = uint32_t(j % C::kKv), ph = free.take(st) ^ 1u;
           const int key = x.key0 + j * kRowTile;
@@ -1008,8 +1012,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 2) {
-    ptx::grid_dependency_wait();
-    ptx::grid_launch_dependents();
     if (lane == 0) {
       Phases<C::kKv> free;
       for (uint32_t n = 0;; ++n) {
@@ -1034,6 +1036,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // and tells the other CTA.
     const uint32_t mail = base + C::kSmExch + 3088;
     for (uint32_t n = 0;; ++n) {
+      if (n == 1) ptx::grid_dependency_wait();
       int u = int(blockIdx.x) >> 1;
       if (n == 0) {
       } else if (rank == 0) {
