@@ -314,6 +314,33 @@ def test_heads_in_several_passes(cuda_device, fmt):
     torch.cuda.empty_cache()
 
 
+def test_passes_without_a_join_between_them(cuda_device):
+    """So many query blocks that none is split: the next pass's expansion directly follows an
+    attention. The same sums in the same order as in one pass, so the same bits."""
+    c = Case(cuda_device, 2, [1100, 500], [0, 300], heads=80, seed=22)
+    c.launch()()
+    torch.cuda.synchronize()
+    want, want_lse = c.out, c.lse
+    launch = c.launch(max_keys=280000)           # 59 heads a pass
+    for _ in range(4):
+        c.out.fill_(7.0)
+        c.lse.fill_(7.0)
+        launch()
+        assert launch.device_error() == 0
+        assert torch.equal(c.out, want) and torch.equal(c.lse, want_lse)
+    sample = [0, 58, 59, 79]                     # heads of both passes against the oracle
+    small = Case.__new__(Case)
+    small.__dict__.update(c.__dict__)
+    small.heads = len(sample)
+    for name in ("q", "out", "lse"):
+        setattr(small, name, getattr(c, name)[:, sample].contiguous())
+    for name in ("w_uk", "w_uv"):
+        setattr(small, name, getattr(c, name)[sample].contiguous())
+    small.check()
+    del launch
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("fmt", [0, 2])
 def test_a_query_that_is_not_finite_stays_in_its_row(cuda_device, fmt):
     c = Case(cuda_device, fmt, [140], [20], seed=5)
