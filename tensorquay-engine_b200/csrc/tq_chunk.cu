@@ -749,6 +749,11 @@ namespace attend {
 
 constexpr int kThreads = 384;
 constexpr float kSlack = 8.f;  // log2 units
+// A pair takes its next unit when the load warp comes to this many tiles before the end of the one
+// at work, itself up to three tiles ahead: late enough that units go to the pairs that are free
+// (taken a whole unit ahead, pairs ended 357 to 432 us into the attention of 4096 tokens, now 398
+// to 408), early enough that the unit's rows are there in time (1, 2 and 4 measure alike).
+constexpr int kClaimAhead = 2;
 
 // A unit as the warps of a CTA take it, fetched ahead by warp 3. tiles < 0: there are no more.
 struct Info {
@@ -781,14 +786,15 @@ struct Shape {
   static constexpr int kPvDone = kPFull + 2 * kS, kOFree = kPvDone + kS, kDrain = kOFree + 1;
   static constexpr int kInfoFull = kDrain + 1, kInfoEmpty = kInfoFull + 2;
   static constexpr int kMailFull = kInfoEmpty + 2, kMailEmpty = kMailFull + 1;
-  static constexpr int kBars = kMailEmpty + 1;
+  static constexpr int kClaim = kMailEmpty + 1;
+  static constexpr int kBars = kClaim + 1;
   static constexpr uint32_t kSmMisc = kSmBars + 8 * kBars;
   static constexpr uint32_t kSmBytes = kSmMisc + 16 + 1024;
   static constexpr uint32_t kTmemO = kS * 128;
   // With two score buffers a tile's own chain (scores, softmax, PV, the next scores in the buffer)
   // is the limit, and both softmax groups work on every tile, half of its keys each (4096 tokens,
-  // 64 heads of 256: 622 us a call, in turn 645); with three the groups take the tiles in turn
-  // (2 x 2048 tokens, 128 heads of 192: 2030 us, by halves 2117).
+  // 64 heads of 256: 622 us a call where in turn took 645); with three the groups take the tiles in
+  // turn (2 x 2048 tokens, 128 heads of 192: 2030 us, by halves 2117).
   static constexpr bool kHalves = kS == 2;
   // In turn: the quarter of a tile's exponentials after which the turn passes. The earlier, the
   // more the two groups' exponentials overlap and slow each other; the later, the longer a tile
@@ -826,9 +832,7 @@ struct Unit {
 
 // Units in the order in which they are taken: head by head, so that the pairs at work at one time
 // share the keys and values of few heads in L2, and within a head the longest piece first. The last
-// two rounds' worth of heads go piece by piece instead, so that the call ends on short units (with
-// a fixed round-robin of units the longest pair had 11% more than the mean at 4096 tokens, 12% in
-// a ragged batch; now about 2%).
+// two rounds' worth of heads go piece by piece instead, so that the call ends on short units.
 __device__ __forceinline__ Unit unit_at(const Args& a, int u, int pieces, int pairs) {
   const int last = min(a.pass_heads, (2 * pairs + pieces - 1) / pieces);
   const int first = (a.pass_heads - last) * pieces;  // units of the heads before those
@@ -891,10 +895,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   Waiter wt{base + C::kSmMisc + 4, false};
-  // The expansion lets this grid start after its own wait for the gather, so the plan and the pieces
-  // are in place ahead of the wait for the keys and values: warps 0 and 3 fetch the first unit's
-  // rows and queries before it (from L2: lines of an earlier call may lie in L1), then they wait
-  // like the others. All 512 columns are this CTA's, so they start at 0.
+  // The expansion lets this grid start after its own wait for the gather, so the plan and the
+  // pieces are in place ahead of the wait for the keys and values: warps 0 and 3 fetch the first
+  // unit's rows and queries before it (from L2: lines of an earlier call may lie in L1), then they
+  // wait like the others. All 512 columns are this CTA's, so they start at 0.
   if (warp != 0 && warp != 3) {
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
@@ -930,7 +934,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ++useq;
         }
         if (n == 0) ptx::grid_dependency_wait();
+        if (!x.tiles && rank == 0) ptx::mbar_arrive(bar(C::kClaim));
         for (int j = 0; j < x.tiles; ++j) {
+          if (j == max(0, x.tiles - kClaimAhead) && rank == 0) ptx::mbar_arrive(bar(C::kClaim));
           const uint32_t st = uint32_t(j % C::kKv), ph = free.take(st) ^ 1u;
           const int key = x.key0 + j * kRowTile;
           if (!wt.on(bar(C::kKEmpty + st), ph)) break;
@@ -1032,14 +1038,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 3) {
-    // The first unit is the pair's own; then the leader takes the next one from the pass's counter
-    // and tells the other CTA.
+    // The first unit is the pair's own; then, near the end of each, the leader takes the next one
+    // from the pass's counter and tells the other CTA.
     const uint32_t mail = base + C::kSmExch + 3088;
     for (uint32_t n = 0;; ++n) {
       if (n == 1) ptx::grid_dependency_wait();
       int u = int(blockIdx.x) >> 1;
       if (n == 0) {
       } else if (rank == 0) {
+        if (!wt.all(bar(C::kClaim), (n & 1u) ^ 1u)) break;
         if (!wt.all(bar(C::kMailEmpty), n & 1u)) break;
         if (lane == 0) {
           u = pairs + atomicAdd(a.w.header + kHdrNext + a.pass, 1);
