@@ -411,9 +411,9 @@ int32_t tq_block_norm(const TqBlockNormSpec* spec, void* stream, TqContractError
  * weights folded into the query and the output: a (query, key, head) triple costs
  * 2 (Dn + Dr + Dv) FLOP instead of 2 (1024 + Dr), and each cached row costs 1024 (Dn + Dv) FLOP
  * a head once per call. So it is the cheaper form for sequences of many new tokens: at 128 heads
- * of 576-wide rows, one sequence over 8000 cached rows takes 377 us for 128 tokens and 382 for 256
- * where tq_mla_prefill takes 312 and 597, eight over 1000 rows 435 and 475 where it takes 474 and
- * 915 (and its caller still folds the weights). A sequence of fewer tokens over a long cache
+ * of 576-wide rows, one sequence over 8000 cached rows takes 375 us for 128 tokens and 379 for 256
+ * where tq_mla_prefill takes 311 and 595, eight over 1000 rows 433 and 474 where it takes 464 and
+ * 922 (and its caller still folds the weights). A sequence of fewer tokens over a long cache
  * belongs in a tq_mla_prefill or tq_mla_decode call beside this one. For sequence s, rows
  * t in [q_start[s], q_start[s + 1]) and cached rows n < kv_len[s]:
  *   k[n, h] = bf16(latent[n] . w_uk[h]^T), followed by the row's Dr RoPE values

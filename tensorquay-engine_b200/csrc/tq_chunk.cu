@@ -530,7 +530,7 @@ namespace expand {
 constexpr int kThreads = 256;  // warp 0 loads, warp 1 MMA, warps 4-7 epilogue
 constexpr int kChunks = kLatent / 64;
 constexpr uint32_t kBox = 128 * 128;  // 128 rows x 64 values
-constexpr int kStages = 5;
+constexpr int kStages = 6;  // what shared memory holds (5: 65492 rows, 32 heads 440 us, now 427)
 constexpr uint32_t kSmW = 0;                              // [kChunks] boxes of weights
 constexpr uint32_t kSmA = kChunks * kBox;                 // [kStages] boxes of rows
 constexpr uint32_t kSmBars = kSmA + kStages * kBox;
@@ -739,8 +739,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 //
 // What bounds it: per 128 x 128 tile and CTA the tensor cores need (2 (Dqk + Dv) 128 128) / 8192
 // cycles (1280 at 192 + 128, 2048 at 256 + 256), the exponentials 128 128 / 16 = 1024. Measured:
-// 64 heads of 192 + 128, 2048 tokens over 4096 cached rows 369 us, the tensor pipe active in 65% of
-// the cycles and the exponentials' unit in 52%; 64 heads of 256 + 256, 4096 tokens 419 us, 80% and
+// 64 heads of 192 + 128, 2048 tokens over 4096 cached rows 376 us, the tensor pipe active in 65% of
+// the cycles and the exponentials' unit in 52%; 64 heads of 256 + 256, 4096 tokens 403 us, 80% and
 // 40%. What is lost lies in the handoffs between a tile's scores, weights and product, and in
 // instruction fetch: the roles are seven different loops that share the caches, so that code added
 // to any of them (unrolled loops, weights by a polynomial, a second MMA warp) cost more than it
