@@ -1206,6 +1206,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                   !grow ? 1.f : m == -INFINITY ? 0.f : ptx::ex2((m - high) * c);
               if (grow) m = high;
               rescale(j, keep, group * (kDv / 2), kDv / 2);
+              // The first half of PV_j starts on group 0's weights alone and adds to all columns of
+              // O, so group 1's are rescaled before group 0 goes on. Both warps of these rows are
+              // here: their maxima and references are the same.
+              ptx::tmem_wait_st();
+              ptx::tc_fence_before();
+              ptx::named_barrier(5 + quad, 64);
+              ptx::tc_fence_after();
               sum[0][0] *= keep;
               sum[0][1] *= keep;
               sum[1][0] *= keep;
