@@ -434,8 +434,9 @@ int32_t tq_block_norm(const TqBlockNormSpec* spec, void* stream, TqContractError
  * gets zeros and lse -inf; rows of q before q_start[0] and from q_start[S] on are not computed and
  * their outputs are left as they were. A cached row that is not finite makes every output that sees
  * it NaN and no other; FP8 rows are dequantized to bf16 first. Rounding points: k and v to bf16
- * (the model's own; a value past bf16's range becomes its largest), the softmax weights to bf16
- * before the value product; statistics and sums are f32 (a score past f32's range gives NaN).
+ * (the model's own; a value past bf16's range, or whose partial sums pass f32's, becomes its
+ * largest), the softmax weights to bf16 before the value product; statistics and sums are f32 (a
+ * score past f32's range gives NaN).
  * Device error flags (tq_mla_read_device_error): TQ_DEV_PAGE_RANGE (a page-table entry outside
  * the pool: its rows read as zeros), TQ_DEV_TABLE_SHORT (kv_len past 64 L, cut),
  * TQ_DEV_SEQ_RANGE (q_start not ascending within [0, T]: nothing is computed),
