@@ -127,17 +127,18 @@ def context_merge(comm: Comm, part_out, part_lse, out=None, lse=None, stream=Non
     import torch
 
     from . import _abi
-    from .ops import _TORCH_DTYPE, _stream_handle
+    from .ops import _TORCH_DTYPE, _allocating_on, _returned, _stream_handle
 
     t, h, d = part_out.shape
     if d != 512 or part_out.dtype != torch.float32 or part_lse.shape != (t, h):
         raise ValueError("partials must be f32 [T, H, 512] and f32 [T, H]")
-    part_out, part_lse = part_out.contiguous(), part_lse.contiguous()
-    if out is None:
-        out = torch.empty((t, h, 512), dtype=torch.bfloat16, device=part_out.device)
-    if lse is None:
-        lse = torch.empty((t, h), dtype=torch.float32, device=part_out.device)
-    g_out, g_lse = comm.gather_buffers(t, h, part_out.device)
+    with _allocating_on(stream):
+        part_out, part_lse = part_out.contiguous(), part_lse.contiguous()
+        if out is None:
+            out = torch.empty((t, h, 512), dtype=torch.bfloat16, device=part_out.device)
+        if lse is None:
+            lse = torch.empty((t, h), dtype=torch.float32, device=part_out.device)
+        g_out, g_lse = comm.gather_buffers(t, h, part_out.device)
     p = _abi.TqContextMergeParams()
     p.tokens, p.heads = t, h
     p.part_out, p.part_lse = part_out.data_ptr(), part_lse.data_ptr()
@@ -150,7 +151,7 @@ def context_merge(comm: Comm, part_out, part_lse, out=None, lse=None, stream=Non
     p.out_dtype = _TORCH_DTYPE[out.dtype]
     _abi.raise_for(_abi.lib.tq_mla_context_merge(ctypes.byref(p), comm.handle,
                                                  _stream_handle(stream)))
-    return out, lse
+    return _returned(stream, out, lse)
 
 
 class _DeviceArray:

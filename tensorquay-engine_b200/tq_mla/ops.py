@@ -131,6 +131,22 @@ def _stream_handle(stream):
     return ctypes.c_void_p(stream.cuda_stream)
 
 
+def _allocating_on(stream):
+    """What is allocated within belongs to ``stream``: memory freed after a launch there is not
+    handed to work of another stream while the launch still uses it."""
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
+def _returned(stream, *results):
+    """Results that were allocated on ``stream``, for a caller that reads them on its current stream
+    (once that waits for ``stream``): dropped there, they are not reused before it has read them."""
+    if stream is not None:
+        for t in results:
+            if t is not None:
+                t.record_stream(torch.cuda.current_stream(t.device))
+    return results
+
+
 class MlaLaunch:
     """A validated dense paged MLA launch bound to its tensors and a workspace.
 
@@ -198,16 +214,17 @@ def mla_decode(q, kv, page_table, seq_id, q_pos, kv_len, *, scale, query_counts=
     ``idx[t, j]`` with ``j < k_len[t]``, ``0 <= idx <= q_pos[t]`` and ``idx < kv_len``.
     """
     t, h = q.shape[0], q.shape[1]
-    if out is None:
-        out = torch.empty((t, h, 512), dtype=out_dtype, device=q.device)
-    if lse is None:
-        lse = torch.empty((t, h), dtype=torch.float32, device=q.device)
     if query_counts is None:
         query_counts = torch.bincount(seq_id.cpu().long(), minlength=page_table.shape[0]).tolist()
-    launch = MlaLaunch(q, kv, page_table, seq_id, q_pos, kv_len, out, lse, scale=scale,
-                       query_counts=query_counts, prefill=prefill, kv_format=kv_format, idx=idx,
-                       k_len=k_len)
-    return launch(stream)
+    with _allocating_on(stream):
+        if out is None:
+            out = torch.empty((t, h, 512), dtype=out_dtype, device=q.device)
+        if lse is None:
+            lse = torch.empty((t, h), dtype=torch.float32, device=q.device)
+        MlaLaunch(q, kv, page_table, seq_id, q_pos, kv_len, out, lse, scale=scale,
+                  query_counts=query_counts, prefill=prefill, kv_format=kv_format, idx=idx,
+                  k_len=k_len)(stream)
+    return _returned(stream, out, lse)
 
 
 def kv_write_spec(src, kv, page_table, seq_id, pos, *, kv_format=None, norm_weight=None,
@@ -303,8 +320,9 @@ def mla_prologue(x, w_qa, q_norm, w_qb, w_uk, w_kva, kv_norm, pos, seq_id, page_
         if q is None:
             width = (512 if w_uk is not None else nope_dim) + rope_dim
             q = torch.empty((x.shape[0], heads, width), dtype=torch.bfloat16, device=x.device)
-        return MlaPrologue(x, w_qa, q_norm, w_qb, w_uk, w_kva, kv_norm, pos, seq_id, page_table, kv,
-                           q, heads=heads, nope_dim=nope_dim, rope_dim=rope_dim, **kw)(flags, stream)
+        MlaPrologue(x, w_qa, q_norm, w_qb, w_uk, w_kva, kv_norm, pos, seq_id, page_table, kv, q,
+                    heads=heads, nope_dim=nope_dim, rope_dim=rope_dim, **kw)(flags, stream)
+    return _returned(stream, q)[0]
 
 
 class _Launch:
@@ -337,12 +355,6 @@ class _Launch:
         status = fn(self._spec_ref, *args, handle, self._err_ref)
         if status:
             raise_for(status, self._err)
-
-
-def _allocating_on(stream):
-    """What is allocated within belongs to ``stream``: memory freed after a launch there is not
-    handed to work of another stream while the launch still uses it."""
-    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
 
 
 def _flags_pointer(flags):
@@ -398,8 +410,9 @@ def step_plan(cached_len, new_len, page_table, free_pages, free_count, *, tokens
               stream=None):
     """One step plan (see ``StepPlan``); returns its ``StepTables``."""
     with _allocating_on(stream):
-        return StepPlan(cached_len, new_len, page_table, free_pages, free_count,
-                        tokens=tokens)(flags, stream)
+        tables = StepPlan(cached_len, new_len, page_table, free_pages, free_count,
+                          tokens=tokens)(flags, stream)
+    return StepTables(*_returned(stream, *tables))
 
 
 def block_norm_spec(y, residual, out, x=None, *, post_weight=None, gate=None, scale=1.0,
@@ -443,7 +456,8 @@ def block_norm(y, residual, *, pre_weight=None, out=None, x=None, stream=None, *
             out = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
         if x is None and pre_weight is not None:
             x = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-        return BlockNorm(y, residual, out, x, pre_weight=pre_weight, **kw)(stream)
+        BlockNorm(y, residual, out, x, pre_weight=pre_weight, **kw)(stream)
+    return _returned(stream, out, x)
 
 
 def chunk_spec(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse=None, *, scale,
@@ -512,17 +526,19 @@ def mla_chunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, *, scale, m
             out = torch.empty((t, h, w_uv.shape[1]), dtype=out_dtype, device=q.device)
         if lse is None:
             lse = torch.empty((t, h), dtype=torch.float32, device=q.device)
-        return MlaChunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse, scale=scale,
-                        max_keys=max_keys, kv_format=kv_format)(stream)
+        MlaChunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse, scale=scale,
+                 max_keys=max_keys, kv_format=kv_format)(stream)
+    return _returned(stream, out, lse)
 
 
 def combine_parts(part_out, part_lse, out=None, lse=None, stream=None):
     """Merge ``G`` partial results (``part_out f32 [G,T,H,512]``, ``part_lse f32 [G,T,H]``)."""
     g, t, h, _ = part_out.shape
-    if out is None:
-        out = torch.empty((t, h, 512), dtype=torch.bfloat16, device=part_out.device)
-    if lse is None:
-        lse = torch.empty((t, h), dtype=torch.float32, device=part_out.device)
+    with _allocating_on(stream):
+        if out is None:
+            out = torch.empty((t, h, 512), dtype=torch.bfloat16, device=part_out.device)
+        if lse is None:
+            lse = torch.empty((t, h), dtype=torch.float32, device=part_out.device)
     p = _abi.TqCombineParams()
     p.parts, p.tokens, p.heads = g, t, h
     p.part_out, p.part_lse = part_out.data_ptr(), part_lse.data_ptr()
@@ -531,7 +547,7 @@ def combine_parts(part_out, part_lse, out=None, lse=None, stream=None):
     p.out_stride_head = out.stride(1) * out.element_size()
     p.out_dtype = _TORCH_DTYPE[out.dtype]
     raise_for(lib.tq_mla_combine(ctypes.byref(p), _stream_handle(stream)))
-    return out, lse
+    return _returned(stream, out, lse)
 
 
 def default_scale(width):
