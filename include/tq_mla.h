@@ -441,6 +441,8 @@ int32_t tq_block_norm(const TqBlockNormSpec* spec, void* stream, TqContractError
  * the pool: its rows read as zeros), TQ_DEV_TABLE_SHORT (kv_len past 64 L, cut),
  * TQ_DEV_SEQ_RANGE (q_start not ascending within [0, T]: nothing is computed),
  * TQ_DEV_WORK_OVERFLOW (more rows than max_keys: nothing is computed), TQ_DEV_WAIT_TIMEOUT.
+ * A call without tokens or sequences launches nothing and clears the flags of its workspace, which
+ * may then be null.
  * The workspace is 256-byte aligned; calls that share one must be ordered on one stream. It holds
  * the cached rows as bf16 (1.2 KB for each of max_keys) and their expanded keys and values, of as
  * many heads at a time as fit 8 GiB (for one head 512 or 1024 bytes a row). The launches depend

@@ -1558,7 +1558,14 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
   if (st != TQ_OK) return st;
   const TqMlaChunkSpec& s = *spec;
   const uint64_t T = s.q.shape[0], S = s.page_table.shape[0];
-  if (T == 0 || S == 0) return fail(nullptr, TQ_OK);
+  if (T == 0 || S == 0) {
+    // Nothing to launch; what the workspace holds is not this call's error word.
+    if (workspace && workspace_bytes >= sizeof(int) &&
+        cudaMemsetAsync(workspace, 0, sizeof(int), static_cast<cudaStream_t>(stream)) !=
+            cudaSuccess)
+      return fail("workspace", TQ_ERR_CUDA);
+    return fail(nullptr, TQ_OK);
+  }
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return fail("device", TQ_ERR_CUDA);
   const int pairs = pairs_on(device);
