@@ -520,16 +520,26 @@ class MlaChunk(_Launch):
 
 
 def mla_chunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, *, scale, max_keys, out=None,
-              lse=None, out_dtype=torch.bfloat16, kv_format=None, stream=None):
-    """One chunk attention call (see ``MlaChunk``); returns ``(out, lse)``."""
+              lse=None, out_dtype=torch.bfloat16, kv_format=None, flags=None, stream=None):
+    """One chunk attention call (see ``MlaChunk``); returns ``(out, lse)``.
+
+    ``flags`` is an optional device ``int32`` tensor that collects the call's error flags
+    (``TQ_DEV_*``): with more cached rows than ``max_keys``, or ``q_start`` out of order, nothing is
+    computed. Rows that are not computed hold NaN where the call allocates ``out`` and ``lse``, and
+    keep their values where the caller gives them.
+    """
     t, h = q.shape[0], q.shape[1]
     with _allocating_on(stream):
         if out is None:
-            out = torch.empty((t, h, w_uv.shape[1]), dtype=out_dtype, device=q.device)
+            out = torch.full((t, h, w_uv.shape[1]), math.nan, dtype=out_dtype, device=q.device)
         if lse is None:
-            lse = torch.empty((t, h), dtype=torch.float32, device=q.device)
-        MlaChunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse, scale=scale,
-                 max_keys=max_keys, kv_format=kv_format)(stream)
+            lse = torch.full((t, h), math.nan, dtype=torch.float32, device=q.device)
+        launch = MlaChunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse, scale=scale,
+                          max_keys=max_keys, kv_format=kv_format)
+        launch(stream)
+        if flags is not None:
+            # The error word is the workspace's first.
+            flags.view(-1)[:1].bitwise_or_(launch.workspace[:4].view(torch.int32))
     return _returned(stream, out, lse)
 
 
