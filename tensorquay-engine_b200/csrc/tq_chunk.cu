@@ -51,8 +51,6 @@ enum Header : int {
   kHdrBlocks = 2,  // query blocks
   kHdrPieces = 3,  // pieces of all blocks: units of one head
   kHdrSplit = 4,   // 1 if some block has more than one piece
-  kHdrWhere = 5,   // first wait that ran out: shared address of its barrier
-  kHdrWho = 6,     // its block, and the kernel's block size << 16
   kHdrNext = 8,    // [128] next unit of each pass over the heads
   kHdrWords = 136
 };
@@ -63,7 +61,6 @@ struct Block {
   int key0, tiles;      // first compact row, row tiles seen
   int seq;
   int piece0, pieces;   // its pieces
-  int unused;
 };
 
 // Row tiles tile0 .. tile0 + tiles - 1 of a block.
@@ -101,9 +98,7 @@ struct Args {
   const int* kv_len;
   uint8_t* out;
   float* lse;  // may be null
-  long long q_st, q_sh, out_st, out_sh;           // bytes
-  long long uk_sh, uk_sr, uv_sh, uv_sr;           // elements
-  long long row_stride;
+  long long out_st, out_sh, row_stride;           // bytes
   int tokens, heads, seqs, slots, pages, cap, max_blocks;
   int head0, pass_heads, pass;
   int split_units;  // most units of a pass after splitting; 0: blocks are not split
@@ -336,7 +331,7 @@ __device__ void plan_pieces(const Args& a, PlanShared& sh) {
       const int s = last_at_or_below(seq_block, a.seqs, b);
       const int row0 = q_start[s] + (b - seq_block[s]) * kQueryTile;
       const int rows = min(kQueryTile, q_start[s + 1] - row0), key0 = seq_key0[s];
-      w.blocks[b] = {row0, rows, key0, tiles, s, at, n, 0};
+      w.blocks[b] = {row0, rows, key0, tiles, s, at, n};
       // Pieces of one length, the last ones shorter.
       const int each = max(1, (tiles + n - 1) / n);
 #pragma unroll 1
@@ -501,13 +496,8 @@ struct Waiter {
   // The end of an aborted CTA: the error flag, and a millisecond in which the pair's copies and
   // MMAs in flight land.
   __device__ void settle(int* header) {
-    const uint32_t bar = ptx::ld_shared_u32(abort);
-    if (!bar) return;
-    if (threadIdx.x == 0) {
-      atomicOr(header + kHdrError, TQ_DEV_WAIT_TIMEOUT);
-      if (atomicCAS(header + kHdrWhere, 0, int(bar)) == 0)
-        header[kHdrWho] = int(blockIdx.x | (blockDim.x << 16));
-    }
+    if (!ptx::ld_shared_u32(abort)) return;
+    if (threadIdx.x == 0) atomicOr(header + kHdrError, TQ_DEV_WAIT_TIMEOUT);
     const uint64_t t0 = ptx::global_timer_ns();
     for (uint32_t i = 0; i < (1u << 20) && ptx::global_timer_ns() - t0 < 1000000ull; ++i) {
     }
@@ -1600,14 +1590,8 @@ extern "C" int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace,
   a.kv_len = ints(s.kv_len);
   a.out = reinterpret_cast<uint8_t*>(s.out.device_address);
   a.lse = s.lse.rank ? reinterpret_cast<float*>(s.lse.device_address) : nullptr;
-  a.q_st = (long long)s.q.strides_bytes[0];
-  a.q_sh = (long long)s.q.strides_bytes[1];
   a.out_st = (long long)s.out.strides_bytes[0];
   a.out_sh = (long long)s.out.strides_bytes[1];
-  a.uk_sh = (long long)(s.w_uk.strides_bytes[0] / 2);
-  a.uk_sr = (long long)(s.w_uk.strides_bytes[1] / 2);
-  a.uv_sh = (long long)(s.w_uv.strides_bytes[0] / 2);
-  a.uv_sr = (long long)(s.w_uv.strides_bytes[1] / 2);
   a.row_stride = (long long)s.kv.strides_bytes[1];
   a.tokens = int(T);
   a.heads = int(s.q.shape[1]);

@@ -433,12 +433,13 @@ extern "C" int32_t tq_step_plan(const TqStepPlanSpec* spec, int32_t* device_flag
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   if (a.requests <= kNear && a.tokens < kNearCount && a.columns < kNearCount) {
     // A quarter of the threads where that many hold the requests: fewer to start and to wait for.
-    // (The larger form's shared memory passes the 48 KB of a plain launch.)
+    // (The larger form's shared memory passes the 48 KB of a plain launch; its 1024 threads of 56
+    // registers are one CTA an SM, and at kNearCount token rows it has 128 of them.)
     cudaError_t e;
     if (a.requests <= kNear / 4) {
       e = launch_near<kThreads / 4>(a, cs);
     } else {
-      static_assert(sizeof(NearShared<kNear>) <= 50 * 1024, "two CTAs an SM");
+      static_assert(sizeof(NearShared<kNear>) <= 232448, "shared memory per CTA");
       e = cudaFuncSetAttribute(near_kernel<kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                int(sizeof(NearShared<kNear>)));
       if (e == cudaSuccess) e = launch_near<kThreads>(a, cs);
