@@ -444,9 +444,11 @@ int32_t tq_block_norm(const TqBlockNormSpec* spec, void* stream, TqContractError
  * A call without tokens or sequences launches nothing and clears the flags of its workspace, which
  * may then be null.
  * The workspace is 256-byte aligned; calls that share one must be ordered on one stream. It holds
- * the cached rows as bf16 (1.2 KB for each of max_keys) and their expanded keys and values, of as
- * many heads at a time as fit 8 GiB (for one head 512 or 1024 bytes a row). The launches depend
- * only on the spec, so a captured call replays for new contents. */
+ * the cached rows as bf16 (1.2 KB for each of max_keys), their expanded keys and values, of as many
+ * heads at a time as fit 8 GiB (for one head 512 or 1024 bytes a row), and, where ceil(T / 256)
+ * times the heads at a time is at most 320 so that work may be split along the keys, 320 partial
+ * outputs of 256 rows (42 MB at Dv = 128, 84 MB at 256, whatever T is). The launches depend only on
+ * the spec, so a captured call replays for new contents. */
 typedef struct {
   TqTensorSpec q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, out, lse;
   int32_t kv_format;

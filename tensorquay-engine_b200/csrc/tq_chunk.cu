@@ -512,9 +512,11 @@ struct Waiter {
 // 512 B written a row. The weights of a column block (256 x 512, half of them in each CTA of the
 // pair) therefore stay in shared memory while the pair walks over row tiles; only the rows
 // stream (16 KB boxes through a ring), half as many bytes per FLOP as with both operands streamed.
-// Two TMEM accumulators: the epilogue of one item runs under the MMAs of the next. Products past
-// bf16's range become its largest value: an infinite value would reach the tile's other query rows
-// as 0 * infinity.
+// Two TMEM accumulators: the epilogue of one item runs under the MMAs of the next. Sums past bf16's
+// range become its largest value: an infinite value would reach the tile's other query rows as
+// 0 * infinity. NaN does not arise from finite operands: a single product does not overflow inside
+// the tensor core and an infinite partial sum stays infinite (rows of 3e38 against weights of both
+// signs and magnitudes up to 3e38).
 namespace expand {
 
 constexpr int kThreads = 256;  // warp 0 loads, warp 1 MMA, warps 4-7 epilogue

@@ -17,7 +17,10 @@
 // Beyond kNear, clusters of C CTAs split the requests: each CTA sums its share, the CTAs exchange
 // their totals through distributed shared memory, scan their share with that base, and after a
 // cluster barrier fill the tokens. With more than one cluster, every cluster does the whole scan
-// (they write the same values) and the clusters split only the tokens.
+// (they write the same values) and the clusters split only the tokens. Back to back 16 us a call for
+// 9001 requests with 13469 tokens, 25 for 4097 with 202793 (one request less, and the other form
+// takes 8.3), 39 for 65536 with 163416, 15.5 for 300 over 2^19 token rows: three dependent passes
+// over the requests, a bisection in global memory for each token, and no programmatic launch.
 
 #include <cuda_runtime.h>
 
