@@ -147,6 +147,15 @@ def _returned(stream, *results):
     return results
 
 
+def _flags_pointer(flags, device):
+    """The address of a call's error flags: a kernel writes there, so it is checked like the tensors."""
+    if flags is None:
+        return None
+    if flags.device != device or flags.dtype != torch.int32 or not flags.numel():
+        raise ValueError(f"flags have to be int32 on {device}")
+    return flags.data_ptr()
+
+
 class MlaLaunch:
     """A validated dense paged MLA launch bound to its tensors and a workspace.
 
@@ -259,7 +268,7 @@ def kv_write(src, kv, page_table, seq_id, pos, *, kv_format=None, flags=None, st
     s = kv_write_spec(src, kv, page_table, seq_id, pos, kv_format=kv_format,
                       norm_weight=norm_weight, norm_eps=norm_eps)
     err = _abi.TqContractError()
-    fp = ctypes.c_void_p(flags.data_ptr()) if flags is not None else None
+    fp = _flags_pointer(flags, kv.device)
     raise_for(lib.tq_kv_write(ctypes.byref(s), fp, _stream_handle(stream), ctypes.byref(err)), err)
     return kv
 
@@ -307,7 +316,7 @@ class MlaPrologue:
 
     def __call__(self, flags=None, stream=None):
         err = _abi.TqContractError()
-        fp = ctypes.c_void_p(flags.data_ptr()) if flags is not None else None
+        fp = _flags_pointer(flags, self.q.device)
         raise_for(lib.tq_mla_prologue(ctypes.byref(self.spec),
                                       ctypes.c_void_p(self.workspace.data_ptr()),
                                       self.workspace.numel(), fp, _stream_handle(stream),
@@ -359,10 +368,6 @@ class _Launch:
             raise_for(status, self._err)
 
 
-def _flags_pointer(flags):
-    return flags.data_ptr() if flags is not None else None
-
-
 #: What ``StepPlan`` fills: the step's metadata as the other operators take it.
 StepTables = collections.namedtuple(
     "StepTables", "q_start kv_len seq_id q_pos slot page_table free_left")
@@ -404,7 +409,7 @@ class StepPlan(_Launch):
         self._check(lib.tq_step_plan_validate)
 
     def __call__(self, flags=None, stream=None):
-        self._run(lib.tq_step_plan, (_flags_pointer(flags),), stream)
+        self._run(lib.tq_step_plan, (_flags_pointer(flags, self.device),), stream)
         return self.tables
 
 
@@ -529,6 +534,7 @@ def mla_chunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, *, scale, m
     keep their values where the caller gives them.
     """
     t, h = q.shape[0], q.shape[1]
+    _flags_pointer(flags, q.device)
     with _allocating_on(stream):
         if out is None:
             out = torch.full((t, h, w_uv.shape[1]), math.nan, dtype=out_dtype, device=q.device)
