@@ -555,6 +555,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::tma_prefetch_desc(&tm_uk);
     ptx::tma_prefetch_desc(&tm_uv);
   }
+  // The allocation is one operation of both CTAs: neither may ask for it before the other runs.
+  ptx::cluster_sync_relaxed();
   if (warp == 1) {
     ptx::tmem_alloc_pair(ptx::smem_addr(tmem_holder), 512);
     ptx::tmem_relinquish_pair();
@@ -699,7 +701,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc_pair(tmem, 512);
+    __syncwarp();
   }
+  ptx::cluster_sync_relaxed();  // both CTAs run until both have given their columns back
 }
 
 }  // namespace expand
@@ -878,6 +882,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::tma_prefetch_desc(&tm_v);
     if (kRope) ptx::tma_prefetch_desc(&tm_rope);
   }
+  // The allocation is one operation of both CTAs: neither may ask for it before the other runs.
+  ptx::cluster_sync_relaxed();
   if (warp == 1) {
     ptx::tmem_alloc_pair(ptx::smem_addr(tmem_holder), 512);
     ptx::tmem_relinquish_pair();
@@ -1360,7 +1366,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc_pair(tmem, 512);
+    __syncwarp();
   }
+  ptx::cluster_sync_relaxed();  // both CTAs run until both have given their columns back
 }
 
 }  // namespace attend

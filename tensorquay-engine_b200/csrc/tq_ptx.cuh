@@ -340,6 +340,9 @@ __device__ __forceinline__ void tmem_wait_st() {
 // One thread of the pair's leader (cluster rank 0) issues an MMA of M = 256: each CTA holds its
 // own 128 rows of A and D, and half of B's N rows, at the same offsets in both CTAs.
 
+// Both CTAs issue it, and only once both are known to run (a cluster barrier before it): issued
+// while the peer had not started, it did not return, once in some 40000 calls that ran beside
+// other streams' kernels.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t holder_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
                :: "r"(holder_smem), "r"(ncols) : "memory");
