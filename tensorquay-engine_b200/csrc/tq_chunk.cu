@@ -8,7 +8,9 @@
 //                     (every sequence padded to kRowTile rows) and its query blocks of kQueryTile
 //                     tokens.
 //   2. gather_kernel  the cached rows through the page table into that space, as bf16 (FP8 rows
-//                     dequantized, rounded once): zeros past kv_len and for a row that is not
+//                     dequantized and rounded once, as this library's other attention takes them:
+//                     a scale belongs to 128 values of a row, so it does not come out of the
+//                     expansion's sum over all 512): zeros past kv_len and for a row that is not
 //                     finite, so that neither stale rows nor such a row can reach an output that
 //                     does not see it through 0 * NaN. The first such row of a sequence is kept:
 //                     the outputs of the tokens that see it become NaN at the end. One block of
@@ -38,6 +40,9 @@ constexpr int kLatent = 512;
 constexpr int kRopeDim = 64;
 constexpr int kRowTile = 128;    // keys per attention step; sequences are padded to it
 constexpr int kQueryTile = 256;  // query tokens of one attention unit
+// Keys and values of one pass over the heads. It bounds the workspace on a GPU that also holds the
+// cache and keeps the serving sizes in one pass; smaller passes, whose keys and values would stay in
+// L2, are not measured.
 constexpr uint64_t kScratchBytes = 8ull << 30;
 // Splitting: at most this many units once split, about four per CTA pair (their partial outputs are
 // kept in the workspace), and what a piece costs beside its tiles (query load, pipeline fill,
@@ -512,7 +517,9 @@ struct Waiter {
 // 512 B written a row. The weights of a column block (256 x 512, half of them in each CTA of the
 // pair) therefore stay in shared memory while the pair walks over row tiles; only the rows
 // stream (16 KB boxes through a ring), half as many bytes per FLOP as with both operands streamed.
-// Two TMEM accumulators: the epilogue of one item runs under the MMAs of the next. Sums past bf16's
+// Two TMEM accumulators: the epilogue of one item runs under the MMAs of the next. The f32 sums are
+// rounded to bf16, the type of the attention's operands and of a model's own keys and values (each
+// such rounding adds 0.0017 in the relative 2-norm, as much as the output's own). Sums past bf16's
 // range become its largest value: an infinite value would reach the tile's other query rows as
 // 0 * infinity. NaN does not arise from finite operands: a single product does not overflow inside
 // the tensor core and an infinite partial sum stays infinite (rows of 3e38 against weights of both
@@ -1148,7 +1155,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 4; ++k)
             top[k] = fmaxf(fmaxf(top[k], __uint_as_float(r[i + k])), __uint_as_float(r[i + 4 + k]));
       };
-      // 32 softmax weights, against mc = -c * reference, to TMEM as 16 columns of bf16 pairs.
+      // 32 softmax weights, against mc = -c * reference, to TMEM as 16 columns of bf16 pairs (PV's
+      // operands have one type, V's); their sum takes them unrounded.
       auto weigh = [&](const uint32_t (&r)[32], float mc, uint32_t dst) {
         uint32_t p[16];
 #pragma unroll
