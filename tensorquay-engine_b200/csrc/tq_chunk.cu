@@ -563,6 +563,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::tma_prefetch_desc(&tm_uv);
   }
   // The allocation is one operation of both CTAs: neither may ask for it before the other runs.
+  __syncwarp();
   ptx::cluster_sync_relaxed();
   if (warp == 1) {
     ptx::tmem_alloc_pair(ptx::smem_addr(tmem_holder), 512);
@@ -703,6 +704,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // it; the others go on to the cluster barrier, which costs no issue slots.
   if (warp == 0) wt.on(bar(kBarDrain), 0);
   wt.settle(a.w.header);
+  __syncwarp();
   ptx::tc_fence_before();
   ptx::cluster_sync();
   if (warp == 1) {
@@ -890,6 +892,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (kRope) ptx::tma_prefetch_desc(&tm_rope);
   }
   // The allocation is one operation of both CTAs: neither may ask for it before the other runs.
+  __syncwarp();
   ptx::cluster_sync_relaxed();
   if (warp == 1) {
     ptx::tmem_alloc_pair(ptx::smem_addr(tmem_holder), 512);
@@ -1369,6 +1372,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
   if (warp == 0) wt.on(bar(C::kDrain), 0);
   wt.settle(a.w.header);
+  __syncwarp();
   ptx::tc_fence_before();
   ptx::cluster_sync();
   if (warp == 1) {
