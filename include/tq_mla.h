@@ -460,6 +460,93 @@ int32_t tq_mla_chunk_workspace_bytes(const TqMlaChunkSpec* spec, int32_t device,
 int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace, uint64_t workspace_bytes,
                      void* stream, TqContractError* err);
 
+/* Index branch of a sparse step: what finds the rows that tq_mla_sparse_validate's plans attend to.
+ * Three calls, then tq_mla_decode:
+ *   tq_index_write    index queries and keys rotated, quantized, the keys written to their cache
+ *   tq_index_scores   a cheap score of every cached row for every query token
+ *   tq_index_select   each token's best rows (idx and k_len of a sparse plan), or its best pages (a
+ *                     page table and a length of its own for each token, for a dense plan)
+ * The reference's contract takes the selected indices as given (contracts.rs:196-200); it has no
+ * code that makes them.
+ *
+ * An index row is 128 E4M3 codes and one f32 scale: TQ_INDEX_ROW_BYTES of payload in rows of
+ * r >= 144 bytes, r a multiple of 16, paged like the attention's cache: u8 [P, 64, 132] with strides
+ * [64 r, r, 1]. The same page table may serve both caches. */
+#define TQ_INDEX_DIM 128
+#define TQ_INDEX_ROW_BYTES 132
+
+/* Index write. With R = 2 * (length of freq), for every token t:
+ *   q', k'  = the R values from rope_start on turned by the angles pos[t] * freq[i], the others as
+ *             they are: pair i is (2 i, 2 i + 1), or (i, i + R / 2) where rope_half is not 0; cosine
+ *             and sine are multiplied by rope_mscale. k is normalised first:
+ *             norm_weight alone: k / sqrt(mean(k^2) + eps) * norm_weight
+ *             and norm_bias:     (k - mean(k)) / sqrt(var(k) + eps) * norm_weight + norm_bias
+ *   row     = 128 codes and a scale of k'; q_out[t, h] = the codes of q'[t, h]
+ *   w_out[t, h] = w[t, h] * scale * (the scale of q'[t, h])
+ * A scale is amax / 448 and a code E4M3(x * (448 / amax)), as tq_kv_write quantizes a tile. All is
+ * f32 up to the code (angles f64, reduced before the sine and cosine). Frequencies are the caller's,
+ * so any scaling of positions for long contexts is theirs; rope_mscale goes with it.
+ *   q      bf16 [T, H, 128], w bf16 or f32 [T, H], q_out u8 [T, H, 128], w_out f32 [T, H]: all or
+ *          none (rank 0: only keys are written); H is 1 to 128
+ *   k      bf16 [T, 128]      norm_weight, norm_bias bf16 [128] or rank 0
+ *   freq   f32 [R / 2] or rank 0 (R = 0); R a multiple of 16, rope_start of 8, their sum <= 128
+ *   page_table i32 [S, L]     seq_id, pos i32 [T]     kv u8 [P, 64, 132]
+ * Outer strides of q and k may be padded (multiples of 16, addresses too); w, q_out and w_out are
+ * packed. Rows that have no place are skipped with the flags of tq_kv_write; their q_out and w_out
+ * are still made. One launch; the grid depends only on the shapes. */
+typedef struct {
+  TqTensorSpec q, k, w, page_table, seq_id, pos, kv, q_out, w_out, norm_weight, norm_bias, freq;
+  int32_t rope_start, rope_half;
+  float rope_mscale, norm_eps, scale;
+} TqIndexWriteSpec;
+int32_t tq_index_write_validate(const TqIndexWriteSpec* spec, TqContractError* err);
+int32_t tq_index_write(const TqIndexWriteSpec* spec, int32_t* device_flags, void* stream,
+                       TqContractError* err);
+
+/* Index scores. With sees(t) = min(kv_len[seq_id[t]], q_pos[t] + 1), for n < sees(t):
+ *   scores[t, n] = key_scale[n] * sum_h w[t, h] * max(0, q[t, h] . k[n])
+ * over the codes, in f32. Columns from sees(t) on keep their values.
+ *   q      u8 [T, H, 128] E4M3 codes and w f32 [T, H], as tq_index_write makes them; H is a
+ *          multiple of 8 up to 128
+ *   kv     u8 [P, 64, 132]    page_table i32 [S, L]    seq_id, q_pos i32 [T]    kv_len i32 [S]
+ *   scores f32 [T, N], outer stride may be padded
+ * A code or scale that is NaN makes the scores that use it NaN and no others. In `device_flags`:
+ * TQ_DEV_SEQ_RANGE (the token's row is left as it was), TQ_DEV_TABLE_SHORT (sees(t) past 64 L, cut),
+ * TQ_DEV_WORK_OVERFLOW (sees(t) past N, cut), TQ_DEV_PAGE_RANGE (a page outside the pool: its rows
+ * read as zeros), TQ_DEV_WAIT_TIMEOUT. Consecutive tokens of one sequence share its rows' loads.
+ * One launch; the grid depends only on the device. */
+typedef struct {
+  TqTensorSpec q, w, kv, page_table, seq_id, q_pos, kv_len, scores;
+} TqIndexScoresSpec;
+int32_t tq_index_scores_validate(const TqIndexScoresSpec* spec, TqContractError* err);
+int32_t tq_index_scores(const TqIndexScoresSpec* spec, int32_t* device_flags, void* stream,
+                        TqContractError* err);
+
+/* Index select, over the first sees(t) = min(kv_len[seq_id[t]], q_pos[t] + 1, N) scores of a row.
+ * Row form (page_table of rank 0): idx[t] holds the positions of the K largest scores in ascending
+ * order, then -1; len[t] is their number. They are the idx and k_len of tq_mla_sparse_validate.
+ * Page form: a page's score is the largest of its (up to 64) visible scores; idx[t] holds the entries
+ * page_table[seq_id[t]][j] of the K best pages j in ascending order of j, then -1, and len[t] the
+ * rows that they hold: 64 each, fewer in the page that sees(t) ends in. They are the page table and
+ * kv_len of a tq_mla_validate plan with one sequence per token, seq_id[t] = t and the q_pos of this
+ * call, for rows of any format.
+ * The first keep_first and the last keep_last of the positions (pages) that a token sees are always
+ * selected. Equal scores go to the lowest position. A score of -inf (masked) or NaN is not selected
+ * (where it is not kept), so a row may end with fewer than K, or none.
+ *   scores f32 [T, N], N < 2^24, outer stride may be padded      seq_id, q_pos i32 [T]
+ *   kv_len i32 [S]    idx i32 [T, K], packed, K is 1 to TQ_MLA_MAX_TOPK    len i32 [T]
+ *   keep_first, keep_last >= 0, their sum <= K
+ * A token without a sequence (seq_id outside [0, S)) selects nothing and sets TQ_DEV_SEQ_RANGE.
+ * TQ_DEV_WORK_OVERFLOW: kv_len and q_pos see more than N columns; TQ_DEV_TABLE_SHORT (page form): more
+ * than 64 L rows, cut. One launch; the grid depends only on the shapes and the device. */
+typedef struct {
+  TqTensorSpec scores, seq_id, q_pos, kv_len, page_table, idx, len;
+  int32_t keep_first, keep_last;
+} TqIndexSelectSpec;
+int32_t tq_index_select_validate(const TqIndexSelectSpec* spec, TqContractError* err);
+int32_t tq_index_select(const TqIndexSelectSpec* spec, int32_t* device_flags, void* stream,
+                        TqContractError* err);
+
 /* Measurement hook, no reference counterpart. Makes later tq_mla_decode / tq_mla_prefill calls
  * on the calling thread record `begin_event` right before and `end_event` right after the
  * attention kernel, on the launch stream (both are cudaEvent_t created by the caller). Pass two

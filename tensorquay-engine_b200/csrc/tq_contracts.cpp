@@ -576,7 +576,180 @@ int32_t chunk_validate_impl(const TqMlaChunkSpec* spec, TqContractError* err) {
   return TQ_OK;
 }
 
+// Index branch. An index pool is declared like the attention's, with rows of TQ_INDEX_ROW_BYTES.
+int32_t index_write_validate_impl(const TqIndexWriteSpec* spec, TqContractError* err) {
+  Failure f{nullptr, TQ_OK};
+  auto fail = [&](const char* field, int32_t kind) {
+    if (err) { err->field = field; err->kind = kind; }
+    return kind;
+  };
+  if (!spec) return fail("spec", TQ_ERR_INVALID_ARGUMENT);
+  const TqIndexWriteSpec& s = *spec;
+  if (s.k.rank != 2) return fail("k", TQ_SHAPE);
+  if (s.page_table.rank != 2) return fail("page_table", TQ_SHAPE);
+  const uint64_t T = s.k.shape[0], D = TQ_INDEX_DIM;
+  if (T > (1u << 24)) return fail("k", TQ_SHAPE);
+  const bool queries = s.q.rank != 0, launching = T != 0;
+  if ((s.w.rank != 0) != queries) return fail("w", TQ_SHAPE);
+  if ((s.q_out.rank != 0) != queries) return fail("q_out", TQ_SHAPE);
+  if ((s.w_out.rank != 0) != queries) return fail("w_out", TQ_SHAPE);
+  if (queries && s.q.rank != 3) return fail("q", TQ_SHAPE);
+  const uint64_t H = queries ? s.q.shape[1] : 0;
+  if (queries && (H < 1 || H > 128)) return fail("q", TQ_SHAPE);
+  if (!check_kv_strides(s.kv, TQ_INDEX_ROW_BYTES, &f)) return fail(f.field, f.kind);
+  const uint64_t q[3] = {T, H, D}, k[2] = {T, D}, w[2] = {T, H}, tok[1] = {T}, dim[1] = {D};
+  const uint64_t table[2] = {s.page_table.shape[0], s.page_table.shape[1]};
+  const uint64_t pool[3] = {s.kv.shape[0], kPageRows, TQ_INDEX_ROW_BYTES};
+  const int32_t bf = TQ_DTYPE_BF16, i32 = TQ_DTYPE_I32;
+  const Layout padded = Layout::PaddedOuter, packed = Layout::Packed;
+  Extent in[9], out[3];
+  for (Extent& e : in) e.present = false;
+  for (Extent& e : out) e.present = false;
+  const int32_t w_type = s.w.dtype == TQ_DTYPE_F32 ? TQ_DTYPE_F32 : TQ_DTYPE_BF16;
+  if (queries &&
+      (!check("q", s.q, q, 3, bf, padded, launching, &in[0], &f) ||
+       !check("w", s.w, w, 2, w_type, packed, launching, &in[1], &f)))
+    return fail(f.field, f.kind);
+  if (!check("k", s.k, k, 2, bf, padded, launching, &in[2], &f) ||
+      !check("page_table", s.page_table, table, 2, i32, packed, launching, &in[3], &f) ||
+      !check("seq_id", s.seq_id, tok, 1, i32, packed, launching, &in[4], &f) ||
+      !check("pos", s.pos, tok, 1, i32, packed, launching, &in[5], &f) ||
+      !check("kv", s.kv, pool, 3, TQ_DTYPE_U8, Layout::Checked, launching, &out[0], &f))
+    return fail(f.field, f.kind);
+  if (queries &&
+      (!check("q_out", s.q_out, q, 3, TQ_DTYPE_U8, packed, launching, &out[1], &f) ||
+       !check("w_out", s.w_out, w, 2, TQ_DTYPE_F32, packed, launching, &out[2], &f)))
+    return fail(f.field, f.kind);
+  if (s.norm_bias.rank != 0 && s.norm_weight.rank == 0) return fail("norm_weight", TQ_SHAPE);
+  if (s.norm_weight.rank != 0) {
+    if (!check("norm_weight", s.norm_weight, dim, 1, bf, packed, launching, &in[6], &f))
+      return fail(f.field, f.kind);
+    if (s.norm_bias.rank != 0 &&
+        !check("norm_bias", s.norm_bias, dim, 1, bf, packed, launching, &in[7], &f))
+      return fail(f.field, f.kind);
+    if (!(std::isfinite(s.norm_eps) && s.norm_eps > 0.f)) return fail("norm_eps", TQ_SCALE);
+  }
+  if (s.freq.rank != 0) {
+    const uint64_t half[1] = {s.freq.shape[0]};
+    if (s.freq.rank != 1 || half[0] == 0 || half[0] % 8 || half[0] > D / 2)
+      return fail("freq", TQ_SHAPE);
+    if (!check("freq", s.freq, half, 1, TQ_DTYPE_F32, packed, launching, &in[8], &f))
+      return fail(f.field, f.kind);
+    if (s.rope_start < 0 || s.rope_start % 8 || uint64_t(s.rope_start) + 2 * half[0] > D)
+      return fail("rope_start", TQ_SHAPE);
+    if (!std::isfinite(s.rope_mscale)) return fail("rope_mscale", TQ_SCALE);
+  }
+  if (queries && !std::isfinite(s.scale)) return fail("scale", TQ_SCALE);
+  if (launching) {
+    const TqTensorSpec* all[5] = {&s.q, &s.k, &s.q_out, &s.norm_weight, &s.norm_bias};
+    const char* names[5] = {"q", "k", "q_out", "norm_weight", "norm_bias"};
+    for (int i = 0; i < 5; ++i) {
+      if (all[i]->rank == 0) continue;
+      if (all[i]->device_address % 16) return fail(names[i], TQ_ALIGNMENT);
+      for (int a = 0; a + 1 < all[i]->rank; ++a)
+        if (all[i]->strides_bytes[a] % 16) return fail(names[i], TQ_STRIDE);
+    }
+  }
+  if (!check_aliases(in, 9, out, 3, &f)) return fail(f.field, f.kind);
+  if (err) { err->field = nullptr; err->kind = TQ_OK; }
+  return TQ_OK;
+}
+
+int32_t index_scores_validate_impl(const TqIndexScoresSpec* spec, TqContractError* err) {
+  Failure f{nullptr, TQ_OK};
+  auto fail = [&](const char* field, int32_t kind) {
+    if (err) { err->field = field; err->kind = kind; }
+    return kind;
+  };
+  if (!spec) return fail("spec", TQ_ERR_INVALID_ARGUMENT);
+  const TqIndexScoresSpec& s = *spec;
+  if (s.q.rank != 3) return fail("q", TQ_SHAPE);
+  if (s.page_table.rank != 2) return fail("page_table", TQ_SHAPE);
+  if (s.scores.rank != 2) return fail("scores", TQ_SHAPE);
+  const uint64_t T = s.q.shape[0], H = s.q.shape[1], N = s.scores.shape[1];
+  const uint64_t S = s.page_table.shape[0], L = s.page_table.shape[1];
+  // T H rows of codes are addressed by one 31-bit coordinate.
+  if (H < 8 || H > 128 || H % 8 || T > (1u << 24)) return fail("q", TQ_SHAPE);
+  const bool launching = T != 0;
+  if (!check_kv_strides(s.kv, TQ_INDEX_ROW_BYTES, &f)) return fail(f.field, f.kind);
+  if (s.kv.shape[0] >= kDimensionLimit / kPageRows) return fail("kv", TQ_DIMENSION);
+  if (T * H >= kDimensionLimit) return fail("q", TQ_DIMENSION);
+  const uint64_t q[3] = {T, H, TQ_INDEX_DIM}, w[2] = {T, H}, tok[1] = {T}, seqs[1] = {S};
+  const uint64_t pool[3] = {s.kv.shape[0], kPageRows, TQ_INDEX_ROW_BYTES}, table[2] = {S, L};
+  const uint64_t o[2] = {T, N};
+  const int32_t i32 = TQ_DTYPE_I32;
+  const Layout packed = Layout::Packed;
+  Extent in[7], out[1];
+  if (!check("q", s.q, q, 3, TQ_DTYPE_U8, packed, launching, &in[0], &f) ||
+      !check("w", s.w, w, 2, TQ_DTYPE_F32, packed, launching, &in[1], &f) ||
+      !check("kv", s.kv, pool, 3, TQ_DTYPE_U8, Layout::Checked, launching, &in[2], &f) ||
+      !check("page_table", s.page_table, table, 2, i32, packed, launching, &in[3], &f) ||
+      !check("seq_id", s.seq_id, tok, 1, i32, packed, launching, &in[4], &f) ||
+      !check("q_pos", s.q_pos, tok, 1, i32, packed, launching, &in[5], &f) ||
+      !check("kv_len", s.kv_len, seqs, 1, i32, packed, launching, &in[6], &f) ||
+      !check("scores", s.scores, o, 2, TQ_DTYPE_F32, Layout::PaddedOuter, launching, &out[0], &f))
+    return fail(f.field, f.kind);
+  if (launching && s.q.device_address % 16) return fail("q", TQ_ALIGNMENT);
+  if (launching && s.w.device_address % 16) return fail("w", TQ_ALIGNMENT);
+  if (!check_aliases(in, 7, out, 1, &f)) return fail(f.field, f.kind);
+  if (err) { err->field = nullptr; err->kind = TQ_OK; }
+  return TQ_OK;
+}
+
+int32_t index_select_validate_impl(const TqIndexSelectSpec* spec, TqContractError* err) {
+  Failure f{nullptr, TQ_OK};
+  auto fail = [&](const char* field, int32_t kind) {
+    if (err) { err->field = field; err->kind = kind; }
+    return kind;
+  };
+  if (!spec) return fail("spec", TQ_ERR_INVALID_ARGUMENT);
+  const TqIndexSelectSpec& s = *spec;
+  if (s.scores.rank != 2 || s.scores.shape[1] >= (1u << 24)) return fail("scores", TQ_SHAPE);
+  if (s.kv_len.rank != 1) return fail("kv_len", TQ_SHAPE);
+  if (s.idx.rank != 2) return fail("idx", TQ_SHAPE);
+  const uint64_t T = s.scores.shape[0], N = s.scores.shape[1], K = s.idx.shape[1];
+  if (T > (1u << 24)) return fail("scores", TQ_SHAPE);
+  if (K < 1 || K > TQ_MLA_MAX_TOPK) return fail("idx", TQ_SHAPE);
+  if (s.keep_first < 0 || uint64_t(s.keep_first) > K) return fail("keep_first", TQ_SHAPE);
+  if (s.keep_last < 0 || uint64_t(s.keep_last) + uint64_t(s.keep_first) > K)
+    return fail("keep_last", TQ_SHAPE);
+  const bool launching = T != 0, pages = s.page_table.rank != 0;
+  if (pages && s.page_table.rank != 2) return fail("page_table", TQ_SHAPE);
+  const uint64_t S = s.kv_len.shape[0];
+  const uint64_t scores[2] = {T, N}, tok[1] = {T}, seqs[1] = {S}, picks[2] = {T, K};
+  const uint64_t table[2] = {S, s.page_table.shape[1]};
+  const int32_t i32 = TQ_DTYPE_I32;
+  const Layout packed = Layout::Packed;
+  Extent in[5], out[2];
+  in[4].present = false;
+  if (!check("scores", s.scores, scores, 2, TQ_DTYPE_F32, Layout::PaddedOuter, launching, &in[0],
+             &f) ||
+      !check("seq_id", s.seq_id, tok, 1, i32, packed, launching, &in[1], &f) ||
+      !check("q_pos", s.q_pos, tok, 1, i32, packed, launching, &in[2], &f) ||
+      !check("kv_len", s.kv_len, seqs, 1, i32, packed, launching, &in[3], &f) ||
+      (pages &&
+       !check("page_table", s.page_table, table, 2, i32, packed, launching, &in[4], &f)) ||
+      !check("idx", s.idx, picks, 2, i32, packed, launching, &out[0], &f) ||
+      !check("len", s.len, tok, 1, i32, packed, launching, &out[1], &f))
+    return fail(f.field, f.kind);
+  if (!check_aliases(in, 5, out, 2, &f)) return fail(f.field, f.kind);
+  if (err) { err->field = nullptr; err->kind = TQ_OK; }
+  return TQ_OK;
+}
+
 }  // namespace
+
+int32_t index_write_validate(const TqIndexWriteSpec* spec, TqContractError* err) {
+  return index_write_validate_impl(spec, err);
+}
+
+int32_t index_scores_validate(const TqIndexScoresSpec* spec, TqContractError* err) {
+  return index_scores_validate_impl(spec, err);
+}
+
+int32_t index_select_validate(const TqIndexSelectSpec* spec, TqContractError* err) {
+  return index_select_validate_impl(spec, err);
+}
 
 int32_t chunk_validate(const TqMlaChunkSpec* spec, TqContractError* err) {
   return chunk_validate_impl(spec, err);
@@ -683,6 +856,18 @@ int32_t tq_block_norm_validate(const TqBlockNormSpec* spec, TqContractError* err
 
 int32_t tq_mla_chunk_validate(const TqMlaChunkSpec* spec, TqContractError* err) {
   return tq::chunk_validate(spec, err);
+}
+
+int32_t tq_index_write_validate(const TqIndexWriteSpec* spec, TqContractError* err) {
+  return tq::index_write_validate(spec, err);
+}
+
+int32_t tq_index_scores_validate(const TqIndexScoresSpec* spec, TqContractError* err) {
+  return tq::index_scores_validate(spec, err);
+}
+
+int32_t tq_index_select_validate(const TqIndexSelectSpec* spec, TqContractError* err) {
+  return tq::index_select_validate(spec, err);
 }
 
 int32_t tq_mla_should_launch(const TqMlaParams* params) {

@@ -24,6 +24,9 @@ int32_t prologue_validate(const TqPrologueSpec* spec, TqContractError* err);
 int32_t step_plan_validate(const TqStepPlanSpec* spec, TqContractError* err);
 int32_t block_norm_validate(const TqBlockNormSpec* spec, TqContractError* err);
 int32_t chunk_validate(const TqMlaChunkSpec* spec, TqContractError* err);
+int32_t index_write_validate(const TqIndexWriteSpec* spec, TqContractError* err);
+int32_t index_scores_validate(const TqIndexScoresSpec* spec, TqContractError* err);
+int32_t index_select_validate(const TqIndexSelectSpec* spec, TqContractError* err);
 void philox_block(const uint32_t counter[4], const uint32_t key[2], uint32_t out[4]);
 int32_t philox_words(uint64_t seed, uint64_t stream, uint64_t start, uint32_t* out,
                      uint64_t count);

@@ -123,6 +123,24 @@ class TqMlaChunkSpec(ctypes.Structure):
             ("max_keys", ctypes.c_uint64)]
 
 
+class TqIndexWriteSpec(ctypes.Structure):
+    _fields_ = [(name, TqTensorSpec) for name in (
+        "q", "k", "w", "page_table", "seq_id", "pos", "kv", "q_out", "w_out", "norm_weight",
+        "norm_bias", "freq")] + [(name, ctypes.c_int32) for name in ("rope_start", "rope_half")] + [
+            (name, ctypes.c_float) for name in ("rope_mscale", "norm_eps", "scale")]
+
+
+class TqIndexScoresSpec(ctypes.Structure):
+    _fields_ = [(name, TqTensorSpec) for name in (
+        "q", "w", "kv", "page_table", "seq_id", "q_pos", "kv_len", "scores")]
+
+
+class TqIndexSelectSpec(ctypes.Structure):
+    _fields_ = [(name, TqTensorSpec) for name in (
+        "scores", "seq_id", "q_pos", "kv_len", "page_table", "idx", "len")] + [
+            (name, ctypes.c_int32) for name in ("keep_first", "keep_last")]
+
+
 # Every exported symbol of include/tq_mla.h, with its ctypes prototype.
 _P = ctypes.POINTER
 _U64, _I32, _VP = ctypes.c_uint64, ctypes.c_int32, ctypes.c_void_p
@@ -167,6 +185,12 @@ PROTOTYPES = {
     "tq_mla_chunk_validate": (_I32, [_P(TqMlaChunkSpec), _P(TqContractError)]),
     "tq_mla_chunk_workspace_bytes": (_I32, [_P(TqMlaChunkSpec), _I32, _P(_U64)]),
     "tq_mla_chunk": (_I32, [_P(TqMlaChunkSpec), _VP, _U64, _VP, _P(TqContractError)]),
+    "tq_index_write_validate": (_I32, [_P(TqIndexWriteSpec), _P(TqContractError)]),
+    "tq_index_write": (_I32, [_P(TqIndexWriteSpec), _VP, _VP, _P(TqContractError)]),
+    "tq_index_scores_validate": (_I32, [_P(TqIndexScoresSpec), _P(TqContractError)]),
+    "tq_index_scores": (_I32, [_P(TqIndexScoresSpec), _VP, _VP, _P(TqContractError)]),
+    "tq_index_select_validate": (_I32, [_P(TqIndexSelectSpec), _P(TqContractError)]),
+    "tq_index_select": (_I32, [_P(TqIndexSelectSpec), _VP, _VP, _P(TqContractError)]),
     "tq_philox_block": (None, [_P(ctypes.c_uint32), _P(ctypes.c_uint32), _P(ctypes.c_uint32)]),
     "tq_philox_words": (_I32, [_U64, _U64, _U64, _P(ctypes.c_uint32), _U64]),
     "tq_philox_uniform_f32": (ctypes.c_float, [ctypes.c_uint32]),

@@ -10,7 +10,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG.parent / "csrc"
 SOURCES = ["tq_mla_kernels.cu", "tq_kv_write.cu", "tq_prologue.cu", "tq_proj.cu", "tq_peer_merge.cu",
            "tq_step.cu", "tq_block_norm.cu",
-           "tq_chunk.cu", "tq_contracts.cpp", "tq_comm.cpp"]
+           "tq_chunk.cu", "tq_index_write.cu", "tq_index_scores.cu", "tq_index_select.cu", "tq_contracts.cpp", "tq_comm.cpp"]
 HEADERS = ["tq_ptx.cuh", "tq_mla_layout.h", "tq_contracts.h"]
 TARGET = PKG / "libtq_mla.so"
 NVCC_FLAGS = [

@@ -549,6 +549,175 @@ def mla_chunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, *, scale, m
     return _returned(stream, out, lse)
 
 
+INDEX_ROW_BYTES = 132
+
+
+def index_pool_spec(kv):
+    """An index cache u8 ``[P, 64, r]`` (rows of 128 E4M3 codes and an f32 scale in ``r`` >= 144
+    bytes, a multiple of 16), declared as ``[P, 64, 132]``."""
+    return tensor_spec([kv.shape[0], kv.shape[1], INDEX_ROW_BYTES],
+                       [kv.stride(0) * kv.element_size(), kv.stride(1) * kv.element_size(), 1],
+                       _abi.DTYPE_U8, kv.data_ptr(), _capacity(kv))
+
+
+def rope_frequencies(width, base=10000.0, *, factor=1.0, original=None, beta_fast=32.0,
+                     beta_slow=1.0):
+    """Frequencies ``[width / 2]`` (f64) of a rotary part of ``width`` values, and the factor of its
+    cosines and sines. ``factor`` > 1 stretches positions for long contexts: all of them alike, or,
+    with ``original`` (the context length the model was trained at), only the slow frequencies.
+    One that turns more than ``beta_fast`` times in ``original`` positions stays, one that turns
+    less than ``beta_slow`` times is divided by ``factor``, those between are blended over their
+    place, and the factor is ``0.1 ln(factor) + 1``."""
+    if width <= 0 or width % 2 or not base > 1.0 or not factor >= 1.0:
+        raise ValueError("rope_frequencies needs an even width, a base above 1 and a factor of 1 or more")
+    at = torch.arange(0, width, 2, dtype=torch.float64)
+    freq = base ** (-at / width)
+    if original is None or factor == 1.0:
+        return freq / factor, 1.0
+    place = lambda turns: width * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+    low = max(math.floor(place(beta_fast)), 0)
+    high = min(math.ceil(place(beta_slow)), width - 1)
+    slow = ((at / 2 - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
+    return freq * (1.0 - slow) + freq / factor * slow, 0.1 * math.log(factor) + 1.0
+
+
+def index_write_spec(q, k, w, page_table, seq_id, pos, kv, q_out, w_out, *, scale=1.0,
+                     norm_weight=None, norm_bias=None, eps=1e-6, freq=None, rope_start=0,
+                     rope_half=False, rope_mscale=1.0):
+    """Declaration of an index write (``tq_index_write``); ``q``, ``w`` and their outputs may be None."""
+    s = _abi.TqIndexWriteSpec()
+    for name, t in (("q", q), ("k", k), ("w", w), ("page_table", page_table), ("seq_id", seq_id),
+                    ("pos", pos), ("q_out", q_out), ("w_out", w_out), ("norm_weight", norm_weight),
+                    ("norm_bias", norm_bias), ("freq", freq)):
+        if t is not None:
+            setattr(s, name, spec_of(t))
+    s.kv = index_pool_spec(kv)
+    s.rope_start, s.rope_half = int(rope_start), int(bool(rope_half))
+    s.rope_mscale, s.norm_eps, s.scale = float(rope_mscale), float(eps), float(scale)
+    return s
+
+
+class IndexWrite(_Launch):
+    """The index queries and keys of a step: rotated, quantized to E4M3, and the keys written to
+    position ``pos`` of sequence ``seq_id`` in the paged index cache ``kv`` (u8 ``[P, 64, r]``).
+
+    ``q`` bf16 ``[T, H, 128]``, ``k`` bf16 ``[T, 128]``, ``w`` bf16 or f32 ``[T, H]``. The call fills
+    ``q_out`` u8 ``[T, H, 128]`` (codes) and ``w_out`` f32 ``[T, H]``: ``w * scale`` times the scale of
+    the query's codes. Without ``q`` (None, as ``w``, ``q_out`` and ``w_out``) it writes keys only.
+    ``norm_weight``, with ``norm_bias`` or without, normalises ``k`` first (mean and variance, or root
+    mean square). ``freq`` f32 ``[R / 2]`` (see ``rope_frequencies``) turns the ``R`` values from
+    ``rope_start`` on: neighbours, or with ``rope_half`` the halves against each other.
+    """
+
+    def __init__(self, q, k, w, page_table, seq_id, pos, kv, q_out, w_out, **kw):
+        self._bind(q, k, w, page_table, seq_id, pos, kv, q_out, w_out, kw.get("norm_weight"),
+                   kw.get("norm_bias"), kw.get("freq"))
+        self.spec = index_write_spec(q, k, w, page_table, seq_id, pos, kv, q_out, w_out, **kw)
+        self._check(lib.tq_index_write_validate)
+        self.q_out, self.w_out = q_out, w_out
+
+    def __call__(self, flags=None, stream=None):
+        self._run(lib.tq_index_write, (_flags_pointer(flags, self.device),), stream)
+        return self.q_out, self.w_out
+
+
+def index_write(q, k, w, page_table, seq_id, pos, kv, *, flags=None, stream=None, **kw):
+    """One index write (see ``IndexWrite``); returns ``(q_out, w_out)``, Nones without ``q``."""
+    q_out = w_out = None
+    with _allocating_on(stream):
+        if q is not None:
+            q_out = torch.empty(q.shape, dtype=torch.uint8, device=q.device)
+            w_out = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        IndexWrite(q, k, w, page_table, seq_id, pos, kv, q_out, w_out, **kw)(flags, stream)
+    return _returned(stream, q_out, w_out)
+
+
+def index_scores_spec(q, w, kv, page_table, seq_id, q_pos, kv_len, scores):
+    """Declaration of index scores (``tq_index_scores``)."""
+    s = _abi.TqIndexScoresSpec()
+    for name, t in (("q", q), ("w", w), ("page_table", page_table), ("seq_id", seq_id),
+                    ("q_pos", q_pos), ("kv_len", kv_len), ("scores", scores)):
+        setattr(s, name, spec_of(t))
+    s.kv = index_pool_spec(kv)
+    return s
+
+
+class IndexScores(_Launch):
+    """A cheap score of every cached row for every query token: ``scores[t, n] = key_scale[n] *
+    sum_h w[t, h] * max(0, q[t, h] . k[n])`` for the rows ``n < min(kv_len, q_pos + 1)`` of token
+    ``t``'s sequence. Columns behind them keep their values.
+
+    ``q`` u8 ``[T, H, 128]`` and ``w`` f32 ``[T, H]`` from ``IndexWrite``, ``kv`` its cache; ``scores``
+    f32 ``[T, N]``.
+    """
+
+    def __init__(self, q, w, kv, page_table, seq_id, q_pos, kv_len, scores):
+        self._bind(q, w, kv, page_table, seq_id, q_pos, kv_len, scores)
+        self.spec = index_scores_spec(q, w, kv, page_table, seq_id, q_pos, kv_len, scores)
+        self._check(lib.tq_index_scores_validate)
+        self.scores = scores
+
+    def __call__(self, flags=None, stream=None):
+        self._run(lib.tq_index_scores, (_flags_pointer(flags, self.device),), stream)
+        return self.scores
+
+
+def index_scores(q, w, kv, page_table, seq_id, q_pos, kv_len, *, columns=None, scores=None,
+                 flags=None, stream=None):
+    """One call of ``IndexScores``; returns ``scores``, -inf where nothing is seen if the call
+    allocates them (``columns`` of them; as many as the page table holds rows by default)."""
+    with _allocating_on(stream):
+        if scores is None:
+            n = 64 * page_table.shape[1] if columns is None else int(columns)
+            scores = torch.full((q.shape[0], n), -math.inf, dtype=torch.float32, device=q.device)
+        IndexScores(q, w, kv, page_table, seq_id, q_pos, kv_len, scores)(flags, stream)
+    return _returned(stream, scores)[0]
+
+
+def index_select_spec(scores, seq_id, q_pos, kv_len, idx, length, *, page_table=None, keep_first=0,
+                      keep_last=0):
+    """Declaration of an index select (``tq_index_select``)."""
+    s = _abi.TqIndexSelectSpec()
+    for name, t in (("scores", scores), ("seq_id", seq_id), ("q_pos", q_pos), ("kv_len", kv_len),
+                    ("page_table", page_table), ("idx", idx), ("len", length)):
+        if t is not None:
+            setattr(s, name, spec_of(t))
+    s.keep_first, s.keep_last = int(keep_first), int(keep_last)
+    return s
+
+
+class IndexSelect(_Launch):
+    """Each token's best rows or pages by ``scores`` f32 ``[T, N]``, over the rows that it sees.
+
+    Without ``page_table``: ``idx`` i32 ``[T, K]`` gets the positions of the ``K`` largest scores in
+    ascending order, then -1, ``length`` i32 ``[T]`` their number: the ``idx`` and ``k_len`` of a sparse
+    ``mla_decode``. With it: ``idx`` gets the pool pages of the ``K`` best pages of 64 rows (by their
+    largest score), ``length`` the rows that they hold: the ``page_table`` and ``kv_len`` of a dense
+    ``mla_decode`` with ``seq_id = arange(T)`` and one query a sequence. The first ``keep_first`` and
+    last ``keep_last`` positions (pages) are always taken. Equal scores go to the lowest position;
+    -inf and NaN are not taken.
+    """
+
+    def __init__(self, scores, seq_id, q_pos, kv_len, idx, length, **kw):
+        self._bind(scores, seq_id, q_pos, kv_len, idx, length, kw.get("page_table"))
+        self.spec = index_select_spec(scores, seq_id, q_pos, kv_len, idx, length, **kw)
+        self._check(lib.tq_index_select_validate)
+        self.idx, self.length = idx, length
+
+    def __call__(self, flags=None, stream=None):
+        self._run(lib.tq_index_select, (_flags_pointer(flags, self.device),), stream)
+        return self.idx, self.length
+
+
+def index_select(scores, seq_id, q_pos, kv_len, k, *, flags=None, stream=None, **kw):
+    """One index select (see ``IndexSelect``) of ``k`` rows or pages; returns ``(idx, length)``."""
+    with _allocating_on(stream):
+        idx = torch.empty((scores.shape[0], int(k)), dtype=torch.int32, device=scores.device)
+        length = torch.empty((scores.shape[0],), dtype=torch.int32, device=scores.device)
+        IndexSelect(scores, seq_id, q_pos, kv_len, idx, length, **kw)(flags, stream)
+    return _returned(stream, idx, length)
+
+
 def combine_parts(part_out, part_lse, out=None, lse=None, stream=None):
     """Merge ``G`` partial results (``part_out f32 [G,T,H,512]``, ``part_lse f32 [G,T,H]``)."""
     g, t, h, _ = part_out.shape
