@@ -1,9 +1,28 @@
 // Index scores (tq_index_scores): a cheap score of every cached row for every query token,
 //   scores[t, n] = key_scale[n] * sum_h w[t, h] * max(0, q[t, h] . k[n]),  n < sees(t).
+//
+// The dots are E4M3 products on tcgen05 (kind::f8f6f4, f32 sums): 128 keys are the M of a tile, the
+// heads of up to 256 columns of query tokens its N, K = 128 in four steps. A key is then one lane
+// of TMEM, so the sum over heads stays in a thread: it reads its columns, cuts them at zero and
+// adds them up with the tokens' weights, and a warp writes 32 consecutive scores.
+//
+// Work: G consecutive tokens are a group (512 columns, 32 tokens at most); a run is a part of a group
+// with one sequence, and a unit of work a run over 128 keys. Every CTA sums the costs of all groups,
+// takes its even share of the sum and walks it; a run's keys are loaded once for all its tokens.
+// Warps of the one CTA on an SM:
+//   0     walks the runs: describes each (tokens, what they see), loads its codes and weights, and
+//         its keys two pages at a time (TMA through the page table, 128-byte swizzle), their scales
+//         with 4-byte copies beside them
+//   1     issues the MMAs, a sub-tile (the keys by half of a group's tokens) into one of two halves
+//         of TMEM
+//   4-11  two groups of warps, one for each half of TMEM: the sums over heads
+// Waits are bounded (2 s); one that gives up sets TQ_DEV_WAIT_TIMEOUT and ends the CTA's work.
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <mutex>
 
 #include "tq_contracts.h"
 #include "tq_ptx.cuh"
@@ -13,102 +32,534 @@ namespace index_scores {
 
 constexpr int kDim = TQ_INDEX_DIM;
 constexpr int kPageRows = 64;
-constexpr int kKeys = 128;   // keys of a block, one a thread
-constexpr int kHeads = 16;   // heads staged at a time
+constexpr int kKeys = 128;  // keys of a tile, two pages
+constexpr int kThreads = 384;
+constexpr int kWarps = kThreads / 32;
+constexpr int kEpilogueWarp = 4;  // first of eight
+constexpr int kColumns = 256;     // of a sub-tile
+constexpr int kSubTokens = 16;    // tokens of a sub-tile at most
+constexpr int kStages = 5;        // key tiles in flight
+constexpr int kScaleSlots = 8;    // see the producer
+constexpr uint32_t kKeyBytes = kKeys * kDim;
+constexpr uint32_t kQueryBytes = 2 * kColumns * kDim;
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+struct Unit {
+  int t0, tokens;          // run of tokens; 0 tokens: no more work
+  int tile0, tiles;        // its key tiles
+  int sees[2 * kSubTokens];
+};
+
+struct Shared {  // behind 1024-byte alignment
+  uint8_t query[2][kQueryBytes];
+  uint8_t key[kStages][kKeyBytes];
+  float weight[2][2 * kColumns];
+  float scale[kScaleSlots][kKeys];
+  Unit unit[2];
+  uint64_t bar_key_full[kStages], bar_key_empty[kStages];
+  uint64_t bar_scale[kScaleSlots];
+  uint64_t bar_unit_full[2], bar_unit_empty[2];
+  uint64_t bar_acc_full[2], bar_acc_empty[2];
+  uint64_t bar_drain;
+  long long part[kWarps];
+  long long start_cost;
+  int start_group;
+  int stop;  // a wait has given up
+  uint32_t tmem;
+};
+constexpr uint32_t kSharedBytes = sizeof(Shared) + 1024;
+static_assert(kSharedBytes <= 227 * 1024, "shared memory per CTA");
 
 struct Args {
-  const uint8_t* q;
-  const float* w;
   const uint8_t* kv;
+  const float* w;
   const int* page_table;
   const int* seq_id;
   const int* q_pos;
   const int* kv_len;
-  float* scores;
+  uint8_t* scores;
   int* flags;
   long long row_stride;    // bytes
   long long score_stride;  // bytes
   int tokens, heads, sequences, slots, pages, columns;
+  int sub;      // tokens of a sub-tile
+  int nowhere;  // a row past the key map's end: reads as zeros
+};
+
+// A bounded wait; `stop` ends all waits of the CTA once one has given up.
+struct Wait {
+  int* flags;
+  volatile int* stop;
+  bool failed = false;
+  __device__ bool on(uint64_t& barrier, uint32_t parity) {
+    if (failed) return false;
+    const uint32_t bar = ptx::smem_addr(&barrier);
+    if (ptx::mbar_test(bar, parity)) return true;
+    const uint64_t t0 = ptx::global_timer_ns();
+    for (uint32_t i = 1;; ++i) {
+      if (ptx::mbar_test(bar, parity)) return true;
+      if ((i & 255) == 0 &&
+          (ptx::global_timer_ns() - t0 > kWaitNs || i > (1u << 26) || *stop)) {
+        if (flags) atomicOr(flags, TQ_DEV_WAIT_TIMEOUT);
+        *stop = 1;
+        failed = true;
+        return false;
+      }
+    }
+  }
+  // For a converged warp: all lanes go on, or none.
+  __device__ bool warp_on(uint64_t& barrier, uint32_t parity) {
+    return __all_sync(0xFFFFFFFFu, on(barrier, parity));
+  }
 };
 
 // Rows that token t sees, 0 without a sequence; `bad` gets the flags of what is cut.
-__device__ __forceinline__ int sees(const Args& a, int t, int* bad) {
-  const int s = a.seq_id[t];
+__device__ __forceinline__ int sees(const Args& a, int s, int pos, int* bad) {
   if (s < 0 || s >= a.sequences) { *bad |= TQ_DEV_SEQ_RANGE; return 0; }
-  const long long n = min((long long)a.kv_len[s], (long long)a.q_pos[t] + 1);
+  const long long n = min((long long)a.kv_len[s], (long long)pos + 1);
   const long long held = (long long)a.slots * kPageRows;
   if (n > held) *bad |= TQ_DEV_TABLE_SHORT;
   if (min(n, held) > a.columns) *bad |= TQ_DEV_WORK_OVERFLOW;
   return int(max(0ll, min(min(n, held), (long long)a.columns)));
 }
 
-__device__ __forceinline__ float2 e4m3_pair(uint32_t codes) {
-  uint32_t h2;
-  asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}"
-      : "=r"(h2) : "r"(codes));
-  float lo, hi;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
-      : "=f"(lo), "=f"(hi) : "r"(h2));
-  return make_float2(lo, hi);
+// Cost of a key tile for a run: its load, and 64 columns at a time the products and sums. (A tile
+// of one token with 64 heads takes about 0.4 of the time of one with 512 columns.)
+__device__ __forceinline__ int tile_cost(const Args& a, int tokens) {
+  return 4 + (tokens * a.heads + 63) / 64;
+}
+__device__ __forceinline__ int tiles_of(int most) { return (most + kKeys - 1) / kKeys; }
+
+// Cost of group g: its tokens in order, run by run; a few of their loads in flight together.
+__device__ __forceinline__ long long group_cost(const Args& a, int g, int* bad) {
+  const int size = 2 * a.sub, t0 = g * size, end = min(a.tokens, t0 + size);
+  long long cost = 0;
+  int seq = 0, run = 0, most = 0;
+  for (int t = t0; t < end; t += 4) {
+    int s[4], p[4], n[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = t + i < end ? a.seq_id[t + i] : 0;
+      p[i] = t + i < end ? a.q_pos[t + i] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = t + i < end ? sees(a, s[i], p[i], bad) : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (t + i >= end) break;
+      if (run && s[i] != seq) {
+        cost += (long long)tiles_of(most) * tile_cost(a, run);
+        run = most = 0;
+      }
+      seq = s[i];
+      ++run;
+      most = max(most, n[i]);
+    }
+  }
+  return cost + (long long)tiles_of(most) * tile_cost(a, run);
 }
 
-__global__ void __launch_bounds__(kKeys) index_scores_kernel(const Args a) {
-  __shared__ float4 q[kHeads][kDim / 4];
-  const int n = blockIdx.x * kKeys + threadIdx.x;
-  for (int t = blockIdx.y; t < a.tokens; t += gridDim.y) {
-    int bad = 0;
-    const int count = sees(a, t, &bad);
-    if (n == 0 && bad && a.flags) atomicOr(a.flags, bad);
-    if (int(blockIdx.x) * kKeys >= count) continue;
-    float k[kDim], scale = 0.f;
-    for (int i = 0; i < kDim; ++i) k[i] = 0.f;
-    if (n < count) {
-      const int page = a.page_table[(long long)a.seq_id[t] * a.slots + n / kPageRows];
-      if (page >= 0 && page < a.pages) {
-        const uint8_t* row = a.kv + ((long long)page * kPageRows + n % kPageRows) * a.row_stride;
-        scale = *reinterpret_cast<const float*>(row + kDim);
-        for (int i = 0; i < kDim / 16; ++i) {
-          const uint4 c = reinterpret_cast<const uint4*>(row)[i];
-          const uint32_t u[4] = {c.x, c.y, c.z, c.w};
-          for (int j = 0; j < 8; ++j) {
-            const float2 v = e4m3_pair(u[j / 2] >> (16 * (j & 1)));
-            k[16 * i + 2 * j] = v.x;
-            k[16 * i + 2 * j + 1] = v.y;
+// The CTA's share [lo, hi) of all costs, and the group that lo falls in.
+__device__ __forceinline__ void find_share(const Args& a, Shared& sh, long long* lo, long long* hi) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int groups = (a.tokens + 2 * a.sub - 1) / (2 * a.sub);
+  const int each = (groups + kThreads - 1) / kThreads;
+  const int g0 = min(groups, tid * each), g1 = min(groups, g0 + each);
+  int bad = 0;
+  long long mine = 0;
+  for (int g = g0; g < g1; ++g) mine += group_cost(a, g, &bad);
+  if (blockIdx.x == 0 && bad && a.flags) atomicOr(a.flags, bad);
+  long long sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+    if (lane >= o) sum += v;
+  }
+  if (lane == 31) sh.part[warp] = sum;
+  __syncthreads();
+  long long total = 0;
+  for (int i = 0; i < kWarps; ++i) {
+    if (i == warp) sum += total;
+    total += sh.part[i];
+  }
+  *lo = total * blockIdx.x / gridDim.x;
+  *hi = total * (blockIdx.x + 1) / gridDim.x;
+  long long at = sum - mine;
+  if (*lo < *hi && at <= *lo && *lo < sum) {
+    int unused = 0, g = g0;
+    for (; g < g1; ++g) {
+      const long long cost = group_cost(a, g, &unused);
+      if (*lo < at + cost) break;
+      at += cost;
+    }
+    sh.start_group = g;
+    sh.start_cost = at;
+  }
+  __syncthreads();
+}
+
+// Warp 0. A unit's slot is free once the MMAs that read its codes and the eight warps that read its
+// weights are done. A key stage is free once its MMAs are; by then the sums of the tile three
+// before it are done (each half of TMEM is taken in turn), so a scale slot that comes back after
+// kStages + 3 tiles is free too.
+__device__ __forceinline__ void produce(const Args& a, Shared& sh, const CUtensorMap* tm_q,
+                                        const CUtensorMap* tm_k, long long lo, long long hi) {
+  const int lane = threadIdx.x & 31;
+  Wait wait{a.flags, &sh.stop};
+  const int size = 2 * a.sub;
+  int tile = 0, units = 0;
+  bool ok = true;
+  long long at = sh.start_cost;
+  for (int g = sh.start_group; ok && at < hi && (long long)g * size < a.tokens; ++g) {
+    const int end = min(a.tokens, (g + 1) * size);
+    for (int t = g * size; ok && at < hi && t < end;) {
+      // One token a lane: the run that starts at t.
+      int seq = 0, n = 0, unused = 0;
+      if (t + lane < end) {
+        seq = a.seq_id[t + lane];
+        n = sees(a, seq, a.q_pos[t + lane], &unused);
+      }
+      const int first = __shfl_sync(0xFFFFFFFFu, seq, 0);
+      const unsigned same = __ballot_sync(0xFFFFFFFFu, t + lane < end && seq == first);
+      const int run = same == 0xFFFFFFFFu ? 32 : __ffs(~same) - 1;
+      if (lane >= run) n = 0;
+      const int most = __reduce_max_sync(0xFFFFFFFFu, n), tiles = tiles_of(most);
+      const int cost = tile_cost(a, run);
+      // Tiles that start within the share.
+      const int j0 = int(min((long long)tiles, max(0ll, (lo - at + cost - 1) / cost)));
+      const int j1 = int(min((long long)tiles, (hi - at + cost - 1) / cost));
+      at += (long long)tiles * cost;
+      if (j0 < j1) {
+        const int u = units & 1;
+        ok = units < 2 || wait.warp_on(sh.bar_unit_empty[u], uint32_t((units >> 1) - 1) & 1u);
+        if (!ok) break;
+        Unit& unit = sh.unit[u];
+        unit.sees[lane] = n;
+        if (lane == 0) {
+          unit.t0 = t;
+          unit.tokens = run;
+          unit.tile0 = j0;
+          unit.tiles = j1 - j0;
+        }
+        __syncwarp();
+        if (lane == 0) {
+          const uint32_t bar = ptx::smem_addr(&sh.bar_unit_full[u]);
+          const uint32_t rows = uint32_t(run * a.heads);
+          ptx::mbar_expect_tx(bar, rows * (kDim + 4));
+          for (int i = 0; i < run; ++i)
+            ptx::tma_load_2d(ptx::smem_addr(sh.query[u]) + uint32_t(i * a.heads * kDim), tm_q, bar, 0,
+                             (t + i) * a.heads);
+          ptx::bulk_load(ptx::smem_addr(sh.weight[u]), a.w + (long long)t * a.heads, rows * 4, bar);
+        }
+        __syncwarp();
+        ++units;
+        const int* table = a.page_table + (long long)first * a.slots;
+        int pages = 0, base = -64;
+        for (int j = j0; j < j1; ++j, ++tile) {
+          // Page entries 32 at a time; behind the last row that the run sees there are none.
+          if (2 * j - base >= 32) {
+            base = 2 * j;
+            const bool seen = base + lane < a.slots && (base + lane) * kPageRows < most;
+            pages = seen ? table[base + lane] : -1;
+            if (seen && (pages < 0 || pages >= a.pages) && a.flags)
+              atomicOr(a.flags, TQ_DEV_PAGE_RANGE);
+          }
+          const int s = tile % kStages;
+          ok = tile < kStages || wait.warp_on(sh.bar_key_empty[s], uint32_t(tile / kStages - 1) & 1u);
+          if (!ok) break;
+          const int p0 = __shfl_sync(0xFFFFFFFFu, pages, 2 * j - base);
+          const int p1 = __shfl_sync(0xFFFFFFFFu, pages, 2 * j - base + 1);
+          const bool in0 = p0 >= 0 && p0 < a.pages, in1 = p1 >= 0 && p1 < a.pages;
+          const int slot = tile % kScaleSlots;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = 32 * (i & 1) + lane;
+            const bool in = i < 2 ? in0 : in1;
+            const uint8_t* src =
+                a.kv + ((long long)(i < 2 ? p0 : p1) * kPageRows + row) * a.row_stride + kDim;
+            ptx::cp_async_4(ptx::smem_addr(&sh.scale[slot][32 * i + lane]), in ? src : a.kv, in ? 4 : 0);
+          }
+          ptx::cp_async_arrive(ptx::smem_addr(&sh.bar_scale[slot]));
+          if (lane == 0) {
+            const uint32_t bar = ptx::smem_addr(&sh.bar_key_full[s]), dst = ptx::smem_addr(sh.key[s]);
+            ptx::mbar_expect_tx(bar, kKeyBytes);
+            ptx::tma_load_2d(dst, tm_k, bar, 0, in0 ? p0 * kPageRows : a.nowhere);
+            ptx::tma_load_2d(dst + kKeyBytes / 2, tm_k, bar, 0, in1 ? p1 * kPageRows : a.nowhere);
+          }
+          __syncwarp();
+        }
+      }
+      t += run;
+    }
+  }
+  // No more work.
+  const int u = units & 1;
+  if (ok) ok = units < 2 || wait.warp_on(sh.bar_unit_empty[u], uint32_t((units >> 1) - 1) & 1u);
+  if (ok && lane == 0) {
+    sh.unit[u].tokens = 0;
+    ptx::mbar_arrive(ptx::smem_addr(&sh.bar_unit_full[u]));
+  }
+  __syncwarp();
+  ptx::cp_async_wait_all();
+  if (!ok) {
+    // What is on its way lands before the CTA ends.
+    int keep = 0;
+    Wait last{a.flags, &keep};
+    for (int i = max(0, tile - kStages); i < tile; ++i)
+      last.on(sh.bar_key_full[i % kStages], uint32_t(i / kStages) & 1u);
+    for (int i = max(0, units - 2); i < units; ++i)
+      last.on(sh.bar_unit_full[i & 1], uint32_t(i >> 1) & 1u);
+  }
+}
+
+// Warp 1. False when a wait has given up.
+__device__ __forceinline__ bool multiply(const Args& a, Shared& sh) {
+  Wait wait{a.flags, &sh.stop};
+  int tile = 0, subs = 0;
+  for (int units = 0;; ++units) {
+    const int u = units & 1;
+    if (!wait.warp_on(sh.bar_unit_full[u], uint32_t(units >> 1) & 1u)) return false;
+    const int tokens = sh.unit[u].tokens, tiles = sh.unit[u].tiles;
+    if (tokens == 0) return true;
+    for (int j = 0; j < tiles; ++j, ++tile) {
+      const int s = tile % kStages;
+      if (!wait.warp_on(sh.bar_key_full[s], uint32_t(tile / kStages) & 1u)) return false;
+      for (int t = 0; t < tokens; t += a.sub, ++subs) {
+        const int half = subs & 1;
+        if (subs >= 2 && !wait.warp_on(sh.bar_acc_empty[half], uint32_t((subs >> 1) - 1) & 1u)) return false;
+        ptx::tc_fence_after();
+        // Columns in whole sixteens: the last ones may be of no token, and nobody reads them.
+        const uint32_t n = uint32_t(min(a.sub, tokens - t) * a.heads + 15) & ~15u;
+        const uint32_t idesc = ptx::idesc_e4m3(kKeys, n);
+        const uint64_t kd = ptx::smem_desc(ptx::smem_addr(sh.key[s]), 16, 1024, 2);
+        const uint64_t qd = ptx::smem_desc(
+            ptx::smem_addr(sh.query[u]) + uint32_t(t * a.heads * kDim), 16, 1024, 2);
+#pragma unroll
+        for (int k = 0; k < kDim / 32; ++k)
+          ptx::mma_f8_ss_warp(sh.tmem + uint32_t(half * kColumns), kd + 2 * k, qd + 2 * k, idesc, k > 0);
+        ptx::mma_commit_warp(ptx::smem_addr(&sh.bar_acc_full[half]));
+      }
+      ptx::mma_commit_warp(ptx::smem_addr(&sh.bar_key_empty[s]));
+    }
+    ptx::mma_commit_warp(ptx::smem_addr(&sh.bar_unit_empty[u]));
+  }
+}
+
+// After a wait that gave up: what the tensor core still does ends before the CTA does.
+__device__ __forceinline__ void drain(const Args& a, Shared& sh) {
+  int keep = 0;
+  Wait last{a.flags, &keep};
+  ptx::mma_commit_warp(ptx::smem_addr(&sh.bar_drain));
+  last.warp_on(sh.bar_drain, 0);
+}
+
+template <int C>
+__device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[C]) {
+  if constexpr (C == 32) ptx::tmem_ld32(at, r);
+  else if constexpr (C == 16) ptx::tmem_ld16(at, r);
+  else ptx::tmem_ld8(at, r);
+}
+
+// Waits for the loads; what reads `r` stays behind it.
+template <int C>
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[C]) {
+  ptx::tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < C; ++i) asm volatile("" : "+r"(r[i]));
+}
+
+// max(0, x), NaN stays NaN.
+__device__ __forceinline__ float cut(uint32_t bits) {
+  float r;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(__uint_as_float(bits)));
+  return r;
+}
+
+__device__ __forceinline__ void fma2(float2& acc, float x, float y, float wx, float wy) {
+  asm("{\n\t.reg .b64 p, q, r;\n\t"
+      "mov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 r, {%0, %1};\n\t"
+      "fma.rn.f32x2 r, p, q, r;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "+f"(acc.x), "+f"(acc.y) : "f"(x), "f"(y), "f"(wx), "f"(wy));
+}
+
+template <int C>
+__device__ __forceinline__ void add_up(const uint32_t (&r)[C], const float* w, float2 (&acc)[4]) {
+#pragma unroll
+  for (int i = 0; i < C; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(w + i);
+    fma2(acc[(i / 2) & 3], cut(r[i]), cut(r[i + 1]), v.x, v.y);
+    fma2(acc[(i / 2 + 1) & 3], cut(r[i + 2]), cut(r[i + 3]), v.z, v.w);
+  }
+}
+
+// Warps 4-11: half `half` of TMEM, lanes 32 (warp % 4) on. C divides the heads: a token's columns are
+// read C at a time, the next ones while the last are added up.
+template <int C>
+__device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half) {
+  const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, key = 32 * quad + lane;
+  const uint32_t tmem = sh.tmem + uint32_t(half * kColumns) + (uint32_t(32 * quad) << 16);
+  const int chunks = a.heads / C;
+  Wait wait{a.flags, &sh.stop};
+  int tile = 0, subs = 0;
+  for (int units = 0;; ++units) {
+    const int u = units & 1;
+    if (!wait.warp_on(sh.bar_unit_full[u], uint32_t(units >> 1) & 1u)) return;
+    const Unit& unit = sh.unit[u];
+    const int tokens = unit.tokens, tiles = unit.tiles, tile0 = unit.tile0, t0 = unit.t0;
+    if (tokens == 0) return;
+    for (int j = 0; j < tiles; ++j, ++tile) {
+      for (int t = 0; t < tokens; t += a.sub, ++subs) {
+        if ((subs & 1) != half) continue;
+        if (!wait.warp_on(sh.bar_scale[tile % kScaleSlots], uint32_t(tile / kScaleSlots) & 1u)) return;
+        if (!wait.warp_on(sh.bar_acc_full[half], uint32_t(subs >> 1) & 1u)) return;
+        ptx::tc_fence_after();
+        const float scale = sh.scale[tile % kScaleSlots][key];
+        const int n = (tile0 + j) * kKeys + key;
+        const int steps = min(a.sub, tokens - t) * chunks;
+        const float* w = sh.weight[u] + t * a.heads;
+        const int* seen = unit.sees + t;
+        uint8_t* out = a.scores + (long long)(t0 + t) * a.score_stride + 4ll * n;
+        uint32_t r[2][C];
+        float2 acc[4] = {};
+        int left = chunks;
+        tmem_load<C>(tmem, r[0]);
+#pragma unroll 1
+        for (int i = 0; i < steps; i += 2) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            if (i + b < steps) {
+              tmem_wait(r[b]);
+              if (i + b + 1 < steps) {
+                tmem_load<C>(tmem + uint32_t((i + b + 1) * C), r[b ^ 1]);
+              } else {
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sh.bar_acc_empty[half]));
+              }
+              add_up<C>(r[b], w, acc);
+              w += C;
+              if (--left == 0) {
+                const float sum = ((acc[0].x + acc[0].y) + (acc[1].x + acc[1].y)) +
+                                  ((acc[2].x + acc[2].y) + (acc[3].x + acc[3].y));
+                if (n < *seen) *reinterpret_cast<float*>(out) = sum * scale;
+                ++seen;
+                out += a.score_stride;
+                left = chunks;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] = make_float2(0.f, 0.f);
+              }
+            }
           }
         }
-      } else if (a.flags) {
-        atomicOr(a.flags, TQ_DEV_PAGE_RANGE);
       }
     }
-    float sum = 0.f;
-    for (int h0 = 0; h0 < a.heads; h0 += kHeads) {
-      const int heads = min(kHeads, a.heads - h0);
-      __syncthreads();
-      for (int i = threadIdx.x; i < heads * (kDim / 4); i += kKeys) {
-        const uint32_t c = reinterpret_cast<const uint32_t*>(
-            a.q + ((long long)t * a.heads + h0) * kDim)[i];
-        const float2 lo = e4m3_pair(c), hi = e4m3_pair(c >> 16);
-        q[i / (kDim / 4)][i % (kDim / 4)] = make_float4(lo.x, lo.y, hi.x, hi.y);
-      }
-      __syncthreads();
-      for (int h = 0; h < heads; ++h) {
-        float dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < kDim / 4; ++i) {
-          const float4 v = q[h][i];
-          dot = fmaf(v.x, k[4 * i], dot);
-          dot = fmaf(v.y, k[4 * i + 1], dot);
-          dot = fmaf(v.z, k[4 * i + 2], dot);
-          dot = fmaf(v.w, k[4 * i + 3], dot);
-        }
-        const float r = dot < 0.f ? 0.f : dot;  // NaN stays NaN
-        sum = fmaf(a.w[(long long)t * a.heads + h0 + h], r, sum);
-      }
-    }
-    if (n < count)
-      reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.scores) + t * a.score_stride)[n] =
-          sum * scale;
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sh.bar_unit_empty[u]));
   }
+}
+
+template <int C>
+__global__ void __launch_bounds__(kThreads, 1)
+    index_scores_kernel(const __grid_constant__ CUtensorMap tm_q,
+                        const __grid_constant__ CUtensorMap tm_k, const Args a) {
+  extern __shared__ uint8_t raw[];
+  Shared& sh = *reinterpret_cast<Shared*>(raw + ((1024u - (ptx::smem_addr(raw) & 1023u)) & 1023u));
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    auto init = [](uint64_t& bar, uint32_t count) { ptx::mbar_init(ptx::smem_addr(&bar), count); };
+    for (int s = 0; s < kStages; ++s) {
+      init(sh.bar_key_full[s], 1);
+      init(sh.bar_key_empty[s], 1);
+    }
+    for (int s = 0; s < kScaleSlots; ++s) init(sh.bar_scale[s], 32);
+    for (int b = 0; b < 2; ++b) {
+      init(sh.bar_unit_full[b], 1);
+      init(sh.bar_unit_empty[b], 9);
+      init(sh.bar_acc_full[b], 1);
+      init(sh.bar_acc_empty[b], 4);
+    }
+    init(sh.bar_drain, 1);
+    sh.stop = 0;
+    ptx::fence_mbar_init_cluster();
+    ptx::tma_prefetch_desc(&tm_q);
+    ptx::tma_prefetch_desc(&tm_k);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_addr(&sh.tmem), 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  long long lo, hi;
+  find_share(a, sh, &lo, &hi);
+  if (lo < hi) {
+    if (warp == 0) {
+      produce(a, sh, &tm_q, &tm_k, lo, hi);
+    } else if (warp == 1) {
+      if (!multiply(a, sh)) drain(a, sh);
+    } else if (warp >= kEpilogueWarp) {
+      sum_heads<C>(a, sh, (warp - kEpilogueWarp) >> 2);
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(sh.tmem, 512);
+  }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// Rows of 128 codes as a 2D map with boxes of `box` rows and 128-byte swizzle.
+bool encode_rows(CUtensorMap* map, const void* addr, uint64_t rows, uint64_t stride, uint32_t box) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {kDim, rows};
+  const cuuint64_t strides[1] = {stride};
+  const cuuint32_t boxes[2] = {kDim, box};
+  const cuuint32_t elem[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(addr), dims, strides, boxes,
+            elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// SMs of the current device, once the kernels have their shared memory granted on it; 0 on failure.
+int sms_on(int device) {
+  static std::mutex mu;
+  static int cached[128] = {0};
+  if (device < 0 || device >= 128) return 0;
+  std::lock_guard<std::mutex> lock(mu);
+  if (cached[device]) return cached[device];
+  int n = 0;
+  const cudaFuncAttribute most = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
+      cudaFuncSetAttribute(index_scores_kernel<32>, most, int(kSharedBytes)) != cudaSuccess ||
+      cudaFuncSetAttribute(index_scores_kernel<16>, most, int(kSharedBytes)) != cudaSuccess ||
+      cudaFuncSetAttribute(index_scores_kernel<8>, most, int(kSharedBytes)) != cudaSuccess)
+    return 0;
+  cached[device] = n;
+  return n;
 }
 
 }  // namespace index_scores
@@ -124,17 +575,20 @@ extern "C" int32_t tq_index_scores(const TqIndexScoresSpec* spec, int32_t* devic
   const int32_t st = tq::index_scores_validate(spec, err);
   if (st != TQ_OK) return st;
   const TqIndexScoresSpec& s = *spec;
-  if (s.q.shape[0] == 0 || s.scores.shape[1] == 0) return fail(nullptr, TQ_OK);
+  if (s.q.shape[0] == 0) return fail(nullptr, TQ_OK);
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return fail("device", TQ_ERR_CUDA);
+  const int sms = sms_on(device);
+  if (sms <= 0) return fail("device", TQ_ERR_CUDA);
   auto ints = [](const TqTensorSpec& t) { return reinterpret_cast<const int*>(t.device_address); };
   Args a = {};
-  a.q = reinterpret_cast<const uint8_t*>(s.q.device_address);
-  a.w = reinterpret_cast<const float*>(s.w.device_address);
   a.kv = reinterpret_cast<const uint8_t*>(s.kv.device_address);
+  a.w = reinterpret_cast<const float*>(s.w.device_address);
   a.page_table = ints(s.page_table);
   a.seq_id = ints(s.seq_id);
   a.q_pos = ints(s.q_pos);
   a.kv_len = ints(s.kv_len);
-  a.scores = reinterpret_cast<float*>(s.scores.device_address);
+  a.scores = reinterpret_cast<uint8_t*>(s.scores.device_address);
   a.flags = device_flags;
   a.row_stride = (long long)s.kv.strides_bytes[1];
   a.score_stride = (long long)s.scores.strides_bytes[0];
@@ -144,9 +598,31 @@ extern "C" int32_t tq_index_scores(const TqIndexScoresSpec* spec, int32_t* devic
   a.slots = int(s.page_table.shape[1]);
   a.pages = int(s.kv.shape[0]);
   a.columns = int(s.scores.shape[1]);
-  const unsigned blocks = unsigned((a.columns + kKeys - 1) / kKeys);
-  const unsigned rows = unsigned(a.tokens < 65535 ? a.tokens : 65535);
-  index_scores_kernel<<<dim3(blocks, rows), kKeys, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  if (cudaGetLastError() != cudaSuccess) return fail("launch", TQ_ERR_CUDA);
+  a.sub = kColumns / a.heads < kSubTokens ? kColumns / a.heads : kSubTokens;
+  CUtensorMap tm_q, tm_k;
+  const void* codes = reinterpret_cast<const void*>(s.q.device_address);
+  // A pool without pages has no memory to describe: every page reads past the end of one row of q.
+  const uint64_t rows = a.pages ? uint64_t(a.pages) * kPageRows : 1;
+  a.nowhere = int(rows);
+  if (!encode_rows(&tm_q, codes, s.q.shape[0] * s.q.shape[1], kDim, uint32_t(a.heads)) ||
+      !encode_rows(&tm_k, a.pages ? a.kv : codes, rows, a.pages ? uint64_t(a.row_stride) : kDim,
+                   kPageRows))
+    return fail("tensor map", TQ_ERR_CUDA);
+  if (!a.pages) a.kv = reinterpret_cast<const uint8_t*>(codes);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(sms), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = kSharedBytes;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  cudaError_t e;
+  if (a.heads % 32 == 0) e = cudaLaunchKernelEx(&cfg, index_scores_kernel<32>, tm_q, tm_k, a);
+  else if (a.heads % 16 == 0) e = cudaLaunchKernelEx(&cfg, index_scores_kernel<16>, tm_q, tm_k, a);
+  else e = cudaLaunchKernelEx(&cfg, index_scores_kernel<8>, tm_q, tm_k, a);
+  if (e != cudaSuccess) return fail("launch", TQ_ERR_CUDA);
   return fail(nullptr, TQ_OK);
 }
