@@ -15,7 +15,7 @@
 //         with 4-byte copies beside them
 //   1     issues the MMAs, a sub-tile (the keys by half of a group's tokens) into one of two halves
 //         of TMEM
-//   4-11  two groups of warps, one for each half of TMEM: the sums over heads
+//   2-17  four groups of warps, two for each half of TMEM: the sums over heads
 // Waits are bounded (2 s); one that gives up sets TQ_DEV_WAIT_TIMEOUT and ends the CTA's work.
 
 #include <cuda.h>
@@ -33,9 +33,9 @@ namespace index_scores {
 constexpr int kDim = TQ_INDEX_DIM;
 constexpr int kPageRows = 64;
 constexpr int kKeys = 128;  // keys of a tile, two pages
-constexpr int kThreads = 384;
+constexpr int kThreads = 576;
 constexpr int kWarps = kThreads / 32;
-constexpr int kEpilogueWarp = 4;  // first of eight
+constexpr int kSumWarp = 2;  // first of sixteen
 constexpr int kColumns = 256;     // of a sub-tile
 constexpr int kSubTokens = 16;    // tokens of a sub-tile at most
 constexpr int kStages = 5;        // key tiles in flight
@@ -43,6 +43,7 @@ constexpr int kScaleSlots = 8;    // see the producer
 constexpr uint32_t kKeyBytes = kKeys * kDim;
 constexpr uint32_t kQueryBytes = 2 * kColumns * kDim;
 constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr uint32_t kWaitPolls = 1u << 26;
 
 struct Unit {
   int t0, tokens;          // run of tokens; 0 tokens: no more work
@@ -86,7 +87,8 @@ struct Args {
   int nowhere;  // a row past the key map's end: reads as zeros
 };
 
-// A bounded wait; `stop` ends all waits of the CTA once one has given up.
+// A bounded wait; `stop` ends all waits of the CTA once one has given up. Reading the timer is slow:
+// only a wait of many polls does.
 struct Wait {
   int* flags;
   volatile int* stop;
@@ -94,16 +96,18 @@ struct Wait {
   __device__ bool on(uint64_t& barrier, uint32_t parity) {
     if (failed) return false;
     const uint32_t bar = ptx::smem_addr(&barrier);
-    if (ptx::mbar_test(bar, parity)) return true;
-    const uint64_t t0 = ptx::global_timer_ns();
+    uint64_t t0 = 0;
     for (uint32_t i = 1;; ++i) {
-      if (ptx::mbar_test(bar, parity)) return true;
-      if ((i & 255) == 0 &&
-          (ptx::global_timer_ns() - t0 > kWaitNs || i > (1u << 26) || *stop)) {
-        if (flags) atomicOr(flags, TQ_DEV_WAIT_TIMEOUT);
-        *stop = 1;
-        failed = true;
-        return false;
+      if (ptx::mbar_try(bar, parity)) return true;
+      if ((i & 63) == 0) {
+        const uint64_t now = ptx::global_timer_ns();
+        if (t0 == 0) t0 = now;
+        if (now - t0 > kWaitNs || i > kWaitPolls || *stop) {
+          if (flags) atomicOr(flags, TQ_DEV_WAIT_TIMEOUT);
+          *stop = 1;
+          failed = true;
+          return false;
+        }
       }
     }
   }
@@ -198,7 +202,7 @@ __device__ __forceinline__ void find_share(const Args& a, Shared& sh, long long*
   __syncthreads();
 }
 
-// Warp 0. A unit's slot is free once the MMAs that read its codes and the eight warps that read its
+// Warp 0. A unit's slot is free once the MMAs that read its codes and the sixteen that read its
 // weights are done. A key stage is free once its MMAs are; by then the sums of the tile three
 // before it are done (each half of TMEM is taken in turn), so a scale slot that comes back after
 // kStages + 3 tiles is free too.
@@ -355,8 +359,7 @@ __device__ __forceinline__ void drain(const Args& a, Shared& sh) {
 
 template <int C>
 __device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[C]) {
-  if constexpr (C == 32) ptx::tmem_ld32(at, r);
-  else if constexpr (C == 16) ptx::tmem_ld16(at, r);
+  if constexpr (C == 16) ptx::tmem_ld16(at, r);
   else ptx::tmem_ld8(at, r);
 }
 
@@ -375,27 +378,121 @@ __device__ __forceinline__ float cut(uint32_t bits) {
   return r;
 }
 
-__device__ __forceinline__ void fma2(float2& acc, float x, float y, float wx, float wy) {
-  asm("{\n\t.reg .b64 p, q, r;\n\t"
-      "mov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 r, {%0, %1};\n\t"
-      "fma.rn.f32x2 r, p, q, r;\n\tmov.b64 {%0, %1}, r;\n\t}"
-      : "+f"(acc.x), "+f"(acc.y) : "f"(x), "f"(y), "f"(wx), "f"(wy));
-}
+// Two sums at once (one instruction for two products and additions).
+__device__ __forceinline__ void fma2(float2& acc, float2 x, float2 w) { acc = __ffma2_rn(x, w, acc); }
+__device__ __forceinline__ float both(float2 acc) { return acc.x + acc.y; }
 
 template <int C>
 __device__ __forceinline__ void add_up(const uint32_t (&r)[C], const float* w, float2 (&acc)[4]) {
 #pragma unroll
   for (int i = 0; i < C; i += 4) {
     const float4 v = *reinterpret_cast<const float4*>(w + i);
-    fma2(acc[(i / 2) & 3], cut(r[i]), cut(r[i + 1]), v.x, v.y);
-    fma2(acc[(i / 2 + 1) & 3], cut(r[i + 2]), cut(r[i + 3]), v.z, v.w);
+    fma2(acc[(i / 2) & 3], make_float2(cut(r[i]), cut(r[i + 1])), make_float2(v.x, v.y));
+    fma2(acc[(i / 2 + 1) & 3], make_float2(cut(r[i + 2]), cut(r[i + 3])), make_float2(v.z, v.w));
   }
 }
 
-// Warps 4-11: half `half` of TMEM, lanes 32 (warp % 4) on. C divides the heads: a token's columns are
+// Warps 2-17, heads 32, 64 or 128 (kH): the first or second part of a sub-tile's tokens, in half
+// `half` of TMEM, lanes 32 (warp % 4) on. A thread has two columns of each eight and four keys, so a
+// weight serves four sums, and the weights of its part, 32 a thread, stay in registers for all tiles
+// of a unit. (One key a thread needs a weight from
+// shared memory for each product: 4 cycles a warp for 128 of them.) A token's four sums end spread
+// over four lanes: three exchanges leave one key's in each.
+// What bounds it: the instructions, 1.5 for each head of a key and token (its cut at zero, half of a
+// product and addition), a cut at half their rate. So the last of the four keys adds |x| to x
+// instead, twice the same, and halves its sum.
+template <int kH>
+__device__ __forceinline__ void sum_heads_in_registers(const Args& a, Shared& sh, int half, int part) {
+  constexpr int kSub = kColumns / kH, kTokens = kSub / 2;  // tokens of a sub-tile, of a part of it
+  constexpr int kStep = 32, kChunks = kH / kStep;  // columns read at a time, of a token
+  const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3;
+  const uint32_t tmem = sh.tmem + uint32_t(half * kColumns) + (uint32_t(32 * quad) << 16);
+  // After the exchanges: lanes with bit 0 hold keys 16 on, with bit 1 the odd eights.
+  const int key = 32 * quad + 16 * (lane & 1) + 4 * (lane & 2) + (lane >> 2);
+  Wait wait{a.flags, &sh.stop};
+  int tile = 0, subs = 0;
+  for (int units = 0;; ++units) {
+    const int u = units & 1;
+    if (!wait.warp_on(sh.bar_unit_full[u], uint32_t(units >> 1) & 1u)) return;
+    const Unit& unit = sh.unit[u];
+    const int tokens = unit.tokens, tiles = unit.tiles;
+    if (tokens == 0) return;
+    // A tile is two sub-tiles, of which this half of TMEM always has the same one, or one, and this
+    // half has every other tile.
+    const bool two = tokens > kSub;
+    const int t0 = two && (subs & 1) != half ? kSub : 0, all = min(kSub, tokens - t0);
+    const int mine = part ? all / 2 : (all + 1) / 2, place = part ? (all + 1) / 2 : 0;
+    const int first = t0 + place;
+    float2 w[kTokens * kH / 8];
+#pragma unroll
+    for (int i = 0; i < kTokens * kH / 8; ++i)
+      w[i] = make_float2(sh.weight[u][first * kH + 8 * i + (lane & 3)],
+                         sh.weight[u][first * kH + 8 * i + 4 + (lane & 3)]);
+    uint8_t* const out0 = a.scores + (long long)(unit.t0 + first) * a.score_stride +
+                          4ll * (unit.tile0 * kKeys + key);
+    const int* seen = unit.sees + first;
+    for (int j = 0; j < tiles; ++j, ++tile) {
+      const int sub = subs + (t0 != 0);
+      subs += two ? 2 : 1;
+      if ((sub & 1) != half) continue;
+      if (!wait.warp_on(sh.bar_scale[tile % kScaleSlots], uint32_t(tile / kScaleSlots) & 1u)) return;
+      if (!wait.warp_on(sh.bar_acc_full[half], uint32_t(sub >> 1) & 1u)) return;
+      ptx::tc_fence_after();
+      const float scale = sh.scale[tile % kScaleSlots][key];
+      const int n = (unit.tile0 + j) * kKeys + key;
+      uint8_t* out = out0 + 4ll * kKeys * j;
+      auto done = [&] {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sh.bar_acc_empty[half]));
+      };
+      if (mine == 0) {
+        done();
+        continue;
+      }
+      const uint32_t from = tmem + uint32_t(place * kH);
+#pragma unroll
+      for (int i = 0; i < kTokens; ++i) {
+        if (i >= mine) break;
+        float2 acc[4] = {};
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const int now = i * kChunks + c;
+          uint32_t x[kStep];
+          ptx::tmem_ld_16x128b_x8(from + uint32_t(kStep * now), x);
+          ptx::tmem_ld_16x128b_x8(from + uint32_t(kStep * now) + (16u << 16), x + kStep / 2);
+          tmem_wait(x);
+          if (c + 1 == kChunks && i + 1 >= mine) done();
+#pragma unroll
+          for (int g = 0; g < kStep / 8; ++g) {
+            const float2 wg = w[now * (kStep / 8) + g];
+            const uint32_t* y = x + 4 * g;
+            fma2(acc[0], make_float2(cut(y[0]), cut(y[2])), wg);
+            fma2(acc[1], make_float2(cut(y[1]), cut(y[3])), wg);
+            y += kStep / 2;
+            fma2(acc[2], make_float2(cut(y[0]), cut(y[2])), wg);
+            const float z0 = __uint_as_float(y[1]), z1 = __uint_as_float(y[3]);
+            fma2(acc[3], make_float2(z0 + fabsf(z0), z1 + fabsf(z1)), wg);
+          }
+        }
+        const float s0 = both(acc[0]), s1 = both(acc[1]), s2 = both(acc[2]), s3 = 0.5f * both(acc[3]);
+        const bool b0 = lane & 1, b1 = lane & 2;
+        const float p = (b0 ? s2 : s0) + __shfl_xor_sync(0xFFFFFFFFu, b0 ? s0 : s2, 1);
+        const float q = (b0 ? s3 : s1) + __shfl_xor_sync(0xFFFFFFFFu, b0 ? s1 : s3, 1);
+        const float sum = (b1 ? q : p) + __shfl_xor_sync(0xFFFFFFFFu, b1 ? p : q, 2);
+        if (n < seen[i]) *reinterpret_cast<float*>(out) = sum * scale;
+        out += a.score_stride;
+      }
+    }
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sh.bar_unit_empty[u]));
+  }
+}
+
+// The same for other numbers of heads, one key a thread. C divides the heads: a token's columns are
 // read C at a time, the next ones while the last are added up.
 template <int C>
-__device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half) {
+__device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half, int part) {
   const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, key = 32 * quad + lane;
   const uint32_t tmem = sh.tmem + uint32_t(half * kColumns) + (uint32_t(32 * quad) << 16);
   const int chunks = a.heads / C;
@@ -415,14 +512,22 @@ __device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half) {
         ptx::tc_fence_after();
         const float scale = sh.scale[tile % kScaleSlots][key];
         const int n = (tile0 + j) * kKeys + key;
-        const int steps = min(a.sub, tokens - t) * chunks;
-        const float* w = sh.weight[u] + t * a.heads;
-        const int* seen = unit.sees + t;
-        uint8_t* out = a.scores + (long long)(t0 + t) * a.score_stride + 4ll * n;
+        const int all = min(a.sub, tokens - t), place = part ? (all + 1) / 2 : 0;
+        const int steps = (part ? all / 2 : (all + 1) / 2) * chunks;
+        if (steps == 0) {
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sh.bar_acc_empty[half]));
+          continue;
+        }
+        const uint32_t from = tmem + uint32_t(place * a.heads);
+        const float* w = sh.weight[u] + (t + place) * a.heads;
+        const int* seen = unit.sees + t + place;
+        uint8_t* out = a.scores + (long long)(t0 + t + place) * a.score_stride + 4ll * n;
         uint32_t r[2][C];
         float2 acc[4] = {};
         int left = chunks;
-        tmem_load<C>(tmem, r[0]);
+        tmem_load<C>(from, r[0]);
 #pragma unroll 1
         for (int i = 0; i < steps; i += 2) {
 #pragma unroll
@@ -430,7 +535,7 @@ __device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half) {
             if (i + b < steps) {
               tmem_wait(r[b]);
               if (i + b + 1 < steps) {
-                tmem_load<C>(tmem + uint32_t((i + b + 1) * C), r[b ^ 1]);
+                tmem_load<C>(from + uint32_t((i + b + 1) * C), r[b ^ 1]);
               } else {
                 ptx::tc_fence_before();
                 __syncwarp();
@@ -439,8 +544,7 @@ __device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half) {
               add_up<C>(r[b], w, acc);
               w += C;
               if (--left == 0) {
-                const float sum = ((acc[0].x + acc[0].y) + (acc[1].x + acc[1].y)) +
-                                  ((acc[2].x + acc[2].y) + (acc[3].x + acc[3].y));
+                const float sum = (both(acc[0]) + both(acc[1])) + (both(acc[2]) + both(acc[3]));
                 if (n < *seen) *reinterpret_cast<float*>(out) = sum * scale;
                 ++seen;
                 out += a.score_stride;
@@ -458,7 +562,8 @@ __device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half) {
   }
 }
 
-template <int C>
+// kH: the heads if they are 32, 64 or 128; else 0, and C as above.
+template <int kH, int C>
 __global__ void __launch_bounds__(kThreads, 1)
     index_scores_kernel(const __grid_constant__ CUtensorMap tm_q,
                         const __grid_constant__ CUtensorMap tm_k, const Args a) {
@@ -474,9 +579,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < kScaleSlots; ++s) init(sh.bar_scale[s], 32);
     for (int b = 0; b < 2; ++b) {
       init(sh.bar_unit_full[b], 1);
-      init(sh.bar_unit_empty[b], 9);
+      init(sh.bar_unit_empty[b], 17);
       init(sh.bar_acc_full[b], 1);
-      init(sh.bar_acc_empty[b], 4);
+      init(sh.bar_acc_empty[b], 8);
     }
     init(sh.bar_drain, 1);
     sh.stop = 0;
@@ -500,8 +605,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       produce(a, sh, &tm_q, &tm_k, lo, hi);
     } else if (warp == 1) {
       if (!multiply(a, sh)) drain(a, sh);
-    } else if (warp >= kEpilogueWarp) {
-      sum_heads<C>(a, sh, (warp - kEpilogueWarp) >> 2);
+    } else {
+      const int group = (warp - kSumWarp) >> 2;
+      if constexpr (kH) sum_heads_in_registers<kH>(a, sh, group & 1, group >> 1);
+      else sum_heads<C>(a, sh, group & 1, group >> 1);
     }
   }
   ptx::tc_fence_before();
@@ -544,6 +651,17 @@ bool encode_rows(CUtensorMap* map, const void* addr, uint64_t rows, uint64_t str
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+typedef void (*Kernel)(CUtensorMap, CUtensorMap, Args);
+
+Kernel kernel_for(int heads) {
+  switch (heads) {
+    case 32: return index_scores_kernel<32, 0>;
+    case 64: return index_scores_kernel<64, 0>;
+    case 128: return index_scores_kernel<128, 0>;
+  }
+  return heads % 16 == 0 ? index_scores_kernel<0, 16> : index_scores_kernel<0, 8>;
+}
+
 // SMs of the current device, once the kernels have their shared memory granted on it; 0 on failure.
 int sms_on(int device) {
   static std::mutex mu;
@@ -552,12 +670,11 @@ int sms_on(int device) {
   std::lock_guard<std::mutex> lock(mu);
   if (cached[device]) return cached[device];
   int n = 0;
-  const cudaFuncAttribute most = cudaFuncAttributeMaxDynamicSharedMemorySize;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
-      cudaFuncSetAttribute(index_scores_kernel<32>, most, int(kSharedBytes)) != cudaSuccess ||
-      cudaFuncSetAttribute(index_scores_kernel<16>, most, int(kSharedBytes)) != cudaSuccess ||
-      cudaFuncSetAttribute(index_scores_kernel<8>, most, int(kSharedBytes)) != cudaSuccess)
-    return 0;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+  for (int heads : {8, 16, 32, 64, 128})
+    if (cudaFuncSetAttribute(kernel_for(heads), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             int(kSharedBytes)) != cudaSuccess)
+      return 0;
   cached[device] = n;
   return n;
 }
@@ -619,10 +736,7 @@ extern "C" int32_t tq_index_scores(const TqIndexScoresSpec* spec, int32_t* devic
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = pdl;
   cfg.numAttrs = 1;
-  cudaError_t e;
-  if (a.heads % 32 == 0) e = cudaLaunchKernelEx(&cfg, index_scores_kernel<32>, tm_q, tm_k, a);
-  else if (a.heads % 16 == 0) e = cudaLaunchKernelEx(&cfg, index_scores_kernel<16>, tm_q, tm_k, a);
-  else e = cudaLaunchKernelEx(&cfg, index_scores_kernel<8>, tm_q, tm_k, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel_for(a.heads), tm_q, tm_k, a);
   if (e != cudaSuccess) return fail("launch", TQ_ERR_CUDA);
   return fail(nullptr, TQ_OK);
 }
