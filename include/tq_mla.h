@@ -533,7 +533,7 @@ int32_t tq_index_scores(const TqIndexScoresSpec* spec, int32_t* device_flags, vo
  * The first keep_first and the last keep_last of the positions (pages) that a token sees are always
  * selected. Equal scores go to the lowest position. A score of -inf (masked) or NaN is not selected
  * (where it is not kept), so a row may end with fewer than K, or none.
- *   scores f32 [T, N], N < 2^24, outer stride may be padded      seq_id, q_pos i32 [T]
+ *   scores f32 [T, N], N <= 2^20, outer stride may be padded      seq_id, q_pos i32 [T]
  *   kv_len i32 [S]    idx i32 [T, K], packed, K is 1 to TQ_MLA_MAX_TOPK    len i32 [T]
  *   keep_first, keep_last >= 0, their sum <= K
  * A token without a sequence (seq_id outside [0, S)) selects nothing and sets TQ_DEV_SEQ_RANGE.

@@ -704,7 +704,7 @@ int32_t index_select_validate_impl(const TqIndexSelectSpec* spec, TqContractErro
   };
   if (!spec) return fail("spec", TQ_ERR_INVALID_ARGUMENT);
   const TqIndexSelectSpec& s = *spec;
-  if (s.scores.rank != 2 || s.scores.shape[1] >= (1u << 24)) return fail("scores", TQ_SHAPE);
+  if (s.scores.rank != 2 || s.scores.shape[1] > (1u << 20)) return fail("scores", TQ_SHAPE);
   if (s.kv_len.rank != 1) return fail("kv_len", TQ_SHAPE);
   if (s.idx.rank != 2) return fail("idx", TQ_SHAPE);
   const uint64_t T = s.scores.shape[0], N = s.scores.shape[1], K = s.idx.shape[1];

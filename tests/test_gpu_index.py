@@ -308,7 +308,8 @@ def check_select(device, score, seq, pos, kv_len, k, table=None, first=0, last=0
     assert int(flags) == want_flags
 
 
-VALUES = ["normal", "coarse", "equal", "zeros", "tiny", "wide", "one high", "falling", "rising", "masked", "clusters"]
+VALUES = ["normal", "coarse", "equal", "zeros", "tiny", "wide", "one high", "falling", "rising", "masked", "clusters", "runs high",
+          "runs low", "two values"]
 
 
 def values(kind, rng, t, n):
@@ -336,6 +337,12 @@ def values(kind, rng, t, n):
         v[rng.random((t, n)) < 0.03] = np.nan
         v[rng.random((t, n)) < 0.03] = np.finfo(np.float32).min
         v[0] = -np.inf
+    if kind in ("runs high", "runs low"):       # evenly spaced neighbours unlike the rest
+        for part in range(512):
+            at = part * max(n - 8, 0) // 512
+            v[:, at:at + 8] += 20 if kind == "runs high" else -20
+    if kind == "two values":
+        v = np.where(rng.random((t, n)) < 0.5, 3.0, -1.5).astype(np.float32)
     if kind == "clusters":
         v = (np.where(rng.random((t, n)) < 0.97, 1.0, 8.0) + v * 1e-6).astype(np.float32)
     return v
@@ -401,6 +408,15 @@ def test_select_of_many_rows(cuda_device):
     rng = np.random.default_rng(23)
     t, n = 700, 3001
     check_select(cuda_device, values("normal", rng, t, n), np.zeros(t, int), np.arange(n - t, n), np.array([n]), 512)
+
+
+@pytest.mark.parametrize("kind", ["normal", "equal", "runs low"])
+def test_select_of_the_longest_rows(cuda_device, kind):
+    rng = np.random.default_rng(24)
+    n = 1 << 20
+    score = values(kind, rng, 1, n)
+    check_select(cuda_device, score, np.array([0]), np.array([n - 1]), np.array([n]), 2051)
+    check_select(cuda_device, score, np.array([0]), np.array([n - 1]), np.array([n]), 2051, rng.permutation(n // PAGE)[None], 1, 2)
 
 
 def test_select_of_no_columns(cuda_device):

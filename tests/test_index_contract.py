@@ -95,7 +95,7 @@ OK = (None, 0)
     write(norm=1), write(rope=0), write(rope=128), write(rope=16, start=112), write(tokens=0),
     scores(), scores(heads=8), scores(heads=128), scores(tokens=0), scores(columns=0),
     select(), select(k=2051), select(k=1), select(pages=True), select(first=7, last=13), select(tokens=0),
-    select(columns=0)])
+    select(columns=0), select(columns=1 << 20)])
 def test_accepted(s):
     assert verdict(s) == OK
 
@@ -168,7 +168,7 @@ def with_(s, **fields):
     # select
     (select(k=0), ("idx", SHAPE)),
     (select(k=2052), ("idx", SHAPE)),
-    (select(columns=1 << 24), ("scores", SHAPE)),
+    (select(columns=(1 << 20) + 1), ("scores", SHAPE)),
     (select(first=21), ("keep_first", SHAPE)),
     (select(first=-1), ("keep_first", SHAPE)),
     (select(first=10, last=11), ("keep_last", SHAPE)),
