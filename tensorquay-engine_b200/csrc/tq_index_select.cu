@@ -1,20 +1,23 @@
 // Index select (tq_index_select): each token's K best rows or pages, in ascending order.
 //
-// One block a token. Up to kDirect scores are held in registers, counted into kBins bins of even width
-// between the least and the largest, and the few in the bin that the K-th largest falls into are
-// ranked against each other. Of a longer row a sample is counted first, for a threshold that a little
-// more than K scores reach (how much more: six standard deviations of the sample's count); the row is
-// streamed once, what reaches the threshold is kept with its position (1 to 2 K candidates), and these
-// are counted and ranked. Where too few or too many reach the threshold it is moved and the row
-// streamed again; where that does not help (more equal scores than candidates fit), and where the bins
-// do not tell the values apart, the K-th largest is searched by halving. What is taken, ties by
-// position, is put into a bitmap of the row, and the bitmap's order is the order of the answer: nothing
-// depends on the order in which candidates arrive.
-// In the page form the scores are first reduced to a value a page, in shared memory, and the same is
-// done with those.
+// The K-th largest of a row's scores is found by counting: into kBins bins of even width between the
+// least and the largest; the scores in the one bin that it falls into, a few dozen as a rule, are ranked
+// against each other, equal ones by position. Where more than kRanked are in it, they are counted
+// again into bins of their own, now by their bits as whole numbers, 10 of 32 a time, so that no
+// distribution takes more than five counts. What is taken goes into a bitmap, whose order is the order
+// of the answer; nothing depends on timing. Two kernels:
+//   hold_kernel    few rows: a cluster of one to eight blocks a token, each with a run of the row in
+//                  registers, their bins added up through distributed shared memory. The page form
+//                  reduces its scores to a value a page first, and does the same with those
+//   stream_kernel  many rows, and longer ones than a cluster holds: a small block a token, six on an SM. A
+//                  sample of the row gives a threshold that a little more than K scores reach (how much
+//                  more: six standard deviations of the sample's count); the row is read once and what
+//                  reaches the threshold is listed; these are counted and ranked. Where too few or too
+//                  many reach it, it is moved and the row read again; where that does not help (more
+//                  equal scores than the list holds) the whole row is counted.
 //
-// What bounds it: reading the scores (4 bytes a row seen) for many tokens, the chain of loads, counts
-// and barriers for few.
+// What bounds it: reading the scores (4 bytes a row seen) and counting them for many tokens, the chain of
+// loads and barriers for few.
 
 #include <cuda_runtime.h>
 
@@ -29,20 +32,17 @@
 namespace tq {
 namespace index_select {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+constexpr int kThreads = 512;          // of hold_kernel
+constexpr int kN = 16;                 // scores that one of them holds
+constexpr int kHold = kN * kThreads;   // and a block
+constexpr int kMaxCluster = 8;
+constexpr int kStreamThreads = 256;
+constexpr int kCandidates = 4096;      // of stream_kernel
+constexpr int kSample = 16;            // scores that one of its threads samples
 constexpr int kPageRows = 64;
-constexpr int kDirect = 8192;
-constexpr int kCandidates = 3840;  // (4096 and the bitmap of 2^20 columns do not fit)
-constexpr int kSample = 8;      // sampled scores of a thread, at a time
-constexpr int kMaxSample = 16;
-constexpr int kBins = 1024;     // two a thread
-constexpr int kRanked = kThreads / 8;  // scores that are ranked against each other, 8 threads each
-static_assert(kBins == 2 * kThreads, "two bins a thread");
-constexpr int kVectors = 4;     // 16-byte vectors of a lane in a stage of the stream
-constexpr int kRing = 2;        // stages on their way
-constexpr uint32_t kRingBytes = kThreads * kVectors * kRing * 16;
-constexpr uint32_t kNever = 0x007FFFFFu;       // key of -inf: this and below is never selected
+constexpr int kBins = 1024;
+constexpr int kRanked = 64;            // scores that are ranked against each other
+constexpr float kLowest = -3.402823466e38f;
 
 struct Args {
   const float* scores;
@@ -55,11 +55,13 @@ struct Args {
   int* flags;
   long long stride;  // bytes between rows of scores
   int columns, sequences, slots, k, keep_first, keep_last;
-  int words;  // of the bitmap
+  int blocks;  // of a cluster
+  int words;   // of the bitmaps
 };
 
-// Scores in their order as whole numbers. (-0 is below 0 here; values are compared as floats, where
-// they are equal.)
+// Scores as they are compared: -0 is 0, NaN is -inf, which is never selected.
+__device__ __forceinline__ float score_of(float v) { return v > -INFINITY ? v + 0.f : -INFINITY; }
+// In their order as whole numbers.
 __device__ __forceinline__ uint32_t key_of(float v) {
   const uint32_t u = __float_as_uint(v);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
@@ -69,567 +71,660 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 
 struct Shared {
-  int sums[2][kWarps][2];  // block sums, two buffers taken in turn
-  int hist[kBins];
-  float2 ranked[kRanked];  // value and position (as bits)
-  int count, bin, above, inside;
-  float cut;
-  int last;
+  int2 sums[2][kThreads / 32];  // of the warps, two buffers taken in turn
+  int2 total[2];                // of the block, for the cluster's others, in turn
+  uint2 range[2];               // least and largest key of the block, in turn
+  int hist[2][kBins];           // in turn; zero when they are not in use
+  float2 own[kRanked];          // the block's scores in the one bin, and their positions (as bits)
+  float2 ranked[kRanked];       // the cluster's
+  int owned, bin, above, inside;
 };
 
-// What is selected: above `t`, and of those equal to it the ones up to position `last`.
-struct Cut {
-  float t;
-  int last;
-  __device__ bool takes(float v, int at) const { return v > t || (v == t && at <= last); }
+// The T threads of a block, and the others of its cluster.
+template <int T>
+struct Team {
+  static constexpr int kWarps = T / 32;
+  Shared& sh;
+  int blocks, rank;
+  int turn = 0, turn2 = 0;
+
+  // (The cluster's barrier is one of whole warps.)
+  __device__ static void cluster_sync() {
+    __syncwarp();
+    ptx::cluster_sync();
+  }
+  __device__ void sync() const {
+    if (blocks > 1) cluster_sync();
+    else __syncthreads();
+  }
+  // Eight bytes of another block's shared memory, at the place of `p` in this one's.
+  __device__ long long peer(const void* p, int block) const {
+    return ptx::ld_cluster_s64(ptx::map_peer(ptx::smem_addr(p), uint32_t(block)));
+  }
+  __device__ static int2 halves(long long v) { return make_int2(int(v), int(v >> 32)); }
+
+  // The sum over the cluster's blocks of a number that each has, and over the ones before this.
+  __device__ int sum(int mine, int* before) {
+    *before = 0;
+    if (blocks == 1) return mine;
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) sh.total[turn2] = make_int2(mine, 0);
+    cluster_sync();
+    const int v = lane < blocks ? halves(peer(&sh.total[turn2], lane)).x : 0;
+    turn2 ^= 1;
+    *before = __reduce_add_sync(0xFFFFFFFFu, lane < rank ? v : 0);
+    return __reduce_add_sync(0xFFFFFFFFu, v);
+  }
+  // Inclusive sum over the block's threads, and the whole; one barrier.
+  __device__ int block_scan(int v, int* all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) sh.sums[turn][warp] = make_int2(v, 0);
+    __syncthreads();
+    const int w = lane < kWarps ? sh.sums[turn][lane].x : 0;
+    turn ^= 1;
+    *all = __reduce_add_sync(0xFFFFFFFFu, w);
+    return v + __reduce_add_sync(0xFFFFFFFFu, lane < warp ? w : 0);
+  }
+  // Least and largest key over the team.
+  __device__ uint2 range(uint32_t least, uint32_t most) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    least = __reduce_min_sync(0xFFFFFFFFu, least);
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
+    if (lane == 0) sh.sums[turn][warp] = make_int2(int(least), int(most));
+    __syncthreads();
+    int2 m = sh.sums[turn][lane & (kWarps - 1)];
+    turn ^= 1;
+    least = __reduce_min_sync(0xFFFFFFFFu, uint32_t(m.x));
+    most = __reduce_max_sync(0xFFFFFFFFu, uint32_t(m.y));
+    if (blocks > 1) {
+      if (threadIdx.x == 0) sh.range[turn2] = make_uint2(least, most);
+      cluster_sync();
+      m = halves(peer(&sh.range[turn2], lane < blocks ? lane : 0));
+      turn2 ^= 1;
+      least = __reduce_min_sync(0xFFFFFFFFu, uint32_t(m.x));
+      most = __reduce_max_sync(0xFFFFFFFFu, uint32_t(m.y));
+    }
+    return make_uint2(least, most);
+  }
 };
 
-// Sums of two numbers over the block, the same in all threads. `turn` flips: one barrier a call.
-__device__ __forceinline__ int2 block_sum(Shared& sh, int x, int y, int& turn) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  x = __reduce_add_sync(0xFFFFFFFFu, x);
-  y = __reduce_add_sync(0xFFFFFFFFu, y);
-  if (lane == 0) *reinterpret_cast<int2*>(sh.sums[turn][warp]) = make_int2(x, y);
-  __syncthreads();
-  const int2 v = lane < kWarps ? *reinterpret_cast<const int2*>(sh.sums[turn][lane]) : make_int2(0, 0);
-  turn ^= 1;
-  return make_int2(__reduce_add_sync(0xFFFFFFFFu, v.x), __reduce_add_sync(0xFFFFFFFFu, v.y));
-}
-
-// What is searched: `want` of the values at x[0, count), of which those outside [lo, hi) are taken
-// anyway.
-struct Row {
+// The block's run of the scores that are searched: those at [begin, end) of a row.
+// In registers, score i of a thread at begin + i * T + threadIdx.x.
+template <int T, int N>
+struct Held {
+  int begin, end;
+  float v[N];
+  __device__ int at(int i) const { return begin + i * T + int(threadIdx.x); }
+  __device__ void load(const float* x) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = at(i) < end ? x[at(i)] : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = score_of(v[i]);
+  }
+  // fn(value, its number) for all of the thread's scores, lanes together.
+  template <typename Fn>
+  __device__ __forceinline__ void each(Fn fn) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) fn(v[i], i);
+  }
+};
+// In memory, read in each pass.
+template <int T>
+struct Read {
+  int begin, end;
   const float* x;
-  int count, lo, hi, want;
+  __device__ int at(int i) const { return begin + i * T + int(threadIdx.x); }
+  __device__ float read(int j) const { return score_of(j < end ? x[j] : -INFINITY); }
+  template <typename Fn>
+  __device__ __forceinline__ void each(Fn fn) const {
+    const int n = (end - begin + T - 1) / T;
+    int i = 0;
+#pragma unroll 1
+    for (; i + 4 <= n; i += 4) {
+      float f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = read(at(i + j));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fn(f[j], i + j);
+    }
+#pragma unroll 1
+    for (; i < n; ++i) fn(read(at(i)), i);
+  }
 };
 
-// Calls fn(values, position of the first, number) for four neighbours at a time, all values of
-// [lo, hi) once; the block's threads share them.
-template <typename Fn>
-__device__ __forceinline__ void each_four(const Row& r, Fn fn) {
-  const int head = min(r.hi - r.lo, int((16 - (reinterpret_cast<uintptr_t>(r.x + r.lo) & 15)) & 15) / 4);
-  const int body = (r.hi - r.lo - head) / 4, tail = r.hi - r.lo - head - 4 * body;
-  const int first = r.lo + head;
-  if (threadIdx.x == 0 && head) {
-    float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    v.x = r.x[r.lo];
-    if (head > 1) v.y = r.x[r.lo + 1];
-    if (head > 2) v.z = r.x[r.lo + 2];
-    fn(v, r.lo);
-  }
-  if (threadIdx.x == 32 && tail) {
-    const int at = first + 4 * body;
-    float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    v.x = r.x[at];
-    if (tail > 1) v.y = r.x[at + 1];
-    if (tail > 2) v.z = r.x[at + 2];
-    fn(v, at);
-  }
-  const float4* x = reinterpret_cast<const float4*>(r.x + first);
-  int i = threadIdx.x;
-  for (; i + 3 * kThreads < body; i += 4 * kThreads) {
-    float4 v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = x[i + j * kThreads];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) fn(v[j], first + 4 * (i + j * kThreads));
-  }
-  for (; i < body; i += kThreads) fn(x[i], first + 4 * i);
-}
-
-__device__ __forceinline__ int reach(const float4& v, float t) {
-  return (v.x >= t) + (v.y >= t) + (v.z >= t) + (v.w >= t);
-}
-
-// Inclusive sum over the block; `total` gets the whole.
-__device__ __forceinline__ int block_scan(Shared& sh, int v, int& turn, int* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
-    if (lane >= o) v += u;
-  }
-  if (lane == 31) sh.sums[turn][warp][0] = v;
-  __syncthreads();
-  const int w = lane < kWarps ? sh.sums[turn][lane][0] : 0;
-  turn ^= 1;
-  *total = __reduce_add_sync(0xFFFFFFFFu, w);
-  return v + __reduce_add_sync(0xFFFFFFFFu, lane < warp ? w : 0);
-}
-
-// The bin of a value; larger values never have lower bins. (-inf, which is no candidate, has none.)
+// Bins between the least and the largest of some values. Larger values never have lower bins.
 struct Bins {
-  float least, scale;
-  bool apart;  // the bins can tell values apart
-  __device__ int of(float v) const { return min(int((v - least) * scale), kBins - 1); }
+  uint32_t least, most;  // keys
+  float low, scale;      // by value: even widths
+  int shift;             // by key
+  __device__ explicit Bins(uint2 range) : least(range.x), most(range.y) {
+    low = value_of(least);
+    const float wide = least < most ? value_of(most) - low : 0.f;
+    scale = float(kBins) / wide;
+    if (!(wide > 0.f && scale > 0.f && scale < INFINITY)) scale = 0.f;
+    shift = max(0, 22 - __clz(int((most - least) | 1u)));
+  }
+  __device__ bool has(float v) const { return key_of(v) >= least && key_of(v) <= most; }
+  // The sum with 2^23 leaves the bin in the low bits, at the rate of an addition (a conversion has an
+  // eighth of it).
+  __device__ int by_value(float v) const {
+    return min(__float_as_int(fmaf(v - low, scale, 8388608.f)), 0x4B000000 + kBins - 1) - 0x4B000000;
+  }
+  __device__ int by_key(float v) const { return int((key_of(v) - least) >> shift); }
 };
 
-// Counts the values (-inf: none) into bins and finds the one that the `want`-th largest is in: sh.bin,
+// The bin that the `want`-th largest is in, from counts that the team has put into hist[which]: sh.bin,
 // with sh.above values in higher bins and sh.inside in it. Returns how many values there are; with
-// fewer than `want` there is no bin. sh.hist is zero before and after.
-template <int N>
-__device__ __forceinline__ int count_bins(Shared& sh, const float* v, int want, Bins* bins, int& turn) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float low = INFINITY, high = -INFINITY;
+// fewer than `want` there is no bin. Leaves the other hist zero, and ends with a barrier.
+template <int T>
+__device__ __forceinline__ int find_bin(Team<T>& team, int which, int want) {
+  constexpr int kEach = kBins / T;
+  Shared& sh = team.sh;
+  team.sync();
+  // From the highest bin down, kEach a thread.
+  const int first = kBins - kEach * (1 + int(threadIdx.x));
+  int n[kEach], mine = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    low = fminf(low, v[i] > -INFINITY ? v[i] : INFINITY);
-    high = fmaxf(high, v[i]);
+  for (int i = 0; i < kEach; i += 2) {
+    const int* at = &sh.hist[which][first + i];
+    int2 two = *reinterpret_cast<const int2*>(at);
+    if (team.blocks > 1) {
+      long long both = 0;  // (counts do not carry: 2^20 at most)
+      for (int b = 0; b < team.blocks; ++b) both += team.peer(at, b);
+      two = Team<T>::halves(both);
+    }
+    n[i] = two.x;
+    n[i + 1] = two.y;
+    mine += two.x + two.y;
+    *reinterpret_cast<int2*>(&sh.hist[which ^ 1][first + i]) = make_int2(0, 0);
   }
-  // (Without values: more than any key, and the key of -inf.)
-  uint32_t least = high > -INFINITY ? key_of(low) : 0xFFFFFFFFu, most = key_of(high);
-  least = __reduce_min_sync(0xFFFFFFFFu, least);
-  most = __reduce_max_sync(0xFFFFFFFFu, most);
-  if (lane == 0) *reinterpret_cast<int2*>(sh.sums[turn][warp]) = make_int2(int(least), int(most));
-  __syncthreads();
-  const int2 m = *reinterpret_cast<const int2*>(sh.sums[turn][lane & (kWarps - 1)]);
-  turn ^= 1;
-  least = __reduce_min_sync(0xFFFFFFFFu, uint32_t(m.x));
-  most = __reduce_max_sync(0xFFFFFFFFu, uint32_t(m.y));
-  bins->least = value_of(least);
-  const float range = value_of(most) - bins->least;
-  bins->scale = float(kBins) / range;
-  bins->apart = least < most && range > 0.f && bins->scale > 0.f && bins->scale < INFINITY;
-  if (bins->apart) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (v[i] > -INFINITY) atomicAdd(&sh.hist[bins->of(v[i])], 1);
-  } else {
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) n += v[i] > -INFINITY;
-    if (n) atomicAdd(&sh.hist[0], n);
-  }
-  __syncthreads();
-  // From the highest bin down, two a thread.
-  int2& mine = reinterpret_cast<int2*>(sh.hist)[kThreads - 1 - threadIdx.x];
-  const int2 n = mine;
-  mine = make_int2(0, 0);
   int total;
-  const int sum = block_scan(sh, n.x + n.y, turn, &total), before = sum - n.x - n.y;
-  if (before < want && want <= sum) {
-    const int top = kBins - 1 - 2 * int(threadIdx.x);
-    const bool upper = before + n.y >= want;
-    sh.bin = upper ? top : top - 1;
-    sh.above = upper ? before : before + n.y;
-    sh.inside = upper ? n.y : n.x;
+  int before = team.block_scan(mine, &total) - mine;
+  if (before < want && want <= before + mine) {
+#pragma unroll
+    for (int i = kEach - 1; i >= 0; --i) {
+      if (before < want && want <= before + n[i]) {
+        sh.bin = first + i;
+        sh.above = before;
+        sh.inside = n[i];
+      }
+      before += n[i];
+    }
   }
   __syncthreads();
   return total;
 }
 
-// By halving: the `want`-th largest of the values, more of which are above -inf, and of those equal to
-// it the last position that is still wanted. at(i) is value i's position, below `end`.
-template <int N, typename At>
-__device__ __forceinline__ Cut cut_by_halving(Shared& sh, const float* v, At at, int want, int end,
-                                              int& turn) {
-  uint32_t lo = kNever + 1, hi = 0xFF800001u;  // `want` reach lo, fewer reach hi
-  while (hi - lo > 1) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    const float t = value_of(mid);
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) n += v[i] >= t;
-    if (block_sum(sh, n, 0, turn).x >= want) lo = mid; else hi = mid;
+// Puts the block's share of the team's `want` best into its bitmap, bits from run.begin on. hist[0],
+// owned and the bitmap are zero.
+template <int T, typename R>
+__device__ __forceinline__ void mark_best(Team<T>& team, const R& run, int want, uint32_t* map) {
+  Shared& sh = team.sh;
+  constexpr int kWarps = T / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto put = [&](bool take, int i) {  // 32 neighbours a warp: a word
+    const unsigned word = __ballot_sync(0xFFFFFFFFu, take);
+    if (lane == 0 && word) map[i * kWarps + warp] |= word;
+  };
+  // The range of all values; -inf is none.
+  float low = INFINITY, high = -INFINITY;
+  run.each([&](float v, int) {
+    low = fminf(low, v > -INFINITY ? v : INFINITY);
+    high = fmaxf(high, v);
+  });
+  Bins bins(team.range(high > -INFINITY ? key_of(low) : 0xFFFFFFFFu, key_of(high)));
+  int which = 0;
+  bool by_value = bins.scale > 0.f;
+  if (by_value) {
+    run.each([&](float v, int) {
+      if (v > -INFINITY) atomicAdd(&sh.hist[0][bins.by_value(v)], 1);
+    });
+  } else {
+    run.each([&](float v, int) {
+      if (v > -INFINITY) atomicAdd(&sh.hist[0][bins.by_key(v)], 1);
+    });
   }
-  const float t = value_of(lo);
-  int n = 0, m = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    n += v[i] > t;
-    m += v[i] == t;
+  if (find_bin(team, 0, want) <= want) {  // all of them
+    run.each([&](float v, int i) { put(v > -INFINITY, i); });
+    return;
   }
-  const int2 both = block_sum(sh, n, m, turn);
-  const int need = want - both.x;
-  if (need >= both.y) return {t, INT_MAX};
-  int a = -1, b = end;  // positions <= a hold fewer than `need` of the equal ones, <= b enough
-  while (b - a > 1) {
-    const int mid = a + (b - a) / 2;
-    int c = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) c += v[i] == t && at(i) <= mid;
-    if (block_sum(sh, c, 0, turn).x >= need) b = mid; else a = mid;
-  }
-  return {t, b};
-}
-
-// The cut that takes the `want` largest of the values (-inf: none), or all if they are no more.
-template <int N, typename At>
-__device__ __forceinline__ Cut best_cut(Shared& sh, const float* v, At at, int want, int end, int& turn) {
-  Bins bins;
-  if (count_bins<N>(sh, v, want, &bins, turn) <= want) return {-INFINITY, -1};
-  const int bin = sh.bin, inside = sh.inside, need = want - sh.above;
-  if (!bins.apart || inside > kRanked) return cut_by_halving<N>(sh, v, at, want, end, turn);
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (v[i] > -INFINITY && bins.of(v[i]) == bin)
-      sh.ranked[atomicAdd(&sh.count, 1)] = make_float2(v[i], __int_as_float(at(i)));
-  __syncthreads();
-  // Rank `need` of them, counted from the largest; equal ones from the lowest position. Eight
-  // threads compare one with an eighth of them each.
-  const int c = threadIdx.x >> 3;
-  const float2 mine = sh.ranked[c];
-  int rank = 0;
-  if (c < inside)
-    for (int j = threadIdx.x & 7; j < inside; j += 8) {
-      const float2 x = sh.ranked[j];
-      rank += x.x > mine.x || (x.x == mine.x && __float_as_int(x.y) < __float_as_int(mine.y));
-    }
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, o);
-  if (c < inside && (threadIdx.x & 7) == 0 && rank == need - 1) {
-    sh.cut = mine.x;
-    sh.last = __float_as_int(mine.y);
-    sh.count = 0;
-  }
-  __syncthreads();
-  return {sh.cut, sh.last};
-}
-
-// A threshold that about `rank` of the sampled values reach.
-template <int N>
-__device__ __forceinline__ float sample_threshold(Shared& sh, const float* v, int rank, int& turn) {
-  Bins bins;
-  if (count_bins<N>(sh, v, rank, &bins, turn) <= rank) return -3.402823466e38f;
-  if (bins.apart && sh.inside <= rank / 8 + 1) return bins.least + float(sh.bin) / bins.scale;
-  return cut_by_halving<N>(sh, v, [](int) { return 0; }, rank, 0, turn).t;
-}
-
-__device__ __forceinline__ void mark(uint32_t* map, int i) { atomicOr(&map[i >> 5], 1u << (i & 31)); }
-
-// 16-byte vectors of global memory, each read by the lane that asked for it: kRing stages of kVectors a
-// lane are on their way while one is worked on, without a register for them and without a barrier.
-struct Stream {
-  const float4* x;
-  int vectors;
-  uint32_t ring;  // this thread's first vector of the ring
-  __device__ Stream(const float* from, int n, float4* buffer)
-      : x(reinterpret_cast<const float4*>(reinterpret_cast<uintptr_t>(from) & ~uintptr_t(15))),
-        vectors(n),
-        ring(ptx::smem_addr(buffer + threadIdx.x)) {}
-  // Vector j of stage k; a warp's are neighbours.
-  __device__ int index(int k, int j) const {
-    return (k * kWarps + int(threadIdx.x >> 5)) * 32 * kVectors + 32 * j + int(threadIdx.x & 31);
-  }
-  __device__ void ask(int k) {
-#pragma unroll
-    for (int j = 0; j < kVectors; ++j) {
-      const int i = index(k, j);
-      const uint32_t to = ring + uint32_t(((k % kRing) * kVectors + j) * kThreads * 16);
-      ptx::cp_async_16(to, i < vectors ? x + i : x, i < vectors ? 16 : 0);
-    }
-    ptx::cp_async_commit();
-  }
-  __device__ void start() {
-#pragma unroll
-    for (int k = 0; k < kRing; ++k) ask(k);
-  }
-  // fn(values, index) for each of the warp's vectors in stages, lanes together; those past the end are
-  // -inf.
-  template <typename Fn>
-  __device__ void run(Fn fn) {
-    const int stages = (vectors + kThreads * kVectors - 1) / (kThreads * kVectors);
-#pragma unroll 1
-    for (int k = 0; k < stages; ++k) {
-      ptx::cp_async_wait_group<kRing - 1>();
-      float4 v[kVectors];
-#pragma unroll
-      for (int j = 0; j < kVectors; ++j) {
-        const uint32_t from = ring + uint32_t(((k % kRing) * kVectors + j) * kThreads * 16);
-        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(v[j].x), "=f"(v[j].y), "=f"(v[j].z), "=f"(v[j].w) : "r"(from) : "memory");
-        if (index(k, j) >= vectors) v[j] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  int need = want;
+  for (;;) {
+    need -= sh.above;
+    if (sh.inside <= kRanked || bins.least == bins.most) break;
+    // Too many to rank: their own range and bins.
+    const int bin = sh.bin;
+    uint32_t least = 0xFFFFFFFFu, most = 0;
+    run.each([&](float v, int) {
+      if (v > -INFINITY && bins.has(v) && (by_value ? bins.by_value(v) : bins.by_key(v)) == bin) {
+        least = min(least, key_of(v));
+        most = max(most, key_of(v));
       }
-      fn(v, k);
-      ask(k + kRing);
+    });
+    bins = Bins(team.range(least, most));
+    by_value = false;
+    which ^= 1;
+    run.each([&](float v, int) {
+      if (bins.has(v)) atomicAdd(&sh.hist[which][bins.by_key(v)], 1);
+    });
+    find_bin(team, which, need);
+  }
+  const int bin = sh.bin, inside = sh.inside;
+  if (inside > kRanked) {
+    // All equal: of these the first `need`, and then what is above them.
+    run.each([&](float v, int i) { put(bins.has(v), i); });
+    __syncthreads();
+    const int words = (run.end - run.begin + 31) / 32, per = (words + T - 1) / T;
+    const int w0 = min(words, int(threadIdx.x) * per), w1 = min(words, w0 + per);
+    int mine = 0, block, lower;
+    for (int w = w0; w < w1; ++w) mine += __popc(map[w]);
+    int place = team.block_scan(mine, &block) - mine;
+    team.sum(block, &lower);
+    place += lower;
+    for (int w = w0; w < w1; ++w) {
+      uint32_t take = 0;
+      for (uint32_t left = map[w]; left && place < need; left &= left - 1, ++place) take |= left & -left;
+      map[w] = take;
     }
-    ptx::cp_async_wait_all();
+    __syncthreads();
+    run.each([&](float v, int i) { put(v > -INFINITY && key_of(v) > bins.most, i); });
+    return;
+  }
+  // All above the bin, and those in it by rank: eight threads compare one with an eighth of them each.
+  run.each([&](float v, int i) {
+    bool above = false;
+    if (v > -INFINITY) {
+      int b = bin + (key_of(v) > bins.most);
+      if (bins.has(v)) b = by_value ? bins.by_value(v) : bins.by_key(v);
+      else if (key_of(v) < bins.least) b = -1;
+      above = b > bin;
+      if (b == bin) sh.own[atomicAdd(&sh.owned, 1)] = make_float2(v, __int_as_float(run.at(i)));
+    }
+    put(above, i);
+  });
+  team.sync();
+  for (int c0 = 0; c0 < inside; c0 += T / 8) {
+    const int c = c0 + (threadIdx.x >> 3);
+    float2 it = make_float2(-INFINITY, 0.f);
+    const float2* all = sh.own;
+    if (team.blocks > 1) {  // (T / 8 is kRanked: once)
+      if (c < inside) {
+        int left = c, b = 0;
+        for (; b < team.blocks - 1; ++b) {
+          const int count = int(ptx::ld_cluster_u32(ptx::map_peer(ptx::smem_addr(&sh.owned), uint32_t(b))));
+          if (left < count) break;
+          left -= count;
+        }
+        const int2 two = Team<T>::halves(team.peer(&sh.own[left], b));
+        it = make_float2(__int_as_float(two.x), __int_as_float(two.y));
+        if ((threadIdx.x & 7) == 0) sh.ranked[c] = it;
+      }
+      all = sh.ranked;
+      __syncthreads();
+    } else if (c < inside) {
+      it = sh.own[c];
+    }
+    int rank = 0;
+    if (c < inside)
+      for (int j = threadIdx.x & 7; j < inside; j += 8) {
+        const float2 x = all[j];
+        rank += x.x > it.x || (x.x == it.x && __float_as_int(x.y) < __float_as_int(it.y));
+      }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, o);
+    // A block marks what is its own.
+    const int at = __float_as_int(it.y) - run.begin;
+    if (c < inside && (threadIdx.x & 7) == 0 && rank < need && at >= 0 && at < run.end - run.begin)
+      atomicOr(&map[at >> 5], 1u << (at & 31));
+  }
+}
+
+// Lists the positions of a bitmap's bits, in order, from to[0] on: each thread numbers a run of its 16
+// bits. Returns how many; the list is there after the next barrier.
+template <int T, typename Fn>
+__device__ __forceinline__ int list_bits(Team<T>& team, const uint32_t* map, int bits, Fn put) {
+  const int units = (bits + 15) / 16, per = (units + T - 1) / T;
+  const int u0 = min(units, int(threadIdx.x) * per), u1 = min(units, u0 + per);
+  const uint16_t* half = reinterpret_cast<const uint16_t*>(map);
+  int mine = 0, total;
+  for (int u = u0; u < u1; ++u) mine += __popc(uint32_t(half[u]));
+  int at = team.block_scan(mine, &total) - mine;
+  for (int u = u0; u < u1; ++u)
+    for (uint32_t b = half[u]; b; b &= b - 1) put(at++, 16 * u + __ffs(b) - 1);
+  return total;
+}
+
+// The largest score of each of the pages [p0, p1) of a row, 16 lanes a page; NaN does not count.
+__device__ __forceinline__ void page_maxima(const float* scores, int seen, int p0, int p1, float* best) {
+  constexpr int kWarps = kThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto largest = [](const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); };
+  auto either = [&](float x, float y, int bit) {  // this lane's part of x or y, with its partner's
+    const bool b = lane & bit;
+    return fmaxf(b ? y : x, __shfl_xor_sync(0xFFFFFFFFu, b ? x : y, bit));
+  };
+  const bool aligned = (reinterpret_cast<uintptr_t>(scores) & 15) == 0;
+  // Eight pages a half warp, all on their way at once: the exchanges leave each lane two of the eight.
+  constexpr int kBatch = 8;
+  for (int p = p0 + 2 * kBatch * warp; p < p1; p += 2 * kBatch * kWarps) {
+    float4 v[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int at = (p + 2 * j + (lane >> 4)) * kPageRows + 4 * (lane & 15);
+      v[j] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (aligned && at + 4 <= seen) {
+        v[j] = *reinterpret_cast<const float4*>(scores + at);
+      } else {
+        if (at < seen) v[j].x = scores[at];
+        if (at + 1 < seen) v[j].y = scores[at + 1];
+        if (at + 2 < seen) v[j].z = scores[at + 2];
+        if (at + 3 < seen) v[j].w = scores[at + 3];
+      }
+    }
+    float m[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) m[j] = largest(v[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m[j] = either(m[j], m[j + 4], 8);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) m[j] = either(m[j], m[j + 2], 4);
+    m[0] = either(m[0], m[1], 2);
+    m[0] = fmaxf(m[0], __shfl_xor_sync(0xFFFFFFFFu, m[0], 1));
+    const int j = ((lane & 8) >> 1) | ((lane & 4) >> 1) | ((lane & 2) >> 1);
+    const int page = p + 2 * j + (lane >> 4);
+    if ((lane & 1) == 0 && page < p1) best[page - p0] = m[0];
+  }
+}
+
+// The rows that token t sees, and where its scores are.
+struct Token {
+  const float* scores;
+  int seq, seen;
+  template <bool kPages>
+  __device__ static Token of(const Args& a, int t, bool tell) {
+    Token k;
+    k.scores = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.scores) + t * a.stride);
+    k.seq = a.seq_id[t];
+    k.seen = 0;
+    const int pos = a.q_pos[t];
+    int bad = 0;
+    if (k.seq < 0 || k.seq >= a.sequences) {
+      bad = TQ_DEV_SEQ_RANGE;
+    } else {
+      long long n = min((long long)a.kv_len[k.seq], (long long)pos + 1);
+      if (kPages) {
+        if (n > (long long)a.slots * kPageRows) bad |= TQ_DEV_TABLE_SHORT;
+        n = min(n, (long long)a.slots * kPageRows);
+      }
+      if (n > a.columns) bad |= TQ_DEV_WORK_OVERFLOW;
+      k.seen = int(max(0ll, min(n, (long long)a.columns)));
+    }
+    if (bad && tell && a.flags) atomicOr(a.flags, bad);
+    return k;
   }
 };
 
-// Keeps the scores of a row that reach `t`; returns how many do (kCandidates of them are kept).
-// `stream` has been started on the row's aligned part.
-__device__ __forceinline__ int collect(Shared& sh, const Row& r, float t, float2* cand, Stream& stream,
-                                       int first) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // One run of places in the list for a warp's; their order does not matter.
-  auto keep = [&](const float4* v, auto position) {
-    auto part = [&](int i) {
-      const float4& f = v[i / 4];
-      return i % 4 == 0 ? f.x : i % 4 == 1 ? f.y : i % 4 == 2 ? f.z : f.w;
-    };
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < 4 * kVectors; ++i) n += part(i) >= t;
-    int sum = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xFFFFFFFFu, sum, o);
-      if (lane >= o) sum += u;
-    }
-    int to = 0;
-    if (lane == 31 && sum) to = atomicAdd(&sh.count, sum);
-    to = __shfl_sync(0xFFFFFFFFu, to, 31) + sum - n;
-    if (n == 0 || to + n > kCandidates) return;  // (too many: they are counted only)
-#pragma unroll
-    for (int i = 0; i < 4 * kVectors; ++i)
-      if (part(i) >= t) cand[to++] = make_float2(part(i), __int_as_float(position(i / 4) + i % 4));
-  };
-  stream.run([&](const float4* v, int k) {
-    keep(v, [&](int j) { return first + 4 * stream.index(k, j); });
-  });
-  if (warp == 0) {  // up to three values before the aligned ones, up to three behind them
-    const int head = first - r.lo, behind = first + 4 * stream.vectors, tail = r.hi - behind;
-    const int i = lane < head ? r.lo + lane : behind + lane - head;
-    const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    float4 v[kVectors];
-#pragma unroll
-    for (int j = 0; j < kVectors; ++j) v[j] = none;
-    if (lane < head + tail) v[0].x = r.x[i];
-    keep(v, [&](int) { return i; });
+// What a token keeps anyway, [0, lo) and [hi, count), and how many of those between it may have.
+struct Kept {
+  int count, lo, hi, want;
+  __device__ Kept(const Args& a, int n) : count(n) {
+    lo = min(a.keep_first, count);
+    hi = max(lo, count - a.keep_last);
+    want = a.k - lo - (count - hi);
   }
-  __syncthreads();
-  const int count = sh.count;
-  __syncthreads();
-  if (threadIdx.x == 0) sh.count = 0;
-  return count;
-}
-
-// The same over the whole row, for what the candidates do not hold.
-__device__ __forceinline__ void mark_best_of_all(Shared& sh, const Row& r, float guess, uint32_t* map,
-                                                 int& turn) {
-  // The largest key that `want` values reach, if that many are above -inf; else the lowest.
-  uint32_t lo = kNever + 1, hi = 0xFF800001u, key = lo;
-  float t = value_of(lo);
-  int need = 0;
-  for (int round = 0;; ++round) {
-    const float x = value_of(key);
-    int n = 0, m = 0;
-    each_four(r, [&](const float4& v, int) {
-      m += reach(v, x);
-      n += (v.x > x) + (v.y > x) + (v.z > x) + (v.w > x);
-    });
-    const int2 both = block_sum(sh, n, m, turn);
-    if (round == 0 || both.y >= r.want) {
-      lo = key;
-      t = x;
-      need = r.want - both.x;
-      if (need > 0) break;  // what equals t is enough, or all that there is
-    } else {
-      hi = key;
-    }
-    if (hi - lo <= 1) break;
-    key = lo + (hi - lo) / 2;
-    if (round == 0 && key_of(guess) > lo && key_of(guess) < hi) key = key_of(guess);
-  }
-  // In order, one position a thread at a time.
-  for (int i0 = r.lo; i0 < r.hi; i0 += kThreads) {
-    const int i = i0 + int(threadIdx.x), lane = threadIdx.x & 31;
-    const float v = i < r.hi ? r.x[i] : -INFINITY;
-    const bool tie = v == t && v > -INFINITY;
-    const unsigned ties = __ballot_sync(0xFFFFFFFFu, tie);
-    if (lane == 0) sh.sums[turn][threadIdx.x >> 5][0] = __popc(ties);
-    __syncthreads();
-    int before = __popc(ties & ((1u << lane) - 1)), all = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      const int c = sh.sums[turn][w][0];
-      if (w < int(threadIdx.x >> 5)) before += c;
-      all += c;
-    }
-    turn ^= 1;
-    if (v > t || (tie && before < need)) mark(map, i);
-    need -= min(need, all);
-  }
-}
-
-// Marks the best of a row of at most N * kThreads scores, held in registers.
-template <int N>
-__device__ __forceinline__ void mark_direct(Shared& sh, const Row& r, uint32_t* map, int& turn) {
-  // Value i of a thread is at r.lo + i * kThreads + threadIdx.x: 32 neighbours a warp, so a ballot is 32
-  // bits of the answer (of the row from r.lo on, which need not begin a word).
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = r.hi - r.lo;
-  float v[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int j = i * kThreads + int(threadIdx.x);
-    v[i] = j < n ? r.x[r.lo + j] : -INFINITY;
-    if (!(v[i] > -INFINITY)) v[i] = -INFINITY;  // no NaN
-  }
-  auto at = [&](int i) { return r.lo + i * kThreads + int(threadIdx.x); };
-  const Cut cut = best_cut<N>(sh, v, at, r.want, r.hi, turn);
-  unsigned bits = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const unsigned taken = __ballot_sync(0xFFFFFFFFu, cut.takes(v[i], at(i)));
-    if (lane == i) bits = taken;
-  }
-  if (bits) {  // lane i's are value i's
-    const int j = r.lo + lane * kThreads + 32 * warp, shift = j & 31;
-    atomicOr(&map[j >> 5], bits << shift);
-    if (shift && bits >> (32 - shift)) atomicOr(&map[(j >> 5) + 1], bits >> (32 - shift));
-  }
-}
+};
 
 template <bool kPages>
-__global__ void __launch_bounds__(kThreads, 2) index_select_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 2) hold_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t raw[];
-  float2* cand = reinterpret_cast<float2*>(raw);
-  float4* ring = reinterpret_cast<float4*>(cand + kCandidates);
-  uint32_t* map = reinterpret_cast<uint32_t*>(ring + kRingBytes / 16);
-  float* page_best = reinterpret_cast<float*>(map + a.words);
+  int* list = reinterpret_cast<int*>(raw);
+  uint32_t* map = reinterpret_cast<uint32_t*>(list + (a.k + 3) / 4 * 4);
+  float* best = reinterpret_cast<float*>(map + a.words);
   __shared__ Shared sh;
-  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int turn = 0;
+  const int tid = threadIdx.x, t = int(blockIdx.x) / a.blocks;
+  Team<kThreads> team{sh, a.blocks, int(blockIdx.x) % a.blocks};
   for (int i = tid; i < a.words; i += kThreads) map[i] = 0;
-  reinterpret_cast<int2*>(sh.hist)[tid] = make_int2(0, 0);
-  if (tid == 0) sh.count = 0;
+  for (int i = tid; i < kBins; i += kThreads) sh.hist[0][i] = 0;
+  if (tid == 0) sh.owned = 0;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const float* scores = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.scores) + t * a.stride);
-  const int s = a.seq_id[t], pos = a.q_pos[t];
-  int bad = 0, seen = 0;
-  if (s < 0 || s >= a.sequences) {
-    bad = TQ_DEV_SEQ_RANGE;
-  } else {
-    long long n = min((long long)a.kv_len[s], (long long)pos + 1);
+  const Token token = Token::of<kPages>(a, t, tid == 0 && team.rank == 0);
+  const Kept kept(a, kPages ? (token.seen + kPageRows - 1) / kPageRows : token.seen);
+  // An even run of what is searched for each block.
+  const int n = kept.want > 0 ? kept.hi - kept.lo : 0, each = (n + a.blocks - 1) / a.blocks;
+  Held<kThreads, kN> run;
+  run.begin = kept.lo + min(n, team.rank * each);
+  run.end = kept.lo + min(n, (team.rank + 1) * each);
+  if (n > 0) {
+    const float* x = token.scores;
     if (kPages) {
-      if (n > (long long)a.slots * kPageRows) bad |= TQ_DEV_TABLE_SHORT;
-      n = min(n, (long long)a.slots * kPageRows);
+      page_maxima(token.scores, token.seen, run.begin, run.end, best);
+      x = best - run.begin;
     }
-    if (n > a.columns) bad |= TQ_DEV_WORK_OVERFLOW;
-    seen = int(max(0ll, min(n, (long long)a.columns)));
-  }
-  if (bad && tid == 0 && a.flags) atomicOr(a.flags, bad);
-  Row r;
-  r.x = scores;
-  r.count = seen;
-  if (kPages) {
-    // The largest score of each page, 16 lanes a page; NaN does not count.
-    r.x = page_best;
-    r.count = (seen + kPageRows - 1) / kPageRows;
-    auto largest = [](const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); };
-    auto either = [&](float x, float y, int bit) {  // this lane's part of x or y, with its partner's
-      const bool b = lane & bit;
-      return fmaxf(b ? y : x, __shfl_xor_sync(0xFFFFFFFFu, b ? x : y, bit));
-    };
-    // Whole pages of an aligned row are streamed, four a half warp: the exchanges leave each lane one
-    // of the four. What is left is read as it is.
-    static_assert(kVectors == 4, "four pages a half warp");
-    const bool aligned = (reinterpret_cast<uintptr_t>(scores) & 15) == 0;
-    const int whole = aligned ? seen / kPageRows : 0;
-    Stream stream(scores, whole * (kPageRows / 4), ring);
-    stream.start();
-    stream.run([&](const float4* v, int k) {
-      float m = either(either(largest(v[0]), largest(v[2]), 8), either(largest(v[1]), largest(v[3]), 8), 4);
-      m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-      m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-      const int p = stream.index(k, 2 * ((lane >> 3) & 1) + ((lane >> 2) & 1)) / (kPageRows / 4);
-      if ((lane & 3) == 0 && p < whole) page_best[p] = m;
-    });
-    for (int p0 = whole + 2 * warp; p0 < r.count; p0 += 2 * kWarps) {
-      const int p = p0 + (lane >> 4), at = p * kPageRows + 4 * (lane & 15);
-      float m = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (at + i < seen) m = fmaxf(m, scores[at + i]);
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-      if ((lane & 15) == 0 && p < r.count) page_best[p] = m;
-    }
+    __syncthreads();
+    run.load(x);
+    mark_best(team, run, kept.want, map);
   }
   __syncthreads();
-  // What is kept anyway is marked, and the rest is searched.
-  r.lo = min(a.keep_first, r.count);
-  r.hi = max(r.lo, r.count - a.keep_last);
-  r.want = a.k - r.lo - (r.count - r.hi);
-  for (int i = tid; i < r.lo; i += kThreads) mark(map, i);
-  for (int i = r.hi + tid; i < r.count; i += kThreads) mark(map, i);
-  const int n = r.hi - r.lo;
-  const float lowest = -3.402823466e38f;
-  if (n > 0 && r.want > 0) {
-    if (n <= kDirect / 4) {
-      mark_direct<kDirect / kThreads / 4>(sh, r, map, turn);
-    } else if (n <= kDirect) {
-      mark_direct<kDirect / kThreads>(sh, r, map, turn);
-    } else if (kPages) {  // more pages than registers hold, already in shared memory
-      mark_best_of_all(sh, r, lowest, map, turn);
-    } else {
-      // The stream is asked for first; it arrives while the sample is read and counted.
-      const int head = int((16 - (reinterpret_cast<uintptr_t>(r.x + r.lo) & 15)) & 15) / 4;
-      const int first = r.lo + head;
-      Stream stream(r.x + first, (r.hi - first) / 4, ring);
-      stream.start();
-      // Sampled in runs of sixteen neighbours (two a warp's load), evenly over the row.
-      float x[kMaxSample];
-      const int rounds = n > 65536 ? kMaxSample / kSample : 1;
-#pragma unroll
-      for (int j = 0; j < kMaxSample; ++j) {
-        x[j] = -INFINITY;
-        if (j < rounds * kSample) {
-          const int run = j * 2 * kWarps + (tid >> 4);
-          const int from = int((long long)run * (n - 16) / (rounds * kSample * 2 * kWarps));
-          const float v = r.x[r.lo + from + (tid & 15)];
-          x[j] = v >= lowest ? v : -INFINITY;
-        }
-      }
-      const float sampled = float(rounds * kThreads * kSample), share = sampled / float(n);
-      const float expect = float(r.want) * share;
-      float rank = expect + 6.f * sqrtf(expect) + 16.f, t0 = lowest;
-      rank = fmaxf(fminf(rank, 0.8f * float(kCandidates) * share), expect + 1.f);
-      bool found = false;
-      for (int attempt = 0; attempt < 3 && !found; ++attempt) {
-        t0 = rank >= sampled ? lowest
-             : rounds > 1    ? sample_threshold<kMaxSample>(sh, x, int(rank), turn)
-                             : sample_threshold<kSample>(sh, x, int(rank), turn);
-        if (attempt) stream.start();
-        const int count = collect(sh, r, t0, cand, stream, first);
-        if (count <= kCandidates && (count >= r.want || t0 == lowest)) {
-          found = true;
-          constexpr int kHeld = (kCandidates + kThreads - 1) / kThreads;
-          float v[kHeld];
-          int place[kHeld];
-#pragma unroll
-          for (int i = 0; i < kHeld; ++i) {
-            const int j = i * kThreads + tid;
-            const float2 c = j < count ? cand[j] : make_float2(-INFINITY, 0.f);
-            v[i] = c.x;
-            place[i] = __float_as_int(c.y);
-          }
-          const Cut cut = best_cut<kHeld>(sh, v, [&](int i) { return place[i]; }, r.want, r.hi, turn);
-#pragma unroll
-          for (int i = 0; i < kHeld; ++i)
-            if (cut.takes(v[i], place[i])) mark(map, place[i]);
-        } else if (count < r.want) {
-          rank *= 1.5f * float(r.want) / float(max(count, r.want / 8 + 1));
-        } else {
-          rank *= 0.75f * float(kCandidates) / float(count);
-          if (rank < expect) break;
-        }
-      }
-      if (!found) mark_best_of_all(sh, r, t0, map, turn);
-    }
-  }
+  int before;
+  const int block = list_bits(team, map, run.end - run.begin,
+                              [&](int i, int bit) { list[i] = run.begin + bit; });
+  const int taken = team.sum(block, &before);
   __syncthreads();
-  // The bitmap in order: each thread numbers a run of its words.
-  int* out = reinterpret_cast<int*>(cand);  // candidates are no longer needed
-  const int words = (r.count + 31) / 32, each = (words + kThreads - 1) / kThreads;
-  const int w0 = min(words, tid * each), w1 = min(words, w0 + each);
-  int mine = 0, taken;
-  for (int w = w0; w < w1; ++w) mine += __popc(map[w]);
-  int at = block_scan(sh, mine, turn, &taken) - mine;
-  for (int w = w0; w < w1; ++w)
-    for (uint32_t bits = map[w]; bits; bits &= bits - 1) out[at++] = 32 * w + __ffs(bits) - 1;
-  __syncthreads();
+  const int* table = kPages ? a.page_table + (long long)max(token.seq, 0) * a.slots : nullptr;
   int* idx = a.idx + (long long)t * a.k;
-  for (int i = tid; i < a.k; i += kThreads) {
-    int v = i < taken ? out[i] : -1;
-    if (kPages && v >= 0) v = a.page_table[(long long)s * a.slots + v];
-    idx[i] = v;
+  auto answer = [&](int i, int v) { idx[i] = kPages ? table[v] : v; };
+  for (int i = tid; i < block; i += kThreads) answer(kept.lo + before + i, list[i]);
+  // What is kept, and -1 behind the last.
+  const int behind = kept.count - kept.hi, all = kept.lo + taken + behind;
+  const int first = team.rank * kThreads + tid, step = a.blocks * kThreads;
+  for (int i = first; i < kept.lo; i += step) answer(i, i);
+  for (int i = first; i < behind; i += step) answer(kept.lo + taken + i, kept.hi + i);
+  for (int i = all + first; i < a.k; i += step) idx[i] = -1;
+  // The block that has the last page of those searched knows whether it is taken.
+  const bool last_kept = behind > 0 || kept.count == kept.lo;
+  const bool mine = n == 0 || last_kept ? team.rank == 0 : run.end == kept.hi && run.begin < run.end;
+  if (tid == 0 && mine) {
+    const int bit = kept.hi - 1 - run.begin;
+    const bool ends = last_kept || (n > 0 && (map[bit >> 5] >> (bit & 31) & 1));
+    a.len[t] = !kPages ? all : all * kPageRows - (ends ? kept.count * kPageRows - token.seen : 0);
   }
-  if (tid == 0) {
-    const bool ends = taken > 0 && out[taken - 1] == r.count - 1;
-    a.len[t] = kPages ? taken * kPageRows - (ends ? r.count * kPageRows - seen : 0) : taken;
+  if (a.blocks > 1) Team<kThreads>::cluster_sync();  // nobody reads this block's memory any more
+}
+
+// ------------------------------------------------------------------------------ stream
+
+// Bits 4 i of the result are bits i of the low byte.
+__device__ __forceinline__ uint32_t spread(uint32_t x) {
+  x &= 0xFFu;
+  x = (x | x << 12) & 0x000F000Fu;
+  x = (x | x << 6) & 0x03030303u;
+  return (x | x << 3) & 0x11111111u;
+}
+
+// A bitmap of the scores x[lo, hi) that reach `t` > -inf, from position `base` on (a multiple of 16 bytes
+// at or before lo), and how many they are. Vectors of four are read; those that reach over an end, one
+// score at a time.
+__device__ __forceinline__ int map_reach(Team<kStreamThreads>& team, const float* x, int base, int lo, int hi,
+                                         float t, uint32_t* map) {
+  constexpr int kWarps = kStreamThreads / 32, kVectors = 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int vectors = (hi - base + 3) >> 2, whole0 = lo > base, whole1 = (hi - base) >> 2;
+#pragma unroll 1
+  for (int g0 = warp * kVectors; 32 * g0 < vectors; g0 += kWarps * kVectors) {
+    float4 v[kVectors];
+#pragma unroll
+    for (int j = 0; j < kVectors; ++j) {
+      const int i = 32 * (g0 + j) + lane, at = base + 4 * i;
+      if (i >= whole0 && i < whole1) {
+        v[j] = *reinterpret_cast<const float4*>(x + at);
+      } else {
+        v[j].x = at >= lo && at < hi ? x[at] : -INFINITY;
+        v[j].y = at + 1 >= lo && at + 1 < hi ? x[at + 1] : -INFINITY;
+        v[j].z = at + 2 >= lo && at + 2 < hi ? x[at + 2] : -INFINITY;
+        v[j].w = at + 3 >= lo && at + 3 < hi ? x[at + 3] : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kVectors; ++j) {
+      // Four ballots: word c has lane l's score c. Lanes 0 to 3 write one each.
+      const unsigned b0 = __ballot_sync(0xFFFFFFFFu, v[j].x >= t), b1 = __ballot_sync(0xFFFFFFFFu, v[j].y >= t);
+      const unsigned b2 = __ballot_sync(0xFFFFFFFFu, v[j].z >= t), b3 = __ballot_sync(0xFFFFFFFFu, v[j].w >= t);
+      if (lane < 4 && 32 * (g0 + j) < vectors)
+        map[4 * (g0 + j) + lane] = lane == 0 ? b0 : lane == 1 ? b1 : lane == 2 ? b2 : b3;
+    }
   }
+  __syncthreads();
+  // Each group of four words into the order of positions.
+  int n = 0;
+  for (int g = threadIdx.x; g < (vectors + 31) / 32; g += kStreamThreads) {
+    uint4& w = reinterpret_cast<uint4*>(map)[g];
+    const uint4 b = w;
+    n += __popc(b.x) + __popc(b.y) + __popc(b.z) + __popc(b.w);
+    auto part = [&](int s) {
+      return spread(b.x >> s) | spread(b.y >> s) << 1 | spread(b.z >> s) << 2 | spread(b.w >> s) << 3;
+    };
+    w = make_uint4(part(0), part(8), part(16), part(24));
+  }
+  int total;
+  team.block_scan(n, &total);  // (its barrier: the words are there)
+  return total;
+}
+
+__global__ void __launch_bounds__(kStreamThreads, 5) stream_kernel(const Args a) {
+  constexpr int kWarps = kStreamThreads / 32;
+  extern __shared__ __align__(16) uint8_t raw[];
+  int* place = reinterpret_cast<int*>(raw);                        // candidates: positions
+  float* value = reinterpret_cast<float*>(place + kCandidates);    // and scores
+  uint32_t* map = reinterpret_cast<uint32_t*>(value + kCandidates);
+  __shared__ Shared sh;
+  __shared__ uint32_t chosen[kCandidates / 32];                  // bitmap of the candidates
+  const int tid = threadIdx.x, t = blockIdx.x;
+  Team<kStreamThreads> team{sh, 1, 0};
+  for (int i = tid; i < kBins; i += kStreamThreads) sh.hist[0][i] = 0;
+  for (int i = tid; i < kCandidates / 32; i += kStreamThreads) chosen[i] = 0;
+  if (tid == 0) sh.owned = 0;
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  const Token token = Token::of<false>(a, t, tid == 0);
+  const Kept kept(a, token.seen);
+  const float* x = token.scores;
+  int* idx = a.idx + (long long)t * a.k;
+  const int n = kept.want > 0 ? kept.hi - kept.lo : 0;
+  int count = 0;         // candidates
+  bool listed = false;   // they are all that is needed
+  if (n > 0) {
+    const int base = kept.lo - int(reinterpret_cast<uintptr_t>(x + kept.lo) & 15) / 4;
+    float t0 = kLowest, sampled = float(kSample * kStreamThreads), share = sampled / float(n);
+    const float expect = float(kept.want) * share;
+    float rank = fminf(expect + 6.f * sqrtf(expect) + 16.f, 0.8f * float(kCandidates) * share);
+    rank = fmaxf(rank, expect + 1.f);
+    float s[kSample];
+    if (n > kCandidates) {
+      // In runs of sixteen neighbours (two a warp's load), evenly over the row.
+#pragma unroll
+      for (int j = 0; j < kSample; ++j) {
+        const int r = j * 2 * kWarps + (tid >> 4);
+        s[j] = x[kept.lo + int((long long)r * (n - 16) / (kSample * 2 * kWarps)) + (tid & 15)];
+      }
+#pragma unroll
+      for (int j = 0; j < kSample; ++j) s[j] = score_of(s[j]);
+    }
+    for (int attempt = 0; attempt < 3; ++attempt) {
+      if (n > kCandidates && rank < sampled) {
+        // About `rank` of the sample reach the low edge of the bin that the rank-th largest is in.
+        float low = INFINITY, high = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kSample; ++j) {
+          low = fminf(low, s[j] > -INFINITY ? s[j] : INFINITY);
+          high = fmaxf(high, s[j]);
+        }
+        const Bins bins(team.range(high > -INFINITY ? key_of(low) : 0xFFFFFFFFu, key_of(high)));
+        const int which = attempt & 1;
+#pragma unroll
+        for (int j = 0; j < kSample; ++j)
+          if (s[j] > -INFINITY)
+            atomicAdd(&sh.hist[which][bins.scale > 0.f ? bins.by_value(s[j]) : bins.by_key(s[j])], 1);
+        t0 = kLowest;
+        if (find_bin(team, which, int(rank)) > int(rank))
+          t0 = bins.scale > 0.f ? bins.low + (float(sh.bin) - 0.5f) / bins.scale
+                                : value_of(bins.least + (uint32_t(sh.bin) << bins.shift));
+        if (!(t0 >= kLowest)) t0 = kLowest;
+      } else {
+        t0 = kLowest;
+      }
+      __syncthreads();
+      for (int i = tid; i < kBins; i += kStreamThreads) sh.hist[0][i] = sh.hist[1][i] = 0;
+      count = map_reach(team, x, base, kept.lo, kept.hi, t0, map);
+      if (count <= kCandidates && (count >= kept.want || t0 == kLowest)) {
+        listed = true;
+        break;
+      }
+      if (count < kept.want) {
+        rank *= 1.5f * float(kept.want) / float(max(count, kept.want / 8 + 1));
+      } else {
+        rank *= 0.75f * float(kCandidates) / float(count);
+        if (rank < expect) break;
+      }
+    }
+    if (listed) {
+      list_bits(team, map, kept.hi - base, [&](int i, int bit) { place[i] = base + bit; });
+      __syncthreads();
+      for (int i = tid; i < count; i += kStreamThreads) value[i] = x[place[i]];
+      __syncthreads();
+      const Read<kStreamThreads> run = {0, count, value};
+      if (count > kept.want) mark_best(team, run, kept.want, chosen);
+    } else {
+      // The whole row, with a bitmap of it.
+      for (int i = tid; i < a.words; i += kStreamThreads) map[i] = 0;
+      __syncthreads();
+      const Read<kStreamThreads> run = {kept.lo, kept.hi, x};
+      mark_best(team, run, kept.want, map);
+    }
+    __syncthreads();
+  }
+  int taken = 0;
+  if (listed && count <= kept.want) {
+    taken = count;
+    for (int i = tid; i < taken; i += kStreamThreads) idx[kept.lo + i] = place[i];
+  } else if (listed) {
+    int* order = reinterpret_cast<int*>(value);
+    taken = list_bits(team, chosen, count, [&](int i, int bit) { order[i] = place[bit]; });
+    __syncthreads();
+    for (int i = tid; i < taken; i += kStreamThreads) idx[kept.lo + i] = order[i];
+  } else if (n > 0) {
+    taken = list_bits(team, map, n, [&](int i, int bit) { place[i] = kept.lo + bit; });
+    __syncthreads();
+    for (int i = tid; i < taken; i += kStreamThreads) idx[kept.lo + i] = place[i];
+  }
+  const int behind = kept.count - kept.hi, all = kept.lo + taken + behind;
+  for (int i = tid; i < kept.lo; i += kStreamThreads) idx[i] = i;
+  for (int i = tid; i < behind; i += kStreamThreads) idx[kept.lo + taken + i] = kept.hi + i;
+  for (int i = all + tid; i < a.k; i += kStreamThreads) idx[i] = -1;
+  if (tid == 0) a.len[t] = all;
+}
+
+// SMs of the current device, once the kernels have their shared memory granted on it; 0 on failure.
+int sms_on(int device) {
+  static std::mutex mu;
+  static int cached[128] = {0};
+  if (device < 0 || device >= 128) return 0;
+  std::lock_guard<std::mutex> lock(mu);
+  int n = 0;
+  const cudaFuncAttribute most = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  const int room = 200 * 1024;
+  if (!cached[device] &&
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess &&
+      cudaFuncSetAttribute(hold_kernel<false>, most, room) == cudaSuccess &&
+      cudaFuncSetAttribute(hold_kernel<true>, most, room) == cudaSuccess &&
+      cudaFuncSetAttribute(stream_kernel, most, room) == cudaSuccess)
+    cached[device] = n;
+  return cached[device];
 }
 
 }  // namespace index_select
@@ -646,6 +741,10 @@ extern "C" int32_t tq_index_select(const TqIndexSelectSpec* spec, int32_t* devic
   if (st != TQ_OK) return st;
   const TqIndexSelectSpec& s = *spec;
   if (s.scores.shape[0] == 0) return fail(nullptr, TQ_OK);
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return fail("device", TQ_ERR_CUDA);
+  const int sms = sms_on(device);
+  if (sms <= 0) return fail("device", TQ_ERR_CUDA);
   auto ints = [](const TqTensorSpec& t) {
     return t.rank ? reinterpret_cast<int*>(t.device_address) : nullptr;
   };
@@ -666,25 +765,47 @@ extern "C" int32_t tq_index_select(const TqIndexSelectSpec* spec, int32_t* devic
   a.keep_first = s.keep_first;
   a.keep_last = s.keep_last;
   const bool pages = s.page_table.rank != 0;
+  const long long rows = (long long)s.scores.shape[0];
   const int items = pages ? (a.columns + kPageRows - 1) / kPageRows : a.columns;
-  a.words = (items + 31) / 32;
-  static_assert(kCandidates * 8 + kRingBytes + (1u << 15) * 4 + sizeof(Shared) <= 227 * 1024 &&
-                    kCandidates * 8 + kRingBytes + (1u << 9) * 4 + (1u << 14) * 4 + sizeof(Shared) <= 227 * 1024,
-                "shared memory of 2^20 columns");
-  const uint32_t bytes = kCandidates * 8u + kRingBytes + uint32_t(a.words) * 4u + (pages ? uint32_t(items) * 4u : 0u);
-  auto kernel = pages ? index_select_kernel<true> : index_select_kernel<false>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) != cudaSuccess)
-    return fail("launch", TQ_ERR_CUDA);
+  // A cluster's blocks: while the card has room for two on each SM and a block would still have kFew
+  // scores, more of them; and as many as it takes to hold a row, pages one a 16th of a block's threads.
+  constexpr int kFew = 8192;
+  a.blocks = 1;
+  while (a.blocks < kMaxCluster && (items > a.blocks * kHold || (rows * a.blocks * 2 <= 2ll * sms &&
+                                                                 a.columns >= 2 * kFew * a.blocks)))
+    a.blocks *= 2;
+  // The row form streams its rows instead where clusters would not all run at once, or cannot hold a row.
+  const bool stream_rows = !pages && (rows * a.blocks > 2ll * sms || items > a.blocks * kHold);
+  const int list = (a.k + 3) / 4 * 16;
+  uint32_t bytes;
+  if (stream_rows) {
+    a.blocks = 1;
+    a.words = ((items + 127) / 128 + 1) * 4;
+    bytes = uint32_t(kCandidates * 8 + a.words * 4);
+  } else {
+    const int each = (items + a.blocks - 1) / a.blocks;
+    a.words = (each + 31) / 32;
+    bytes = uint32_t(list + a.words * 4 + (pages ? each * 4 : 0));
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(s.scores.shape[0]), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.gridDim = dim3(unsigned(rows * a.blocks), 1, 1);
+  cfg.blockDim = dim3(stream_rows ? kStreamThreads : kThreads, 1, 1);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute pdl[1];
-  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  pdl[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = pdl;
+  cudaLaunchAttribute attr[1];
+  // Not both: clusters that were launched early took the places of the ones before them.
+  if (a.blocks == 1) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+  } else {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(a.blocks);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr;
   cfg.numAttrs = 1;
+  const auto kernel = stream_rows ? stream_kernel : pages ? hold_kernel<true> : hold_kernel<false>;
   if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return fail("launch", TQ_ERR_CUDA);
   return fail(nullptr, TQ_OK);
 }
