@@ -33,8 +33,7 @@ namespace tq {
 namespace index_select {
 
 constexpr int kThreads = 512;          // of hold_kernel
-constexpr int kN = 16;                 // scores that one of them holds
-constexpr int kHold = kN * kThreads;   // and a block
+constexpr int kHold = 32 * kThreads;   // scores that a block of it holds, in registers
 constexpr int kMaxCluster = 8;
 constexpr int kStreamThreads = 256;
 constexpr int kCandidates = 4096;      // of stream_kernel
@@ -172,6 +171,20 @@ struct Held {
 #pragma unroll
     for (int i = 0; i < N; ++i) fn(v[i], i);
   }
+  // A bitmap of the scores that take(value, number): a ballot is a word, 32 neighbours a warp. Lane i
+  // keeps the i-th.
+  template <typename Fn>
+  __device__ __forceinline__ void mark(uint32_t* map, Fn take) const {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    static_assert(N <= 32, "a word a lane");
+    unsigned mine = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const unsigned word = __ballot_sync(0xFFFFFFFFu, take(v[i], i));
+      if (lane == i) mine = word;
+    }
+    if (mine) map[lane * (T / 32) + warp] |= mine;
+  }
 };
 // In memory, read in each pass.
 template <int T>
@@ -195,6 +208,14 @@ struct Read {
 #pragma unroll 1
     for (; i < n; ++i) fn(read(at(i)), i);
   }
+  template <typename Fn>
+  __device__ __forceinline__ void mark(uint32_t* map, Fn take) const {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    each([&](float v, int i) {
+      const unsigned word = __ballot_sync(0xFFFFFFFFu, take(v, i));
+      if (lane == 0 && word) map[i * (T / 32) + warp] |= word;
+    });
+  }
 };
 
 // Bins between the least and the largest of some values. Larger values never have lower bins.
@@ -212,9 +233,9 @@ struct Bins {
   __device__ bool has(float v) const { return key_of(v) >= least && key_of(v) <= most; }
   // The sum with 2^23 leaves the bin in the low bits, at the rate of an addition (a conversion has an
   // eighth of it).
-  __device__ int by_value(float v) const {
-    return min(__float_as_int(fmaf(v - low, scale, 8388608.f)), 0x4B000000 + kBins - 1) - 0x4B000000;
-  }
+  static constexpr int kZero = 0x4B000000;
+  __device__ int sum(float v) const { return __float_as_int(fmaf(v - low, scale, 8388608.f)); }
+  __device__ int by_value(float v) const { return min(sum(v), kZero + kBins - 1) - kZero; }
   __device__ int by_key(float v) const { return int((key_of(v) - least) >> shift); }
 };
 
@@ -265,12 +286,6 @@ __device__ __forceinline__ int find_bin(Team<T>& team, int which, int want) {
 template <int T, typename R>
 __device__ __forceinline__ void mark_best(Team<T>& team, const R& run, int want, uint32_t* map) {
   Shared& sh = team.sh;
-  constexpr int kWarps = T / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto put = [&](bool take, int i) {  // 32 neighbours a warp: a word
-    const unsigned word = __ballot_sync(0xFFFFFFFFu, take);
-    if (lane == 0 && word) map[i * kWarps + warp] |= word;
-  };
   // The range of all values; -inf is none.
   float low = INFINITY, high = -INFINITY;
   run.each([&](float v, int) {
@@ -290,7 +305,7 @@ __device__ __forceinline__ void mark_best(Team<T>& team, const R& run, int want,
     });
   }
   if (find_bin(team, 0, want) <= want) {  // all of them
-    run.each([&](float v, int i) { put(v > -INFINITY, i); });
+    run.mark(map, [](float v, int) { return v > -INFINITY; });
     return;
   }
   int need = want;
@@ -317,7 +332,7 @@ __device__ __forceinline__ void mark_best(Team<T>& team, const R& run, int want,
   const int bin = sh.bin, inside = sh.inside;
   if (inside > kRanked) {
     // All equal: of these the first `need`, and then what is above them.
-    run.each([&](float v, int i) { put(bins.has(v), i); });
+    run.mark(map, [&](float v, int) { return bins.has(v); });
     __syncthreads();
     const int words = (run.end - run.begin + 31) / 32, per = (words + T - 1) / T;
     const int w0 = min(words, int(threadIdx.x) * per), w1 = min(words, w0 + per);
@@ -332,21 +347,27 @@ __device__ __forceinline__ void mark_best(Team<T>& team, const R& run, int want,
       map[w] = take;
     }
     __syncthreads();
-    run.each([&](float v, int i) { put(v > -INFINITY && key_of(v) > bins.most, i); });
+    run.mark(map, [&](float v, int) { return v > -INFINITY && key_of(v) > bins.most; });
     return;
   }
   // All above the bin, and those in it by rank: eight threads compare one with an eighth of them each.
-  run.each([&](float v, int i) {
-    bool above = false;
-    if (v > -INFINITY) {
-      int b = bin + (key_of(v) > bins.most);
-      if (bins.has(v)) b = by_value ? bins.by_value(v) : bins.by_key(v);
-      else if (key_of(v) < bins.least) b = -1;
-      above = b > bin;
-      if (b == bin) sh.own[atomicAdd(&sh.owned, 1)] = make_float2(v, __int_as_float(run.at(i)));
-    }
-    put(above, i);
-  });
+  auto own = [&](float v, int i) {
+    sh.own[atomicAdd(&sh.owned, 1)] = make_float2(v, __int_as_float(run.at(i)));
+  };
+  if (by_value) {
+    // (-inf has a negative sum; what rounds up past the last bin is in it.)
+    const int in = Bins::kZero + bin, top = bin == kBins - 1 ? INT_MAX : in;
+    run.mark(map, [&](float v, int i) {
+      const int sum = bins.sum(v);
+      if (sum >= in && sum <= top) own(v, i);
+      return sum > top;
+    });
+  } else {
+    run.mark(map, [&](float v, int i) {
+      if (bins.has(v) && bins.by_key(v) == bin) own(v, i);
+      return v > -INFINITY && (key_of(v) > bins.most || (bins.has(v) && bins.by_key(v) > bin));
+    });
+  }
   team.sync();
   for (int c0 = 0; c0 < inside; c0 += T / 8) {
     const int c = c0 + (threadIdx.x >> 3);
@@ -479,8 +500,9 @@ struct Kept {
   }
 };
 
-template <bool kPages>
-__global__ void __launch_bounds__(kThreads, 2) hold_kernel(const Args a) {
+// N: scores (pages) of a thread.
+template <bool kPages, int N>
+__global__ void __launch_bounds__(kThreads, 1) hold_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t raw[];
   int* list = reinterpret_cast<int*>(raw);
   uint32_t* map = reinterpret_cast<uint32_t*>(list + (a.k + 3) / 4 * 4);
@@ -497,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 2) hold_kernel(const Args a) {
   const Kept kept(a, kPages ? (token.seen + kPageRows - 1) / kPageRows : token.seen);
   // An even run of what is searched for each block.
   const int n = kept.want > 0 ? kept.hi - kept.lo : 0, each = (n + a.blocks - 1) / a.blocks;
-  Held<kThreads, kN> run;
+  Held<kThreads, N> run;
   run.begin = kept.lo + min(n, team.rank * each);
   run.end = kept.lo + min(n, (team.rank + 1) * each);
   if (n > 0) {
@@ -596,7 +618,7 @@ __device__ __forceinline__ int map_reach(Team<kStreamThreads>& team, const float
   return total;
 }
 
-__global__ void __launch_bounds__(kStreamThreads, 5) stream_kernel(const Args a) {
+__global__ void __launch_bounds__(kStreamThreads, 4) stream_kernel(const Args a) {
   constexpr int kWarps = kStreamThreads / 32;
   extern __shared__ __align__(16) uint8_t raw[];
   int* place = reinterpret_cast<int*>(raw);                        // candidates: positions
@@ -625,6 +647,9 @@ __global__ void __launch_bounds__(kStreamThreads, 5) stream_kernel(const Args a)
     float rank = fminf(expect + 6.f * sqrtf(expect) + 16.f, 0.8f * float(kCandidates) * share);
     rank = fmaxf(rank, expect + 1.f);
     float s[kSample];
+    if (tid == 0 && kept.hi - base >= 4)  // the whole row is on its way to L2 while it is sampled
+      ptx::bulk_prefetch_l2(x + base + (kept.lo > base ? 4 : 0),
+                            uint32_t(((kept.hi - base) / 4 - (kept.lo > base)) * 16));
     if (n > kCandidates) {
       // In runs of sixteen neighbours (two a warp's load), evenly over the row.
 #pragma unroll
@@ -675,7 +700,17 @@ __global__ void __launch_bounds__(kStreamThreads, 5) stream_kernel(const Args a)
     if (listed) {
       list_bits(team, map, kept.hi - base, [&](int i, int bit) { place[i] = base + bit; });
       __syncthreads();
-      for (int i = tid; i < count; i += kStreamThreads) value[i] = x[place[i]];
+      for (int i0 = tid; i0 < count; i0 += 4 * kStreamThreads) {
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = i0 + j * kStreamThreads;
+          f[j] = i < count ? x[place[i]] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i0 + j * kStreamThreads < count) value[i0 + j * kStreamThreads] = f[j];
+      }
       __syncthreads();
       const Read<kStreamThreads> run = {0, count, value};
       if (count > kept.want) mark_best(team, run, kept.want, chosen);
@@ -720,8 +755,10 @@ int sms_on(int device) {
   const int room = 200 * 1024;
   if (!cached[device] &&
       cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess &&
-      cudaFuncSetAttribute(hold_kernel<false>, most, room) == cudaSuccess &&
-      cudaFuncSetAttribute(hold_kernel<true>, most, room) == cudaSuccess &&
+      cudaFuncSetAttribute(hold_kernel<false, 16>, most, room) == cudaSuccess &&
+      cudaFuncSetAttribute(hold_kernel<false, 32>, most, room) == cudaSuccess &&
+      cudaFuncSetAttribute(hold_kernel<true, 16>, most, room) == cudaSuccess &&
+      cudaFuncSetAttribute(hold_kernel<true, 32>, most, room) == cudaSuccess &&
       cudaFuncSetAttribute(stream_kernel, most, room) == cudaSuccess)
     cached[device] = n;
   return cached[device];
@@ -767,15 +804,16 @@ extern "C" int32_t tq_index_select(const TqIndexSelectSpec* spec, int32_t* devic
   const bool pages = s.page_table.rank != 0;
   const long long rows = (long long)s.scores.shape[0];
   const int items = pages ? (a.columns + kPageRows - 1) / kPageRows : a.columns;
-  // A cluster's blocks: while the card has room for two on each SM and a block would still have kFew
-  // scores, more of them; and as many as it takes to hold a row, pages one a 16th of a block's threads.
+  // A cluster's blocks: as many as it takes to hold a row, and more while the card has room for one on
+  // each SM and a block would still have kFew scores (the barriers of a cluster, about 1000 cycles each,
+  // take as long as a block takes for that many).
   constexpr int kFew = 8192;
   a.blocks = 1;
-  while (a.blocks < kMaxCluster && (items > a.blocks * kHold || (rows * a.blocks * 2 <= 2ll * sms &&
-                                                                 a.columns >= 2 * kFew * a.blocks)))
+  while (a.blocks < kMaxCluster && (items > a.blocks * kHold || (rows * a.blocks * 2 <= sms &&
+                                                                 a.columns > 2 * kFew * a.blocks)))
     a.blocks *= 2;
   // The row form streams its rows instead where clusters would not all run at once, or cannot hold a row.
-  const bool stream_rows = !pages && (rows * a.blocks > 2ll * sms || items > a.blocks * kHold);
+  const bool stream_rows = !pages && (rows * a.blocks > sms || items > a.blocks * kHold);
   const int list = (a.k + 3) / 4 * 16;
   uint32_t bytes;
   if (stream_rows) {
@@ -805,7 +843,10 @@ extern "C" int32_t tq_index_select(const TqIndexSelectSpec* spec, int32_t* devic
   }
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const auto kernel = stream_rows ? stream_kernel : pages ? hold_kernel<true> : hold_kernel<false>;
+  const int n = (items + a.blocks - 1) / a.blocks;
+  const auto kernel = stream_rows ? stream_kernel
+                      : pages     ? n <= kHold / 2 ? hold_kernel<true, 16> : hold_kernel<true, 32>
+                                  : n <= kHold / 2 ? hold_kernel<false, 16> : hold_kernel<false, 32>;
   if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return fail("launch", TQ_ERR_CUDA);
   return fail(nullptr, TQ_OK);
 }

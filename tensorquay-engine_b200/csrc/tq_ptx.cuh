@@ -235,6 +235,11 @@ __device__ __forceinline__ void prefetch_l2(const void* p) {
   asm volatile("prefetch.global.L2 [%0];" :: "l"(p));
 }
 
+// Brings `bytes` (a multiple of 16, from a 16-byte aligned address) into L2.
+__device__ __forceinline__ void bulk_prefetch_l2(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p), "r"(bytes) : "memory");
+}
+
 // Programmatic dependent launch: the dependent grid may start early; it waits here until the
 // grids it depends on have completed and their memory is visible.
 __device__ __forceinline__ void grid_dependency_wait() {
