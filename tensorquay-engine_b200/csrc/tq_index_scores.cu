@@ -11,12 +11,13 @@
 // takes its even share of the sum and walks it; a run's keys are loaded once for all its tokens.
 // Warps of the one CTA on an SM:
 //   0     walks the runs: describes each (tokens, what they see), loads its codes and weights, and
-//         its keys two pages at a time (TMA through the page table, 128-byte swizzle), their scales
-//         with 4-byte copies beside them
+//         its keys and their scales two pages at a time (TMA through the page table, the codes with
+//         128-byte swizzle). With the scales fetched by 4-byte copies of its lanes a tile took it 1100
+//         cycles, and 64 requests over 16K to 32K rows 62 us instead of FIXME
 //   1     issues the MMAs, a sub-tile (the keys by half of a group's tokens) into one of two halves
 //         of TMEM
 //   2-17  four groups of warps, two for each half of TMEM: the sums over heads
-// Waits are bounded (2 s); one that gives up sets TQ_DEV_WAIT_TIMEOUT and ends the CTA's work.
+// Waits are bounded (about 2 s); one that gives up sets TQ_DEV_WAIT_TIMEOUT and ends its warp's work.
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -38,12 +39,11 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kSumWarp = 2;  // first of sixteen
 constexpr int kColumns = 256;     // of a sub-tile
 constexpr int kSubTokens = 16;    // tokens of a sub-tile at most
-constexpr int kStages = 5;        // key tiles in flight
+constexpr int kStages = 4;        // key tiles in flight
 constexpr int kScaleSlots = 8;    // see the producer
 constexpr uint32_t kKeyBytes = kKeys * kDim;
 constexpr uint32_t kQueryBytes = 2 * kColumns * kDim;
-constexpr uint64_t kWaitNs = 2000000000ull;
-constexpr uint32_t kWaitPolls = 1u << 26;
+constexpr uint32_t kTries = 1u << 21;
 
 struct Unit {
   int t0, tokens;          // run of tokens; 0 tokens: no more work
@@ -55,7 +55,7 @@ struct Shared {  // behind 1024-byte alignment
   uint8_t query[2][kQueryBytes];
   uint8_t key[kStages][kKeyBytes];
   float weight[2][2 * kColumns];
-  float scale[kScaleSlots][kKeys];
+  float4 scale[kScaleSlots][kKeys];  // the first of four; TMA moves 16 bytes at least
   Unit unit[2];
   uint64_t bar_key_full[kStages], bar_key_empty[kStages];
   uint64_t bar_scale[kScaleSlots];
@@ -65,14 +65,12 @@ struct Shared {  // behind 1024-byte alignment
   long long part[kWarps];
   long long start_cost;
   int start_group;
-  int stop;  // a wait has given up
   uint32_t tmem;
 };
 constexpr uint32_t kSharedBytes = sizeof(Shared) + 1024;
 static_assert(kSharedBytes <= 227 * 1024, "shared memory per CTA");
 
 struct Args {
-  const uint8_t* kv;
   const float* w;
   const int* page_table;
   const int* seq_id;
@@ -80,39 +78,27 @@ struct Args {
   const int* kv_len;
   uint8_t* scores;
   int* flags;
-  long long row_stride;    // bytes
   long long score_stride;  // bytes
   int tokens, heads, sequences, slots, pages, columns;
   int sub;      // tokens of a sub-tile
   int nowhere;  // a row past the key map's end: reads as zeros
 };
 
-// A bounded wait; `stop` ends all waits of the CTA once one has given up. Reading the timer is slow:
-// only a wait of many polls does.
+// A bounded wait: kTries suspensions of at most a microsecond. No more instructions than it needs: it
+// stands in a dozen places and competes for the instruction caches with the loops around it (with a
+// timer in its loop, a wait that had long been satisfied took 200 to 400 cycles).
 struct Wait {
   int* flags;
-  volatile int* stop;
-  bool failed = false;
-  __device__ bool on(uint64_t& barrier, uint32_t parity) {
-    if (failed) return false;
+  __device__ __forceinline__ bool on(uint64_t& barrier, uint32_t parity) {
     const uint32_t bar = ptx::smem_addr(&barrier);
-    uint64_t t0 = 0;
-    for (uint32_t i = 1;; ++i) {
-      if (ptx::mbar_try(bar, parity)) return true;
-      if ((i & 63) == 0) {
-        const uint64_t now = ptx::global_timer_ns();
-        if (t0 == 0) t0 = now;
-        if (now - t0 > kWaitNs || i > kWaitPolls || *stop) {
-          if (flags) atomicOr(flags, TQ_DEV_WAIT_TIMEOUT);
-          *stop = 1;
-          failed = true;
-          return false;
-        }
-      }
-    }
+#pragma unroll 1
+    for (uint32_t i = 0; i < kTries; ++i)
+      if (ptx::mbar_try(bar, parity, 1000)) return true;
+    if (flags) atomicOr(flags, TQ_DEV_WAIT_TIMEOUT);
+    return false;
   }
   // For a converged warp: all lanes go on, or none.
-  __device__ bool warp_on(uint64_t& barrier, uint32_t parity) {
+  __device__ __forceinline__ bool warp_on(uint64_t& barrier, uint32_t parity) {
     return __all_sync(0xFFFFFFFFu, on(barrier, parity));
   }
 };
@@ -207,9 +193,10 @@ __device__ __forceinline__ void find_share(const Args& a, Shared& sh, long long*
 // before it are done (each half of TMEM is taken in turn), so a scale slot that comes back after
 // kStages + 3 tiles is free too.
 __device__ __forceinline__ void produce(const Args& a, Shared& sh, const CUtensorMap* tm_q,
-                                        const CUtensorMap* tm_k, long long lo, long long hi) {
+                                        const CUtensorMap* tm_k, const CUtensorMap* tm_s, long long lo,
+                                        long long hi) {
   const int lane = threadIdx.x & 31;
-  Wait wait{a.flags, &sh.stop};
+  Wait wait{a.flags};
   const int size = 2 * a.sub;
   int tile = 0, units = 0;
   bool ok = true;
@@ -258,37 +245,36 @@ __device__ __forceinline__ void produce(const Args& a, Shared& sh, const CUtenso
         __syncwarp();
         ++units;
         const int* table = a.page_table + (long long)first * a.slots;
-        int pages = 0, base = -64;
+        // Page entries 32 at a time, the next ones on their way; behind the last row that the run sees
+        // there are none.
+        auto entries = [&](int base) {
+          const bool seen = base + lane < a.slots && (base + lane) * kPageRows < most;
+          const int page = seen ? table[base + lane] : -1;
+          return page >= 0 && page < a.pages ? page * kPageRows : seen ? -2 : -1;
+        };
+        int base = 2 * j0, rows_now = entries(base), rows_next = entries(base + 32);
         for (int j = j0; j < j1; ++j, ++tile) {
-          // Page entries 32 at a time; behind the last row that the run sees there are none.
           if (2 * j - base >= 32) {
-            base = 2 * j;
-            const bool seen = base + lane < a.slots && (base + lane) * kPageRows < most;
-            pages = seen ? table[base + lane] : -1;
-            if (seen && (pages < 0 || pages >= a.pages) && a.flags)
-              atomicOr(a.flags, TQ_DEV_PAGE_RANGE);
+            base += 32;
+            rows_now = rows_next;
+            rows_next = entries(base + 32);
           }
-          const int s = tile % kStages;
+          if (2 * j == base && rows_now == -2 && a.flags) atomicOr(a.flags, TQ_DEV_PAGE_RANGE);
+          const int s = tile % kStages, slot = tile % kScaleSlots;
           ok = tile < kStages || wait.warp_on(sh.bar_key_empty[s], uint32_t(tile / kStages - 1) & 1u);
           if (!ok) break;
-          const int p0 = __shfl_sync(0xFFFFFFFFu, pages, 2 * j - base);
-          const int p1 = __shfl_sync(0xFFFFFFFFu, pages, 2 * j - base + 1);
-          const bool in0 = p0 >= 0 && p0 < a.pages, in1 = p1 >= 0 && p1 < a.pages;
-          const int slot = tile % kScaleSlots;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = 32 * (i & 1) + lane;
-            const bool in = i < 2 ? in0 : in1;
-            const uint8_t* src =
-                a.kv + ((long long)(i < 2 ? p0 : p1) * kPageRows + row) * a.row_stride + kDim;
-            ptx::cp_async_4(ptx::smem_addr(&sh.scale[slot][32 * i + lane]), in ? src : a.kv, in ? 4 : 0);
-          }
-          ptx::cp_async_arrive(ptx::smem_addr(&sh.bar_scale[slot]));
+          const int r0 = __shfl_sync(0xFFFFFFFFu, rows_now, 2 * j - base);
+          const int r1 = __shfl_sync(0xFFFFFFFFu, rows_now, 2 * j - base + 1);
           if (lane == 0) {
             const uint32_t bar = ptx::smem_addr(&sh.bar_key_full[s]), dst = ptx::smem_addr(sh.key[s]);
+            const uint32_t bar2 = ptx::smem_addr(&sh.bar_scale[slot]), dst2 = ptx::smem_addr(sh.scale[slot]);
+            const int y0 = r0 >= 0 ? r0 : a.nowhere, y1 = r1 >= 0 ? r1 : a.nowhere;
             ptx::mbar_expect_tx(bar, kKeyBytes);
-            ptx::tma_load_2d(dst, tm_k, bar, 0, in0 ? p0 * kPageRows : a.nowhere);
-            ptx::tma_load_2d(dst + kKeyBytes / 2, tm_k, bar, 0, in1 ? p1 * kPageRows : a.nowhere);
+            ptx::tma_load_2d(dst, tm_k, bar, 0, y0);
+            ptx::tma_load_2d(dst + kKeyBytes / 2, tm_k, bar, 0, y1);
+            ptx::mbar_expect_tx(bar2, kKeys * 16);
+            ptx::tma_load_2d(dst2, tm_s, bar2, 0, y0);
+            ptx::tma_load_2d(dst2 + kKeys * 8, tm_s, bar2, 0, y1);
           }
           __syncwarp();
         }
@@ -304,57 +290,64 @@ __device__ __forceinline__ void produce(const Args& a, Shared& sh, const CUtenso
     ptx::mbar_arrive(ptx::smem_addr(&sh.bar_unit_full[u]));
   }
   __syncwarp();
-  ptx::cp_async_wait_all();
   if (!ok) {
     // What is on its way lands before the CTA ends.
-    int keep = 0;
-    Wait last{a.flags, &keep};
-    for (int i = max(0, tile - kStages); i < tile; ++i)
+    Wait last{a.flags};
+    for (int i = max(0, tile - kStages); i < tile; ++i) {
       last.on(sh.bar_key_full[i % kStages], uint32_t(i / kStages) & 1u);
+      last.on(sh.bar_scale[i % kScaleSlots], uint32_t(i / kScaleSlots) & 1u);
+    }
     for (int i = max(0, units - 2); i < units; ++i)
       last.on(sh.bar_unit_full[i & 1], uint32_t(i >> 1) & 1u);
   }
 }
 
-// Warp 1. False when a wait has given up.
+// Warp 1, one lane of it. False when a wait has given up.
 __device__ __forceinline__ bool multiply(const Args& a, Shared& sh) {
-  Wait wait{a.flags, &sh.stop};
-  int tile = 0, subs = 0;
+  Wait wait{a.flags};
+  const uint32_t tmem = sh.tmem;
+  // Rows of 128 bytes, K-major, 128-byte swizzle: 8-row groups 1 KB apart.
+  const uint64_t keys0 = ptx::smem_desc(ptx::smem_addr(sh.key[0]), 16, 1024, 2);
+  const uint64_t queries0 = ptx::smem_desc(ptx::smem_addr(sh.query[0]), 16, 1024, 2);
+  int s = 0;
+  uint32_t key_parity = 0, subs = 0;
   for (int units = 0;; ++units) {
     const int u = units & 1;
-    if (!wait.warp_on(sh.bar_unit_full[u], uint32_t(units >> 1) & 1u)) return false;
+    if (!wait.on(sh.bar_unit_full[u], uint32_t(units >> 1) & 1u)) return false;
     const int tokens = sh.unit[u].tokens, tiles = sh.unit[u].tiles;
     if (tokens == 0) return true;
-    for (int j = 0; j < tiles; ++j, ++tile) {
-      const int s = tile % kStages;
-      if (!wait.warp_on(sh.bar_key_full[s], uint32_t(tile / kStages) & 1u)) return false;
-      for (int t = 0; t < tokens; t += a.sub, ++subs) {
-        const int half = subs & 1;
-        if (subs >= 2 && !wait.warp_on(sh.bar_acc_empty[half], uint32_t((subs >> 1) - 1) & 1u)) return false;
+    const uint64_t queries = queries0 + uint64_t(u) * (kQueryBytes >> 4);
+    // Columns in whole sixteens: the last ones may be of no token, and nobody reads them.
+    auto idesc = [&](int n) { return ptx::idesc_e4m3(kKeys, uint32_t(n * a.heads + 15) & ~15u); };
+    const bool two = tokens > a.sub;
+    const uint32_t id0 = idesc(two ? a.sub : tokens), id1 = idesc(tokens - a.sub);
+    const uint64_t second = queries + uint64_t(a.sub * a.heads * kDim >> 4);
+    for (int j = 0; j < tiles; ++j) {
+      const uint64_t keys = keys0 + uint64_t(s) * (kKeyBytes >> 4);
+      if (!wait.on(sh.bar_key_full[s], key_parity)) return false;
+#pragma unroll 1
+      for (int part = 0; part <= int(two); ++part, ++subs) {
+        const uint32_t half = subs & 1;
+        if (subs >= 2 && !wait.on(sh.bar_acc_empty[half], (subs >> 1 & 1u) ^ 1u)) return false;
         ptx::tc_fence_after();
-        // Columns in whole sixteens: the last ones may be of no token, and nobody reads them.
-        const uint32_t n = uint32_t(min(a.sub, tokens - t) * a.heads + 15) & ~15u;
-        const uint32_t idesc = ptx::idesc_e4m3(kKeys, n);
-        const uint64_t kd = ptx::smem_desc(ptx::smem_addr(sh.key[s]), 16, 1024, 2);
-        const uint64_t qd = ptx::smem_desc(
-            ptx::smem_addr(sh.query[u]) + uint32_t(t * a.heads * kDim), 16, 1024, 2);
-#pragma unroll
-        for (int k = 0; k < kDim / 32; ++k)
-          ptx::mma_f8_ss_warp(sh.tmem + uint32_t(half * kColumns), kd + 2 * k, qd + 2 * k, idesc, k > 0);
-        ptx::mma_commit_warp(ptx::smem_addr(&sh.bar_acc_full[half]));
+        ptx::mma_f8_ss_x4(tmem + half * kColumns, keys, part ? second : queries, part ? id1 : id0);
+        ptx::mma_commit(ptx::smem_addr(&sh.bar_acc_full[half]));
       }
-      ptx::mma_commit_warp(ptx::smem_addr(&sh.bar_key_empty[s]));
+      ptx::mma_commit(ptx::smem_addr(&sh.bar_key_empty[s]));
+      if (++s == kStages) {
+        s = 0;
+        key_parity ^= 1;
+      }
     }
-    ptx::mma_commit_warp(ptx::smem_addr(&sh.bar_unit_empty[u]));
+    ptx::mma_commit(ptx::smem_addr(&sh.bar_unit_empty[u]));
   }
 }
 
 // After a wait that gave up: what the tensor core still does ends before the CTA does.
 __device__ __forceinline__ void drain(const Args& a, Shared& sh) {
-  int keep = 0;
-  Wait last{a.flags, &keep};
-  ptx::mma_commit_warp(ptx::smem_addr(&sh.bar_drain));
-  last.warp_on(sh.bar_drain, 0);
+  Wait last{a.flags};
+  ptx::mma_commit(ptx::smem_addr(&sh.bar_drain));
+  last.on(sh.bar_drain, 0);
 }
 
 template <int C>
@@ -409,7 +402,7 @@ __device__ __forceinline__ void sum_heads_in_registers(const Args& a, Shared& sh
   const uint32_t tmem = sh.tmem + uint32_t(half * kColumns) + (uint32_t(32 * quad) << 16);
   // After the exchanges: lanes with bit 0 hold keys 16 on, with bit 1 the odd eights.
   const int key = 32 * quad + 16 * (lane & 1) + 4 * (lane & 2) + (lane >> 2);
-  Wait wait{a.flags, &sh.stop};
+  Wait wait{a.flags};
   int tile = 0, subs = 0;
   for (int units = 0;; ++units) {
     const int u = units & 1;
@@ -435,10 +428,9 @@ __device__ __forceinline__ void sum_heads_in_registers(const Args& a, Shared& sh
       const int sub = subs + (t0 != 0);
       subs += two ? 2 : 1;
       if ((sub & 1) != half) continue;
-      if (!wait.warp_on(sh.bar_scale[tile % kScaleSlots], uint32_t(tile / kScaleSlots) & 1u)) return;
       if (!wait.warp_on(sh.bar_acc_full[half], uint32_t(sub >> 1) & 1u)) return;
       ptx::tc_fence_after();
-      const float scale = sh.scale[tile % kScaleSlots][key];
+      float scale = 0.f;  // read before the half is given back
       const int n = (unit.tile0 + j) * kKeys + key;
       uint8_t* out = out0 + 4ll * kKeys * j;
       auto done = [&] {
@@ -462,6 +454,10 @@ __device__ __forceinline__ void sum_heads_in_registers(const Args& a, Shared& sh
           ptx::tmem_ld_16x128b_x8(from + uint32_t(kStep * now), x);
           ptx::tmem_ld_16x128b_x8(from + uint32_t(kStep * now) + (16u << 16), x + kStep / 2);
           tmem_wait(x);
+          if (now == 0) {
+            if (!wait.warp_on(sh.bar_scale[tile % kScaleSlots], uint32_t(tile / kScaleSlots) & 1u)) return;
+            scale = sh.scale[tile % kScaleSlots][key].x;
+          }
           if (c + 1 == kChunks && i + 1 >= mine) done();
 #pragma unroll
           for (int g = 0; g < kStep / 8; ++g) {
@@ -496,7 +492,7 @@ __device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half, i
   const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, key = 32 * quad + lane;
   const uint32_t tmem = sh.tmem + uint32_t(half * kColumns) + (uint32_t(32 * quad) << 16);
   const int chunks = a.heads / C;
-  Wait wait{a.flags, &sh.stop};
+  Wait wait{a.flags};
   int tile = 0, subs = 0;
   for (int units = 0;; ++units) {
     const int u = units & 1;
@@ -510,7 +506,7 @@ __device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half, i
         if (!wait.warp_on(sh.bar_scale[tile % kScaleSlots], uint32_t(tile / kScaleSlots) & 1u)) return;
         if (!wait.warp_on(sh.bar_acc_full[half], uint32_t(subs >> 1) & 1u)) return;
         ptx::tc_fence_after();
-        const float scale = sh.scale[tile % kScaleSlots][key];
+        const float scale = sh.scale[tile % kScaleSlots][key].x;
         const int n = (tile0 + j) * kKeys + key;
         const int all = min(a.sub, tokens - t), place = part ? (all + 1) / 2 : 0;
         const int steps = (part ? all / 2 : (all + 1) / 2) * chunks;
@@ -566,7 +562,8 @@ __device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half, i
 template <int kH, int C>
 __global__ void __launch_bounds__(kThreads, 1)
     index_scores_kernel(const __grid_constant__ CUtensorMap tm_q,
-                        const __grid_constant__ CUtensorMap tm_k, const Args a) {
+                        const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_s, const Args a) {
   extern __shared__ uint8_t raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw + ((1024u - (ptx::smem_addr(raw) & 1023u)) & 1023u));
   const int warp = threadIdx.x >> 5;
@@ -576,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       init(sh.bar_key_full[s], 1);
       init(sh.bar_key_empty[s], 1);
     }
-    for (int s = 0; s < kScaleSlots; ++s) init(sh.bar_scale[s], 32);
+    for (int s = 0; s < kScaleSlots; ++s) init(sh.bar_scale[s], 1);
     for (int b = 0; b < 2; ++b) {
       init(sh.bar_unit_full[b], 1);
       init(sh.bar_unit_empty[b], 17);
@@ -584,10 +581,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       init(sh.bar_acc_empty[b], 8);
     }
     init(sh.bar_drain, 1);
-    sh.stop = 0;
     ptx::fence_mbar_init_cluster();
     ptx::tma_prefetch_desc(&tm_q);
     ptx::tma_prefetch_desc(&tm_k);
+    ptx::tma_prefetch_desc(&tm_s);
   }
   if (warp == 1) {
     ptx::tmem_alloc(ptx::smem_addr(&sh.tmem), 512);
@@ -602,9 +599,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   find_share(a, sh, &lo, &hi);
   if (lo < hi) {
     if (warp == 0) {
-      produce(a, sh, &tm_q, &tm_k, lo, hi);
+      produce(a, sh, &tm_q, &tm_k, &tm_s, lo, hi);
     } else if (warp == 1) {
-      if (!multiply(a, sh)) drain(a, sh);
+      if ((threadIdx.x & 31) == 0 && !multiply(a, sh)) drain(a, sh);
+      __syncwarp();
     } else {
       const int group = (warp - kSumWarp) >> 2;
       if constexpr (kH) sum_heads_in_registers<kH>(a, sh, group & 1, group >> 1);
@@ -651,7 +649,21 @@ bool encode_rows(CUtensorMap* map, const void* addr, uint64_t rows, uint64_t str
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-typedef void (*Kernel)(CUtensorMap, CUtensorMap, Args);
+// A page's scales, one f32 a row, in boxes of 16 bytes a row: the three columns past the map's only one
+// read as zeros.
+bool encode_scales(CUtensorMap* map, const void* addr, uint64_t rows, uint64_t stride) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {1, rows};
+  const cuuint64_t strides[1] = {stride};
+  const cuuint32_t boxes[2] = {4, kPageRows};
+  const cuuint32_t elem[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(addr), dims, strides, boxes,
+            elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+            CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+typedef void (*Kernel)(CUtensorMap, CUtensorMap, CUtensorMap, Args);
 
 Kernel kernel_for(int heads) {
   switch (heads) {
@@ -699,7 +711,6 @@ extern "C" int32_t tq_index_scores(const TqIndexScoresSpec* spec, int32_t* devic
   if (sms <= 0) return fail("device", TQ_ERR_CUDA);
   auto ints = [](const TqTensorSpec& t) { return reinterpret_cast<const int*>(t.device_address); };
   Args a = {};
-  a.kv = reinterpret_cast<const uint8_t*>(s.kv.device_address);
   a.w = reinterpret_cast<const float*>(s.w.device_address);
   a.page_table = ints(s.page_table);
   a.seq_id = ints(s.seq_id);
@@ -707,7 +718,6 @@ extern "C" int32_t tq_index_scores(const TqIndexScoresSpec* spec, int32_t* devic
   a.kv_len = ints(s.kv_len);
   a.scores = reinterpret_cast<uint8_t*>(s.scores.device_address);
   a.flags = device_flags;
-  a.row_stride = (long long)s.kv.strides_bytes[1];
   a.score_stride = (long long)s.scores.strides_bytes[0];
   a.tokens = int(s.q.shape[0]);
   a.heads = int(s.q.shape[1]);
@@ -716,16 +726,17 @@ extern "C" int32_t tq_index_scores(const TqIndexScoresSpec* spec, int32_t* devic
   a.pages = int(s.kv.shape[0]);
   a.columns = int(s.scores.shape[1]);
   a.sub = kColumns / a.heads < kSubTokens ? kColumns / a.heads : kSubTokens;
-  CUtensorMap tm_q, tm_k;
+  CUtensorMap tm_q, tm_k, tm_s;
   const void* codes = reinterpret_cast<const void*>(s.q.device_address);
   // A pool without pages has no memory to describe: every page reads past the end of one row of q.
   const uint64_t rows = a.pages ? uint64_t(a.pages) * kPageRows : 1;
+  const uint64_t stride = a.pages ? s.kv.strides_bytes[1] : kDim;
+  const uint8_t* keys = reinterpret_cast<const uint8_t*>(a.pages ? s.kv.device_address : s.q.device_address);
   a.nowhere = int(rows);
   if (!encode_rows(&tm_q, codes, s.q.shape[0] * s.q.shape[1], kDim, uint32_t(a.heads)) ||
-      !encode_rows(&tm_k, a.pages ? a.kv : codes, rows, a.pages ? uint64_t(a.row_stride) : kDim,
-                   kPageRows))
+      !encode_rows(&tm_k, keys, rows, stride, kPageRows) ||
+      !encode_scales(&tm_s, a.pages ? keys + kDim : keys, rows, stride))
     return fail("tensor map", TQ_ERR_CUDA);
-  if (!a.pages) a.kv = reinterpret_cast<const uint8_t*>(codes);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(sms), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
@@ -736,7 +747,7 @@ extern "C" int32_t tq_index_scores(const TqIndexScoresSpec* spec, int32_t* devic
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = pdl;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel_for(a.heads), tm_q, tm_k, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel_for(a.heads), tm_q, tm_k, tm_s, a);
   if (e != cudaSuccess) return fail("launch", TQ_ERR_CUDA);
   return fail(nullptr, TQ_OK);
 }

@@ -149,15 +149,15 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
-// As mbar_test, but the thread may be suspended for a while: a wait costs its neighbours fewer issue
-// slots.
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+// As mbar_test, but the thread may be suspended for up to `ns` nanoseconds: a wait costs its neighbours
+// fewer issue slots.
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity, uint32_t ns) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+      : "=r"(ok) : "r"(bar), "r"(parity), "r"(ns) : "memory");
   return ok != 0;
 }
 
@@ -307,15 +307,22 @@ __device__ __forceinline__ void mma_ss_warp(uint32_t d_tmem, uint64_t a_desc, ui
       :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// As mma_ss_warp, kind::f8f6f4 (E4M3 in, f32 accumulate; K = 32 a step).
-__device__ __forceinline__ void mma_f8_ss_warp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                               uint32_t idesc, uint32_t accumulate) {
+// D[tmem] = A[smem desc] * B[smem desc]^T over K = 128 of E4M3 (kind::f8f6f4, f32 sums), by one thread:
+// four steps of 32, 32 bytes apart inside the 128-byte swizzle (2 descriptor units; a descriptor's
+// 14-bit address field does not carry).
+__device__ __forceinline__ void mma_f8_ss_x4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                             uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-      :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+      "{\n\t.reg .pred f, t;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 f, 0, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, f;\n\t"
+      "add.u64 a, %1, 2;\n\tadd.u64 b, %2, 2;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, t;\n\t"
+      "add.u64 a, %1, 4;\n\tadd.u64 b, %2, 4;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, t;\n\t"
+      "add.u64 a, %1, 6;\n\tadd.u64 b, %2, 6;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, t;\n\t}"
+      :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc) : "memory");
 }
 
 __device__ __forceinline__ void mma_ts_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
@@ -619,15 +626,6 @@ __device__ __forceinline__ void bulk_copy_to_peer(uint32_t dst_cluster, uint32_t
       :: "r"(dst_cluster), "r"(src_cta), "r"(bytes), "r"(remote_bar) : "memory");
 }
 
-// As cp_async_16, 4 bytes.
-__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, uint32_t src_bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(src_bytes)
-               : "memory");
-}
-// One of the arrivals that `bar` was initialised for, once this thread's earlier cp.async are done.
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
 // Bulk copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) from global into this
 // CTA's shared memory, completing `bytes` transactions on `bar`.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
