@@ -40,7 +40,9 @@ constexpr int kSumWarp = 2;  // first of sixteen
 constexpr int kColumns = 256;     // of a sub-tile
 constexpr int kSubTokens = 16;    // tokens of a sub-tile at most
 constexpr int kStages = 4;        // key tiles in flight
-constexpr int kScaleSlots = 8;    // see the producer
+constexpr int kPack = 4;          // key tiles of a step at most
+constexpr int kScaleSlots = 12;   // see the producer
+constexpr int kCached = 512;      // tokens that are looked up once
 constexpr uint32_t kKeyBytes = kKeys * kDim;
 constexpr uint32_t kQueryBytes = 2 * kColumns * kDim;
 constexpr uint32_t kTries = 1u << 21;
@@ -48,6 +50,7 @@ constexpr uint32_t kTries = 1u << 21;
 struct Unit {
   int t0, tokens;          // run of tokens; 0 tokens: no more work
   int tile0, tiles;        // its key tiles
+  int pack;                // of them in one step
   int sees[2 * kSubTokens];
 };
 
@@ -57,6 +60,7 @@ struct Shared {  // behind 1024-byte alignment
   float weight[2][2 * kColumns];
   float4 scale[kScaleSlots][kKeys];  // the first of four; TMA moves 16 bytes at least
   Unit unit[2];
+  int2 token[kCached];     // sequence, rows seen
   uint64_t bar_key_full[kStages], bar_key_empty[kStages];
   uint64_t bar_scale[kScaleSlots];
   uint64_t bar_unit_full[2], bar_unit_empty[2];
@@ -68,6 +72,7 @@ struct Shared {  // behind 1024-byte alignment
   uint32_t tmem;
 };
 constexpr uint32_t kSharedBytes = sizeof(Shared) + 1024;
+static_assert(kScaleSlots >= 2 * kPack + kStages, "scale slots");
 static_assert(kSharedBytes <= 227 * 1024, "shared memory per CTA");
 
 struct Args {
@@ -81,6 +86,7 @@ struct Args {
   long long score_stride;  // bytes
   int tokens, heads, sequences, slots, pages, columns;
   int sub;      // tokens of a sub-tile
+  int pack;     // several tiles of a short run may share a step
   int nowhere;  // a row past the key map's end: reads as zeros
 };
 
@@ -120,30 +126,43 @@ __device__ __forceinline__ int tile_cost(const Args& a, int tokens) {
 }
 __device__ __forceinline__ int tiles_of(int most) { return (most + kKeys - 1) / kKeys; }
 
-// Cost of group g: its tokens in order, run by run; a few of their loads in flight together.
-__device__ __forceinline__ long long group_cost(const Args& a, int g, int* bad) {
+// Sequence and rows seen of four tokens from t on, up to `end`: from the cache, or with their loads in
+// flight together.
+__device__ __forceinline__ void look_up(const Args& a, const Shared& sh, int t, int end, int2 (&to)[4],
+                                        int* bad) {
+  if (a.tokens <= kCached) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = sh.token[min(t + i, end - 1)];
+    return;
+  }
+  int p[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    to[i].x = a.seq_id[min(t + i, end - 1)];
+    p[i] = a.q_pos[min(t + i, end - 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) to[i].y = sees(a, to[i].x, p[i], bad);
+}
+
+// Cost of group g: its tokens in order, run by run.
+__device__ __forceinline__ long long group_cost(const Args& a, const Shared& sh, int g, int* bad) {
   const int size = 2 * a.sub, t0 = g * size, end = min(a.tokens, t0 + size);
   long long cost = 0;
   int seq = 0, run = 0, most = 0;
   for (int t = t0; t < end; t += 4) {
-    int s[4], p[4], n[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[i] = t + i < end ? a.seq_id[t + i] : 0;
-      p[i] = t + i < end ? a.q_pos[t + i] : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) n[i] = t + i < end ? sees(a, s[i], p[i], bad) : 0;
+    int2 token[4];
+    look_up(a, sh, t, end, token, bad);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (t + i >= end) break;
-      if (run && s[i] != seq) {
+      if (run && token[i].x != seq) {
         cost += (long long)tiles_of(most) * tile_cost(a, run);
         run = most = 0;
       }
-      seq = s[i];
+      seq = token[i].x;
       ++run;
-      most = max(most, n[i]);
+      most = max(most, token[i].y);
     }
   }
   return cost + (long long)tiles_of(most) * tile_cost(a, run);
@@ -156,8 +175,15 @@ __device__ __forceinline__ void find_share(const Args& a, Shared& sh, long long*
   const int each = (groups + kThreads - 1) / kThreads;
   const int g0 = min(groups, tid * each), g1 = min(groups, g0 + each);
   int bad = 0;
+  if (a.tokens <= kCached) {
+    if (tid < a.tokens) {
+      const int s = a.seq_id[tid];
+      sh.token[tid] = make_int2(s, sees(a, s, a.q_pos[tid], &bad));
+    }
+    __syncthreads();
+  }
   long long mine = 0;
-  for (int g = g0; g < g1; ++g) mine += group_cost(a, g, &bad);
+  for (int g = g0; g < g1; ++g) mine += group_cost(a, sh, g, &bad);
   if (blockIdx.x == 0 && bad && a.flags) atomicOr(a.flags, bad);
   long long sum = mine;
 #pragma unroll
@@ -178,7 +204,7 @@ __device__ __forceinline__ void find_share(const Args& a, Shared& sh, long long*
   if (*lo < *hi && at <= *lo && *lo < sum) {
     int unused = 0, g = g0;
     for (; g < g1; ++g) {
-      const long long cost = group_cost(a, g, &unused);
+      const long long cost = group_cost(a, sh, g, &unused);
       if (*lo < at + cost) break;
       at += cost;
     }
@@ -189,9 +215,9 @@ __device__ __forceinline__ void find_share(const Args& a, Shared& sh, long long*
 }
 
 // Warp 0. A unit's slot is free once the MMAs that read its codes and the sixteen that read its
-// weights are done. A key stage is free once its MMAs are; by then the sums of the tile three
-// before it are done (each half of TMEM is taken in turn), so a scale slot that comes back after
-// kStages + 3 tiles is free too.
+// weights are done. A key stage is free once its MMAs are. By then the sums of the step two before theirs
+// are done (each half of TMEM is taken in turn), and with them those of the tile 2 kPack before it: a
+// scale slot that comes back after 2 kPack + kStages tiles is free too.
 __device__ __forceinline__ void produce(const Args& a, Shared& sh, const CUtensorMap* tm_q,
                                         const CUtensorMap* tm_k, const CUtensorMap* tm_s, long long lo,
                                         long long hi) {
@@ -207,8 +233,13 @@ __device__ __forceinline__ void produce(const Args& a, Shared& sh, const CUtenso
       // One token a lane: the run that starts at t.
       int seq = 0, n = 0, unused = 0;
       if (t + lane < end) {
-        seq = a.seq_id[t + lane];
-        n = sees(a, seq, a.q_pos[t + lane], &unused);
+        if (a.tokens <= kCached) {
+          seq = sh.token[t + lane].x;
+          n = sh.token[t + lane].y;
+        } else {
+          seq = a.seq_id[t + lane];
+          n = sees(a, seq, a.q_pos[t + lane], &unused);
+        }
       }
       const int first = __shfl_sync(0xFFFFFFFFu, seq, 0);
       const unsigned same = __ballot_sync(0xFFFFFFFFu, t + lane < end && seq == first);
@@ -231,6 +262,7 @@ __device__ __forceinline__ void produce(const Args& a, Shared& sh, const CUtenso
           unit.tokens = run;
           unit.tile0 = j0;
           unit.tiles = j1 - j0;
+          unit.pack = a.pack ? max(1, min(kPack, a.sub / run)) : 1;
         }
         __syncwarp();
         if (lane == 0) {
@@ -250,7 +282,9 @@ __device__ __forceinline__ void produce(const Args& a, Shared& sh, const CUtenso
         auto entries = [&](int base) {
           const bool seen = base + lane < a.slots && (base + lane) * kPageRows < most;
           const int page = seen ? table[base + lane] : -1;
-          return page >= 0 && page < a.pages ? page * kPageRows : seen ? -2 : -1;
+          if (page >= 0 && page < a.pages) return page * kPageRows;
+          if (seen && a.flags) atomicOr(a.flags, TQ_DEV_PAGE_RANGE);
+          return a.nowhere;
         };
         int base = 2 * j0, rows_now = entries(base), rows_next = entries(base + 32);
         for (int j = j0; j < j1; ++j, ++tile) {
@@ -259,7 +293,6 @@ __device__ __forceinline__ void produce(const Args& a, Shared& sh, const CUtenso
             rows_now = rows_next;
             rows_next = entries(base + 32);
           }
-          if (2 * j == base && rows_now == -2 && a.flags) atomicOr(a.flags, TQ_DEV_PAGE_RANGE);
           const int s = tile % kStages, slot = tile % kScaleSlots;
           ok = tile < kStages || wait.warp_on(sh.bar_key_empty[s], uint32_t(tile / kStages - 1) & 1u);
           if (!ok) break;
@@ -268,13 +301,12 @@ __device__ __forceinline__ void produce(const Args& a, Shared& sh, const CUtenso
           if (lane == 0) {
             const uint32_t bar = ptx::smem_addr(&sh.bar_key_full[s]), dst = ptx::smem_addr(sh.key[s]);
             const uint32_t bar2 = ptx::smem_addr(&sh.bar_scale[slot]), dst2 = ptx::smem_addr(sh.scale[slot]);
-            const int y0 = r0 >= 0 ? r0 : a.nowhere, y1 = r1 >= 0 ? r1 : a.nowhere;
             ptx::mbar_expect_tx(bar, kKeyBytes);
-            ptx::tma_load_2d(dst, tm_k, bar, 0, y0);
-            ptx::tma_load_2d(dst + kKeyBytes / 2, tm_k, bar, 0, y1);
+            ptx::tma_load_2d(dst, tm_k, bar, 0, r0);
+            ptx::tma_load_2d(dst + kKeyBytes / 2, tm_k, bar, 0, r1);
             ptx::mbar_expect_tx(bar2, kKeys * 16);
-            ptx::tma_load_2d(dst2, tm_s, bar2, 0, y0);
-            ptx::tma_load_2d(dst2 + kKeys * 8, tm_s, bar2, 0, y1);
+            ptx::tma_load_2d(dst2, tm_s, bar2, 0, r0);
+            ptx::tma_load_2d(dst2 + kKeys * 8, tm_s, bar2, 0, r1);
           }
           __syncwarp();
         }
@@ -310,7 +342,7 @@ __device__ __forceinline__ bool multiply(const Args& a, Shared& sh) {
   const uint64_t keys0 = ptx::smem_desc(ptx::smem_addr(sh.key[0]), 16, 1024, 2);
   const uint64_t queries0 = ptx::smem_desc(ptx::smem_addr(sh.query[0]), 16, 1024, 2);
   int s = 0;
-  uint32_t key_parity = 0, subs = 0;
+  uint32_t key_parity = 0, steps = 0;
   for (int units = 0;; ++units) {
     const int u = units & 1;
     if (!wait.on(sh.bar_unit_full[u], uint32_t(units >> 1) & 1u)) return false;
@@ -322,22 +354,35 @@ __device__ __forceinline__ bool multiply(const Args& a, Shared& sh) {
     const bool two = tokens > a.sub;
     const uint32_t id0 = idesc(two ? a.sub : tokens), id1 = idesc(tokens - a.sub);
     const uint64_t second = queries + uint64_t(a.sub * a.heads * kDim >> 4);
-    for (int j = 0; j < tiles; ++j) {
-      const uint64_t keys = keys0 + uint64_t(s) * (kKeyBytes >> 4);
-      if (!wait.on(sh.bar_key_full[s], key_parity)) return false;
+    const int pack = sh.unit[u].pack;
+    // A step fills half of TMEM: with a tile's first or second sub-tile, or with `pack` tiles.
+    auto begin = [&] {
+      if (steps >= 2 && !wait.on(sh.bar_acc_empty[steps & 1], (steps >> 1 & 1u) ^ 1u)) return false;
+      ptx::tc_fence_after();
+      return true;
+    };
+    for (int j = 0; j < tiles;) {
+      if (!begin()) return false;
 #pragma unroll 1
-      for (int part = 0; part <= int(two); ++part, ++subs) {
-        const uint32_t half = subs & 1;
-        if (subs >= 2 && !wait.on(sh.bar_acc_empty[half], (subs >> 1 & 1u) ^ 1u)) return false;
-        ptx::tc_fence_after();
-        ptx::mma_f8_ss_x4(tmem + half * kColumns, keys, part ? second : queries, part ? id1 : id0);
-        ptx::mma_commit(ptx::smem_addr(&sh.bar_acc_full[half]));
+      for (int p = 0; p < pack && j < tiles; ++p, ++j) {
+        const uint64_t keys = keys0 + uint64_t(s) * (kKeyBytes >> 4);
+        if (!wait.on(sh.bar_key_full[s], key_parity)) return false;
+        const uint32_t half = steps & 1;
+        ptx::mma_f8_ss_x4(tmem + half * kColumns + uint32_t(p * tokens * a.heads), keys, queries, id0);
+        if (two) {
+          ptx::mma_commit(ptx::smem_addr(&sh.bar_acc_full[half]));
+          ++steps;
+          if (!begin()) return false;
+          ptx::mma_f8_ss_x4(tmem + (half ^ 1) * kColumns, keys, second, id1);
+        }
+        ptx::mma_commit(ptx::smem_addr(&sh.bar_key_empty[s]));
+        if (++s == kStages) {
+          s = 0;
+          key_parity ^= 1;
+        }
       }
-      ptx::mma_commit(ptx::smem_addr(&sh.bar_key_empty[s]));
-      if (++s == kStages) {
-        s = 0;
-        key_parity ^= 1;
-      }
+      ptx::mma_commit(ptx::smem_addr(&sh.bar_acc_full[steps & 1]));
+      ++steps;
     }
     ptx::mma_commit(ptx::smem_addr(&sh.bar_unit_empty[u]));
   }
@@ -348,12 +393,6 @@ __device__ __forceinline__ void drain(const Args& a, Shared& sh) {
   Wait last{a.flags};
   ptx::mma_commit(ptx::smem_addr(&sh.bar_drain));
   last.on(sh.bar_drain, 0);
-}
-
-template <int C>
-__device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[C]) {
-  if constexpr (C == 16) ptx::tmem_ld16(at, r);
-  else ptx::tmem_ld8(at, r);
 }
 
 // Waits for the loads; what reads `r` stays behind it.
@@ -375,109 +414,158 @@ __device__ __forceinline__ float cut(uint32_t bits) {
 __device__ __forceinline__ void fma2(float2& acc, float2 x, float2 w) { acc = __ffma2_rn(x, w, acc); }
 __device__ __forceinline__ float both(float2 acc) { return acc.x + acc.y; }
 
-template <int C>
-__device__ __forceinline__ void add_up(const uint32_t (&r)[C], const float* w, float2 (&acc)[4]) {
+__device__ __forceinline__ void add_up(const uint32_t (&r)[8], const float* w, float2 (&acc)[4]) {
 #pragma unroll
-  for (int i = 0; i < C; i += 4) {
+  for (int i = 0; i < 8; i += 4) {
     const float4 v = *reinterpret_cast<const float4*>(w + i);
     fma2(acc[(i / 2) & 3], make_float2(cut(r[i]), cut(r[i + 1])), make_float2(v.x, v.y));
     fma2(acc[(i / 2 + 1) & 3], make_float2(cut(r[i + 2]), cut(r[i + 3])), make_float2(v.z, v.w));
   }
 }
 
-// Warps 2-17, heads 32, 64 or 128 (kH): the first or second part of a sub-tile's tokens, in half
-// `half` of TMEM, lanes 32 (warp % 4) on. A thread has two columns of each eight and four keys, so a
-// weight serves four sums, and the weights of its part, 32 a thread, stay in registers for all tiles
-// of a unit. (One key a thread needs a weight from
-// shared memory for each product: 4 cycles a warp for 128 of them.) A token's four sums end spread
-// over four lanes: three exchanges leave one key's in each.
+// A token's sum over kH heads for 128 keys: columns from `from` on, weights w. A thread has two columns
+// of each eight and four keys, so a weight serves four sums. (One key a thread needs a weight from
+// shared memory for each product: 4 cycles a warp for 128 of them.) The four sums end spread over four
+// lanes: three exchanges leave one key's in each. `last` is called once all columns are read.
 // What bounds it: the instructions, 1.5 for each head of a key and token (its cut at zero, half of a
 // product and addition), a cut at half their rate. So the last of the four keys adds |x| to x
 // instead, twice the same, and halves its sum.
+template <int kH, typename Fn>
+__device__ __forceinline__ float sum_heads_of(uint32_t from, const float2* w, int lane, Fn last) {
+  constexpr int kStep = kH % 32 ? 16 : 32, kChunks = kH / kStep;  // columns read at a time
+  float2 acc[4] = {};
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    uint32_t x[kStep];
+    if constexpr (kStep == 32) {
+      ptx::tmem_ld_16x128b_x8(from + uint32_t(kStep * c), x);
+      ptx::tmem_ld_16x128b_x8(from + uint32_t(kStep * c) + (16u << 16), x + kStep / 2);
+    } else {
+      ptx::tmem_ld_16x128b_x4(from + uint32_t(kStep * c), x);
+      ptx::tmem_ld_16x128b_x4(from + uint32_t(kStep * c) + (16u << 16), x + kStep / 2);
+    }
+    tmem_wait(x);
+    if (c + 1 == kChunks) last();
+#pragma unroll
+    for (int g = 0; g < kStep / 8; ++g) {
+      const float2 wg = w[c * (kStep / 8) + g];
+      const uint32_t* y = x + 4 * g;
+      fma2(acc[0], make_float2(cut(y[0]), cut(y[2])), wg);
+      fma2(acc[1], make_float2(cut(y[1]), cut(y[3])), wg);
+      y += kStep / 2;
+      fma2(acc[2], make_float2(cut(y[0]), cut(y[2])), wg);
+      const float z0 = __uint_as_float(y[1]), z1 = __uint_as_float(y[3]);
+      fma2(acc[3], make_float2(z0 + fabsf(z0), z1 + fabsf(z1)), wg);
+    }
+  }
+  const float s0 = both(acc[0]), s1 = both(acc[1]), s2 = both(acc[2]), s3 = 0.5f * both(acc[3]);
+  const bool b0 = lane & 1, b1 = lane & 2;
+  const float p = (b0 ? s2 : s0) + __shfl_xor_sync(0xFFFFFFFFu, b0 ? s0 : s2, 1);
+  const float q = (b0 ? s3 : s1) + __shfl_xor_sync(0xFFFFFFFFu, b0 ? s1 : s3, 1);
+  return (b1 ? q : p) + __shfl_xor_sync(0xFFFFFFFFu, b1 ? p : q, 2);
+}
+
+// The sum warps, heads a multiple of 16 (kH): the first or second part of a step's columns in half `half` of
+// TMEM, lanes 32 (warp % 4) on. The weights of its part, about 32 a thread, stay in registers for all tiles
+// of a unit.
 template <int kH>
 __device__ __forceinline__ void sum_heads_in_registers(const Args& a, Shared& sh, int half, int part) {
-  constexpr int kSub = kColumns / kH, kTokens = kSub / 2;  // tokens of a sub-tile, of a part of it
-  constexpr int kStep = 32, kChunks = kH / kStep;  // columns read at a time, of a token
+  constexpr int kSub = kColumns / kH < kSubTokens ? kColumns / kH : kSubTokens;  // tokens of a step
+  constexpr int kSlots = (kSub + 1) / 2;                                         // slots of a warp
   const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3;
   const uint32_t tmem = sh.tmem + uint32_t(half * kColumns) + (uint32_t(32 * quad) << 16);
   // After the exchanges: lanes with bit 0 hold keys 16 on, with bit 1 the odd eights.
   const int key = 32 * quad + 16 * (lane & 1) + 4 * (lane & 2) + (lane >> 2);
   Wait wait{a.flags};
-  int tile = 0, subs = 0;
+  auto done = [&] {
+    ptx::tc_fence_before();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sh.bar_acc_empty[half]));
+  };
+  int tile = 0, steps = 0;
   for (int units = 0;; ++units) {
     const int u = units & 1;
     if (!wait.warp_on(sh.bar_unit_full[u], uint32_t(units >> 1) & 1u)) return;
     const Unit& unit = sh.unit[u];
     const int tokens = unit.tokens, tiles = unit.tiles;
     if (tokens == 0) return;
-    // A tile is two sub-tiles, of which this half of TMEM always has the same one, or one, and this
-    // half has every other tile.
-    const bool two = tokens > kSub;
-    const int t0 = two && (subs & 1) != half ? kSub : 0, all = min(kSub, tokens - t0);
-    const int mine = part ? all / 2 : (all + 1) / 2, place = part ? (all + 1) / 2 : 0;
-    const int first = t0 + place;
-    float2 w[kTokens * kH / 8];
+    float2 w[kSlots * kH / 8];
+    auto weights = [&](int i, int t) {
 #pragma unroll
-    for (int i = 0; i < kTokens * kH / 8; ++i)
-      w[i] = make_float2(sh.weight[u][first * kH + 8 * i + (lane & 3)],
-                         sh.weight[u][first * kH + 8 * i + 4 + (lane & 3)]);
-    uint8_t* const out0 = a.scores + (long long)(unit.t0 + first) * a.score_stride +
-                          4ll * (unit.tile0 * kKeys + key);
-    const int* seen = unit.sees + first;
-    for (int j = 0; j < tiles; ++j, ++tile) {
-      const int sub = subs + (t0 != 0);
-      subs += two ? 2 : 1;
-      if ((sub & 1) != half) continue;
-      if (!wait.warp_on(sh.bar_acc_full[half], uint32_t(sub >> 1) & 1u)) return;
-      ptx::tc_fence_after();
-      float scale = 0.f;  // read before the half is given back
-      const int n = (unit.tile0 + j) * kKeys + key;
-      uint8_t* out = out0 + 4ll * kKeys * j;
-      auto done = [&] {
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sh.bar_acc_empty[half]));
-      };
-      if (mine == 0) {
-        done();
-        continue;
+      for (int g = 0; g < kH / 8; ++g) {
+        const float* from = &sh.weight[u][(t * kH + 8 * g + (lane & 3)) & (2 * kColumns - 1)];
+        w[i * (kH / 8) + g] = make_float2(from[0], from[4]);
       }
-      const uint32_t from = tmem + uint32_t(place * kH);
+    };
+    if (tokens > kSub) {
+      // A tile is two steps, of which this half of TMEM always has the same one.
+      const int t0 = (steps & 1) != half ? kSub : 0, all = min(kSub, tokens - t0);
+      const int mine = part ? all / 2 : (all + 1) / 2, place = part ? (all + 1) / 2 : 0;
 #pragma unroll
-      for (int i = 0; i < kTokens; ++i) {
-        if (i >= mine) break;
-        float2 acc[4] = {};
+      for (int i = 0; i < kSlots; ++i) weights(i, t0 + place + i);
+      const int* seen = unit.sees + t0 + place;
+      uint8_t* out = a.scores + (long long)(unit.t0 + t0 + place) * a.score_stride +
+                     4ll * (unit.tile0 * kKeys + key);
+      int n = unit.tile0 * kKeys + key, step = steps + (t0 != 0);
+      for (int j = 0; j < tiles; ++j, step += 2, n += kKeys, out += 4 * kKeys) {
+        const int slot = (tile + j) % kScaleSlots;
+        if (!wait.warp_on(sh.bar_acc_full[half], uint32_t(step >> 1) & 1u)) return;
+        ptx::tc_fence_after();
+        if (mine == 0) {
+          done();
+          continue;
+        }
+        if (!wait.warp_on(sh.bar_scale[slot], uint32_t((tile + j) / kScaleSlots) & 1u)) return;
+        const float scale = sh.scale[slot][key].x;
+        uint8_t* to = out;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const int now = i * kChunks + c;
-          uint32_t x[kStep];
-          ptx::tmem_ld_16x128b_x8(from + uint32_t(kStep * now), x);
-          ptx::tmem_ld_16x128b_x8(from + uint32_t(kStep * now) + (16u << 16), x + kStep / 2);
-          tmem_wait(x);
-          if (now == 0) {
-            if (!wait.warp_on(sh.bar_scale[tile % kScaleSlots], uint32_t(tile / kScaleSlots) & 1u)) return;
-            scale = sh.scale[tile % kScaleSlots][key].x;
-          }
-          if (c + 1 == kChunks && i + 1 >= mine) done();
+        for (int i = 0; i < kSlots; ++i) {
+          if (i >= mine) break;
+          const float sum = sum_heads_of<kH>(tmem + uint32_t((place + i) * kH), w + i * (kH / 8), lane, [&] {
+            if (i + 1 >= mine) done();
+          });
+          if (n < seen[i]) *reinterpret_cast<float*>(to) = sum * scale;
+          to += a.score_stride;
+        }
+      }
+      steps += 2 * tiles;
+      tile += tiles;
+    } else {
+      // A step has `pack` tiles, and this half every other step. Its columns are slots of kH, a tile and
+      // a token each; this warp has `most` of them from `place` on.
+      const int pack = unit.pack, all = pack * tokens;
+      const int most = part ? all / 2 : (all + 1) / 2, place = part ? (all + 1) / 2 : 0;
 #pragma unroll
-          for (int g = 0; g < kStep / 8; ++g) {
-            const float2 wg = w[now * (kStep / 8) + g];
-            const uint32_t* y = x + 4 * g;
-            fma2(acc[0], make_float2(cut(y[0]), cut(y[2])), wg);
-            fma2(acc[1], make_float2(cut(y[1]), cut(y[3])), wg);
-            y += kStep / 2;
-            fma2(acc[2], make_float2(cut(y[0]), cut(y[2])), wg);
-            const float z0 = __uint_as_float(y[1]), z1 = __uint_as_float(y[3]);
-            fma2(acc[3], make_float2(z0 + fabsf(z0), z1 + fabsf(z1)), wg);
+      for (int i = 0; i < kSlots; ++i) weights(i, (place + i) % tokens);
+      for (int j = 0; j < tiles; j += pack, ++steps) {
+        const int tile_now = tile, held = min(pack, tiles - j);
+        tile += held;
+        if ((steps & 1) != half) continue;
+        if (!wait.warp_on(sh.bar_acc_full[half], uint32_t(steps >> 1) & 1u)) return;
+        ptx::tc_fence_after();
+        const int mine = min(most, held * tokens - place);
+        if (mine <= 0) {
+          done();
+          continue;
+        }
+        int p = place / tokens, t = place % tokens;
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+          if (i >= mine) break;
+          const int slot = (tile_now + p) % kScaleSlots;
+          if (!wait.warp_on(sh.bar_scale[slot], uint32_t((tile_now + p) / kScaleSlots) & 1u)) return;
+          const float scale = sh.scale[slot][key].x;  // before the half is given back
+          const float sum = sum_heads_of<kH>(tmem + uint32_t((place + i) * kH), w + i * (kH / 8), lane, [&] {
+            if (i + 1 >= mine) done();
+          });
+          const int n = (unit.tile0 + j + p) * kKeys + key;
+          if (n < unit.sees[t])
+            reinterpret_cast<float*>(a.scores + (long long)(unit.t0 + t) * a.score_stride)[n] = sum * scale;
+          if (++t == tokens) {
+            t = 0;
+            ++p;
           }
         }
-        const float s0 = both(acc[0]), s1 = both(acc[1]), s2 = both(acc[2]), s3 = 0.5f * both(acc[3]);
-        const bool b0 = lane & 1, b1 = lane & 2;
-        const float p = (b0 ? s2 : s0) + __shfl_xor_sync(0xFFFFFFFFu, b0 ? s0 : s2, 1);
-        const float q = (b0 ? s3 : s1) + __shfl_xor_sync(0xFFFFFFFFu, b0 ? s1 : s3, 1);
-        const float sum = (b1 ? q : p) + __shfl_xor_sync(0xFFFFFFFFu, b1 ? p : q, 2);
-        if (n < seen[i]) *reinterpret_cast<float*>(out) = sum * scale;
-        out += a.score_stride;
       }
     }
     __syncwarp();
@@ -485,12 +573,12 @@ __device__ __forceinline__ void sum_heads_in_registers(const Args& a, Shared& sh
   }
 }
 
-// The same for other numbers of heads, one key a thread. C divides the heads: a token's columns are
-// read C at a time, the next ones while the last are added up.
-template <int C>
+// The same for other multiples of 8 heads, one key a thread: a token's columns are read eight at a time,
+// the next ones while the last are added up.
 __device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half, int part) {
   const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, key = 32 * quad + lane;
   const uint32_t tmem = sh.tmem + uint32_t(half * kColumns) + (uint32_t(32 * quad) << 16);
+  constexpr int C = 8;
   const int chunks = a.heads / C;
   Wait wait{a.flags};
   int tile = 0, subs = 0;
@@ -523,7 +611,7 @@ __device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half, i
         uint32_t r[2][C];
         float2 acc[4] = {};
         int left = chunks;
-        tmem_load<C>(from, r[0]);
+        ptx::tmem_ld8(from, r[0]);
 #pragma unroll 1
         for (int i = 0; i < steps; i += 2) {
 #pragma unroll
@@ -531,13 +619,13 @@ __device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half, i
             if (i + b < steps) {
               tmem_wait(r[b]);
               if (i + b + 1 < steps) {
-                tmem_load<C>(from + uint32_t((i + b + 1) * C), r[b ^ 1]);
+                ptx::tmem_ld8(from + uint32_t((i + b + 1) * C), r[b ^ 1]);
               } else {
                 ptx::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sh.bar_acc_empty[half]));
               }
-              add_up<C>(r[b], w, acc);
+              add_up(r[b], w, acc);
               w += C;
               if (--left == 0) {
                 const float sum = (both(acc[0]) + both(acc[1])) + (both(acc[2]) + both(acc[3]));
@@ -558,8 +646,8 @@ __device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half, i
   }
 }
 
-// kH: the heads if they are 32, 64 or 128; else 0, and C as above.
-template <int kH, int C>
+// kH: the heads if they are a multiple of 16; else 0.
+template <int kH>
 __global__ void __launch_bounds__(kThreads, 1)
     index_scores_kernel(const __grid_constant__ CUtensorMap tm_q,
                         const __grid_constant__ CUtensorMap tm_k,
@@ -606,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
       const int group = (warp - kSumWarp) >> 2;
       if constexpr (kH) sum_heads_in_registers<kH>(a, sh, group & 1, group >> 1);
-      else sum_heads<C>(a, sh, group & 1, group >> 1);
+      else sum_heads(a, sh, group & 1, group >> 1);
     }
   }
   ptx::tc_fence_before();
@@ -667,11 +755,16 @@ typedef void (*Kernel)(CUtensorMap, CUtensorMap, CUtensorMap, Args);
 
 Kernel kernel_for(int heads) {
   switch (heads) {
-    case 32: return index_scores_kernel<32, 0>;
-    case 64: return index_scores_kernel<64, 0>;
-    case 128: return index_scores_kernel<128, 0>;
+    case 16: return index_scores_kernel<16>;
+    case 32: return index_scores_kernel<32>;
+    case 48: return index_scores_kernel<48>;
+    case 64: return index_scores_kernel<64>;
+    case 80: return index_scores_kernel<80>;
+    case 96: return index_scores_kernel<96>;
+    case 112: return index_scores_kernel<112>;
+    case 128: return index_scores_kernel<128>;
   }
-  return heads % 16 == 0 ? index_scores_kernel<0, 16> : index_scores_kernel<0, 8>;
+  return index_scores_kernel<0>;
 }
 
 // SMs of the current device, once the kernels have their shared memory granted on it; 0 on failure.
@@ -683,7 +776,7 @@ int sms_on(int device) {
   if (cached[device]) return cached[device];
   int n = 0;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
-  for (int heads : {8, 16, 32, 64, 128})
+  for (int heads : {8, 16, 32, 48, 64, 80, 96, 112, 128})
     if (cudaFuncSetAttribute(kernel_for(heads), cudaFuncAttributeMaxDynamicSharedMemorySize,
                              int(kSharedBytes)) != cudaSuccess)
       return 0;
@@ -725,6 +818,7 @@ extern "C" int32_t tq_index_scores(const TqIndexScoresSpec* spec, int32_t* devic
   a.slots = int(s.page_table.shape[1]);
   a.pages = int(s.kv.shape[0]);
   a.columns = int(s.scores.shape[1]);
+  a.pack = a.heads % 16 == 0;
   a.sub = kColumns / a.heads < kSubTokens ? kColumns / a.heads : kSubTokens;
   CUtensorMap tm_q, tm_k, tm_s;
   const void* codes = reinterpret_cast<const void*>(s.q.device_address);
