@@ -9,7 +9,7 @@
 //   hold_kernel    few rows: a cluster of one to eight blocks a token, each with a run of the row in
 //                  registers, their bins added up through distributed shared memory. The page form
 //                  reduces its scores to a value a page first, and does the same with those
-//   stream_kernel  many rows, and longer ones than a cluster holds: a small block a token, six on an SM. A
+//   stream_kernel  many rows, and longer ones than a cluster holds: a small block a token, four on an SM. A
 //                  sample of the row gives a threshold that a little more than K scores reach (how much
 //                  more: six standard deviations of the sample's count); the row is read once and what
 //                  reaches the threshold is listed; these are counted and ranked. Where too few or too
@@ -37,7 +37,7 @@ constexpr int kHold = 32 * kThreads;   // scores that a block of it holds, in re
 constexpr int kMaxCluster = 8;
 constexpr int kStreamThreads = 256;
 constexpr int kCandidates = 4096;      // of stream_kernel
-constexpr int kSample = 16;            // scores that one of its threads samples
+constexpr int kSample = 8;             // scores that one of its threads samples
 constexpr int kPageRows = 64;
 constexpr int kBins = 1024;
 constexpr int kRanked = 64;            // scores that are ranked against each other
@@ -156,12 +156,26 @@ struct Team {
 // In registers, score i of a thread at begin + i * T + threadIdx.x.
 template <int T, int N>
 struct Held {
+  static constexpr bool kFew = true;  // N <= 32
   int begin, end;
+  const float* x;
+  const int* place;  // null: score i is x[at(i)]; else x[place[at(i)]]
   float v[N];
+  __device__ float value(int i) const { return score_of(place ? x[place[at(i)]] : x[at(i)]); }
   __device__ int at(int i) const { return begin + i * T + int(threadIdx.x); }
-  __device__ void load(const float* x) {
+  __device__ void load(const float* from) {
+    x = from;
+    place = nullptr;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = at(i) < end ? x[at(i)] : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = score_of(v[i]);
+  }
+  __device__ void gather(const float* from, const int* at_place) {
+    x = from;
+    place = at_place;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = at(i) < end ? x[place[at(i)]] : -INFINITY;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = score_of(v[i]);
   }
@@ -189,8 +203,10 @@ struct Held {
 // In memory, read in each pass.
 template <int T>
 struct Read {
+  static constexpr bool kFew = false;
   int begin, end;
   const float* x;
+  __device__ float value(int i) const { return read(at(i)); }
   __device__ int at(int i) const { return begin + i * T + int(threadIdx.x); }
   __device__ float read(int j) const { return score_of(j < end ? x[j] : -INFINITY); }
   template <typename Fn>
@@ -357,11 +373,23 @@ __device__ __forceinline__ void mark_best(Team<T>& team, const R& run, int want,
   if (by_value) {
     // (-inf has a negative sum; what rounds up past the last bin is in it.)
     const int in = Bins::kZero + bin, top = bin == kBins - 1 ? INT_MAX : in;
-    run.mark(map, [&](float v, int i) {
-      const int sum = bins.sum(v);
-      if (sum >= in && sum <= top) own(v, i);
-      return sum > top;
-    });
+    if constexpr (R::kFew) {
+      // Which of a thread's are in the bin is a bit each: a branch a score would take longer than all
+      // the rest, and few threads have any.
+      unsigned mine = 0;
+      run.mark(map, [&](float v, int i) {
+        const int sum = bins.sum(v);
+        mine |= unsigned(unsigned(sum - in) <= unsigned(top - in)) << i;
+        return sum > top;
+      });
+      for (; mine; mine &= mine - 1) own(run.value(__ffs(mine) - 1), __ffs(mine) - 1);
+    } else {
+      run.mark(map, [&](float v, int i) {
+        const int sum = bins.sum(v);
+        if (sum >= in && sum <= top) own(v, i);
+        return sum > top;
+      });
+    }
   } else {
     run.mark(map, [&](float v, int i) {
       if (bins.has(v) && bins.by_key(v) == bin) own(v, i);
@@ -405,18 +433,20 @@ __device__ __forceinline__ void mark_best(Team<T>& team, const R& run, int want,
   }
 }
 
-// Lists the positions of a bitmap's bits, in order, from to[0] on: each thread numbers a run of its 16
-// bits. Returns how many; the list is there after the next barrier.
-template <int T, typename Fn>
-__device__ __forceinline__ int list_bits(Team<T>& team, const uint32_t* map, int bits, Fn put) {
-  const int units = (bits + 15) / 16, per = (units + T - 1) / T;
+// Calls put(i, bit) for the i-th of a bitmap's bits, in order: each thread numbers a run of its units.
+// Returns how many bits there are; what `put` writes is there after the next barrier.
+template <typename Unit, int T, typename Fn>
+__device__ __forceinline__ int list_units(Team<T>& team, const Unit* map, int bits, Fn put) {
+  constexpr int kBits = 8 * sizeof(Unit);
+  const int units = (bits + kBits - 1) / kBits, per = (units + T - 1) / T;
   const int u0 = min(units, int(threadIdx.x) * per), u1 = min(units, u0 + per);
-  const uint16_t* half = reinterpret_cast<const uint16_t*>(map);
   int mine = 0, total;
-  for (int u = u0; u < u1; ++u) mine += __popc(uint32_t(half[u]));
+  for (int u = u0; u < u1; ++u) mine += __popc(uint32_t(map[u]));
   int at = team.block_scan(mine, &total) - mine;
+#pragma unroll 1
   for (int u = u0; u < u1; ++u)
-    for (uint32_t b = half[u]; b; b &= b - 1) put(at++, 16 * u + __ffs(b) - 1);
+#pragma unroll 1
+    for (uint32_t b = map[u]; b; b &= b - 1) put(at++, kBits * u + __ffs(b) - 1);
   return total;
 }
 
@@ -534,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) hold_kernel(const Args a) {
   }
   __syncthreads();
   int before;
-  const int block = list_bits(team, map, run.end - run.begin,
+  const int block = list_units(team, reinterpret_cast<const uint16_t*>(map), run.end - run.begin,
                               [&](int i, int bit) { list[i] = run.begin + bit; });
   const int taken = team.sum(block, &before);
   __syncthreads();
@@ -580,12 +610,16 @@ __device__ __forceinline__ int map_reach(Team<kStreamThreads>& team, const float
 #pragma unroll 1
   for (int g0 = warp * kVectors; 32 * g0 < vectors; g0 += kWarps * kVectors) {
     float4 v[kVectors];
+    // All loads first, without a branch.
+    if (whole1 > whole0) {
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j)
+        v[j] = *reinterpret_cast<const float4*>(x + base + 4 * min(max(32 * (g0 + j) + lane, whole0), whole1 - 1));
+    }
 #pragma unroll
     for (int j = 0; j < kVectors; ++j) {
       const int i = 32 * (g0 + j) + lane, at = base + 4 * i;
-      if (i >= whole0 && i < whole1) {
-        v[j] = *reinterpret_cast<const float4*>(x + at);
-      } else {
+      if (i < whole0 || i >= whole1) {
         v[j].x = at >= lo && at < hi ? x[at] : -INFINITY;
         v[j].y = at + 1 >= lo && at + 1 < hi ? x[at + 1] : -INFINITY;
         v[j].z = at + 2 >= lo && at + 2 < hi ? x[at + 2] : -INFINITY;
@@ -618,12 +652,19 @@ __device__ __forceinline__ int map_reach(Team<kStreamThreads>& team, const float
   return total;
 }
 
+// Marks the best of a whole row, read again in each pass: for what the list does not hold.
+__device__ __noinline__ void mark_row(Shared& sh, const float* x, int lo, int hi, int want, uint32_t* map) {
+  Team<kStreamThreads> team{sh, 1, 0};
+  const Read<kStreamThreads> run = {lo, hi, x};
+  mark_best(team, run, want, map);
+}
+
 __global__ void __launch_bounds__(kStreamThreads, 4) stream_kernel(const Args a) {
   constexpr int kWarps = kStreamThreads / 32;
   extern __shared__ __align__(16) uint8_t raw[];
   int* place = reinterpret_cast<int*>(raw);                        // candidates: positions
-  float* value = reinterpret_cast<float*>(place + kCandidates);    // and scores
-  uint32_t* map = reinterpret_cast<uint32_t*>(value + kCandidates);
+  int* order = place + kCandidates;                                // those selected
+  uint32_t* map = reinterpret_cast<uint32_t*>(order + (a.k + 3) / 4 * 4);
   __shared__ Shared sh;
   __shared__ uint32_t chosen[kCandidates / 32];                  // bitmap of the candidates
   const int tid = threadIdx.x, t = blockIdx.x;
@@ -646,22 +687,20 @@ __global__ void __launch_bounds__(kStreamThreads, 4) stream_kernel(const Args a)
     const float expect = float(kept.want) * share;
     float rank = fminf(expect + 6.f * sqrtf(expect) + 16.f, 0.8f * float(kCandidates) * share);
     rank = fmaxf(rank, expect + 1.f);
-    float s[kSample];
-    if (tid == 0 && kept.hi - base >= 4)  // the whole row is on its way to L2 while it is sampled
-      ptx::bulk_prefetch_l2(x + base + (kept.lo > base ? 4 : 0),
-                            uint32_t(((kept.hi - base) / 4 - (kept.lo > base)) * 16));
-    if (n > kCandidates) {
-      // In runs of sixteen neighbours (two a warp's load), evenly over the row.
-#pragma unroll
-      for (int j = 0; j < kSample; ++j) {
-        const int r = j * 2 * kWarps + (tid >> 4);
-        s[j] = x[kept.lo + int((long long)r * (n - 16) / (kSample * 2 * kWarps)) + (tid & 15)];
-      }
-#pragma unroll
-      for (int j = 0; j < kSample; ++j) s[j] = score_of(s[j]);
-    }
     for (int attempt = 0; attempt < 3; ++attempt) {
       if (n > kCandidates && rank < sampled) {
+        // Sampled in runs of sixteen neighbours (two a warp's load), evenly over the row.
+        float s[kSample];
+#pragma unroll
+        for (int j = 0; j < kSample; ++j) {
+          const int r = j * 2 * kWarps + (tid >> 4);
+          s[j] = x[kept.lo + int((long long)r * (n - 16) / (kSample * 2 * kWarps)) + (tid & 15)];
+        }
+        if (attempt == 0 && tid == 0)  // the whole row is on its way to L2 meanwhile
+          ptx::bulk_prefetch_l2(x + base + (kept.lo > base ? 4 : 0),
+                                uint32_t(((kept.hi - base) / 4 - (kept.lo > base)) * 16));
+#pragma unroll
+        for (int j = 0; j < kSample; ++j) s[j] = score_of(s[j]);
         // About `rank` of the sample reach the low edge of the bin that the rank-th largest is in.
         float low = INFINITY, high = -INFINITY;
 #pragma unroll
@@ -698,28 +737,20 @@ __global__ void __launch_bounds__(kStreamThreads, 4) stream_kernel(const Args a)
       }
     }
     if (listed) {
-      list_bits(team, map, kept.hi - base, [&](int i, int bit) { place[i] = base + bit; });
+      list_units(team, map, kept.hi - base, [&](int i, int bit) { place[i] = base + bit; });
       __syncthreads();
-      for (int i0 = tid; i0 < count; i0 += 4 * kStreamThreads) {
-        float f[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = i0 + j * kStreamThreads;
-          f[j] = i < count ? x[place[i]] : 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (i0 + j * kStreamThreads < count) value[i0 + j * kStreamThreads] = f[j];
+      if (count > kept.want) {
+        Held<kStreamThreads, kCandidates / kStreamThreads> run;
+        run.begin = 0;
+        run.end = count;
+        run.gather(x, place);
+        mark_best(team, run, kept.want, chosen);
       }
-      __syncthreads();
-      const Read<kStreamThreads> run = {0, count, value};
-      if (count > kept.want) mark_best(team, run, kept.want, chosen);
     } else {
       // The whole row, with a bitmap of it.
       for (int i = tid; i < a.words; i += kStreamThreads) map[i] = 0;
       __syncthreads();
-      const Read<kStreamThreads> run = {kept.lo, kept.hi, x};
-      mark_best(team, run, kept.want, map);
+      mark_row(sh, x, kept.lo, kept.hi, kept.want, map);
     }
     __syncthreads();
   }
@@ -728,12 +759,12 @@ __global__ void __launch_bounds__(kStreamThreads, 4) stream_kernel(const Args a)
     taken = count;
     for (int i = tid; i < taken; i += kStreamThreads) idx[kept.lo + i] = place[i];
   } else if (listed) {
-    int* order = reinterpret_cast<int*>(value);
-    taken = list_bits(team, chosen, count, [&](int i, int bit) { order[i] = place[bit]; });
+    taken = list_units(team, reinterpret_cast<const uint16_t*>(chosen), count,
+                       [&](int i, int bit) { order[i] = place[bit]; });
     __syncthreads();
     for (int i = tid; i < taken; i += kStreamThreads) idx[kept.lo + i] = order[i];
   } else if (n > 0) {
-    taken = list_bits(team, map, n, [&](int i, int bit) { place[i] = kept.lo + bit; });
+    taken = list_units(team, map, n, [&](int i, int bit) { place[i] = kept.lo + bit; });
     __syncthreads();
     for (int i = tid; i < taken; i += kStreamThreads) idx[kept.lo + i] = place[i];
   }
@@ -819,7 +850,7 @@ extern "C" int32_t tq_index_select(const TqIndexSelectSpec* spec, int32_t* devic
   if (stream_rows) {
     a.blocks = 1;
     a.words = ((items + 127) / 128 + 1) * 4;
-    bytes = uint32_t(kCandidates * 8 + a.words * 4);
+    bytes = uint32_t(kCandidates * 4 + list + a.words * 4);
   } else {
     const int each = (items + a.blocks - 1) / a.blocks;
     a.words = (each + 31) / 32;
