@@ -12,11 +12,20 @@
 // Warps of the one CTA on an SM:
 //   0     walks the runs: describes each (tokens, what they see), loads its codes and weights, and
 //         its keys and their scales two pages at a time (TMA through the page table, the codes with
-//         128-byte swizzle). With the scales fetched by 4-byte copies of its lanes a tile took it 1100
-//         cycles, and 64 requests over 16K to 32K rows 62 us instead of FIXME
-//   1     issues the MMAs, a sub-tile (the keys by half of a group's tokens) into one of two halves
-//         of TMEM
-//   2-17  four groups of warps, two for each half of TMEM: the sums over heads
+//         128-byte swizzle). A scale arrives as the first of four floats, the least that TMA moves;
+//         4-byte copies by the warp's lanes took 1100 cycles a tile
+//   1     one lane issues the MMAs, a step into one of two halves of TMEM: a tile by half of a group's
+//         tokens, or up to kPack tiles by a run of few
+//   2-17  four groups of warps, two for each half of TMEM: the sums over heads. A warp has the tokens'
+//         weights in registers for a whole run, four keys a thread; what a thread adds for a key and
+//         a head is 1.5 instructions (a maximum, half of a packed multiply-add)
+//
+// What bounds it (times back to back): many tokens, the sum warps' instructions: 2048 tokens of 64 heads
+// over 16384 rows 161 us, where the E4M3 products alone would take 72 and the maximum and the
+// multiply-add of each dot, issued without a pause, about 110. Few tokens: 64 requests of 16384 to 32768
+// rows 60 us at 56% of the copy bandwidth (loads alone take 24, the sums without loads 35: they meet in
+// the four stages of keys, and neither fewer nor more of them or of the tiles a step was faster); one
+// token of 8192 rows 7 us, launch and one chain of loads, products and sums.
 // Waits are bounded (about 2 s); one that gives up sets TQ_DEV_WAIT_TIMEOUT and ends its warp's work.
 
 #include <cuda.h>
@@ -37,8 +46,8 @@ constexpr int kKeys = 128;  // keys of a tile, two pages
 constexpr int kThreads = 576;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSumWarp = 2;  // first of sixteen
-constexpr int kColumns = 256;     // of a sub-tile
-constexpr int kSubTokens = 16;    // tokens of a sub-tile at most
+constexpr int kColumns = 256;     // of a step
+constexpr int kSubTokens = 16;    // tokens of a step at most
 constexpr int kStages = 4;        // key tiles in flight
 constexpr int kPack = 4;          // key tiles of a step at most
 constexpr int kScaleSlots = 12;   // see the producer
@@ -85,7 +94,7 @@ struct Args {
   int* flags;
   long long score_stride;  // bytes
   int tokens, heads, sequences, slots, pages, columns;
-  int sub;      // tokens of a sub-tile
+  int sub;      // tokens of a step
   int pack;     // several tiles of a short run may share a step
   int nowhere;  // a row past the key map's end: reads as zeros
 };
@@ -355,7 +364,7 @@ __device__ __forceinline__ bool multiply(const Args& a, Shared& sh) {
     const uint32_t id0 = idesc(two ? a.sub : tokens), id1 = idesc(tokens - a.sub);
     const uint64_t second = queries + uint64_t(a.sub * a.heads * kDim >> 4);
     const int pack = sh.unit[u].pack;
-    // A step fills half of TMEM: with a tile's first or second sub-tile, or with `pack` tiles.
+    // A step fills half of TMEM: with a tile by the first or second half of the tokens, or with `pack` tiles.
     auto begin = [&] {
       if (steps >= 2 && !wait.on(sh.bar_acc_empty[steps & 1], (steps >> 1 & 1u) ^ 1u)) return false;
       ptx::tc_fence_after();

@@ -9,15 +9,21 @@
 //   hold_kernel    few rows: a cluster of one to eight blocks a token, each with a run of the row in
 //                  registers, their bins added up through distributed shared memory. The page form
 //                  reduces its scores to a value a page first, and does the same with those
-//   stream_kernel  many rows, and longer ones than a cluster holds: a small block a token, four on an SM. A
-//                  sample of the row gives a threshold that a little more than K scores reach (how much
-//                  more: six standard deviations of the sample's count); the row is read once and what
-//                  reaches the threshold is listed; these are counted and ranked. Where too few or too
-//                  many reach it, it is moved and the row read again; where that does not help (more
-//                  equal scores than the list holds) the whole row is counted.
+//   stream_kernel  more rows, or longer ones, than clusters hold at once: a block a token. A sample of
+//                  the row gives a threshold that a little more than K scores reach (how much more: six
+//                  standard deviations of the sample's count); the row is read once and what reaches
+//                  the threshold is listed; these are counted and ranked. Where too few or too many
+//                  reach it, it is moved and the row read again; where that does not help (more equal
+//                  scores than the list holds) the whole row is counted. The blocks are small, four on
+//                  an SM, where there are many, since each has a chain of barriers that the others
+//                  fill; where a row has an SM to itself they are large (64 rows of 131072, K 2048:
+//                  36 us instead of 84).
 //
-// What bounds it: reading the scores (4 bytes a row seen) and counting them for many tokens, the chain of
-// loads and barriers for few.
+// What bounds it (times back to back, scores in L2 where they fit): few rows are a chain of loads and
+// barriers (1 x 8192: 6 us; 64 x 32768, K 2048: 16 us, one count, one rank and the cluster's barriers,
+// for 1.1 us of reading). Many rows are bound by instructions (2048 x 16384, K 2048: 78 us at 28% of
+// the copy bandwidth; about 32000 of a warp a row, two thirds of them for the 2500 candidates). Pages:
+// 64 x 131072 12.5 us, 41% of it: one wave of maxima, then the chain.
 
 #include <cuda_runtime.h>
 
@@ -35,9 +41,10 @@ namespace index_select {
 constexpr int kThreads = 512;          // of hold_kernel
 constexpr int kHold = 32 * kThreads;   // scores that a block of it holds, in registers
 constexpr int kMaxCluster = 8;
-constexpr int kStreamThreads = 256;
+constexpr int kStreamThreads = 256;    // of stream_kernel where there are many rows,
+constexpr int kLongThreads = 1024;     // and where a row has an SM to itself
 constexpr int kCandidates = 4096;      // of stream_kernel
-constexpr int kSample = 8;             // scores that one of its threads samples
+constexpr int kSampled = 2048;         // scores that it samples
 constexpr int kPageRows = 64;
 constexpr int kBins = 1024;
 constexpr int kRanked = 64;            // scores that are ranked against each other
@@ -70,7 +77,7 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 
 struct Shared {
-  int2 sums[2][kThreads / 32];  // of the warps, two buffers taken in turn
+  int2 sums[2][32];             // of the warps, two buffers taken in turn
   int2 total[2];                // of the block, for the cluster's others, in turn
   uint2 range[2];               // least and largest key of the block, in turn
   int hist[2][kBins];           // in turn; zero when they are not in use
@@ -260,14 +267,16 @@ struct Bins {
 // fewer than `want` there is no bin. Leaves the other hist zero, and ends with a barrier.
 template <int T>
 __device__ __forceinline__ int find_bin(Team<T>& team, int which, int want) {
-  constexpr int kEach = kBins / T;
+  constexpr int kEach = kBins / T < 2 ? 2 : kBins / T;
+  const bool active = kBins / kEach == T || threadIdx.x < kBins / kEach;
   Shared& sh = team.sh;
   team.sync();
   // From the highest bin down, kEach a thread.
   const int first = kBins - kEach * (1 + int(threadIdx.x));
-  int n[kEach], mine = 0;
+  int n[kEach] = {}, mine = 0;
 #pragma unroll
   for (int i = 0; i < kEach; i += 2) {
+    if (!active) break;
     const int* at = &sh.hist[which][first + i];
     int2 two = *reinterpret_cast<const int2*>(at);
     if (team.blocks > 1) {
@@ -530,9 +539,10 @@ struct Kept {
   }
 };
 
-// N: scores (pages) of a thread.
+// N: scores (pages) of a thread. Short rows need few registers, and three blocks are on an SM (2000 rows
+// of 64 pages: 26 us, with N = 16 and one block 62).
 template <bool kPages, int N>
-__global__ void __launch_bounds__(kThreads, 1) hold_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, N <= 4 ? 3 : 1) hold_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t raw[];
   int* list = reinterpret_cast<int*>(raw);
   uint32_t* map = reinterpret_cast<uint32_t*>(list + (a.k + 3) / 4 * 4);
@@ -602,9 +612,10 @@ __device__ __forceinline__ uint32_t spread(uint32_t x) {
 // A bitmap of the scores x[lo, hi) that reach `t` > -inf, from position `base` on (a multiple of 16 bytes
 // at or before lo), and how many they are. Vectors of four are read; those that reach over an end, one
 // score at a time.
-__device__ __forceinline__ int map_reach(Team<kStreamThreads>& team, const float* x, int base, int lo, int hi,
+template <int T>
+__device__ __forceinline__ int map_reach(Team<T>& team, const float* x, int base, int lo, int hi,
                                          float t, uint32_t* map) {
-  constexpr int kWarps = kStreamThreads / 32, kVectors = 4;
+  constexpr int kWarps = T / 32, kVectors = 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int vectors = (hi - base + 3) >> 2, whole0 = lo > base, whole1 = (hi - base) >> 2;
 #pragma unroll 1
@@ -638,7 +649,7 @@ __device__ __forceinline__ int map_reach(Team<kStreamThreads>& team, const float
   __syncthreads();
   // Each group of four words into the order of positions.
   int n = 0;
-  for (int g = threadIdx.x; g < (vectors + 31) / 32; g += kStreamThreads) {
+  for (int g = threadIdx.x; g < (vectors + 31) / 32; g += T) {
     uint4& w = reinterpret_cast<uint4*>(map)[g];
     const uint4 b = w;
     n += __popc(b.x) + __popc(b.y) + __popc(b.z) + __popc(b.w);
@@ -653,14 +664,16 @@ __device__ __forceinline__ int map_reach(Team<kStreamThreads>& team, const float
 }
 
 // Marks the best of a whole row, read again in each pass: for what the list does not hold.
+template <int T>
 __device__ __noinline__ void mark_row(Shared& sh, const float* x, int lo, int hi, int want, uint32_t* map) {
-  Team<kStreamThreads> team{sh, 1, 0};
-  const Read<kStreamThreads> run = {lo, hi, x};
+  Team<T> team{sh, 1, 0};
+  const Read<T> run = {lo, hi, x};
   mark_best(team, run, want, map);
 }
 
-__global__ void __launch_bounds__(kStreamThreads, 4) stream_kernel(const Args a) {
-  constexpr int kWarps = kStreamThreads / 32;
+template <int T>
+__global__ void __launch_bounds__(T, T == kStreamThreads ? 4 : 1) stream_kernel(const Args a) {
+  constexpr int kWarps = T / 32, kSample = kSampled / T;  // of a thread
   extern __shared__ __align__(16) uint8_t raw[];
   int* place = reinterpret_cast<int*>(raw);                        // candidates: positions
   int* order = place + kCandidates;                                // those selected
@@ -668,9 +681,9 @@ __global__ void __launch_bounds__(kStreamThreads, 4) stream_kernel(const Args a)
   __shared__ Shared sh;
   __shared__ uint32_t chosen[kCandidates / 32];                  // bitmap of the candidates
   const int tid = threadIdx.x, t = blockIdx.x;
-  Team<kStreamThreads> team{sh, 1, 0};
-  for (int i = tid; i < kBins; i += kStreamThreads) sh.hist[0][i] = 0;
-  for (int i = tid; i < kCandidates / 32; i += kStreamThreads) chosen[i] = 0;
+  Team<T> team{sh, 1, 0};
+  for (int i = tid; i < kBins; i += T) sh.hist[0][i] = 0;
+  for (int i = tid; i < kCandidates / 32; i += T) chosen[i] = 0;
   if (tid == 0) sh.owned = 0;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
@@ -683,7 +696,7 @@ __global__ void __launch_bounds__(kStreamThreads, 4) stream_kernel(const Args a)
   bool listed = false;   // they are all that is needed
   if (n > 0) {
     const int base = kept.lo - int(reinterpret_cast<uintptr_t>(x + kept.lo) & 15) / 4;
-    float t0 = kLowest, sampled = float(kSample * kStreamThreads), share = sampled / float(n);
+    float t0 = kLowest, sampled = float(kSampled), share = sampled / float(n);
     const float expect = float(kept.want) * share;
     float rank = fminf(expect + 6.f * sqrtf(expect) + 16.f, 0.8f * float(kCandidates) * share);
     rank = fmaxf(rank, expect + 1.f);
@@ -723,7 +736,7 @@ __global__ void __launch_bounds__(kStreamThreads, 4) stream_kernel(const Args a)
         t0 = kLowest;
       }
       __syncthreads();
-      for (int i = tid; i < kBins; i += kStreamThreads) sh.hist[0][i] = sh.hist[1][i] = 0;
+      for (int i = tid; i < kBins; i += T) sh.hist[0][i] = sh.hist[1][i] = 0;
       count = map_reach(team, x, base, kept.lo, kept.hi, t0, map);
       if (count <= kCandidates && (count >= kept.want || t0 == kLowest)) {
         listed = true;
@@ -740,7 +753,7 @@ __global__ void __launch_bounds__(kStreamThreads, 4) stream_kernel(const Args a)
       list_units(team, map, kept.hi - base, [&](int i, int bit) { place[i] = base + bit; });
       __syncthreads();
       if (count > kept.want) {
-        Held<kStreamThreads, kCandidates / kStreamThreads> run;
+        Held<T, kCandidates / T> run;
         run.begin = 0;
         run.end = count;
         run.gather(x, place);
@@ -748,30 +761,30 @@ __global__ void __launch_bounds__(kStreamThreads, 4) stream_kernel(const Args a)
       }
     } else {
       // The whole row, with a bitmap of it.
-      for (int i = tid; i < a.words; i += kStreamThreads) map[i] = 0;
+      for (int i = tid; i < a.words; i += T) map[i] = 0;
       __syncthreads();
-      mark_row(sh, x, kept.lo, kept.hi, kept.want, map);
+      mark_row<T>(sh, x, kept.lo, kept.hi, kept.want, map);
     }
     __syncthreads();
   }
   int taken = 0;
   if (listed && count <= kept.want) {
     taken = count;
-    for (int i = tid; i < taken; i += kStreamThreads) idx[kept.lo + i] = place[i];
+    for (int i = tid; i < taken; i += T) idx[kept.lo + i] = place[i];
   } else if (listed) {
     taken = list_units(team, reinterpret_cast<const uint16_t*>(chosen), count,
                        [&](int i, int bit) { order[i] = place[bit]; });
     __syncthreads();
-    for (int i = tid; i < taken; i += kStreamThreads) idx[kept.lo + i] = order[i];
+    for (int i = tid; i < taken; i += T) idx[kept.lo + i] = order[i];
   } else if (n > 0) {
     taken = list_units(team, map, n, [&](int i, int bit) { place[i] = kept.lo + bit; });
     __syncthreads();
-    for (int i = tid; i < taken; i += kStreamThreads) idx[kept.lo + i] = place[i];
+    for (int i = tid; i < taken; i += T) idx[kept.lo + i] = place[i];
   }
   const int behind = kept.count - kept.hi, all = kept.lo + taken + behind;
-  for (int i = tid; i < kept.lo; i += kStreamThreads) idx[i] = i;
-  for (int i = tid; i < behind; i += kStreamThreads) idx[kept.lo + taken + i] = kept.hi + i;
-  for (int i = all + tid; i < a.k; i += kStreamThreads) idx[i] = -1;
+  for (int i = tid; i < kept.lo; i += T) idx[i] = i;
+  for (int i = tid; i < behind; i += T) idx[kept.lo + taken + i] = kept.hi + i;
+  for (int i = all + tid; i < a.k; i += T) idx[i] = -1;
   if (tid == 0) a.len[t] = all;
 }
 
@@ -786,11 +799,14 @@ int sms_on(int device) {
   const int room = 200 * 1024;
   if (!cached[device] &&
       cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess &&
+      cudaFuncSetAttribute(hold_kernel<false, 4>, most, room) == cudaSuccess &&
+      cudaFuncSetAttribute(hold_kernel<true, 4>, most, room) == cudaSuccess &&
       cudaFuncSetAttribute(hold_kernel<false, 16>, most, room) == cudaSuccess &&
       cudaFuncSetAttribute(hold_kernel<false, 32>, most, room) == cudaSuccess &&
       cudaFuncSetAttribute(hold_kernel<true, 16>, most, room) == cudaSuccess &&
       cudaFuncSetAttribute(hold_kernel<true, 32>, most, room) == cudaSuccess &&
-      cudaFuncSetAttribute(stream_kernel, most, room) == cudaSuccess)
+      cudaFuncSetAttribute(stream_kernel<kLongThreads>, most, room) == cudaSuccess &&
+      cudaFuncSetAttribute(stream_kernel<kStreamThreads>, most, room) == cudaSuccess)
     cached[device] = n;
   return cached[device];
 }
@@ -843,8 +859,12 @@ extern "C" int32_t tq_index_select(const TqIndexSelectSpec* spec, int32_t* devic
   while (a.blocks < kMaxCluster && (items > a.blocks * kHold || (rows * a.blocks * 2 <= sms &&
                                                                  a.columns > 2 * kFew * a.blocks)))
     a.blocks *= 2;
-  // The row form streams its rows instead where clusters would not all run at once, or cannot hold a row.
-  const bool stream_rows = !pages && (rows * a.blocks > sms || items > a.blocks * kHold);
+  // The row form streams its rows instead where clusters would not all run at once, or cannot hold a row,
+  // unless they are short: then there is nothing to sample, and a block that holds its row reads it once
+  // (2000 x 2048, K 512: 29 us, streamed 46).
+  const bool stream_rows =
+      !pages && items > kHold / 8 && (rows * a.blocks > sms || items > a.blocks * kHold);
+  const bool alone = stream_rows && rows <= sms;
   const int list = (a.k + 3) / 4 * 16;
   uint32_t bytes;
   if (stream_rows) {
@@ -858,7 +878,7 @@ extern "C" int32_t tq_index_select(const TqIndexSelectSpec* spec, int32_t* devic
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(rows * a.blocks), 1, 1);
-  cfg.blockDim = dim3(stream_rows ? kStreamThreads : kThreads, 1, 1);
+  cfg.blockDim = dim3(alone ? kLongThreads : stream_rows ? kStreamThreads : kThreads, 1, 1);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
@@ -875,9 +895,12 @@ extern "C" int32_t tq_index_select(const TqIndexSelectSpec* spec, int32_t* devic
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const int n = (items + a.blocks - 1) / a.blocks;
-  const auto kernel = stream_rows ? stream_kernel
-                      : pages     ? n <= kHold / 2 ? hold_kernel<true, 16> : hold_kernel<true, 32>
-                                  : n <= kHold / 2 ? hold_kernel<false, 16> : hold_kernel<false, 32>;
+  const auto kernel = alone            ? stream_kernel<kLongThreads>
+                      : stream_rows    ? stream_kernel<kStreamThreads>
+                      : n <= kHold / 8 ? pages ? hold_kernel<true, 4> : hold_kernel<false, 4>
+                      : n <= kHold / 2 ? pages ? hold_kernel<true, 16> : hold_kernel<false, 16>
+                      : pages          ? hold_kernel<true, 32>
+                                       : hold_kernel<false, 32>;
   if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return fail("launch", TQ_ERR_CUDA);
   return fail(nullptr, TQ_OK);
 }

@@ -13,7 +13,9 @@
 // reduction. A block has one token's heads, 16 at a time, two of them a half warp: a lane's cosines
 // and sines stay in registers for all heads, and four lanes share the divisions of two. Keys, one a
 // token, have blocks of eight tokens of their own. Blocks are small so that many are at work on an SM:
-// their first steps are a chain of loads and the angles.
+// their first steps are a chain of loads and the angles. 8192 tokens of 64 heads take 58 us, 55% of
+// the copy bandwidth (99 with one block a token's 64 heads and the angles in shared memory); 64 tokens 8 us with
+// the launch.
 
 #include <cuda_runtime.h>
 

@@ -410,6 +410,17 @@ def test_select_of_many_rows(cuda_device):
     check_select(cuda_device, values("normal", rng, t, n), np.zeros(t, int), np.arange(n - t, n), np.array([n]), 512)
 
 
+@pytest.mark.parametrize("kind", VALUES)
+@pytest.mark.parametrize("t,n,k", [(40, 40003, 301), (148, 16390, 2051), (149, 16390, 60), (500, 1503, 200), (150, 2049, 9)])
+def test_select_of_rows_that_fill_the_card(cuda_device, kind, t, n, k):
+    """About as many rows as there are SMs, and many short ones."""
+    rng = np.random.default_rng(t + k)
+    score = values(kind, rng, t, n)
+    last = np.arange(n - t, n)
+    check_select(cuda_device, score, np.zeros(t, int), last, np.array([n]), k)
+    check_select(cuda_device, score, np.zeros(t, int), last, np.array([n]), k, None, 3, k // 2)
+
+
 @pytest.mark.parametrize("kind", ["normal", "equal", "runs low"])
 def test_select_of_the_longest_rows(cuda_device, kind):
     rng = np.random.default_rng(24)
