@@ -493,7 +493,8 @@ int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace, uint64_t works
  *   page_table i32 [S, L]     seq_id, pos i32 [T]     kv u8 [P, 64, 132]
  * Outer strides of q and k may be padded (multiples of 16, addresses too); w, q_out and w_out are
  * packed. Rows that have no place are skipped with the flags of tq_kv_write; their q_out and w_out
- * are still made. One launch; the grid depends only on the shapes. */
+ * are still made. The positions of a call's tokens are distinct: where two tokens name one cache row,
+ * it may hold parts of both. One launch; the grid depends only on the shapes. */
 typedef struct {
   TqTensorSpec q, k, w, page_table, seq_id, pos, kv, q_out, w_out, norm_weight, norm_bias, freq;
   int32_t rope_start, rope_half;
