@@ -15,15 +15,18 @@
 //                  the threshold is listed; these are counted and ranked. Where too few or too many
 //                  reach it, it is moved and the row read again; where that does not help (more equal
 //                  scores than the list holds) the whole row is counted. The blocks are small, four on
-//                  an SM, where there are many, since each has a chain of barriers that the others
-//                  fill; where a row has an SM to itself they are large (64 rows of 131072, K 2048:
-//                  36 us instead of 84).
+//                  an SM, where there are many, since each has a chain of barriers that the others fill
+//                  (of half the size: 90 us instead of 74 for 2048 rows of 16384); they are large where a
+//                  row has an SM to itself (64 rows of 131072, K 2048: 26 us instead of 84), and for
+//                  long rows (600 of 65536: 69 us; with the small blocks' sample of 2048 one row in
+//                  thirty missed its threshold, 87)
 //
 // What bounds it (times back to back, scores in L2 where they fit): few rows are a chain of loads and
 // barriers (1 x 8192: 6 us; 64 x 32768, K 2048: 16 us, one count, one rank and the cluster's barriers,
-// for 1.1 us of reading). Many rows are bound by instructions (2048 x 16384, K 2048: 78 us at 28% of
-// the copy bandwidth; about 32000 of a warp a row, two thirds of them for the 2500 candidates). Pages:
-// 64 x 131072 12.5 us, 41% of it: one wave of maxima, then the chain.
+// for 1.1 us of reading). Many rows are bound by the latency of the same chain, four rows an SM at a
+// time, and by instructions: 2048 x 16384, K 2048: 74 us, a third of it the sample and its threshold, a
+// fifth the row's one reading, the rest the 2700 candidates. Pages: 64 x 131072 12.5 us, 41% of the copy
+// bandwidth: one wave of maxima, then the chain.
 
 #include <cuda_runtime.h>
 
@@ -42,10 +45,9 @@ constexpr int kThreads = 512;          // of hold_kernel
 constexpr int kHold = 32 * kThreads;   // scores that a block of it holds, in registers
 constexpr int kMaxCluster = 8;
 constexpr int kStreamThreads = 256;    // of stream_kernel where there are many rows,
-constexpr int kLongThreads = 1024;     // and where a row has an SM to itself
-constexpr int kCandidates = 4096;      // of stream_kernel
-constexpr int kSampled = 2048;         // scores that it samples
+constexpr int kLongThreads = 512;      // and where a row has an SM to itself, or is long
 constexpr int kPageRows = 64;
+constexpr int kLongRow = 32768;        // longer rows want a larger sample than a small block's
 constexpr int kBins = 1024;
 constexpr int kRanked = 64;            // scores that are ranked against each other
 constexpr float kLowest = -3.402823466e38f;
@@ -610,46 +612,40 @@ __device__ __forceinline__ uint32_t spread(uint32_t x) {
 }
 
 // A bitmap of the scores x[lo, hi) that reach `t` > -inf, from position `base` on (a multiple of 16 bytes
-// at or before lo), and how many they are. Vectors of four are read; those that reach over an end, one
-// score at a time.
+// at or before lo), and how many they are.
 template <int T>
 __device__ __forceinline__ int map_reach(Team<T>& team, const float* x, int base, int lo, int hi,
                                          float t, uint32_t* map) {
-  constexpr int kWarps = T / 32, kVectors = 4;
+  constexpr int kWarps = T / 32, kBatch = 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int vectors = (hi - base + 3) >> 2, whole0 = lo > base, whole1 = (hi - base) >> 2;
+  // Four ballots a group of 128 scores: word c has lane l's score c. Lanes 0 to 3 write one each.
+  auto reach = [&](const float4& v, int g) {
+    const unsigned b0 = __ballot_sync(0xFFFFFFFFu, v.x >= t), b1 = __ballot_sync(0xFFFFFFFFu, v.y >= t);
+    const unsigned b2 = __ballot_sync(0xFFFFFFFFu, v.z >= t), b3 = __ballot_sync(0xFFFFFFFFu, v.w >= t);
+    if (lane < 4) map[4 * g + lane] = lane == 0 ? b0 : lane == 1 ? b1 : lane == 2 ? b2 : b3;
+  };
+  // Those within [lo, hi), a batch's loads first; a warp's last group again where a batch reaches past.
+  const int whole0 = lo > base, whole1 = (hi - base) >> 7;
+  const float4* from = reinterpret_cast<const float4*>(x + base) + lane;
 #pragma unroll 1
-  for (int g0 = warp * kVectors; 32 * g0 < vectors; g0 += kWarps * kVectors) {
-    float4 v[kVectors];
-    // All loads first, without a branch.
-    if (whole1 > whole0) {
+  for (int g0 = whole0 + warp * kBatch; g0 < whole1; g0 += kWarps * kBatch) {
+    float4 v[kBatch];
 #pragma unroll
-      for (int j = 0; j < kVectors; ++j)
-        v[j] = *reinterpret_cast<const float4*>(x + base + 4 * min(max(32 * (g0 + j) + lane, whole0), whole1 - 1));
-    }
+    for (int j = 0; j < kBatch; ++j) v[j] = from[32 * min(g0 + j, whole1 - 1)];
 #pragma unroll
-    for (int j = 0; j < kVectors; ++j) {
-      const int i = 32 * (g0 + j) + lane, at = base + 4 * i;
-      if (i < whole0 || i >= whole1) {
-        v[j].x = at >= lo && at < hi ? x[at] : -INFINITY;
-        v[j].y = at + 1 >= lo && at + 1 < hi ? x[at + 1] : -INFINITY;
-        v[j].z = at + 2 >= lo && at + 2 < hi ? x[at + 2] : -INFINITY;
-        v[j].w = at + 3 >= lo && at + 3 < hi ? x[at + 3] : -INFINITY;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < kVectors; ++j) {
-      // Four ballots: word c has lane l's score c. Lanes 0 to 3 write one each.
-      const unsigned b0 = __ballot_sync(0xFFFFFFFFu, v[j].x >= t), b1 = __ballot_sync(0xFFFFFFFFu, v[j].y >= t);
-      const unsigned b2 = __ballot_sync(0xFFFFFFFFu, v[j].z >= t), b3 = __ballot_sync(0xFFFFFFFFu, v[j].w >= t);
-      if (lane < 4 && 32 * (g0 + j) < vectors)
-        map[4 * (g0 + j) + lane] = lane == 0 ? b0 : lane == 1 ? b1 : lane == 2 ? b2 : b3;
-    }
+    for (int j = 0; j < kBatch; ++j) reach(v[j], min(g0 + j, whole1 - 1));
+  }
+  // Those at the ends, if any.
+  const int groups = (hi - base + 127) >> 7;
+  if (warp < 2 && (warp == 0 ? whole0 : groups > max(whole0, whole1))) {
+    const int g = warp == 0 ? 0 : groups - 1, at = base + 128 * g + 4 * lane;
+    auto one = [&](int i) { return i >= lo && i < hi ? x[i] : -INFINITY; };
+    reach(make_float4(one(at), one(at + 1), one(at + 2), one(at + 3)), g);
   }
   __syncthreads();
   // Each group of four words into the order of positions.
   int n = 0;
-  for (int g = threadIdx.x; g < (vectors + 31) / 32; g += T) {
+  for (int g = threadIdx.x; g < groups; g += T) {
     uint4& w = reinterpret_cast<uint4*>(map)[g];
     const uint4 b = w;
     n += __popc(b.x) + __popc(b.y) + __popc(b.z) + __popc(b.w);
@@ -671,15 +667,21 @@ __device__ __noinline__ void mark_row(Shared& sh, const float* x, int lo, int hi
   mark_best(team, run, want, map);
 }
 
+// Scores that it lists: a small block 13 a thread, which leaves it registers, and room beside the most
+// that can be asked for.
 template <int T>
-__global__ void __launch_bounds__(T, T == kStreamThreads ? 4 : 1) stream_kernel(const Args a) {
-  constexpr int kWarps = T / 32, kSample = kSampled / T;  // of a thread
+constexpr int kCandidates = T == kStreamThreads ? 13 * T : 8 * T;
+
+template <int T>
+__global__ void __launch_bounds__(T, T == kStreamThreads ? 4 : 2) stream_kernel(const Args a) {
+  constexpr int kWarps = T / 32, kCandidates = index_select::kCandidates<T>;
+  constexpr int kSample = T == kStreamThreads ? 8 : 16;  // scores of a thread
   extern __shared__ __align__(16) uint8_t raw[];
   int* place = reinterpret_cast<int*>(raw);                        // candidates: positions
   int* order = place + kCandidates;                                // those selected
   uint32_t* map = reinterpret_cast<uint32_t*>(order + (a.k + 3) / 4 * 4);
   __shared__ Shared sh;
-  __shared__ uint32_t chosen[kCandidates / 32];                  // bitmap of the candidates
+  __shared__ __align__(16) uint32_t chosen[kCandidates / 32];    // bitmap of the candidates
   const int tid = threadIdx.x, t = blockIdx.x;
   Team<T> team{sh, 1, 0};
   for (int i = tid; i < kBins; i += T) sh.hist[0][i] = 0;
@@ -696,7 +698,7 @@ __global__ void __launch_bounds__(T, T == kStreamThreads ? 4 : 1) stream_kernel(
   bool listed = false;   // they are all that is needed
   if (n > 0) {
     const int base = kept.lo - int(reinterpret_cast<uintptr_t>(x + kept.lo) & 15) / 4;
-    float t0 = kLowest, sampled = float(kSampled), share = sampled / float(n);
+    float t0 = kLowest, sampled = float(kSample * T), share = sampled / float(n);
     const float expect = float(kept.want) * share;
     float rank = fminf(expect + 6.f * sqrtf(expect) + 16.f, 0.8f * float(kCandidates) * share);
     rank = fmaxf(rank, expect + 1.f);
@@ -707,7 +709,7 @@ __global__ void __launch_bounds__(T, T == kStreamThreads ? 4 : 1) stream_kernel(
 #pragma unroll
         for (int j = 0; j < kSample; ++j) {
           const int r = j * 2 * kWarps + (tid >> 4);
-          s[j] = x[kept.lo + int((long long)r * (n - 16) / (kSample * 2 * kWarps)) + (tid & 15)];
+          s[j] = x[kept.lo + int(uint32_t(r * (n - 16)) / (kSample * 2 * kWarps)) + (tid & 15)];
         }
         if (attempt == 0 && tid == 0)  // the whole row is on its way to L2 meanwhile
           ptx::bulk_prefetch_l2(x + base + (kept.lo > base ? 4 : 0),
@@ -742,12 +744,10 @@ __global__ void __launch_bounds__(T, T == kStreamThreads ? 4 : 1) stream_kernel(
         listed = true;
         break;
       }
-      if (count < kept.want) {
-        rank *= 1.5f * float(kept.want) / float(max(count, kept.want / 8 + 1));
-      } else {
-        rank *= 0.75f * float(kCandidates) / float(count);
-        if (rank < expect) break;
-      }
+      // Half way between too few and too many, by what this threshold gave. (Many equal ones: no use.)
+      rank *= 0.5f * float(kept.want + kCandidates) / float(max(count, kept.want / 8 + 1));
+      if (rank < 0.5f * expect) break;
+      rank = fmaxf(rank, 1.f);
     }
     if (listed) {
       list_units(team, map, kept.hi - base, [&](int i, int bit) { place[i] = base + bit; });
@@ -864,13 +864,13 @@ extern "C" int32_t tq_index_select(const TqIndexSelectSpec* spec, int32_t* devic
   // (2000 x 2048, K 512: 29 us, streamed 46).
   const bool stream_rows =
       !pages && items > kHold / 8 && (rows * a.blocks > sms || items > a.blocks * kHold);
-  const bool alone = stream_rows && rows <= sms;
+  const bool large = stream_rows && (rows <= sms || items > kLongRow);
   const int list = (a.k + 3) / 4 * 16;
   uint32_t bytes;
   if (stream_rows) {
     a.blocks = 1;
     a.words = ((items + 127) / 128 + 1) * 4;
-    bytes = uint32_t(kCandidates * 4 + list + a.words * 4);
+    bytes = uint32_t((large ? kCandidates<kLongThreads> : kCandidates<kStreamThreads>) * 4 + list + a.words * 4);
   } else {
     const int each = (items + a.blocks - 1) / a.blocks;
     a.words = (each + 31) / 32;
@@ -878,7 +878,7 @@ extern "C" int32_t tq_index_select(const TqIndexSelectSpec* spec, int32_t* devic
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(rows * a.blocks), 1, 1);
-  cfg.blockDim = dim3(alone ? kLongThreads : stream_rows ? kStreamThreads : kThreads, 1, 1);
+  cfg.blockDim = dim3(large ? kLongThreads : stream_rows ? kStreamThreads : kThreads, 1, 1);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
@@ -895,7 +895,7 @@ extern "C" int32_t tq_index_select(const TqIndexSelectSpec* spec, int32_t* devic
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const int n = (items + a.blocks - 1) / a.blocks;
-  const auto kernel = alone            ? stream_kernel<kLongThreads>
+  const auto kernel = large            ? stream_kernel<kLongThreads>
                       : stream_rows    ? stream_kernel<kStreamThreads>
                       : n <= kHold / 8 ? pages ? hold_kernel<true, 4> : hold_kernel<false, 4>
                       : n <= kHold / 2 ? pages ? hold_kernel<true, 16> : hold_kernel<false, 16>
