@@ -11,20 +11,22 @@
 //                  reduces its scores to a value a page first, and does the same with those
 //   stream_kernel  more rows, or longer ones, than clusters hold at once: a block a token. A sample of
 //                  the row gives a threshold that a little more than K scores reach (how much more: six
-//                  standard deviations of the sample's count); the row is read once and what reaches
-//                  the threshold is listed; these are counted and ranked. Where too few or too many
-//                  reach it, it is moved and the row read again; where that does not help (more equal
-//                  scores than the list holds) the whole row is counted. The blocks are small, four on
-//                  an SM, where there are many, since each has a chain of barriers that the others fill
-//                  (of half the size: 90 us instead of 74 for 2048 rows of 16384); they are large where a
-//                  row has an SM to itself (64 rows of 131072, K 2048: 26 us instead of 84), and for
-//                  long rows (600 of 65536: 69 us; with the small blocks' sample of 2048 one row in
-//                  thirty missed its threshold, 87)
+//                  standard deviations of the sample's count, or as many as the list has room for); the
+//                  row is read once and what reaches the threshold is listed; these are counted and
+//                  ranked. Where too few or too many reach it, it is moved and the row read again; where
+//                  that does not help (more equal scores than the list holds) the whole row is counted.
+//                  The blocks are small, five on an SM, where there are many, since each has a chain of
+//                  barriers that the others fill (of half the size: 90 us instead of 74 for 2048 rows of
+//                  16384, then with four on an SM). Their sample is 1024 scores: of 2048 the chain
+//                  was longer (74 us, now 67; with the fifth block 64) and a threshold missed more
+//                  seldom than one in a thousand. They are large where a row has an SM to itself (64 rows
+//                  of 131072, K 2048: 26 us instead of 84), and for long rows (600 of 65536: 69 us; one
+//                  small block in thirty missed its threshold, 87).
 //
 // What bounds it (times back to back, scores in L2 where they fit): few rows are a chain of loads and
 // barriers (1 x 8192: 6 us; 64 x 32768, K 2048: 16 us, one count, one rank and the cluster's barriers,
-// for 1.1 us of reading). Many rows are bound by the latency of the same chain, four rows an SM at a
-// time, and by instructions: 2048 x 16384, K 2048: 74 us, a third of it the sample and its threshold, a
+// for 1.1 us of reading). Many rows are bound by the latency of the same chain, five rows an SM at a
+// time, and by instructions: 2048 x 16384, K 2048: 64 us, a third of it the sample and its threshold, a
 // fifth the row's one reading, the rest the 2700 candidates. Pages: 64 x 131072 12.5 us, 41% of the copy
 // bandwidth: one wave of maxima, then the chain.
 
@@ -673,9 +675,9 @@ template <int T>
 constexpr int kCandidates = T == kStreamThreads ? 13 * T : 8 * T;
 
 template <int T>
-__global__ void __launch_bounds__(T, T == kStreamThreads ? 4 : 2) stream_kernel(const Args a) {
+__global__ void __launch_bounds__(T, T == kStreamThreads ? 5 : 2) stream_kernel(const Args a) {
   constexpr int kWarps = T / 32, kCandidates = index_select::kCandidates<T>;
-  constexpr int kSample = T == kStreamThreads ? 8 : 16;  // scores of a thread
+  constexpr int kSample = T == kStreamThreads ? 4 : 16;  // scores of a thread
   extern __shared__ __align__(16) uint8_t raw[];
   int* place = reinterpret_cast<int*>(raw);                        // candidates: positions
   int* order = place + kCandidates;                                // those selected
