@@ -20,12 +20,16 @@
 //         weights in registers for a whole run, four keys a thread; what a thread adds for a key and
 //         a head is 1.5 instructions (a maximum, half of a packed multiply-add)
 //
-// What bounds it (times back to back): many tokens, the sum warps' instructions: 2048 tokens of 64 heads
-// over 16384 rows 161 us, where the E4M3 products alone would take 72 and the maximum and the
-// multiply-add of each dot, issued without a pause, about 110. Few tokens: 64 requests of 16384 to 32768
-// rows 60 us at 56% of the copy bandwidth (loads alone take 24, the sums without loads 35: they meet in
-// the four stages of keys, and neither fewer nor more of them or of the tiles a step was faster); one
-// token of 8192 rows 7 us, launch and one chain of loads, products and sums.
+// What bounds it (times back to back): many tokens, the hand-overs between the MMAs and the sums. 2048
+// tokens of 64 heads over 8192 rows take 163 us, where the products alone would take 72; without the
+// arithmetic of the sums it is 126, without their reads of TMEM 131: a step's MMAs, its commit, its sums
+// and their arrival follow one another in each half of TMEM, and two halves hide half of that. (Sixteen
+// warps a step instead of eight: the same time. MMAs issued by a converged warp cost half as much,
+// 145 cycles for four, and the call took 171 us.) Few tokens, the loads: 64 requests of 16384 to 32768 rows
+// 56 us at 60% of the copy bandwidth, 50 without the scales' loads and the sums. TMA takes about 7 cycles
+// for a row of 128 bytes at a pitch of 144; seven stages instead of four, or pages brought to L2 ahead (the
+// same engine: 76 us), do not help. One token of 8192 rows 7 us, launch and one chain of loads, products
+// and sums.
 // Waits are bounded (about 2 s); one that gives up sets TQ_DEV_WAIT_TIMEOUT and ends its warp's work.
 
 #include <cuda.h>
