@@ -138,7 +138,8 @@ __device__ __forceinline__ int sees(const Args& a, int s, int pos, int* bad) {
 __device__ __forceinline__ int tile_cost(const Args& a, int tokens) {
   return 4 + (tokens * a.heads + 63) / 64;
 }
-__device__ __forceinline__ int tiles_of(int most) { return (most + kKeys - 1) / kKeys; }
+// (No sum with `most`: it may be 2^31 - 1.)
+__device__ __forceinline__ int tiles_of(int most) { return most / kKeys + (most % kKeys != 0); }
 
 // Sequence and rows seen of four tokens from t on, up to `end`: from the cache, or with their loads in
 // flight together.
@@ -292,10 +293,11 @@ __device__ __forceinline__ void produce(const Args& a, Shared& sh, const CUtenso
         __syncwarp();
         ++units;
         const int* table = a.page_table + (long long)first * a.slots;
+        const int seen_pages = most / kPageRows + (most % kPageRows != 0);
         // Page entries 32 at a time, the next ones on their way; behind the last row that the run sees
         // there are none.
         auto entries = [&](int base) {
-          const bool seen = base + lane < a.slots && (base + lane) * kPageRows < most;
+          const bool seen = base + lane < min(a.slots, seen_pages);
           const int page = seen ? table[base + lane] : -1;
           if (page >= 0 && page < a.pages) return page * kPageRows;
           if (seen && a.flags) atomicOr(a.flags, TQ_DEV_PAGE_RANGE);
@@ -528,7 +530,8 @@ __device__ __forceinline__ void sum_heads_in_registers(const Args& a, Shared& sh
       const int* seen = unit.sees + t0 + place;
       uint8_t* out = a.scores + (long long)(unit.t0 + t0 + place) * a.score_stride +
                      4ll * (unit.tile0 * kKeys + key);
-      int n = unit.tile0 * kKeys + key, step = steps + (t0 != 0);
+      uint32_t n = uint32_t(unit.tile0 * kKeys + key);  // (one tile on from the last it may pass 2^31)
+      int step = steps + (t0 != 0);
       for (int j = 0; j < tiles; ++j, step += 2, n += kKeys, out += 4 * kKeys) {
         const int slot = (tile + j) % kScaleSlots;
         if (!wait.warp_on(sh.bar_acc_full[half], uint32_t(step >> 1) & 1u)) return;
@@ -546,7 +549,7 @@ __device__ __forceinline__ void sum_heads_in_registers(const Args& a, Shared& sh
           const float sum = sum_heads_of<kH>(tmem + uint32_t((place + i) * kH), w + i * (kH / 8), lane, [&] {
             if (i + 1 >= mine) done();
           });
-          if (n < seen[i]) *reinterpret_cast<float*>(to) = sum * scale;
+          if (n < uint32_t(seen[i])) *reinterpret_cast<float*>(to) = sum * scale;
           to += a.score_stride;
         }
       }
