@@ -365,13 +365,20 @@ __device__ __forceinline__ bool multiply(const Args& a, Shared& sh) {
   // Rows of 128 bytes, K-major, 128-byte swizzle: 8-row groups 1 KB apart.
   const uint64_t keys0 = ptx::smem_desc(ptx::smem_addr(sh.key[0]), 16, 1024, 2);
   const uint64_t queries0 = ptx::smem_desc(ptx::smem_addr(sh.query[0]), 16, 1024, 2);
-  int s = 0;
+  int s = 0, tile = 0;  // tiles of all units before this
   uint32_t key_parity = 0, steps = 0;
+  // The arrivals that nobody else waits for, of the last key stages and the last unit, must not find a CTA
+  // that has ended, and its shared memory another's. They are there before the last sums are.
+  auto settled = [&](int units) {
+    for (int i = max(0, tile - kStages); i < tile; ++i)
+      if (!wait.on(sh.bar_key_empty[i % kStages], uint32_t(i / kStages) & 1u)) return false;
+    return units == 0 || wait.on(sh.bar_unit_empty[(units - 1) & 1], uint32_t((units - 1) >> 1) & 1u);
+  };
   for (int units = 0;; ++units) {
     const int u = units & 1;
     if (!wait.on(sh.bar_unit_full[u], uint32_t(units >> 1) & 1u)) return false;
     const int tokens = sh.unit[u].tokens, tiles = sh.unit[u].tiles;
-    if (tokens == 0) return true;
+    if (tokens == 0) return settled(units);
     const uint64_t queries = queries0 + uint64_t(u) * (kQueryBytes >> 4);
     // Columns in whole sixteens: the last ones may be of no token, and nobody reads them.
     auto idesc = [&](int n) { return ptx::idesc_e4m3(kKeys, uint32_t(n * a.heads + 15) & ~15u); };
@@ -409,6 +416,7 @@ __device__ __forceinline__ bool multiply(const Args& a, Shared& sh) {
       ++steps;
     }
     ptx::mma_commit(ptx::smem_addr(&sh.bar_unit_empty[u]));
+    tile += tiles;
   }
 }
 
