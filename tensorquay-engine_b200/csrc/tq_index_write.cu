@@ -139,7 +139,8 @@ __device__ __forceinline__ void normalise(const Args& a, const Place<F>& place, 
   s = 0.f;
   each(x, x, [&](float v, float) { s = fmaf(v, v, s); return v; });
   const float r = 1.f / sqrtf(sum16(s) * (1.f / TQ_INDEX_DIM) + a.eps);
-  each(x, w, [&](float v, float by) { return v * (r * by); });
+  // (In this order: r times a large weight may overflow where the value times r is small or 0.)
+  each(x, w, [&](float v, float by) { return v * r * by; });
   if (a.norm_bias) each(x, unpack<F>(place.load(a.norm_bias)), [](float v, float b) { return v + b; });
 }
 
