@@ -491,10 +491,11 @@ int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace, uint64_t works
  *   k      bf16 [T, 128]      norm_weight, norm_bias bf16 [128] or rank 0
  *   freq   f32 [R / 2] or rank 0 (R = 0); R a multiple of 16, rope_start of 8, their sum <= 128
  *   page_table i32 [S, L]     seq_id, pos i32 [T]     kv u8 [P, 64, 132]
- * Outer strides of q and k may be padded (multiples of 16, addresses too); w, q_out and w_out are
- * packed. Rows that have no place are skipped with the flags of tq_kv_write; their q_out and w_out
- * are still made. The positions of a call's tokens are distinct: where two tokens name one cache row,
- * it may hold parts of both. One launch; the grid depends only on the shapes. */
+ * Outer strides of q and k may be padded (multiples of 16, addresses too; heads less than 2^36 bytes
+ * apart); w, q_out and w_out are packed. Rows that have no place are skipped with the flags of
+ * tq_kv_write; their q_out and w_out are still made. The positions of a call's tokens are distinct:
+ * where two tokens name one cache row, it may hold parts of both. One launch; the
+ * grid depends only on the shapes. */
 typedef struct {
   TqTensorSpec q, k, w, page_table, seq_id, pos, kv, q_out, w_out, norm_weight, norm_bias, freq;
   int32_t rope_start, rope_half;

@@ -640,6 +640,9 @@ int32_t index_write_validate_impl(const TqIndexWriteSpec* spec, TqContractError*
     if (!std::isfinite(s.rope_mscale)) return fail("rope_mscale", TQ_SCALE);
   }
   if (queries && !std::isfinite(s.scale)) return fail("scale", TQ_SCALE);
+  // The kernel counts the distance between heads in sixteen bytes, in 32 bits.
+  if (launching && queries && H > 1 && s.q.strides_bytes[1] >= uint64_t(1) << 36)
+    return fail("q", TQ_OVERFLOW);
   if (launching) {
     const TqTensorSpec* all[5] = {&s.q, &s.k, &s.q_out, &s.norm_weight, &s.norm_bias};
     const char* names[5] = {"q", "k", "q_out", "norm_weight", "norm_bias"};
