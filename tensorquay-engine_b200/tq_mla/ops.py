@@ -554,7 +554,11 @@ INDEX_ROW_BYTES = 132
 
 def index_pool_spec(kv):
     """An index cache u8 ``[P, 64, r]`` (rows of 128 E4M3 codes and an f32 scale in ``r`` >= 144
-    bytes, a multiple of 16), declared as ``[P, 64, 132]``."""
+    bytes, a multiple of 16), declared as ``[P, 64, 132]``. Its rows are contiguous."""
+    if kv.dim() != 3 or kv.shape[2] * kv.element_size() < INDEX_ROW_BYTES:
+        raise ContractError("kv", 1)
+    if kv.stride(2) != 1:
+        raise ContractError("kv", 4)
     return tensor_spec([kv.shape[0], kv.shape[1], INDEX_ROW_BYTES],
                        [kv.stride(0) * kv.element_size(), kv.stride(1) * kv.element_size(), 1],
                        _abi.DTYPE_U8, kv.data_ptr(), _capacity(kv))
