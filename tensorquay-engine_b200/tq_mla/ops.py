@@ -552,6 +552,14 @@ def mla_chunk(q, w_uk, w_uv, kv, page_table, q_start, q_pos, kv_len, *, scale, m
 INDEX_ROW_BYTES = 132
 
 
+def _int32(field, value):
+    """A number of a declaration (which would keep its low 32 bits alone)."""
+    value = int(value)
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise ContractError(field, 3)
+    return value
+
+
 def index_pool_spec(kv):
     """An index cache u8 ``[P, 64, r]`` (rows of 128 E4M3 codes and an f32 scale in ``r`` >= 144
     bytes, a multiple of 16), declared as ``[P, 64, 132]``. Its rows are contiguous."""
@@ -596,7 +604,7 @@ def index_write_spec(q, k, w, page_table, seq_id, pos, kv, q_out, w_out, *, scal
         if t is not None:
             setattr(s, name, spec_of(t))
     s.kv = index_pool_spec(kv)
-    s.rope_start, s.rope_half = int(rope_start), int(bool(rope_half))
+    s.rope_start, s.rope_half = _int32("rope_start", rope_start), int(bool(rope_half))
     s.rope_mscale, s.norm_eps, s.scale = float(rope_mscale), float(eps), float(scale)
     return s
 
@@ -686,7 +694,7 @@ def index_select_spec(scores, seq_id, q_pos, kv_len, idx, length, *, page_table=
                     ("page_table", page_table), ("idx", idx), ("len", length)):
         if t is not None:
             setattr(s, name, spec_of(t))
-    s.keep_first, s.keep_last = int(keep_first), int(keep_last)
+    s.keep_first, s.keep_last = _int32("keep_first", keep_first), _int32("keep_last", keep_last)
     return s
 
 

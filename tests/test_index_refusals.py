@@ -4,7 +4,7 @@ it is. CPU only."""
 import pytest
 import torch
 
-from test_index_contract import GiB, OK, SHAPE, STRIDE, changed, verdict, write
+from test_index_contract import DIMENSION, GiB, OK, SHAPE, STRIDE, changed, verdict, write
 from tq_mla import ops
 
 OVERFLOW = 8
@@ -33,3 +33,17 @@ def test_pools_whose_rows_are_not_132_bytes_in_a_row():
         s = ops.index_pool_spec(kv)
         assert list(s.shape) == [3, 64, 132] and s.strides_bytes[2] == 1
         assert s.strides_bytes[1] == kv.stride(1) * kv.element_size()
+
+
+@pytest.mark.parametrize("field", ["keep_first", "keep_last", "rope_start"])
+@pytest.mark.parametrize("value", [2 ** 32, 2 ** 32 + 8, 2 ** 31, -2 ** 32, -2 ** 31 - 1])
+def test_numbers_past_32_bits(field, value):
+    """Their low 32 bits would be numbers that are accepted."""
+    i, f = torch.zeros(1, dtype=torch.int32), torch.zeros((1, 9))
+    with pytest.raises(ops.ContractError) as e:
+        if field == "rope_start":
+            kv = torch.zeros((1, 64, 144), dtype=torch.uint8)
+            ops.index_write_spec(None, torch.zeros((1, 128), dtype=torch.bfloat16), None, i[None], i, i, kv, None, None, rope_start=value)
+        else:
+            ops.index_select_spec(f, i, i, i, i[None], i, **{field: value})
+    assert (e.value.field, e.value.kind) == (field, DIMENSION)
