@@ -31,6 +31,7 @@
 
 #include "tq_contracts.h"
 #include "tq_ptx.cuh"
+#include "tq_tensor_map.h"
 
 namespace tq {
 namespace chunk {
@@ -1488,25 +1489,6 @@ Layout layout_of(const TqMlaChunkSpec& s) {
   l.v = take(l.pass_heads * l.cap * dv * 2);
   l.total = at;
   return l;
-}
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
 }
 
 // bf16 boxes of 64 values by `box` rows (and one of the third axis) with 128-byte swizzle.

@@ -37,6 +37,7 @@
 #include "tq_contracts.h"
 #include "tq_mla_layout.h"
 #include "tq_ptx.cuh"
+#include "tq_tensor_map.h"
 
 namespace tq {
 namespace mla {
@@ -1449,25 +1450,6 @@ __global__ void gen_kv_rows_kernel(char* pool, uint64_t row_stride, uint64_t wid
 
 // ---------------------------------------------------------------------------------------------
 // Host glue.
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
 
 bool encode_bf16(CUtensorMap* map, const void* addr, int rank, const cuuint64_t* dims,
                  const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swz) {

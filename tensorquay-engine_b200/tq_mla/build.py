@@ -9,9 +9,9 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG.parent / "csrc"
 SOURCES = ["tq_mla_kernels.cu", "tq_kv_write.cu", "tq_prologue.cu", "tq_proj.cu", "tq_peer_merge.cu",
-           "tq_step.cu", "tq_block_norm.cu",
-           "tq_chunk.cu", "tq_index_write.cu", "tq_index_scores.cu", "tq_index_select.cu", "tq_contracts.cpp", "tq_comm.cpp"]
-HEADERS = ["tq_ptx.cuh", "tq_mla_layout.h", "tq_contracts.h"]
+           "tq_step.cu", "tq_block_norm.cu", "tq_chunk.cu", "tq_index_write.cu",
+           "tq_index_scores.cu", "tq_index_select.cu", "tq_contracts.cpp", "tq_comm.cpp"]
+HEADERS = ["tq_ptx.cuh", "tq_tensor_map.h", "tq_mla_layout.h", "tq_contracts.h"]
 TARGET = PKG / "libtq_mla.so"
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
