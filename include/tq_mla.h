@@ -487,7 +487,8 @@ int32_t tq_mla_chunk(const TqMlaChunkSpec* spec, void* workspace, uint64_t works
  * f32 up to the code (angles f64, reduced before the sine and cosine). Frequencies are the caller's,
  * so any scaling of positions for long contexts is theirs; rope_mscale goes with it.
  *   q      bf16 [T, H, 128], w bf16 or f32 [T, H], q_out u8 [T, H, 128], w_out f32 [T, H]: all or
- *          none (rank 0: only keys are written); H is 1 to 128
+ *          none (rank 0: only keys are written); H is 1 to 128 (tq_index_scores takes multiples of 8),
+ *          T at most 2^24
  *   k      bf16 [T, 128]      norm_weight, norm_bias bf16 [128] or rank 0
  *   freq   f32 [R / 2] or rank 0 (R = 0); R a multiple of 16, rope_start of 8, their sum <= 128
  *   page_table i32 [S, L]     seq_id, pos i32 [T]     kv u8 [P, 64, 132]
@@ -509,10 +510,13 @@ int32_t tq_index_write(const TqIndexWriteSpec* spec, int32_t* device_flags, void
  *   scores[t, n] = key_scale[n] * sum_h w[t, h] * max(0, q[t, h] . k[n])
  * over the codes, in f32. Columns from sees(t) on keep their values.
  *   q      u8 [T, H, 128] E4M3 codes and w f32 [T, H], as tq_index_write makes them; H is a
- *          multiple of 8 up to 128
- *   kv     u8 [P, 64, 132]    page_table i32 [S, L]    seq_id, q_pos i32 [T]    kv_len i32 [S]
+ *          multiple of 8 up to 128. Other numbers of heads are filled up with heads of zeros, in the
+ *          q and w of tq_index_write already: they change no score. (A multiple of 16 is faster.)
+ *   kv     u8 [P, 64, 132], P < 2^25    page_table i32 [S, L]    seq_id, q_pos i32 [T]    kv_len i32 [S]
  *   scores f32 [T, N], outer stride may be padded
- * A code or scale that is NaN makes the scores that use it NaN and no others. In `device_flags`:
+ * T is at most 2^24 and T H below 2^31.
+ * A code or scale that is NaN makes the scores that use it NaN and no others. Where the magnitudes
+ * |w| max(0, q . k) of a score add up to 2^127 or more, it may become infinite or NaN. In `device_flags`:
  * TQ_DEV_SEQ_RANGE (the token's row is left as it was), TQ_DEV_TABLE_SHORT (sees(t) past 64 L, cut),
  * TQ_DEV_WORK_OVERFLOW (sees(t) past N, cut), TQ_DEV_PAGE_RANGE (a page outside the pool: its rows
  * read as zeros), TQ_DEV_WAIT_TIMEOUT. Consecutive tokens of one sequence share its rows' loads.
@@ -535,7 +539,7 @@ int32_t tq_index_scores(const TqIndexScoresSpec* spec, int32_t* device_flags, vo
  * The first keep_first and the last keep_last of the positions (pages) that a token sees are always
  * selected. Equal scores go to the lowest position. A score of -inf (masked) or NaN is not selected
  * (where it is not kept), so a row may end with fewer than K, or none.
- *   scores f32 [T, N], N <= 2^20, outer stride may be padded      seq_id, q_pos i32 [T]
+ *   scores f32 [T, N], T <= 2^24, N <= 2^20, outer stride may be padded      seq_id, q_pos i32 [T]
  *   kv_len i32 [S]    idx i32 [T, K], packed, K is 1 to TQ_MLA_MAX_TOPK    len i32 [T]
  *   keep_first, keep_last >= 0, their sum <= K
  * A token without a sequence (seq_id outside [0, S)) selects nothing and sets TQ_DEV_SEQ_RANGE.

@@ -2,9 +2,13 @@
 //   scores[t, n] = key_scale[n] * sum_h w[t, h] * max(0, q[t, h] . k[n]),  n < sees(t).
 //
 // The dots are E4M3 products on tcgen05 (kind::f8f6f4, f32 sums): 128 keys are the M of a tile, the
-// heads of up to 256 columns of query tokens its N, K = 128 in four steps. A key is then one lane
-// of TMEM, so the sum over heads stays in a thread: it reads its columns, cuts them at zero and
-// adds them up with the tokens' weights, and a warp writes 32 consecutive scores.
+// heads of up to 256 columns of query tokens its N, K = 128 in four steps. A key is then one lane of
+// TMEM. What reads its columns, cuts them at zero and adds them up with the tokens' weights takes one of
+// two forms, and either way a warp writes 32 consecutive scores:
+//   heads a multiple of 16   a thread has a part of the columns of four keys and its weights in registers;
+//                            the sums of four lanes are joined by three exchanges
+//   other multiples of 8     a thread has all columns of one key; weights from shared memory, no packing of
+//                            several tiles into a step
 //
 // Work: G consecutive tokens are a group (512 columns, 32 tokens at most); a run is a part of a group
 // with one sequence, and a unit of work a run over 128 keys. Every CTA sums the costs of all groups,
@@ -16,17 +20,17 @@
 //         4-byte copies by the warp's lanes took 1100 cycles a tile
 //   1     one lane issues the MMAs, a step into one of two halves of TMEM: a tile by half of a group's
 //         tokens, or up to kPack tiles by a run of few
-//   2-17  four groups of warps, two for each half of TMEM: the sums over heads. A warp has the tokens'
-//         weights in registers for a whole run, four keys a thread; what a thread adds for a key and
-//         a head is 1.5 instructions (a maximum, half of a packed multiply-add)
+//   2-17  four groups of warps, two for each half of TMEM: the sums over heads. In the first form a warp
+//         has the tokens' weights in registers for a whole run; what a thread adds for a key and a head
+//         is 1.5 instructions (a maximum, half of a packed multiply-add)
 //
 // What bounds it (times back to back): many tokens, the hand-overs between the MMAs and the sums. 2048
-// tokens of 64 heads over 8192 rows take 163 us, where the products alone would take 72; without the
+// tokens of 64 heads over 8192 rows take 164 us (151 captured), where the products alone would take 72; without the
 // arithmetic of the sums it is 126, without their reads of TMEM 131: a step's MMAs, its commit, its sums
 // and their arrival follow one another in each half of TMEM, and two halves hide half of that. (Sixteen
 // warps a step instead of eight: the same time. MMAs issued by a converged warp cost half as much,
 // 145 cycles for four, and the call took 171 us.) Few tokens, the loads: 64 requests of 16384 to 32768 rows
-// 56 us at 60% of the copy bandwidth, 50 without the scales' loads and the sums. TMA takes about 7 cycles
+// 56 us (53 captured) at 60% of the copy bandwidth, 50 without the scales' loads and the sums. TMA takes about 7 cycles
 // for a row of 128 bytes at a pitch of 144; seven stages instead of four, or pages brought to L2 ahead (the
 // same engine: 76 us), do not help. One token of 8192 rows 7 us, launch and one chain of loads, products
 // and sums.
@@ -462,7 +466,7 @@ __device__ __forceinline__ void add_up(const uint32_t (&r)[8], const float* w, f
 // lanes: three exchanges leave one key's in each. `last` is called once all columns are read.
 // What bounds it: the instructions, 1.5 for each head of a key and token (its cut at zero, half of a
 // product and addition), a cut at half their rate. So the last of the four keys adds |x| to x
-// instead, twice the same, and halves its sum.
+// instead, twice the same, and halves its sum. (So that sum leaves f32 at half the size of the others.)
 template <int kH, typename Fn>
 __device__ __forceinline__ float sum_heads_of(uint32_t from, const float2* w, int lane, Fn last) {
   constexpr int kStep = kH % 32 ? 16 : 32, kChunks = kH / kStep;  // columns read at a time
@@ -608,7 +612,9 @@ __device__ __forceinline__ void sum_heads_in_registers(const Args& a, Shared& sh
 }
 
 // The same for other multiples of 8 heads, one key a thread: a token's columns are read eight at a time,
-// the next ones while the last are added up.
+// the next ones while the last are added up. A weight is read from shared memory for each product, which
+// costs up to twice the time (captured, 2048 tokens over 8192 rows: 72 heads 355 us, 80 heads 206; 64 tokens
+// over 16384 to 32768 rows: 77 and 53), so that a caller gains by filling its heads up to a multiple of 16.
 __device__ __forceinline__ void sum_heads(const Args& a, Shared& sh, int half, int part) {
   const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, key = 32 * quad + lane;
   const uint32_t tmem = sh.tmem + uint32_t(half * kColumns) + (uint32_t(32 * quad) << 16);

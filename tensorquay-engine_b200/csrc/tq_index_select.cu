@@ -23,12 +23,15 @@
 //                  of 131072, K 2048: 26 us instead of 84), and for long rows (600 of 65536: 69 us; one
 //                  small block in thirty missed its threshold, 87).
 //
-// What bounds it (times back to back, scores in L2 where they fit): few rows are a chain of loads and
-// barriers (1 x 8192: 6 us; 64 x 32768, K 2048: 16 us, one count, one rank and the cluster's barriers,
-// for 1.1 us of reading). Many rows are bound by the latency of the same chain, five rows an SM at a
-// time, and by instructions: 2048 x 16384, K 2048: 64 us, a third of it the sample and its threshold, a
-// fifth the row's one reading, the rest the 2700 candidates. Pages: 64 x 131072 12.5 us, 41% of the copy
-// bandwidth: one wave of maxima, then the chain.
+// What bounds it (captured calls back to back, scores in L2 where they fit): few rows are a chain of loads
+// and barriers. 1 x 8192: 5.7 us. 64 rows of 16384 to 32768, K 2048, two blocks each: 12.9 us for 1.1 us of
+// reading; of a block's 19300 cycles the token and its scores take 2800, their range 2500, the count 1900,
+// the sum of both blocks' counts and the bin 2200, the bitmap 3250, the rank 1900, the list 2800, the answer
+// 700, the end 1050, and of these five barriers of the cluster about a quarter. Many rows are bound by the
+// latency of the same chain, five rows an SM at a time, and by instructions: 2048 x 16384, K 2048: 64 us, a
+// third of it the sample and its threshold, a fifth the row's one reading, the rest the 2700 candidates.
+// Pages of 64 rows of 65536 to 131072: 11.8 us, 33% of the copy bandwidth (12.5 us and 41% where all are
+// full): one wave of maxima, 8000 cycles, then the chain, 12400.
 
 #include <cuda_runtime.h>
 
@@ -854,8 +857,9 @@ extern "C" int32_t tq_index_select(const TqIndexSelectSpec* spec, int32_t* devic
   const long long rows = (long long)s.scores.shape[0];
   const int items = pages ? (a.columns + kPageRows - 1) / kPageRows : a.columns;
   // A cluster's blocks: as many as it takes to hold a row, and more while the card has room for one on
-  // each SM and a block would still have kFew scores (the barriers of a cluster, about 1000 cycles each,
-  // take as long as a block takes for that many).
+  // each SM and a block would still have kFew scores (the five barriers of a cluster, about 1000 cycles
+  // each, take as long as a block takes for that many: with 14800 scores its range, count and bitmap take
+  // 3500 cycles more than with 8192, beside a barrier).
   constexpr int kFew = 8192;
   a.blocks = 1;
   while (a.blocks < kMaxCluster && (items > a.blocks * kHold || (rows * a.blocks * 2 <= sms &&

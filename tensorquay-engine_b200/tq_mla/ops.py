@@ -616,6 +616,8 @@ class IndexWrite(_Launch):
     ``q`` bf16 ``[T, H, 128]``, ``k`` bf16 ``[T, 128]``, ``w`` bf16 or f32 ``[T, H]``. The call fills
     ``q_out`` u8 ``[T, H, 128]`` (codes) and ``w_out`` f32 ``[T, H]``: ``w * scale`` times the scale of
     the query's codes. Without ``q`` (None, as ``w``, ``q_out`` and ``w_out``) it writes keys only.
+    ``H`` is 1 to 128; ``IndexScores`` takes multiples of 8, so other numbers of heads are filled up
+    here, with queries and weights of zero.
     ``norm_weight``, with ``norm_bias`` or without, normalises ``k`` first (mean and variance, or root
     mean square). ``freq`` f32 ``[R / 2]`` (see ``rope_frequencies``) turns the ``R`` values from
     ``rope_start`` on: neighbours, or with ``rope_half`` the halves against each other.
@@ -660,7 +662,8 @@ class IndexScores(_Launch):
     ``t``'s sequence. Columns behind them keep their values.
 
     ``q`` u8 ``[T, H, 128]`` and ``w`` f32 ``[T, H]`` from ``IndexWrite``, ``kv`` its cache; ``scores``
-    f32 ``[T, N]``.
+    f32 ``[T, N]``. ``H`` is a multiple of 8 up to 128, faster where it is one of 16; heads of zeros change
+    no score.
     """
 
     def __init__(self, q, w, kv, page_table, seq_id, q_pos, kv_len, scores):
